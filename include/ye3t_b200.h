@@ -22,13 +22,14 @@
 extern "C" {
 #endif
 
-#define Y3B_ABI_VERSION 8
+#define Y3B_ABI_VERSION 9
 
 /* dtype codes */
 #define Y3B_F32 0
 #define Y3B_F64 1
 #define Y3B_C64 2
 #define Y3B_C128 3
+#define Y3B_BF16 4 /* learned operators only */
 
 /* status codes */
 #define Y3B_OK 0
@@ -613,6 +614,75 @@ int y3b_forces_gather(const int64_t* row_offsets, const int32_t* neighbors, int6
 int y3b_forces_scatter(const int64_t* row_offsets, const int32_t* neighbors, int64_t center_begin,
                        int64_t center_count, int64_t atom_count, const double* edge_grad,
                        double* forces, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Learned per-atom operators (no counterpart in the reference: models built on
+ * its features use them).
+ *
+ * Species embedding: out[i, c] = scale * table[species[i], c], table
+ * [species_count, channels] and out [atom_count, channels] of one dtype
+ * (F32, F64, BF16; products in fp32, fp64 for F64, rounded once).  species holds int32 or int64
+ * (species_bytes 4 or 8); a value outside [0, species_count) sets
+ * Y3B_STATUS_INDEX_RANGE in *status (nullable) and gives a zero row. */
+int y3b_species_embedding(int dtype, const void* table, int64_t species_count, int64_t channels,
+                          const void* species, int species_bytes, int64_t atom_count, double scale, void* out,
+                          int32_t* status, void* stream);
+
+/* table_grad[v, c] = scale * sum over atoms of species v of grad[i, c], every
+ * row written, summed in fp32 (fp64 for F64) in a fixed order: results are bitwise repeatable.  The
+ * workspace is 32-byte aligned and of the size the query gives (-1 for sizes it does not take). */
+int64_t y3b_species_embedding_adjoint_workspace_bytes(int dtype, int64_t atom_count, int64_t species_count,
+                                                      int64_t channels);
+int y3b_species_embedding_adjoint(int dtype, const void* grad, const void* species, int species_bytes,
+                                  int64_t atom_count, int64_t species_count, int64_t channels, double scale,
+                                  void* workspace, int64_t workspace_bytes, void* table_grad, int32_t* status,
+                                  void* stream);
+
+/* Structure attention: queries [query_count, heads, width] attend to the keys and values
+ * [key_count, key_heads, width] of their own structure,
+ *   s_ij = scale q_i . k_j - slope_h |x_i - y_j|,  out_i = sum_j softmax_j(s_ij) v_j,
+ * key head h / (heads / key_heads) serving query head h.  A query whose structure has no
+ * keys gives zeros.  The last dimension is dense; rows and heads have strides in elements.
+ * positions [query_count, 3], key_positions [key_count, 3] and slopes [heads] are fp32 and null
+ * together.  Structure s holds queries query_offsets[s] .. query_offsets[s + 1] and keys
+ * key_offsets[s] .. key_offsets[s + 1]; *_structure names each row's structure. */
+typedef struct {
+  int32_t dtype; /* Y3B_F32 or Y3B_BF16 */
+  int32_t heads;
+  int32_t key_heads; /* divides heads */
+  int32_t width;     /* 1 to 128 */
+  int64_t query_count;
+  int64_t key_count;
+  int64_t structure_count;
+  const void* query;
+  const void* key;
+  const void* value;
+  int64_t query_row_stride, query_head_stride;
+  int64_t key_row_stride, key_head_stride;
+  int64_t value_row_stride, value_head_stride;
+  const float* positions;
+  const float* key_positions;
+  const float* slopes;
+  const int32_t* query_offsets;   /* [structure_count + 1] */
+  const int32_t* key_offsets;     /* [structure_count + 1] */
+  const int32_t* query_structure; /* [query_count], in [0, structure_count) */
+  const int32_t* key_structure;   /* [key_count], in [0, structure_count) */
+  float scale;
+} y3b_structure_attention_args;
+
+/* out [query_count, heads, width] and lse [query_count, heads] (for the
+ * adjoint) are dense. */
+int y3b_structure_attention(const y3b_structure_attention_args* args, void* out, float* lse, void* stream);
+
+/* Gradients of the call above, every array dense and written whole.  With key_positions_grad null, queries and
+ * keys are the same atoms and positions_grad takes both sums.  No floating-point atomics: results are
+ * bitwise repeatable. */
+int64_t y3b_structure_attention_adjoint_workspace_bytes(int64_t query_count, int64_t key_count, int64_t heads,
+                                                        int64_t key_heads);
+int y3b_structure_attention_adjoint(const y3b_structure_attention_args* args, const void* out_grad, const float* lse,
+                                    void* workspace, int64_t workspace_bytes, void* query_grad, void* key_grad,
+                                    void* value_grad, float* positions_grad, float* key_positions_grad,
+                                    float* slopes_grad, void* stream);
 
 /* ------------------------------------------------------------------------
  * Measurement support: an FP64 / FP32 FMA throughput kernel used to measure

@@ -1,0 +1,83 @@
+"""Learned operators: what is checked on the host, without a GPU."""
+
+import ctypes
+
+import pytest
+import torch
+
+
+def test_layout_counts_are_checked():
+    from ye3t_b200.runtime import StructureLayout
+    with pytest.raises(ValueError):
+        StructureLayout([3, -1], heads=1)
+    with pytest.raises(ValueError):
+        StructureLayout([3, 1], [2], heads=1)
+    with pytest.raises(ValueError):
+        StructureLayout([[3, 1]], heads=1)
+    with pytest.raises(ValueError):
+        StructureLayout([1.5], heads=1)
+    with pytest.raises(ValueError):
+        StructureLayout([3], heads=4, key_heads=3)
+    with pytest.raises(ValueError):
+        StructureLayout([3], heads=0)
+    with pytest.raises(ValueError):
+        StructureLayout([2**30, 2**30], heads=1)
+    with pytest.raises(ValueError):
+        StructureLayout([3], heads=1, device="cpu")
+
+
+def test_cpu_tensors_are_refused():
+    from ye3t_b200 import runtime as rt
+    with pytest.raises(ValueError):
+        rt.species_embedding(torch.zeros(2, 2), torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(ValueError):
+        rt.structure_attention(torch.zeros(2, 1, 4), torch.zeros(2, 1, 4), torch.zeros(2, 1, 4), None)
+
+
+def test_entry_points_refuse_bad_arguments():
+    """The C entry points return an error code before they touch the device."""
+    from ye3t_b200 import _native as nat
+    lib = nat.lib()
+    assert lib.y3b_species_embedding(nat.C64, 0, 1, 1, 0, 8, 1, 1.0, 0, 0, 0) == -1
+    assert lib.y3b_species_embedding(nat.F32, 0, 1, 1, 0, 2, 1, 1.0, 0, 0, 0) == -1
+    assert lib.y3b_species_embedding(nat.F32, 0, 1, 0, 0, 8, 1, 1.0, 0, 0, 0) == -1
+    assert lib.y3b_species_embedding(nat.F32, 0, 1, 1, 0, 8, 1, 1.0, 0, 0, 0) == -1
+    assert lib.y3b_species_embedding(nat.F32, 0, 1, 1, 0, 8, 0, 1.0, 0, 0, 0) == 0
+    assert lib.y3b_species_embedding_adjoint_workspace_bytes(nat.F32, -1, 1, 1) == -1
+    assert lib.y3b_species_embedding_adjoint_workspace_bytes(nat.F32, 1 << 31, 1, 1) == -1
+    assert lib.y3b_species_embedding_adjoint_workspace_bytes(nat.F32, 1000, 10, 8) > 0
+    assert lib.y3b_species_embedding_adjoint(nat.F32, 0, 0, 8, 10, 3, 4, 1.0, 0, 0, 0, 0, 0) == -1
+    assert lib.y3b_structure_attention(None, 0, 0, 0) == -1
+    a = nat.StructureAttentionArgs()
+    a.dtype, a.heads, a.key_heads, a.width = nat.F32, 4, 2, 32
+    call = lambda: lib.y3b_structure_attention(ctypes.byref(a), 0, 0, 0)  # noqa: E731
+    assert call() == 0  # nothing to do
+    a.key_heads = 3
+    assert call() == -1 and b"multiple" in lib.y3b_last_error()
+    a.key_heads, a.width = 2, 129
+    assert call() == -1 and b"width" in lib.y3b_last_error()
+    a.width, a.dtype = 32, nat.F64
+    assert call() == -1
+    a.dtype, a.query_count = nat.BF16, 5
+    assert call() == -1
+    a.query_count, a.positions = 0, 16
+    assert call() == -1 and b"slopes" in lib.y3b_last_error()
+
+
+def test_argument_struct_layout(tmp_path):
+    """The ctypes mirror has the header's size and offsets."""
+    import os
+    import subprocess
+    from ye3t_b200 import _native as nat
+    repo = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    cls = nat.StructureAttentionArgs
+    fields = [f[0] for f in cls._fields_]
+    src = tmp_path / "layout.c"
+    lines = "".join(f'printf("%zu\\n", offsetof(y3b_structure_attention_args, {f}));\n' for f in fields)
+    src.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "ye3t_b200.h"\nint main(void) {\n'
+                   'printf("%zu\\n", sizeof(y3b_structure_attention_args));\n' + lines + "return 0;\n}\n")
+    exe = tmp_path / "layout"
+    subprocess.run(["gcc", "-I", os.path.join(repo, "include"), str(src), "-o", str(exe)], check=True)
+    out = [int(v) for v in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
+    assert out[0] == ctypes.sizeof(cls)
+    assert out[1:] == [getattr(cls, f).offset for f in fields]

@@ -16,8 +16,8 @@ import torch
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libye3t_b200.so")
 
-ABI_VERSION = 8
-F32, F64, C64, C128 = 0, 1, 2, 3
+ABI_VERSION = 9
+F32, F64, C64, C128, BF16 = 0, 1, 2, 3, 4
 STATUS_INDEX_RANGE = 1
 STATUS_CAPACITY = 2
 STATUS_TABLE = 4
@@ -91,6 +91,21 @@ class RecoupledTileTables(ctypes.Structure):
     ]
 
 
+class StructureAttentionArgs(ctypes.Structure):
+    """Mirror of y3b_structure_attention_args."""
+
+    _fields_ = [
+        ("dtype", I32), ("heads", I32), ("key_heads", I32), ("width", I32),
+        ("query_count", I64), ("key_count", I64), ("structure_count", I64),
+        ("query", VP), ("key", VP), ("value", VP),
+        ("query_row_stride", I64), ("query_head_stride", I64), ("key_row_stride", I64), ("key_head_stride", I64),
+        ("value_row_stride", I64), ("value_head_stride", I64),
+        ("positions", VP), ("key_positions", VP), ("slopes", VP),
+        ("query_offsets", VP), ("key_offsets", VP), ("query_structure", VP), ("key_structure", VP),
+        ("scale", ctypes.c_float),
+    ]
+
+
 _SIGS = {
     "y3b_abi_version": (I32, []),
     "y3b_last_error": (ctypes.c_char_p, []),
@@ -152,6 +167,14 @@ _SIGS = {
                                          VP, VP]),
     "y3b_forces_gather": (ctypes.c_int, [VP, VP, I64, VP, VP, VP, VP]),
     "y3b_forces_scatter": (ctypes.c_int, [VP, VP, I64, I64, I64, VP, VP, VP]),
+    "y3b_species_embedding": (ctypes.c_int, [ctypes.c_int, VP, I64, I64, VP, ctypes.c_int, I64, DBL, VP, VP, VP]),
+    "y3b_species_embedding_adjoint_workspace_bytes": (I64, [ctypes.c_int, I64, I64, I64]),
+    "y3b_species_embedding_adjoint": (ctypes.c_int, [ctypes.c_int, VP, VP, ctypes.c_int, I64, I64, I64, DBL, VP, I64,
+                                                     VP, VP, VP]),
+    "y3b_structure_attention": (ctypes.c_int, [ctypes.POINTER(StructureAttentionArgs), VP, VP, VP]),
+    "y3b_structure_attention_adjoint_workspace_bytes": (I64, [I64, I64, I64, I64]),
+    "y3b_structure_attention_adjoint": (ctypes.c_int, [ctypes.POINTER(StructureAttentionArgs), VP, VP, VP, I64, VP,
+                                                       VP, VP, VP, VP, VP, VP]),
     "y3b_fma_peak_launch": (ctypes.c_int, [ctypes.c_int, I32, I32, I32, VP, ctypes.POINTER(DBL), VP]),
 }
 
@@ -194,6 +217,14 @@ def dtype_code(dtype: torch.dtype) -> int:
         return _DTYPE_CODE[dtype]
     except KeyError:
         raise TypeError(f"unsupported dtype {dtype}") from None
+
+
+def learned_dtype_code(dtype: torch.dtype) -> int:
+    """Code of a dtype of the learned operators, which also take bfloat16 but nothing complex."""
+    code = {torch.float32: F32, torch.float64: F64, torch.bfloat16: BF16}.get(dtype)
+    if code is None:
+        raise TypeError(f"unsupported dtype {dtype}")
+    return code
 
 
 def ptr(t) -> int:

@@ -15,9 +15,12 @@ status word is set, matching the reference CPU path's eager checks
 
 from __future__ import annotations
 
+import ctypes
 import os
 
+import numpy as np
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as nat
 
@@ -33,6 +36,9 @@ __all__ = [
     "plain_site_basis_product_adjoint",
     "symmetric_power_table_contraction",
     "pace_radial_channel_contraction_with_derivative",
+    "species_embedding",
+    "StructureLayout",
+    "structure_attention",
     "native_execution_plan_capabilities",
 ]
 
@@ -525,6 +531,266 @@ def pace_radial_channel_contraction_with_derivative(values, derivatives, coeffic
     return out, dout
 
 
+# -- learned per-atom operators ----------------------------------------------------------------
+def _embedding_forward(table, species, scale, validate):
+    dev = nat.require_cuda(table, species, what="species_embedding")
+    t, z = table.contiguous(), species.contiguous()
+    out = torch.empty(tuple(species.shape) + (t.shape[1],), dtype=t.dtype, device=dev)
+    status = _status(dev) if validate else None
+    nat.check(nat.lib().y3b_species_embedding(nat.learned_dtype_code(t.dtype), t.data_ptr(), t.shape[0], t.shape[1],
+                                              z.data_ptr(), z.element_size(), z.numel(), scale, out.data_ptr(),
+                                              nat.ptr(status), nat.stream_of(dev)), "species_embedding")
+    if validate:
+        _raise_on_status(status, "species_embedding")
+    return out
+
+
+def _embedding_adjoint(grad, species, species_count, scale):
+    dev = nat.require_cuda(grad, species, what="species_embedding adjoint")
+    g, z = grad.contiguous(), species.contiguous()
+    C = g.shape[-1]
+    code = nat.learned_dtype_code(g.dtype)
+    out = torch.empty((species_count, C), dtype=g.dtype, device=dev)
+    lib = nat.lib()
+    ws_bytes = int(lib.y3b_species_embedding_adjoint_workspace_bytes(code, z.numel(), species_count, C))
+    if ws_bytes < 0:
+        raise ValueError("species_embedding: the gradient takes up to 2^31 - 1 atoms and species")
+    ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=dev)
+    nat.check(lib.y3b_species_embedding_adjoint(code, g.data_ptr(), z.data_ptr(), z.element_size(), z.numel(),
+                                                species_count, C, scale, ws.data_ptr(), ws_bytes, out.data_ptr(), 0,
+                                                nat.stream_of(dev)), "species_embedding adjoint")
+    return out
+
+
+class _SpeciesEmbedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, species, scale, validate):
+        ctx.save_for_backward(species)
+        ctx.species_count, ctx.scale = table.shape[0], scale
+        return _embedding_forward(table, species, scale, validate)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        (species,) = ctx.saved_tensors
+        return _embedding_adjoint(grad, species, ctx.species_count, ctx.scale), None, None, None
+
+
+def species_embedding(table, species, *, scale=1.0, backend="auto", validate=None):
+    """``out[i] = scale * table[species[i]]``: a learned vector per species.
+
+    ``table`` is ``[species_count, channels]`` (float32, float64 or bfloat16) and ``species`` any integer
+    shape (int32 or int64); the result has shape ``species.shape + (channels,)``.  A species outside the
+    table gives a zero row and no gradient, or ``IndexError`` with ``validate``.  Products are formed in
+    float32 (float64 for float64) and rounded once.
+
+    Differentiable once in ``table``: the atoms are sorted by species and each species' gradients are summed
+    in a fixed order, so the gradient is bitwise repeatable.
+    """
+    _check_backend(backend)
+    table = torch.as_tensor(table)
+    species = torch.as_tensor(species, device=table.device)
+    nat.require_cuda(table, species, what="species_embedding")
+    nat.learned_dtype_code(table.dtype)
+    if table.ndim != 2 or table.shape[1] < 1:
+        raise ValueError("table must be [species_count, channels] with at least one channel")
+    if species.dtype not in (torch.int32, torch.int64):
+        raise TypeError("species must be int32 or int64")
+    scale, validate = float(scale), _validate_default(validate)
+    if table.requires_grad and torch.is_grad_enabled():
+        return _SpeciesEmbedding.apply(table, species, scale, validate)
+    return _embedding_forward(table, species, scale, validate)
+
+
+def _host_counts(counts, what):
+    if isinstance(counts, torch.Tensor):
+        counts = counts.detach().cpu().numpy()
+    c = np.asarray(counts)
+    if c.ndim != 1 or (c.size and c.dtype.kind not in "iu"):
+        raise ValueError(f"{what} must be a one-dimensional list of integers")
+    c = c.astype(np.int64)
+    if c.size and int(c.min()) < 0:
+        raise ValueError(f"{what} must not be negative")
+    if int(c.sum()) > 2**31 - 1:
+        raise ValueError(f"{what}: at most 2^31 - 1 atoms in a batch")
+    return c
+
+
+class StructureLayout:
+    """Which rows of a packed batch belong to which structure, for :func:`structure_attention`.
+
+    ``query_counts[s]`` queries and ``key_counts[s]`` keys of structure ``s`` lie one after the other, structure
+    by structure; with ``key_counts`` None the queries and the keys are the same atoms.  Counts are host
+    integers and may be zero.  A layout is built once per batch and used for every layer and head width with
+    its numbers of heads; it holds index tables only.
+    """
+
+    def __init__(self, query_counts, key_counts=None, *, heads, key_heads=None, device="cuda"):
+        queries = _host_counts(query_counts, "query_counts")
+        keys = queries if key_counts is None else _host_counts(key_counts, "key_counts")
+        if keys.size != queries.size:
+            raise ValueError(f"{queries.size} structures of queries, but {keys.size} of keys")
+        self.heads = int(heads)
+        self.key_heads = self.heads if key_heads is None else int(key_heads)
+        if self.heads < 1 or self.key_heads < 1 or self.heads % self.key_heads:
+            raise ValueError(f"heads ({self.heads}) must be a positive multiple of key_heads ({self.key_heads})")
+        self.shared = key_counts is None
+        self.structure_count = int(queries.size)
+        self.query_count, self.key_count = int(queries.sum()), int(keys.sum())
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise ValueError(f"StructureLayout: ye3t_b200 evaluates on CUDA devices only, not on {self.device}")
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        number = np.arange(self.structure_count)
+        tables = [np.concatenate([[0], np.cumsum(queries)]), np.concatenate([[0], np.cumsum(keys)]),
+                  np.repeat(number, queries), np.repeat(number, keys)]
+        # one copy to the device; it is complete when the constructor returns, so any stream may use it
+        packed = torch.as_tensor(np.concatenate(tables).astype(np.int32)).to(self.device)
+        self._stream = nat.stream_of(self.device)
+        self._packed = packed
+        (self._query_offsets, self._key_offsets, self._query_structure, self._key_structure) = packed.split(
+            [t.size for t in tables])
+
+    def _use(self):
+        """Keeps the tables' memory from reuse before the current stream is done with it."""
+        if nat.stream_of(self.device) != self._stream:
+            self._packed.record_stream(torch.cuda.current_stream(self.device))
+
+
+def _attention_args(query, key, value, x, y, slopes, layout, scale):
+    a = nat.StructureAttentionArgs()
+    a.dtype = nat.learned_dtype_code(query.dtype)
+    a.heads, a.key_heads, a.width = query.shape[1], key.shape[1], query.shape[2]
+    a.query_count, a.key_count, a.structure_count = query.shape[0], key.shape[0], layout.structure_count
+    a.query, a.key, a.value = query.data_ptr(), key.data_ptr(), value.data_ptr()
+    a.query_row_stride, a.query_head_stride = query.stride(0), query.stride(1)
+    a.key_row_stride, a.key_head_stride = key.stride(0), key.stride(1)
+    a.value_row_stride, a.value_head_stride = value.stride(0), value.stride(1)
+    a.positions, a.key_positions, a.slopes = nat.ptr(x), nat.ptr(y), nat.ptr(slopes)
+    a.query_offsets, a.key_offsets = layout._query_offsets.data_ptr(), layout._key_offsets.data_ptr()
+    a.query_structure, a.key_structure = layout._query_structure.data_ptr(), layout._key_structure.data_ptr()
+    a.scale = scale
+    layout._use()
+    return a
+
+
+def _dense_rows(t):
+    """The tensor itself where its last dimension is dense."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _attention_forward(query, key, value, x, y, slopes, layout, scale):
+    q, k, v = _dense_rows(query), _dense_rows(key), _dense_rows(value)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+    args = _attention_args(q, k, v, x, y, slopes, layout, scale)
+    nat.check(nat.lib().y3b_structure_attention(ctypes.byref(args), out.data_ptr(), lse.data_ptr(),
+                                                nat.stream_of(q.device)), "structure_attention")
+    return out, lse
+
+
+class _StructureAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, query, key, value, x, y, slopes, layout, scale):
+        same = y is None
+        x = None if x is None else x.contiguous()
+        y = x if same else y.contiguous()
+        slopes = None if slopes is None else slopes.contiguous()
+        out, lse = _attention_forward(query, key, value, x, y, slopes, layout, scale)
+        ctx.save_for_backward(query, key, value, x, y, slopes, lse)
+        ctx.layout, ctx.scale, ctx.same = layout, scale, same
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        query, key, value, x, y, slopes, lse = ctx.saved_tensors
+        layout, dev = ctx.layout, query.device
+        q, k, v, g = _dense_rows(query), _dense_rows(key), _dense_rows(value), grad.contiguous()
+        dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        dk = torch.empty(k.shape, dtype=k.dtype, device=dev)
+        dv = torch.empty(v.shape, dtype=v.dtype, device=dev)
+        dx = dy = dslopes = None
+        if slopes is not None:
+            dx, dslopes = torch.empty_like(x), torch.empty_like(slopes)
+            dy = None if ctx.same else torch.empty_like(y)
+        lib = nat.lib()
+        ws_bytes = int(lib.y3b_structure_attention_adjoint_workspace_bytes(q.shape[0], k.shape[0], q.shape[1],
+                                                                           k.shape[1]))
+        ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=dev)
+        args = _attention_args(q, k, v, x, y, slopes, layout, ctx.scale)
+        nat.check(lib.y3b_structure_attention_adjoint(
+            ctypes.byref(args), g.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws_bytes, dq.data_ptr(), dk.data_ptr(),
+            dv.data_ptr(), nat.ptr(dx), nat.ptr(dy), nat.ptr(dslopes), nat.stream_of(dev)),
+            "structure_attention adjoint")
+        return dq, dk, dv, dx, dy, dslopes, None, None
+
+
+def _check_positions(t, rows, what):
+    if t.dtype != torch.float32 or tuple(t.shape) != (rows, 3):
+        raise ValueError(f"{what} must be float32 [{rows}, 3], got {t.dtype} {tuple(t.shape)}")
+
+
+def structure_attention(query, key, value, layout, *, positions=None, key_positions=None, slopes=None, scale=None,
+                        backend="auto"):
+    """Softmax attention among the atoms of each structure of a packed batch, weaker with distance.
+
+    ``s_ij = scale * q_i . k_j - slopes[h] * |positions_i - key_positions_j|`` over the keys ``j`` of query
+    ``i``'s own structure, ``out_i = sum_j softmax_j(s_ij) v_j``.  ``query`` is ``[queries, heads, width]``,
+    ``key`` and ``value`` ``[keys, key_heads, width]`` (float32 or bfloat16, width 1 to 128); key head
+    ``h // (heads // key_heads)`` serves query head ``h``.  ``layout`` is the batch's
+    :class:`StructureLayout`; one query per structure makes a pooled readout.  ``positions`` and ``slopes``
+    (float32, both or neither) give the distance term; ``key_positions`` is left out where queries and keys
+    are the same atoms.  ``scale`` defaults to ``width ** -0.5``.  A query whose structure has no keys gives
+    zeros.
+
+    Scores, softmax statistics and sums are held in float32.  Differentiable once in query, key, value,
+    positions, key_positions and slopes (a pair at distance zero gives no position gradient); results and
+    gradients are bitwise repeatable.
+    """
+    _check_backend(backend)
+    given = [t for t in (query, key, value, positions, key_positions, slopes) if t is not None]
+    dev = nat.require_cuda(*given, what="structure_attention")
+    if not isinstance(layout, StructureLayout):
+        raise TypeError("layout must be a StructureLayout")
+    if layout.device != dev:
+        raise ValueError(f"structure_attention: the layout is on {layout.device}, the tensors on {dev}")
+    if query.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"structure_attention takes float32 or bfloat16, got {query.dtype}")
+    if key.dtype != query.dtype or value.dtype != query.dtype:
+        raise TypeError("query, key and value must have one dtype")
+    if query.ndim != 3 or key.ndim != 3 or value.shape != key.shape or key.shape[2] != query.shape[2]:
+        raise ValueError("query must be [queries, heads, width], key and value [keys, key_heads, width]")
+    if not 1 <= query.shape[2] <= 128:
+        raise ValueError(f"head width must be 1 to 128, got {query.shape[2]}")
+    if query.shape[1] != layout.heads or key.shape[1] != layout.key_heads:
+        raise ValueError(f"{query.shape[1]} heads and {key.shape[1]} key heads, but the layout was built for "
+                         f"{layout.heads} and {layout.key_heads}")
+    if query.shape[0] != layout.query_count or key.shape[0] != layout.key_count:
+        raise ValueError(f"{query.shape[0]} queries and {key.shape[0]} keys, but the layout holds "
+                         f"{layout.query_count} and {layout.key_count}")
+    if (positions is None) != (slopes is None):
+        raise ValueError("positions and slopes come together")
+    if positions is None and key_positions is not None:
+        raise ValueError("key_positions without positions")
+    if positions is not None:
+        _check_positions(positions, layout.query_count, "positions")
+        if key_positions is not None:
+            _check_positions(key_positions, layout.key_count, "key_positions")
+        elif not layout.shared:
+            raise ValueError("the layout has keys of its own: give key_positions")
+        if slopes.dtype != torch.float32 or tuple(slopes.shape) != (layout.heads,):
+            raise ValueError(f"slopes must be float32 [{layout.heads}], got {slopes.dtype} {tuple(slopes.shape)}")
+    scale = float(query.shape[2]) ** -0.5 if scale is None else float(scale)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
+        return _StructureAttention.apply(query, key, value, positions, key_positions, slopes, layout, scale)
+    x = None if positions is None else positions.contiguous()
+    y = x if key_positions is None else key_positions.contiguous()
+    return _attention_forward(query, key, value, x, y, None if slopes is None else slopes.contiguous(), layout,
+                              scale)[0]
+
+
 def native_execution_plan_capabilities():
     """Capability report; the analogue of ``ye3t/runtime/execution_plan.py:6118``."""
     try:
@@ -556,6 +822,8 @@ def native_execution_plan_capabilities():
             "ace_density_mixed": ["float32 -> complex64", "float64 -> complex128"],
             "pace_radial_channel_contraction_with_derivative": ["float32", "float64"],
             "ace_bundle": ["complex128"],
+            "species_embedding": ["float32", "float64", "bfloat16"],
+            "structure_attention": ["float32", "bfloat16"],
         },
         "density_accumulate_deterministic": True,
         "max_spherical_lmax": 8,
