@@ -667,22 +667,38 @@ typedef struct {
   const int32_t* key_offsets;     /* [structure_count + 1] */
   const int32_t* query_structure; /* [query_count], in [0, structure_count) */
   const int32_t* key_structure;   /* [key_count], in [0, structure_count) */
+  /* Work tables.  Every query is in query_rows (one warp computes it) or in exactly one tile
+   * of up to 128 queries of one structure; a tile is one item, or several items with consecutive slots
+   * that split its keys and one join.  Keys likewise, with queries as the columns.
+   *   item  (first row, rows, first column, columns, slot or -1, 0, 0, 0)
+   *   join  (first row, rows, first slot, slots) */
+  int64_t query_item_count, query_join_count, query_slot_count, query_row_count;
+  int64_t key_item_count, key_join_count, key_slot_count, key_row_count;
+  const int32_t* query_items; /* 32-byte aligned */
+  const int32_t* query_joins; /* 16-byte aligned */
+  const int32_t* query_rows;
+  const int32_t* key_items;
+  const int32_t* key_joins;
+  const int32_t* key_rows;
   float scale;
 } y3b_structure_attention_args;
 
-/* out [query_count, heads, width] and lse [query_count, heads] (for the
- * adjoint) are dense. */
-int y3b_structure_attention(const y3b_structure_attention_args* args, void* out, float* lse, void* stream);
+/* Bytes of workspace (16-byte aligned) of the call below, or with adjoint != 0 of its adjoint; -1 for bad
+ * arguments.  The tables must be filled in. */
+int64_t y3b_structure_attention_workspace_bytes(const y3b_structure_attention_args* args, int adjoint);
+
+/* out [query_count, heads, width] and lse [query_count, heads] (for the adjoint) are dense.  *status
+ * (nullable) takes Y3B_STATUS_TIMEOUT. */
+int y3b_structure_attention(const y3b_structure_attention_args* args, void* workspace, int64_t workspace_bytes,
+                            void* out, float* lse, int32_t* status, void* stream);
 
 /* Gradients of the call above, every array dense and written whole.  With key_positions_grad null, queries and
  * keys are the same atoms and positions_grad takes both sums.  No floating-point atomics: results are
  * bitwise repeatable. */
-int64_t y3b_structure_attention_adjoint_workspace_bytes(int64_t query_count, int64_t key_count, int64_t heads,
-                                                        int64_t key_heads);
-int y3b_structure_attention_adjoint(const y3b_structure_attention_args* args, const void* out_grad, const float* lse,
-                                    void* workspace, int64_t workspace_bytes, void* query_grad, void* key_grad,
-                                    void* value_grad, float* positions_grad, float* key_positions_grad,
-                                    float* slopes_grad, void* stream);
+int y3b_structure_attention_adjoint(const y3b_structure_attention_args* args, const void* out, const void* out_grad,
+                                    const float* lse, void* workspace, int64_t workspace_bytes, void* query_grad,
+                                    void* key_grad, void* value_grad, float* positions_grad,
+                                    float* key_positions_grad, float* slopes_grad, int32_t* status, void* stream);
 
 /* ------------------------------------------------------------------------
  * Measurement support: an FP64 / FP32 FMA throughput kernel used to measure

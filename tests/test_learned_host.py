@@ -47,10 +47,10 @@ def test_entry_points_refuse_bad_arguments():
     assert lib.y3b_species_embedding_adjoint_workspace_bytes(nat.F32, 1 << 31, 1, 1) == -1
     assert lib.y3b_species_embedding_adjoint_workspace_bytes(nat.F32, 1000, 10, 8) > 0
     assert lib.y3b_species_embedding_adjoint(nat.F32, 0, 0, 8, 10, 3, 4, 1.0, 0, 0, 0, 0, 0) == -1
-    assert lib.y3b_structure_attention(None, 0, 0, 0) == -1
+    assert lib.y3b_structure_attention(None, 0, 0, 0, 0, 0, 0) == -1
     a = nat.StructureAttentionArgs()
     a.dtype, a.heads, a.key_heads, a.width = nat.F32, 4, 2, 32
-    call = lambda: lib.y3b_structure_attention(ctypes.byref(a), 0, 0, 0)  # noqa: E731
+    call = lambda: lib.y3b_structure_attention(ctypes.byref(a), 0, 0, 0, 0, 0, 0)  # noqa: E731
     assert call() == 0  # nothing to do
     a.key_heads = 3
     assert call() == -1 and b"multiple" in lib.y3b_last_error()

@@ -102,7 +102,10 @@ class StructureAttentionArgs(ctypes.Structure):
         ("value_row_stride", I64), ("value_head_stride", I64),
         ("positions", VP), ("key_positions", VP), ("slopes", VP),
         ("query_offsets", VP), ("key_offsets", VP), ("query_structure", VP), ("key_structure", VP),
-        ("scale", ctypes.c_float),
+        ("query_item_count", I64), ("query_join_count", I64), ("query_slot_count", I64), ("query_row_count", I64),
+        ("key_item_count", I64), ("key_join_count", I64), ("key_slot_count", I64), ("key_row_count", I64),
+        ("query_items", VP), ("query_joins", VP), ("query_rows", VP), ("key_items", VP), ("key_joins", VP),
+        ("key_rows", VP), ("scale", ctypes.c_float),
     ]
 
 
@@ -171,10 +174,10 @@ _SIGS = {
     "y3b_species_embedding_adjoint_workspace_bytes": (I64, [ctypes.c_int, I64, I64, I64]),
     "y3b_species_embedding_adjoint": (ctypes.c_int, [ctypes.c_int, VP, VP, ctypes.c_int, I64, I64, I64, DBL, VP, I64,
                                                      VP, VP, VP]),
-    "y3b_structure_attention": (ctypes.c_int, [ctypes.POINTER(StructureAttentionArgs), VP, VP, VP]),
-    "y3b_structure_attention_adjoint_workspace_bytes": (I64, [I64, I64, I64, I64]),
-    "y3b_structure_attention_adjoint": (ctypes.c_int, [ctypes.POINTER(StructureAttentionArgs), VP, VP, VP, I64, VP,
-                                                       VP, VP, VP, VP, VP, VP]),
+    "y3b_structure_attention_workspace_bytes": (I64, [ctypes.POINTER(StructureAttentionArgs), ctypes.c_int]),
+    "y3b_structure_attention": (ctypes.c_int, [ctypes.POINTER(StructureAttentionArgs), VP, I64, VP, VP, VP, VP]),
+    "y3b_structure_attention_adjoint": (ctypes.c_int, [ctypes.POINTER(StructureAttentionArgs), VP, VP, VP, VP, I64,
+                                                       VP, VP, VP, VP, VP, VP, VP, VP]),
     "y3b_fma_peak_launch": (ctypes.c_int, [ctypes.c_int, I32, I32, I32, VP, ctypes.POINTER(DBL), VP]),
 }
 

@@ -14,7 +14,9 @@
 //
 // Row kernels: one warp per (row, head); lanes take 32 columns at a time for the scores and
 // then the D components for the sums.
-#include "structure_attention.cuh"
+#include <algorithm>
+
+#include "structure_attention_tile.cuh"
 
 namespace y3b {
 namespace {
@@ -63,15 +65,16 @@ __device__ __forceinline__ Apart apart(float ax, float ay, float az, const float
 }
 
 template <typename T>
-__global__ void __launch_bounds__(32 * kRowWarps) row_forward_kernel(AttArgs a, T* __restrict__ out,
+__global__ void __launch_bounds__(32 * kRowWarps) row_forward_kernel(AttArgs a, const int32_t* __restrict__ rows,
+                                                                     int64_t row_count, T* __restrict__ out,
                                                                      float* __restrict__ lse) {
   __shared__ float s_q[kRowWarps][kAttMaxWidth];
   __shared__ float s_p[kRowWarps][32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t task = blockIdx.x * int64_t(kRowWarps) + w;
-  if (task >= a.nq * a.H) return;
-  const int64_t i = task / a.H;
-  const int h = int(task - i * a.H), hk = h / a.group;
+  if (task >= row_count * a.H) return;
+  const int64_t i = rows[task / a.H];
+  const int h = int(task % a.H), hk = h / a.group;
   const T* q = static_cast<const T*>(a.q) + i * a.q_row + h * a.q_head;
   const T* k = static_cast<const T*>(a.k) + hk * a.k_head;
   const T* v = static_cast<const T*>(a.v) + hk * a.v_head;
@@ -129,16 +132,16 @@ __global__ void __launch_bounds__(32 * kRowWarps) row_forward_kernel(AttArgs a, 
 // Query side of the backward: delta, dq and this row's parts of dslope and dx.
 template <typename T>
 __global__ void __launch_bounds__(32 * kRowWarps) row_backward_query_kernel(
-    AttArgs a, const T* __restrict__ grad, const float* __restrict__ lse, float* __restrict__ delta,
-    T* __restrict__ dq, float* __restrict__ dslope_part, float* __restrict__ dx_part) {
+    AttArgs a, const int32_t* __restrict__ rows, int64_t row_count, const T* __restrict__ grad,
+    const float* __restrict__ lse, float* __restrict__ delta, T* __restrict__ dq, float* __restrict__ dslope_part, float* __restrict__ dx_part) {
   __shared__ float s_q[kRowWarps][kAttMaxWidth];
   __shared__ float s_g[kRowWarps][kAttMaxWidth];
   __shared__ float s_p[kRowWarps][32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t task = blockIdx.x * int64_t(kRowWarps) + w;
-  if (task >= a.nq * a.H) return;
-  const int64_t i = task / a.H;
-  const int h = int(task - i * a.H), hk = h / a.group;
+  if (task >= row_count * a.H) return;
+  const int64_t i = rows[task / a.H];
+  const int h = int(task % a.H), hk = h / a.group;
   const T* q = static_cast<const T*>(a.q) + i * a.q_row + h * a.q_head;
   const T* k = static_cast<const T*>(a.k) + hk * a.k_head;
   const T* v = static_cast<const T*>(a.v) + hk * a.v_head;
@@ -223,17 +226,17 @@ __global__ void __launch_bounds__(32 * kRowWarps) row_backward_query_kernel(
 // Key side: dk, dv and dy of one (key, key head), over the query heads that share it.
 template <typename T>
 __global__ void __launch_bounds__(32 * kRowWarps) row_backward_key_kernel(
-    AttArgs a, const T* __restrict__ grad, const float* __restrict__ lse, const float* __restrict__ delta,
-    T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ dy_part) {
+    AttArgs a, const int32_t* __restrict__ rows, int64_t row_count, const T* __restrict__ grad,
+    const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ dy_part) {
   __shared__ float s_k[kRowWarps][kAttMaxWidth];
   __shared__ float s_v[kRowWarps][kAttMaxWidth];
   __shared__ float s_p[kRowWarps][32];
   __shared__ float s_d[kRowWarps][32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t task = blockIdx.x * int64_t(kRowWarps) + w;
-  if (task >= a.nk * a.Hk) return;
-  const int64_t j = task / a.Hk;
-  const int hk = int(task - j * a.Hk);
+  if (task >= row_count * a.Hk) return;
+  const int64_t j = rows[task / a.Hk];
+  const int hk = int(task % a.Hk);
   const T* k = static_cast<const T*>(a.k) + j * a.k_row + hk * a.k_head;
   const T* v = static_cast<const T*>(a.v) + j * a.v_row + hk * a.v_head;
   for (int d = lane; d < a.D; d += 32) {
@@ -370,6 +373,14 @@ int unpack(const y3b_structure_attention_args* p, const char* what, AttArgs* a) 
     Y3B_CHECK_ARG(p->query_count == 0 || p->positions, "%s: slopes without positions", what);
     Y3B_CHECK_ARG(p->key_count == 0 || p->key_positions, "%s: slopes without key positions", what);
   }
+  Y3B_CHECK_ARG(p->query_item_count >= 0 && p->query_join_count >= 0 && p->query_slot_count >= 0 &&
+                    p->query_row_count >= 0 && p->key_item_count >= 0 && p->key_join_count >= 0 &&
+                    p->key_slot_count >= 0 && p->key_row_count >= 0,
+                "%s: negative table size", what);
+  Y3B_CHECK_ARG((p->query_item_count == 0 || p->query_items) && (p->query_join_count == 0 || p->query_joins) &&
+                    (p->query_row_count == 0 || p->query_rows) && (p->key_item_count == 0 || p->key_items) &&
+                    (p->key_join_count == 0 || p->key_joins) && (p->key_row_count == 0 || p->key_rows),
+                "%s: null table", what);
   a->H = p->heads;
   a->Hk = p->key_heads;
   a->D = p->width;
@@ -397,37 +408,336 @@ int unpack(const y3b_structure_attention_args* p, const char* what, AttArgs* a) 
   return Y3B_OK;
 }
 
-unsigned row_grid(int64_t tasks) { return unsigned((tasks + kRowWarps - 1) / kRowWarps); }
+// ---------------------------------------------------------------------------
+// Operands for the tile kernels: rows padded to a multiple of 8 values, fp32 as three bf16
+// pieces.  A non-finite value keeps its first piece and zeros for the rest.  One thread per 8
+// values of one head of one row.
+struct PackSource {
+  const void* p;
+  int64_t row, head, rows;
+  int heads;
+  __nv_bfloat16* out;
+};
+struct PackArgs {
+  PackSource s[4];
+  int D, chunks;
+};
 
 template <typename T>
-int forward(const AttArgs& a, void* out, float* lse, cudaStream_t s) {
-  row_forward_kernel<T><<<row_grid(a.nq * a.H), 32 * kRowWarps, 0, s>>>(a, static_cast<T*>(out), lse);
-  Y3B_LAUNCH_CHECK();
+__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackArgs a) {
+  const PackSource& o = a.s[blockIdx.y];
+  const int64_t per_row = int64_t(o.heads) * a.chunks, total = o.rows * per_row, piece = total * 8;
+  for (int64_t t = blockIdx.x * int64_t(256) + threadIdx.x; t < total; t += int64_t(gridDim.x) * 256) {
+    const int64_t r = t / per_row;
+    const int u = int(t - r * per_row), h = u / a.chunks, c = u - h * a.chunks;
+    const T* src = static_cast<const T*>(o.p) + r * o.row + h * o.head + c * 8;
+    const int n = a.D - c * 8;
+    uint32_t out[3][4];
+#pragma unroll
+    for (int k = 0; k < 8; k += 2) {
+      const float x = k < n ? to_float(src[k]) : 0.0f, y = k + 1 < n ? to_float(src[k + 1]) : 0.0f;
+      if constexpr (sizeof(T) == 4) {
+        uint32_t q[3];
+        split_pair<3>(x, y, q);
+        // the rest of a value that is not finite in bf16 would be NaN
+        const uint32_t keep = ((q[0] & 0x7f80u) == 0x7f80u ? 0u : 0xffffu) |
+                              ((q[0] & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u);
+        out[0][k / 2] = q[0];
+        out[1][k / 2] = q[1] & keep;
+        out[2][k / 2] = q[2] & keep;
+      } else {
+        out[0][k / 2] = tc::bf16x2(x, y);
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < (sizeof(T) == 4 ? 3 : 1); ++p)
+      *reinterpret_cast<uint4*>(o.out + p * piece + t * 8) = make_uint4(out[p][0], out[p][1], out[p][2], out[p][3]);
+  }
+}
+
+// Joins of split items, one CTA a (join, head), one warp a row; W = floats of a partial row.
+template <typename T>
+__global__ void __launch_bounds__(128) join_forward_kernel(const AttJoin* __restrict__ joins,
+                                                           const float* __restrict__ part, int W, int DP, int D,
+                                                           int H, T* __restrict__ out, float* __restrict__ lse) {
+  const AttJoin jn = joins[blockIdx.x / unsigned(H)];
+  const int h = int(blockIdx.x % unsigned(H)), lane = threadIdx.x & 31;
+  const int64_t step = int64_t(H) * kTileRows * W;
+  for (int r = threadIdx.x >> 5; r < jn.rows; r += 4) {
+    const float* p = part + ((int64_t(jn.first) * H + h) * kTileRows + r) * W;
+    float m = -INFINITY;
+    for (int k = lane; k < jn.count; k += 32) m = fmaxf(m, p[k * step + DP]);
+    m = warp_max(m);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f;
+    for (int k = lane; k < jn.count; k += 32) l += p[k * step + DP + 1] * exp2f(p[k * step + DP] - ref);
+    l = warp_sum(l);
+    const bool none = m == -INFINITY && l == 0.0f;
+    const int64_t at = (int64_t(jn.row) + r) * H + h;
+    const float inv = none ? 0.0f : 1.0f / l;
+    for (int d = lane; d < D; d += 32) {
+      float o = 0.0f;
+      for (int k = 0; k < jn.count; ++k) {
+        // a part without any score above -inf holds no numbers
+        const float mk = p[k * step + DP];
+        if (!(mk == -INFINITY && p[k * step + DP + 1] == 0.0f)) o = fmaf(p[k * step + d], exp2f(mk - ref), o);
+      }
+      out[at * D + d] = from_float<T>(none ? 0.0f : o * inv);
+    }
+    if (lane == 0) lse[at] = none ? INFINITY : m + log2f(l);
+  }
+}
+
+__device__ __forceinline__ float sum_parts(const float* p, int64_t step, int count) {
+  float s = 0.0f;
+  for (int k = 0; k < count; ++k) s += p[k * step];
+  return s;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(128) join_query_kernel(const AttJoin* __restrict__ joins,
+                                                         const float* __restrict__ part, int W, int DP, int D, int H,
+                                                         float scale, const float* __restrict__ slopes,
+                                                         T* __restrict__ dq, float* __restrict__ delta,
+                                                         float* __restrict__ slope_part,
+                                                         float* __restrict__ place_part) {
+  const AttJoin jn = joins[blockIdx.x / unsigned(H)];
+  const int h = int(blockIdx.x % unsigned(H)), lane = threadIdx.x & 31;
+  const int64_t step = int64_t(H) * kTileRows * W;
+  for (int r = threadIdx.x >> 5; r < jn.rows; r += 4) {
+    const float* p = part + ((int64_t(jn.first) * H + h) * kTileRows + r) * W;
+    const int64_t at = (int64_t(jn.row) + r) * H + h;
+    const float s = lane < 10 ? sum_parts(p + DP + lane, step, jn.count) : 0.0f;
+    const float all = __shfl_sync(0xffffffffu, s, 9), inv = all == 0.0f ? 0.0f : 1.0f / all;
+    const float dl = __shfl_sync(0xffffffffu, s, 0) * inv;
+    const float low = __shfl_sync(0xffffffffu, s, lane < 3 ? 6 + lane : 2);  // what delta multiplies
+    const float high = __shfl_sync(0xffffffffu, s, lane < 3 ? 3 + lane : 1);
+    if (lane == 0) delta[at] = dl;
+    for (int d = lane; d < D; d += 32) {
+      float x = sum_parts(p + d, step, jn.count);
+      // one piece: dS was formed with the forward's rounded delta, and P K follows the sums
+      if constexpr (sizeof(T) == 2) x = fmaf(p[DP + 10] - dl, sum_parts(p + DP + 16 + d, step, jn.count), x);
+      dq[at * D + d] = from_float<T>(scale * x);
+    }
+    if (slopes) {
+      if (lane < 3) place_part[at * 3 + lane] = -slopes[h] * inv * (high - dl * low);
+      if (lane == 3) slope_part[at] = -inv * (high - dl * low);
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(128) join_key_kernel(const AttJoin* __restrict__ joins,
+                                                       const float* __restrict__ part, int W, int DP, int D, int Hk,
+                                                       float scale, T* __restrict__ dk, T* __restrict__ dv,
+                                                       float* __restrict__ place_part) {
+  const AttJoin jn = joins[blockIdx.x / unsigned(Hk)];
+  const int h = int(blockIdx.x % unsigned(Hk)), lane = threadIdx.x & 31;
+  const int64_t step = int64_t(Hk) * kTileRows * W;
+  for (int r = threadIdx.x >> 5; r < jn.rows; r += 4) {
+    const float* p = part + ((int64_t(jn.first) * Hk + h) * kTileRows + r) * W;
+    const int64_t at = (int64_t(jn.row) + r) * Hk + h;
+    for (int d = lane; d < D; d += 32) {
+      dv[at * D + d] = from_float<T>(sum_parts(p + d, step, jn.count));
+      dk[at * D + d] = from_float<T>(scale * sum_parts(p + DP + d, step, jn.count));
+    }
+    if (place_part && lane < 3) place_part[at * 3 + lane] = -sum_parts(p + 2 * DP + lane, step, jn.count);
+  }
+}
+
+// ---------------------------------------------------------------------------
+unsigned row_grid(int64_t tasks) { return unsigned((tasks + kRowWarps - 1) / kRowWarps); }
+
+bool on16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// How one call uses its workspace (offsets in bytes, parts 16-byte aligned).
+struct AttPlan {
+  int pieces, DP, chunks, Wf, Wq, Wk;
+  bool tiles;
+  bool direct[3];  // query, key, value are read in place
+  int64_t packed[4], delta, slope, dx, dy, part_q, part_k, bytes;
+};
+
+bool in_place(const y3b_structure_attention_args* p, const void* base, int64_t row, int64_t head) {
+  return p->dtype == Y3B_BF16 && p->width % 8 == 0 && row % 8 == 0 && head % 8 == 0 && on16(base);
+}
+
+AttPlan make_plan(const y3b_structure_attention_args* p, bool adjoint) {
+  AttPlan w;
+  const int64_t H = p->heads, Hk = p->key_heads, nq = p->query_count, nk = p->key_count;
+  w.pieces = p->dtype == Y3B_F32 ? 3 : 1;
+  w.DP = p->width > 64 ? 128 : 64;
+  w.chunks = (p->width + 7) / 8;
+  w.Wf = w.DP + 16;
+  w.Wq = (w.pieces == 1 ? 2 : 1) * w.DP + 16;
+  w.Wk = 2 * w.DP + 16;
+  w.tiles = p->query_item_count > 0 || (adjoint && p->key_item_count > 0);
+  w.direct[0] = in_place(p, p->query, p->query_row_stride, p->query_head_stride);
+  w.direct[1] = in_place(p, p->key, p->key_row_stride, p->key_head_stride);
+  w.direct[2] = in_place(p, p->value, p->value_row_stride, p->value_head_stride);
+  int64_t at = 0;
+  const auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += (bytes + 15) / 16 * 16;
+    return here;
+  };
+  const int64_t row = int64_t(w.pieces) * w.chunks * 16;
+  w.packed[0] = take(w.tiles && !w.direct[0] ? nq * H * row : 0);
+  w.packed[1] = take(w.tiles && !w.direct[1] ? nk * Hk * row : 0);
+  w.packed[2] = take(w.tiles && !w.direct[2] ? nk * Hk * row : 0);
+  w.packed[3] = take(w.tiles && adjoint ? nq * H * row : 0);
+  w.delta = take(adjoint ? nq * H * 4 : 0);
+  w.slope = take(adjoint ? nq * H * 4 : 0);
+  w.dx = take(adjoint ? nq * H * 12 : 0);
+  w.dy = take(adjoint ? nk * Hk * 12 : 0);
+  w.part_q = take(p->query_slot_count * H * kTileRows * w.Wq * 4);
+  w.part_k = take(adjoint ? p->key_slot_count * Hk * kTileRows * w.Wk * 4 : 0);
+  w.bytes = at;
+  return w;
+}
+
+// Operand views of the call, packed where they cannot be read in place.
+int operands(const y3b_structure_attention_args* p, const AttPlan& w, const void* grad, unsigned char* ws,
+             AttTileArgs* t, cudaStream_t s) {
+  const int64_t H = p->heads, Hk = p->key_heads, D = p->width;
+  const PackSource src[4] = {
+      {p->query, p->query_row_stride, p->query_head_stride, p->query_count, int(H), nullptr},
+      {p->key, p->key_row_stride, p->key_head_stride, p->key_count, int(Hk), nullptr},
+      {p->value, p->value_row_stride, p->value_head_stride, p->key_count, int(Hk), nullptr},
+      {grad, H * D, D, p->query_count, int(H), nullptr}};
+  AttOperand* dst[4] = {&t->q, &t->k, &t->v, &t->g};
+  PackArgs a;
+  a.D = int(D);
+  a.chunks = w.chunks;
+  int n = 0;
+  int64_t most = 0;
+  for (int k = 0; k < (grad ? 4 : 3); ++k) {
+    if (k < 3 ? w.direct[k] : in_place(p, grad, H * D, D)) {
+      *dst[k] = {static_cast<const __nv_bfloat16*>(src[k].p), src[k].row, src[k].head, 0};
+      continue;
+    }
+    PackSource o = src[k];
+    o.out = reinterpret_cast<__nv_bfloat16*>(ws + w.packed[k]);
+    const int64_t wide = int64_t(w.chunks) * 8;
+    *dst[k] = {o.out, o.heads * wide, wide, o.rows * o.heads * wide};
+    if (o.rows > 0) {
+      a.s[n++] = o;
+      most = std::max(most, o.rows * o.heads * w.chunks);
+    }
+  }
+  if (n) {
+    const dim3 grid(unsigned(std::min<int64_t>((most + 255) / 256, kSMs * 16)), unsigned(n));
+    if (p->dtype == Y3B_F32) pack_kernel<float><<<grid, 256, 0, s>>>(a);
+    else pack_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a);
+    Y3B_LAUNCH_CHECK();
+  }
   return Y3B_OK;
 }
 
-// Workspace of the backward: delta [nq, H], the rows' parts of dslope [nq, H] and dx
-// [nq, H, 3], and of dy [nk, Hk, 3], all fp32.
-int64_t backward_floats(int64_t nq, int64_t nk, int64_t H, int64_t Hk) { return nq * H * 5 + nk * Hk * 3; }
+AttTileArgs tile_args(const y3b_structure_attention_args* p, const AttArgs& a, const AttPlan& w, int32_t* status) {
+  AttTileArgs t{};
+  t.H = a.H;
+  t.Hk = a.Hk;
+  t.D = a.D;
+  t.group = a.group;
+  t.chunks = w.chunks;
+  t.x = a.x;
+  t.y = a.y;
+  t.slopes = a.slopes;
+  t.scale = a.scale;
+  t.scale2 = a.scale2;
+  t.status = status;
+  return t;
+}
 
 template <typename T>
-int backward(const AttArgs& a, const void* grad, const float* lse, float* ws, void* dq, void* dk, void* dv,
-             float* dx, float* dy, float* dslopes, cudaStream_t s) {
-  float* delta = ws;
-  float* slope_part = delta + a.nq * a.H;
-  float* dx_part = slope_part + a.nq * a.H;
-  float* dy_part = dx_part + a.nq * a.H * 3;
-  const T* g = static_cast<const T*>(grad);
-  if (a.nq > 0) {
-    row_backward_query_kernel<T><<<row_grid(a.nq * a.H), 32 * kRowWarps, 0, s>>>(a, g, lse, delta,
-                                                                                static_cast<T*>(dq), slope_part,
-                                                                                dx_part);
+int forward(const y3b_structure_attention_args* p, const AttArgs& a, const AttPlan& w, unsigned char* ws, void* out,
+            float* lse, int32_t* status, cudaStream_t s) {
+  if (p->query_row_count > 0) {
+    row_forward_kernel<T><<<row_grid(p->query_row_count * a.H), 32 * kRowWarps, 0, s>>>(
+        a, p->query_rows, p->query_row_count, static_cast<T*>(out), lse);
     Y3B_LAUNCH_CHECK();
   }
-  if (a.nk > 0) {
-    row_backward_key_kernel<T><<<row_grid(a.nk * a.Hk), 32 * kRowWarps, 0, s>>>(
-        a, g, lse, delta, static_cast<T*>(dk), static_cast<T*>(dv), dy_part);
+  if (p->query_item_count > 0) {
+    AttTileArgs t = tile_args(p, a, w, status);
+    int rc = operands(p, w, nullptr, ws, &t, s);
+    if (rc) return rc;
+    t.items = reinterpret_cast<const AttItem*>(p->query_items);
+    t.out0 = out;
+    t.lse = lse;
+    t.part = reinterpret_cast<float*>(ws + w.part_q);
+    t.vec = a.D * sizeof(T) % 16 == 0 && on16(out);
+    rc = attention_forward_tiles(w.pieces, t, p->query_item_count, s);
+    if (rc) return rc;
+    if (p->query_join_count > 0) {
+      join_forward_kernel<T><<<unsigned(p->query_join_count * a.H), 128, 0, s>>>(
+          reinterpret_cast<const AttJoin*>(p->query_joins), t.part, w.Wf, w.DP, a.D, a.H, static_cast<T*>(out), lse);
+      Y3B_LAUNCH_CHECK();
+    }
+  }
+  return Y3B_OK;
+}
+
+template <typename T>
+int backward(const y3b_structure_attention_args* p, const AttArgs& a, const AttPlan& w, unsigned char* ws,
+             const void* out, const void* grad, const float* lse, void* dq, void* dk, void* dv, float* dx, float* dy,
+             float* dslopes, int32_t* status, cudaStream_t s) {
+  float* delta = reinterpret_cast<float*>(ws + w.delta);
+  float* slope_part = reinterpret_cast<float*>(ws + w.slope);
+  float* dx_part = reinterpret_cast<float*>(ws + w.dx);
+  float* dy_part = reinterpret_cast<float*>(ws + w.dy);
+  const T* g = static_cast<const T*>(grad);
+  AttTileArgs t = tile_args(p, a, w, status);
+  if (w.tiles) {
+    const int rc = operands(p, w, grad, ws, &t, s);
+    if (rc) return rc;
+  }
+  t.lse = const_cast<float*>(lse);
+  t.delta = delta;
+  t.slope_part = slope_part;
+  // query side: it also gives delta, which the key side reads
+  if (p->query_row_count > 0) {
+    row_backward_query_kernel<T><<<row_grid(p->query_row_count * a.H), 32 * kRowWarps, 0, s>>>(
+        a, p->query_rows, p->query_row_count, g, lse, delta, static_cast<T*>(dq), slope_part, dx_part);
     Y3B_LAUNCH_CHECK();
+  }
+  if (p->query_item_count > 0) {
+    t.items = reinterpret_cast<const AttItem*>(p->query_items);
+    t.out_in = out;
+    t.grad_in = grad;
+    t.place_part = dx_part;
+    t.out0 = dq;
+    t.part = reinterpret_cast<float*>(ws + w.part_q);
+    t.vec = a.D * sizeof(T) % 16 == 0 && on16(dq) && on16(out) && on16(grad);
+    const int rc = attention_query_tiles(w.pieces, t, p->query_item_count, s);
+    if (rc) return rc;
+    if (p->query_join_count > 0) {
+      join_query_kernel<T><<<unsigned(p->query_join_count * a.H), 128, 0, s>>>(
+          reinterpret_cast<const AttJoin*>(p->query_joins), t.part, w.Wq, w.DP, a.D, a.H, a.scale, a.slopes,
+          static_cast<T*>(dq), delta, slope_part, dx_part);
+      Y3B_LAUNCH_CHECK();
+    }
+  }
+  if (p->key_row_count > 0) {
+    row_backward_key_kernel<T><<<row_grid(p->key_row_count * a.Hk), 32 * kRowWarps, 0, s>>>(
+        a, p->key_rows, p->key_row_count, g, lse, delta, static_cast<T*>(dk), static_cast<T*>(dv), dy_part);
+    Y3B_LAUNCH_CHECK();
+  }
+  if (p->key_item_count > 0) {
+    t.items = reinterpret_cast<const AttItem*>(p->key_items);
+    t.place_part = dy_part;
+    t.out0 = dv;
+    t.out1 = dk;
+    t.part = reinterpret_cast<float*>(ws + w.part_k);
+    t.vec = a.D * sizeof(T) % 16 == 0 && on16(dk) && on16(dv);
+    const int rc = attention_key_tiles(w.pieces, t, p->key_item_count, s);
+    if (rc) return rc;
+    if (p->key_join_count > 0) {
+      join_key_kernel<T><<<unsigned(p->key_join_count * a.Hk), 128, 0, s>>>(
+          reinterpret_cast<const AttJoin*>(p->key_joins), t.part, w.Wk, w.DP, a.D, a.Hk, a.scale,
+          static_cast<T*>(dk), static_cast<T*>(dv), a.slopes ? dy_part : nullptr);
+      Y3B_LAUNCH_CHECK();
+    }
   }
   if (a.slopes) {
     // dy == null: queries and keys are the same atoms and dx takes both sums
@@ -447,50 +757,62 @@ int backward(const AttArgs& a, const void* grad, const float* lse, float* ws, vo
 
 using namespace y3b;
 
-extern "C" int y3b_structure_attention(const y3b_structure_attention_args* args, void* out, float* lse,
+extern "C" int64_t y3b_structure_attention_workspace_bytes(const y3b_structure_attention_args* args, int adjoint) {
+  AttArgs a;
+  if (unpack(args, "structure_attention_workspace_bytes", &a)) return -1;
+  return make_plan(args, adjoint != 0).bytes;
+}
+
+namespace {
+int check_workspace(const AttPlan& w, const void* workspace, int64_t bytes, const char* what) {
+  if (w.bytes == 0) return Y3B_OK;
+  Y3B_CHECK_ARG(workspace && on16(workspace), "%s: workspace must be 16-byte aligned", what);
+  if (bytes < w.bytes)
+    return fail(Y3B_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld needed", what, (long long)bytes,
+                (long long)w.bytes);
+  return Y3B_OK;
+}
+}  // namespace
+
+extern "C" int y3b_structure_attention(const y3b_structure_attention_args* args, void* workspace,
+                                       int64_t workspace_bytes, void* out, float* lse, int32_t* status,
                                        void* stream) {
   AttArgs a;
-  const int rc = unpack(args, "structure_attention", &a);
+  int rc = unpack(args, "structure_attention", &a);
   if (rc) return rc;
   if (a.nq == 0) return Y3B_OK;
   Y3B_CHECK_ARG(out && lse, "structure_attention: null output");
-  return args->dtype == Y3B_F32 ? forward<float>(a, out, lse, as_stream(stream))
-                                : forward<__nv_bfloat16>(a, out, lse, as_stream(stream));
-}
-
-extern "C" int64_t y3b_structure_attention_adjoint_workspace_bytes(int64_t query_count, int64_t key_count,
-                                                                   int64_t heads, int64_t key_heads) {
-  if (query_count < 0 || key_count < 0 || heads < 1 || key_heads < 1) return -1;
-  return backward_floats(query_count, key_count, heads, key_heads) * 4;
-}
-
-extern "C" int y3b_structure_attention_adjoint(const y3b_structure_attention_args* args, const void* out_grad,
-                                               const float* lse, void* workspace, int64_t workspace_bytes,
-                                               void* query_grad, void* key_grad, void* value_grad,
-                                               float* positions_grad, float* key_positions_grad, float* slopes_grad,
-                                               void* stream) {
-  AttArgs a;
-  const int rc = unpack(args, "structure_attention_adjoint", &a);
+  const AttPlan w = make_plan(args, false);
+  rc = check_workspace(w, workspace, workspace_bytes, "structure_attention");
   if (rc) return rc;
-  const int64_t need = backward_floats(a.nq, a.nk, a.H, a.Hk) * 4;
-  Y3B_CHECK_ARG(a.nq == 0 || (out_grad && lse && query_grad), "structure_attention_adjoint: null query-side argument");
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  return args->dtype == Y3B_F32 ? forward<float>(args, a, w, ws, out, lse, status, as_stream(stream))
+                                : forward<__nv_bfloat16>(args, a, w, ws, out, lse, status, as_stream(stream));
+}
+
+extern "C" int y3b_structure_attention_adjoint(const y3b_structure_attention_args* args, const void* out,
+                                               const void* out_grad, const float* lse, void* workspace,
+                                               int64_t workspace_bytes, void* query_grad, void* key_grad,
+                                               void* value_grad, float* positions_grad, float* key_positions_grad,
+                                               float* slopes_grad, int32_t* status, void* stream) {
+  AttArgs a;
+  int rc = unpack(args, "structure_attention_adjoint", &a);
+  if (rc) return rc;
+  Y3B_CHECK_ARG(a.nq == 0 || (out && out_grad && lse && query_grad),
+                "structure_attention_adjoint: null query-side argument");
   Y3B_CHECK_ARG(a.nk == 0 || (key_grad && value_grad), "structure_attention_adjoint: null key-side gradient");
   Y3B_CHECK_ARG(!a.slopes || (slopes_grad && (a.nq == 0 || positions_grad)),
                 "structure_attention_adjoint: null position or slope gradient");
   Y3B_CHECK_ARG(!a.slopes || key_positions_grad || a.nk == 0 || a.nq == a.nk,
                 "structure_attention_adjoint: one position gradient needs as many queries as keys");
-  if (need > 0) {
-    Y3B_CHECK_ARG(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
-                  "structure_attention_adjoint: workspace must be 16-byte aligned");
-    if (workspace_bytes < need)
-      return fail(Y3B_ERR_WORKSPACE, "structure_attention_adjoint: workspace of %lld bytes, %lld needed",
-                  (long long)workspace_bytes, (long long)need);
-  }
-  float* ws = static_cast<float*>(workspace);
+  const AttPlan w = make_plan(args, true);
+  rc = check_workspace(w, workspace, workspace_bytes, "structure_attention_adjoint");
+  if (rc) return rc;
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
   cudaStream_t s = as_stream(stream);
   return args->dtype == Y3B_F32
-             ? backward<float>(a, out_grad, lse, ws, query_grad, key_grad, value_grad, positions_grad,
-                               key_positions_grad, slopes_grad, s)
-             : backward<__nv_bfloat16>(a, out_grad, lse, ws, query_grad, key_grad, value_grad, positions_grad,
-                                       key_positions_grad, slopes_grad, s);
+             ? backward<float>(args, a, w, ws, out, out_grad, lse, query_grad, key_grad, value_grad, positions_grad,
+                               key_positions_grad, slopes_grad, status, s)
+             : backward<__nv_bfloat16>(args, a, w, ws, out, out_grad, lse, query_grad, key_grad, value_grad,
+                                       positions_grad, key_positions_grad, slopes_grad, status, s);
 }

@@ -1,0 +1,738 @@
+// Structure attention on the tensor cores: one kernel body for the forward and the two sides
+// of the backward.
+//
+// A CTA takes an item: up to 128 rows of one structure, a range of its columns, one head.
+//   forward    rows = queries, columns = keys     S = Q K^T            O  += P V
+//   query side rows = queries, columns = keys     S = Q K^T, T = G V^T dQ += dS K
+//   key side   rows = keys,    columns = queries  S = K Q^T, T = V G^T dV += P G, dK += dS Q
+// (G = gradient of the output.)  Per tile of BN columns: tcgen05.mma forms the score products in
+// tensor memory; thread r of the four score warps reads row r, does the softmax arithmetic in fp32 and
+// writes P or dS back to tensor memory as bf16, where it is the A operand of the accumulating product
+// (B: the same shared-memory column tile, read MN-major).  One warp issues the MMAs, two
+// warps bring the next column tile with cp.async, rows outside the item as zeros; so
+// nothing of another structure enters a product.
+//
+// What bounds it: the score warps.  A score takes one exp2 and one square root on the special-function
+// unit, 16 lanes a cycle and SM, so at most 8 scores a cycle and SM; the products of a
+// score at D = 64 take 1/32 (forward) cycle.  Positions and sums are therefore in packed fp32
+// pairs, and two or three CTAs share an SM so that one's MMAs and waits lie under another's
+// arithmetic.
+//
+// fp32 data is carried as three bf16 pieces (8 + 8 + 8 bits): six products of pieces give each
+// product to about 2^-24, and P and dS are split likewise.
+#pragma once
+
+#include <type_traits>
+
+#include "structure_attention.cuh"
+#include "tcgen05.cuh"
+
+namespace y3b {
+
+enum AttMode { kForward = 0, kQuerySide = 1, kKeySide = 2 };
+
+constexpr int kTileRows = 128;
+constexpr int kTileThreads = 224;  // 4 score warps, 1 MMA warp, 2 loading warps
+constexpr int kLoadThreads = 64;
+
+struct AttItem {
+  int row, rows, col, cols, slot, pad[3];
+};
+struct AttJoin {
+  int row, rows, first, count;
+};
+
+// A bf16 operand: element (piece, row, head, d) at piece * piece_stride + row * row_stride + head * head_stride + d.
+struct AttOperand {
+  const __nv_bfloat16* p;
+  int64_t row, head, piece;
+};
+
+struct AttTileArgs {
+  AttOperand q, k, v, g;
+  int H, Hk, D, group, chunks;  // chunks: 16-byte pieces of a row of an operand
+  const float* x;
+  const float* y;
+  const float* slopes;
+  float scale, scale2;
+  const AttItem* items;
+  const void* out_in;   // forward result, query side
+  const void* grad_in;  // gradient of it, query side
+  float* lse;           // written by the forward
+  float* delta;         // written by the query side
+  float* slope_part;    // [nq, H]
+  float* place_part;    // [nq, H, 3] or [nk, Hk, 3]
+  void* out0;           // O, dQ or dV
+  void* out1;           // dK
+  float* part;          // partial results of split items
+  int32_t* status;
+  int vec;              // 16-byte stores to out0 / out1 and loads of out_in / grad_in
+};
+
+template <int MODE, int DP, int NP>
+struct AttCfg {
+  static constexpr int BN = NP == 1 ? 64 : DP == 64 ? 32 : MODE == kForward ? 32 : 16;
+  static constexpr int ROWOPS = MODE == kForward ? 1 : 2;
+  static constexpr int PANELS = DP / 64;
+  static constexpr int STAGES = NP == 3 && DP == 128 && MODE != kForward ? 1 : 2;
+  static constexpr int ROW_PIECE = kTileRows * DP * 2;
+  static constexpr int COL_PIECE = BN * DP * 2;
+  static constexpr int COL_STAGE = 2 * NP * COL_PIECE;
+  static constexpr int EXTRA = 5 * BN;  // floats a stage: x, y, z, -lse, delta of the columns
+  static constexpr int SMEM = 1024 + ROWOPS * NP * ROW_PIECE + STAGES * (COL_STAGE + EXTRA * 4);
+  // tensor memory columns; with one piece P and dS take the place of the scores they come from
+  static constexpr int S = 0;
+  static constexpr int T = BN;
+  static constexpr int SCORES = MODE == kForward ? BN : 2 * BN;
+  static constexpr int A0 = NP == 1 ? 0 : SCORES;
+  static constexpr int A1 = NP == 1 ? BN : SCORES + NP * BN / 2;
+  static constexpr int ACC = NP == 1 ? SCORES : SCORES + (MODE == kKeySide ? 2 : 1) * NP * BN / 2;
+  // Accumulators.  OPS results (dV and dK on the key side); a second one of each for three pieces
+  // takes all products but that of the leading pieces: the tensor cores truncate when they accumulate,
+  // once a product, and the sum of the leading pieces then sees a sixth as many.  With one piece the
+  // query side also accumulates P K, to correct dQ for the rounding of delta.
+  static constexpr int OPS = MODE == kKeySide ? 2 : 1;
+  static constexpr int SMALL = NP == 3 ? OPS : 0;
+  static constexpr bool FIX = MODE == kQuerySide && NP == 1;
+  static constexpr int HALVES = MODE == kKeySide && NP == 3 && DP == 128 ? 2 : 1;  // CTAs that share a width
+  static constexpr int W = DP / HALVES;  // columns of one accumulator
+  static constexpr int NEED = ACC + (OPS + SMALL + (FIX ? 1 : 0)) * W;
+  static constexpr int COLUMNS = NEED <= 128 ? 128 : NEED <= 256 ? 256 : 512;
+  static constexpr int PER_SM_TMEM = 512 / COLUMNS;
+  static constexpr int PER_SM_SMEM = (227 * 1024) / (SMEM + 2048);
+  static constexpr int PER_SM_MIN = PER_SM_TMEM < PER_SM_SMEM ? PER_SM_TMEM : PER_SM_SMEM;
+  static constexpr int PER_SM = PER_SM_MIN > 2 ? 2 : PER_SM_MIN;
+  // floats of one row of a split item's partial result
+  static constexpr int PART = (MODE == kKeySide || FIX ? 2 : 1) * DP + 16;
+};
+
+// Two-operand piece products, smallest first.
+template <int NP> struct Pieces;
+template <> struct Pieces<1> {
+  static constexpr int N = 1;
+  __device__ static constexpr int a(int) { return 0; }
+  __device__ static constexpr int b(int) { return 0; }
+};
+template <> struct Pieces<3> {
+  static constexpr int N = 6;
+  __device__ static constexpr int a(int n) { return n == 0 ? 2 : n == 2 ? 1 : n == 3 ? 1 : 0; }
+  __device__ static constexpr int b(int n) { return n == 1 ? 2 : n == 2 ? 1 : n == 4 ? 1 : 0; }
+};
+
+// Rows [0, valid) of an operand into a tile of ROWS x DP in the 128-byte swizzle, zeros elsewhere.
+template <int ROWS, int DP, int NP>
+__device__ __forceinline__ void load_tile(uint32_t dst, const AttOperand& o, int64_t row0, int head, int valid,
+                                          int chunks, int t, int threads) {
+  constexpr int CH = DP / 8;
+  const __nv_bfloat16* base = o.p + row0 * o.row + head * o.head;
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    for (int u = t; u < ROWS * CH; u += threads) {
+      const int r = u / CH, c = u % CH;
+      const uint32_t at = dst + p * (ROWS * DP * 2) + (c >> 3) * (ROWS * 128) + (r >> 3) * 1024 + (r & 7) * 128 +
+                          (((c & 7) ^ (r & 7)) << 4);
+      const bool there = r < valid && c < chunks;
+      const __nv_bfloat16* src = there ? base + p * o.piece + int64_t(r) * o.row + c * 8 : o.p;
+      tc::cp16(at, src, there);
+    }
+  }
+}
+
+// Values (2k, 2k + 1) as NP packed bf16 pieces.
+template <int NP>
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t (&r)[NP]) {
+  r[0] = tc::bf16x2(a, b);
+  if constexpr (NP == 3) {
+    float ra = a - __uint_as_float(r[0] << 16), rb = b - __uint_as_float(r[0] & 0xffff0000u);
+    r[1] = tc::bf16x2(ra, rb);
+    ra -= __uint_as_float(r[1] << 16);
+    rb -= __uint_as_float(r[1] & 0xffff0000u);
+    r[2] = tc::bf16x2(ra, rb);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_row16(T* dst, const float* v, int d0, int D, bool vec) {
+  if (vec && d0 + 16 <= D) {
+    if constexpr (sizeof(T) == 2) {
+      uint32_t r[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) r[k] = tc::bf16x2(v[2 * k], v[2 * k + 1]);
+      reinterpret_cast<uint4*>(dst + d0)[0] = make_uint4(r[0], r[1], r[2], r[3]);
+      reinterpret_cast<uint4*>(dst + d0)[1] = make_uint4(r[4], r[5], r[6], r[7]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        reinterpret_cast<float4*>(dst + d0)[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      if (d0 + k < D) dst[d0 + k] = from_float<T>(v[k]);
+  }
+}
+
+// Distances of a pair of columns and their reciprocals from the squares.  The squares come with a
+// tiny term, so that 1/d stays finite and (x - y) / d is zero at distance zero.  Every mode forms its
+// scores by the same operations: the backward then sees the forward's scores bit for bit.
+struct Distance {
+  tc::f2 d, r;
+};
+__device__ __forceinline__ Distance distance(tc::f2 squares) {
+  float u0, u1;
+  tc::unpack(squares, u0, u1);
+  Distance x;
+  x.r = tc::pack(tc::rsqrt_approx(u0), tc::rsqrt_approx(u1));
+  x.d = tc::mul2(squares, x.r);
+  return x;
+}
+
+template <int MODE, int DP, int NP, bool BIAS>
+__global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) attention_tile_kernel(
+    const __grid_constant__ AttTileArgs a) {
+  using C = AttCfg<MODE, DP, NP>;
+  using T = typename std::conditional<NP == 1, __nv_bfloat16, float>::type;
+  constexpr int BN = C::BN;
+  extern __shared__ __align__(1024) unsigned char tile_smem[];
+  __shared__ __align__(8) uint64_t bars[2 * C::STAGES + 3];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int heads = MODE == kKeySide ? a.Hk : a.H;
+  const int half = C::HALVES == 1 ? 0 : int(blockIdx.x % C::HALVES);
+  const unsigned task = blockIdx.x / C::HALVES;
+  const int head = int(task % unsigned(heads));
+  const AttItem item = a.items[task / unsigned(heads)];
+  const int d_first = half * C::W;                                            // accumulated components: d_first ..
+  const int d_count = C::HALVES == 1 ? a.D : min(a.D - d_first, int(C::W));   // .. d_first + d_count (D > 64 with halves)
+  const int acc_n = (d_count + 15) / 16 * 16;
+  const int ntiles = (item.cols + BN - 1) / BN;
+  const int total = MODE == kKeySide ? ntiles * a.group : ntiles;
+
+  const uint32_t smem = (tc::smem_addr(tile_smem) + 1023u) & ~1023u;
+  const uint32_t row0 = smem, row1 = smem + NP * C::ROW_PIECE;
+  const uint32_t cols = smem + C::ROWOPS * NP * C::ROW_PIECE;
+  float* extra = reinterpret_cast<float*>(tile_smem + (smem - tc::smem_addr(tile_smem)) + C::ROWOPS * NP * C::ROW_PIECE +
+                                          C::STAGES * C::COL_STAGE);
+  const uint32_t bar0 = tc::smem_addr(bars);
+  const auto full = [&](int s) { return bar0 + 8 * s; };
+  const auto empty = [&](int s) { return bar0 + 8 * (C::STAGES + s); };
+  const uint32_t s_ready = bar0 + 8 * (2 * C::STAGES), p_ready = s_ready + 8, drain = s_ready + 16;
+
+  if (warp == 4) tc::alloc(tc::smem_addr(&s_tmem), C::COLUMNS);
+  if (tid == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      tc::mbar_init(full(s), kLoadThreads);
+      tc::mbar_init(empty(s), 1);
+    }
+    tc::mbar_init(s_ready, 1);
+    tc::mbar_init(p_ready, 4);
+    tc::mbar_init(drain, 1);
+    tc::mbar_init_fence();
+    s_abort = 0;
+  }
+  // row operands, by all threads
+  {
+    const AttOperand& r0 = MODE == kKeySide ? a.k : a.q;
+    load_tile<kTileRows, DP, NP>(row0, r0, item.row, head, item.rows, a.chunks, tid, kTileThreads);
+    if constexpr (MODE != kForward) {
+      const AttOperand& r1 = MODE == kKeySide ? a.v : a.g;
+      load_tile<kTileRows, DP, NP>(row1, r1, item.row, head, item.rows, a.chunks, tid, kTileThreads);
+    }
+    tc::cp_commit();
+    tc::cp_wait<0>();
+    tc::fence_async_smem();
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = s_tmem;
+
+  if (warp >= 5) {
+    // ---- loading warps: column tile t into stage t % STAGES, one tile ahead of its arrival
+    const int t = tid - 160;
+    bool ok = true;
+    for (int j = 0; j < total && ok; ++j) {
+      const int s = j % C::STAGES;
+      if (j >= C::STAGES) ok = tc::mbar_wait(empty(s), ((j / C::STAGES) - 1) & 1);
+      if (!ok) break;
+      const int sub = MODE == kKeySide ? j / ntiles : 0, jt = MODE == kKeySide ? j - sub * ntiles : j;
+      const int c0 = jt * BN, n = item.cols - c0 < BN ? item.cols - c0 : BN;
+      const int64_t col = int64_t(item.col) + c0;
+      const uint32_t dst = cols + s * C::COL_STAGE;
+      const int ch = MODE == kKeySide ? head * a.group + sub : head / a.group;
+      load_tile<BN, DP, NP>(dst, MODE == kKeySide ? a.q : a.k, col, ch, n, a.chunks, t, kLoadThreads);
+      load_tile<BN, DP, NP>(dst + NP * C::COL_PIECE, MODE == kKeySide ? a.g : a.v, col, ch, n, a.chunks, t,
+                            kLoadThreads);
+      const uint32_t ex = tc::smem_addr(extra + s * C::EXTRA);
+      if constexpr (BIAS) {
+        const float* pos = MODE == kKeySide ? a.x : a.y;
+        for (int u = t; u < 3 * BN; u += kLoadThreads) {
+          const int r = u / 3, c = u - 3 * r;
+          tc::cp4(ex + (c * BN + r) * 4, r < n ? pos + 3 * (col + r) + c : pos, r < n);
+        }
+      }
+      if constexpr (MODE == kKeySide) {
+        for (int u = t; u < 2 * BN; u += kLoadThreads) {
+          const int r = u >> 1, c = u & 1;
+          const float* src = c ? a.delta : a.lse;
+          tc::cp4(ex + ((3 + c) * BN + r) * 4, r < n ? src + (col + r) * a.H + ch : src, r < n);
+        }
+      }
+      tc::cp_commit();
+      if constexpr (C::STAGES == 1) {
+        tc::cp_wait<0>();
+        tc::fence_async_smem();
+        tc::mbar_arrive(full(s));
+      } else if (j > 0) {
+        tc::cp_wait<1>();
+        tc::fence_async_smem();
+        tc::mbar_arrive(full((j - 1) % C::STAGES));
+      }
+    }
+    tc::cp_wait<0>();
+    if constexpr (C::STAGES > 1) {
+      if (ok && total > 0) {
+        tc::fence_async_smem();
+        tc::mbar_arrive(full((total - 1) % C::STAGES));
+      }
+    }
+    if (!ok) s_abort = 1;
+  } else if (warp == 4) {
+    // ---- MMA issue: scores of tile j, then (when P is back) its accumulating product
+    if (lane == 0) {
+      const int ksteps = (a.D + 15) / 16;
+      const uint32_t id_s = tc::idesc_bf16(kTileRows, BN, false), id_a = tc::idesc_bf16(kTileRows, acc_n, true);
+      bool ok = true;
+      for (int j = 0; j < total; ++j) {
+        const int s = j % C::STAGES;
+        ok = tc::mbar_wait(full(s), (j / C::STAGES) & 1);
+        if (!ok) break;
+        tc::fence_after();
+        const uint32_t c0 = cols + s * C::COL_STAGE, c1 = c0 + NP * C::COL_PIECE;
+#pragma unroll
+        for (int op = 0; op < C::ROWOPS; ++op) {
+          const uint32_t ra = op ? row1 : row0, cb = op ? c1 : c0, d = tmem + (op ? C::T : C::S);
+#pragma unroll
+          for (int n = 0; n < Pieces<NP>::N; ++n) {
+            for (int ks = 0; ks < ksteps; ++ks) {
+              const uint32_t off = (ks & 3) * 32;
+              tc::mma_ss(d,
+                         tc::desc_sw128(ra + Pieces<NP>::a(n) * C::ROW_PIECE + (ks >> 2) * (kTileRows * 128) + off, 16,
+                                        1024),
+                         tc::desc_sw128(cb + Pieces<NP>::b(n) * C::COL_PIECE + (ks >> 2) * (BN * 128) + off, 16, 1024),
+                         id_s, n > 0 || ks > 0);
+            }
+          }
+        }
+        tc::commit(s_ready);
+        ok = tc::mbar_wait(p_ready, j & 1);
+        if (!ok) break;
+        tc::fence_after();
+        // forward: P x V; query side: dS x K (and P x K); key side: P x G and dS x Q
+#pragma unroll
+        for (int op = 0; op < C::OPS + (C::FIX ? 1 : 0); ++op) {
+          const uint32_t A = tmem + (op == 0 ? C::A0 : C::A1);
+          const uint32_t cb = (MODE == kForward || (MODE == kKeySide && op == 0) ? c1 : c0) + half * (BN * 128);
+#pragma unroll
+          for (int n = 0; n < Pieces<NP>::N; ++n) {
+            const bool small = NP == 3 && n < Pieces<NP>::N - 1;
+            const uint32_t d = tmem + C::ACC + (op + (small ? C::OPS : 0)) * C::W;
+#pragma unroll
+            for (int ks = 0; ks < BN / 16; ++ks)
+              tc::mma_ts(d, A + Pieces<NP>::a(n) * (BN / 2) + ks * 8,
+                         tc::desc_sw128(cb + Pieces<NP>::b(n) * C::COL_PIECE + ks * 2048, BN * 128, 1024), id_a,
+                         j > 0 || ks > 0 || (small && n > 0));
+          }
+        }
+        tc::commit(empty(s));
+      }
+      if (!ok) {
+        s_abort = 1;
+        tc::commit(drain);
+        tc::mbar_wait(drain, 0);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- score warps: thread = row
+    const bool valid = tid < item.rows;
+    const int64_t row = int64_t(item.row) + (valid ? tid : 0);
+    const uint32_t lane_base = tmem + (uint32_t(32 * warp) << 16);
+    float px = 0.0f, py = 0.0f, pz = 0.0f, slope = 0.0f;
+    if constexpr (BIAS) {
+      const float* pos = (MODE == kKeySide ? a.y : a.x) + 3 * row;
+      px = pos[0];
+      py = pos[1];
+      pz = pos[2];
+      slope = MODE == kKeySide ? 0.0f : a.slopes[head];
+    }
+    const tc::f2 px2 = tc::pack(px, px), py2 = tc::pack(py, py), pz2 = tc::pack(pz, pz);
+    const tc::f2 scale2 = tc::pack(a.scale2, a.scale2), tiny2 = tc::pack(1e-30f, 1e-30f);
+    tc::f2 nslope2 = tc::pack(-slope * kLog2e, -slope * kLog2e);
+    bool ok = true;
+
+    // state of the forward: reference maximum and sum; of the query side: the ten sums
+    float m = -INFINITY, l = 0.0f;
+    float nL = 0.0f, delta0 = 0.0f;
+    float sum[10];
+#pragma unroll
+    for (int k = 0; k < 10; ++k) sum[k] = 0.0f;
+    if constexpr (MODE == kQuerySide) {
+      if (valid) {
+        nL = -a.lse[row * a.H + head];
+        const T* o = static_cast<const T*>(a.out_in) + (row * a.H + head) * a.D;
+        const T* g = static_cast<const T*>(a.grad_in) + (row * a.H + head) * a.D;
+        constexpr int W = 16 / int(sizeof(T));
+        int d = 0;
+        if (a.vec) {
+          for (; d + W <= a.D; d += W) {
+            const uint4 ou = *reinterpret_cast<const uint4*>(o + d), gu = *reinterpret_cast<const uint4*>(g + d);
+            const T* ov = reinterpret_cast<const T*>(&ou);
+            const T* gv = reinterpret_cast<const T*>(&gu);
+#pragma unroll
+            for (int k = 0; k < W; ++k) delta0 = fmaf(to_float(ov[k]), to_float(gv[k]), delta0);
+          }
+        }
+        for (; d < a.D; ++d) delta0 = fmaf(to_float(o[d]), to_float(g[d]), delta0);
+      }
+    }
+    const tc::f2 nL2 = tc::pack(nL, nL), delta02 = tc::pack(delta0, delta0);
+
+    for (int j = 0; j < total; ++j) {
+      const int s = j % C::STAGES;
+      const int sub = MODE == kKeySide ? j / ntiles : 0, jt = MODE == kKeySide ? j - sub * ntiles : j;
+      const int n = item.cols - jt * BN;  // columns there are, BN or more in a full tile
+      ok = tc::mbar_wait(full(s), (j / C::STAGES) & 1) && tc::mbar_wait(s_ready, j & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc::fence_after();
+      const float* ex = extra + s * C::EXTRA;
+      if (32 * warp >= item.rows) {
+        // no row of the item in this warp: its lanes of P stay as they are and reach no result
+      } else if constexpr (MODE == kForward) {
+        float v[BN];
+#pragma unroll
+        for (int c = 0; c < BN; c += 16) tc::ld16(lane_base + C::S + c, v + c);
+        tc::wait_ld();
+        float top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < BN; c += 4) {
+          tc::f2 s0 = tc::mul2(tc::pack(v[c], v[c + 1]), scale2), s1 = tc::mul2(tc::pack(v[c + 2], v[c + 3]), scale2);
+          if constexpr (BIAS) {
+            const ulonglong2 xx = *reinterpret_cast<const ulonglong2*>(ex + c);
+            const ulonglong2 yy = *reinterpret_cast<const ulonglong2*>(ex + BN + c);
+            const ulonglong2 zz = *reinterpret_cast<const ulonglong2*>(ex + 2 * BN + c);
+            const tc::f2 dx0 = tc::sub2(px2, xx.x), dx1 = tc::sub2(px2, xx.y);
+            const tc::f2 dy0 = tc::sub2(py2, yy.x), dy1 = tc::sub2(py2, yy.y);
+            const tc::f2 dz0 = tc::sub2(pz2, zz.x), dz1 = tc::sub2(pz2, zz.y);
+            s0 = tc::fma2(distance(tc::fma2(dz0, dz0, tc::fma2(dy0, dy0, tc::fma2(dx0, dx0, tiny2)))).d, nslope2, s0);
+            s1 = tc::fma2(distance(tc::fma2(dz1, dz1, tc::fma2(dy1, dy1, tc::fma2(dx1, dx1, tiny2)))).d, nslope2, s1);
+          }
+          tc::unpack(s0, v[c], v[c + 1]);
+          tc::unpack(s1, v[c + 2], v[c + 3]);
+        }
+        if (n < BN) {
+#pragma unroll
+          for (int c = 0; c < BN; ++c)
+            if (c >= n) v[c] = -INFINITY;
+        }
+#pragma unroll
+        for (int c = 0; c < BN; ++c) top = fmaxf(top, v[c]);
+        // the reference maximum moves only when a row would pass 2^8 times it: P stays within 2^8
+        // and the accumulated rows are rescaled seldom
+        if (j == 0) {
+          m = top;
+        } else {
+          const bool move = top > m + 8.0f || (m == -INFINITY && top > m);
+          if (__any_sync(0xffffffffu, move)) {
+            const float f = move ? tc::ex2(m - top) : 1.0f;
+            if (move) m = top;
+            l *= f;
+            ok = tc::mbar_wait(empty((j - 1) % C::STAGES), ((j - 1) / C::STAGES) & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc::fence_after();
+#pragma unroll
+            for (int u = 0; u < C::OPS + C::SMALL; ++u) {
+              for (int d = 0; d < acc_n; d += 16) {
+                float o[16];
+                tc::ld16(lane_base + C::ACC + u * C::W + d, o);
+                tc::wait_ld();
+                uint32_t r[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(o[k] * f);
+                tc::st16(lane_base + C::ACC + u * C::W + d, r);
+              }
+            }
+            tc::wait_st();
+          }
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+        const tc::f2 nref = tc::pack(-ref, -ref);
+        tc::f2 l0 = tc::pack(0.0f, 0.0f), l1 = l0;
+#pragma unroll
+        for (int c0 = 0; c0 < BN; c0 += 16) {
+          uint32_t pr[NP][8];
+#pragma unroll
+          for (int c = 0; c < 16; c += 2) {
+            float e0, e1;
+            tc::unpack(tc::add2(tc::pack(v[c0 + c], v[c0 + c + 1]), nref), e0, e1);
+            e0 = tc::ex2(e0);
+            e1 = tc::ex2(e1);
+            if (c & 2) l1 = tc::add2(l1, tc::pack(e0, e1));
+            else l0 = tc::add2(l0, tc::pack(e0, e1));
+            uint32_t r[NP];
+            split_pair<NP>(e0, e1, r);
+#pragma unroll
+            for (int p = 0; p < NP; ++p) pr[p][c / 2] = r[p];
+          }
+#pragma unroll
+          for (int p = 0; p < NP; ++p) tc::st8(lane_base + C::A0 + p * (BN / 2) + c0 / 2, pr[p]);
+        }
+        float s0, s1;
+        tc::unpack(tc::add2(l0, l1), s0, s1);
+        l += s0 + s1;
+      } else {
+        if constexpr (MODE == kKeySide) {
+          if constexpr (BIAS) {
+            slope = a.slopes[head * a.group + sub];
+            nslope2 = tc::pack(-slope * kLog2e, -slope * kLog2e);
+          }
+        }
+        const tc::f2 zero2 = tc::pack(0.0f, 0.0f);
+        tc::f2 acc[10];
+#pragma unroll
+        for (int k = 0; k < 10; ++k) acc[k] = zero2;
+#pragma unroll
+        for (int c0 = 0; c0 < BN; c0 += 16) {
+          float sv[16], tv[16];
+          tc::ld16(lane_base + C::S + c0, sv);
+          tc::ld16(lane_base + C::T + c0, tv);
+          tc::wait_ld();
+          uint32_t pr[NP][8], dr[NP][8];
+#pragma unroll
+          for (int c = 0; c < 16; c += 2) {
+            const int cc = c0 + c;
+            tc::f2 e, dx, dy, dz, d, r, score = tc::mul2(tc::pack(sv[c], sv[c + 1]), scale2);
+            if constexpr (MODE == kQuerySide) e = nL2;
+            else e = *reinterpret_cast<const tc::f2*>(ex + 3 * BN + cc) ^ 0x8000000080000000ull;  // -lse
+            if constexpr (BIAS) {
+              dx = tc::sub2(px2, *reinterpret_cast<const tc::f2*>(ex + cc));
+              dy = tc::sub2(py2, *reinterpret_cast<const tc::f2*>(ex + BN + cc));
+              dz = tc::sub2(pz2, *reinterpret_cast<const tc::f2*>(ex + 2 * BN + cc));
+              const Distance x = distance(tc::fma2(dz, dz, tc::fma2(dy, dy, tc::fma2(dx, dx, tiny2))));
+              d = x.d;
+              r = x.r;
+              score = tc::fma2(d, nslope2, score);
+            }
+            e = tc::add2(score, e);
+            float p0, p1;
+            tc::unpack(e, p0, p1);
+            p0 = tc::ex2(p0);
+            p1 = tc::ex2(p1);
+            if (n < BN) {
+              if (cc >= n) p0 = 0.0f;
+              if (cc + 1 >= n) p1 = 0.0f;
+            }
+            const tc::f2 p = tc::pack(p0, p1), tt = tc::pack(tv[c], tv[c + 1]);
+            float g0, g1;
+            if constexpr (MODE == kQuerySide) {
+              const tc::f2 pt = tc::mul2(p, tt);
+              tc::unpack(tc::mul2(p, tc::sub2(tt, delta02)), g0, g1);
+              acc[0] = tc::add2(acc[0], pt);
+              acc[9] = tc::add2(acc[9], p);
+              if constexpr (BIAS) {
+                acc[1] = tc::fma2(d, pt, acc[1]);
+                acc[2] = tc::fma2(d, p, acc[2]);
+                const tc::f2 u = tc::mul2(pt, r), w = tc::mul2(p, r);
+                acc[3] = tc::fma2(u, dx, acc[3]);
+                acc[4] = tc::fma2(u, dy, acc[4]);
+                acc[5] = tc::fma2(u, dz, acc[5]);
+                acc[6] = tc::fma2(w, dx, acc[6]);
+                acc[7] = tc::fma2(w, dy, acc[7]);
+                acc[8] = tc::fma2(w, dz, acc[8]);
+              }
+            } else {
+              const tc::f2 ds = tc::mul2(p, tc::sub2(tt, *reinterpret_cast<const tc::f2*>(ex + 4 * BN + cc)));
+              tc::unpack(ds, g0, g1);
+              if constexpr (BIAS) {
+                const tc::f2 u = tc::mul2(ds, r);
+                acc[0] = tc::fma2(u, dx, acc[0]);
+                acc[1] = tc::fma2(u, dy, acc[1]);
+                acc[2] = tc::fma2(u, dz, acc[2]);
+              }
+            }
+            if constexpr (MODE == kKeySide || C::FIX) {
+              uint32_t q[NP];
+              split_pair<NP>(p0, p1, q);
+#pragma unroll
+              for (int k = 0; k < NP; ++k) pr[k][c / 2] = q[k];
+            }
+            uint32_t q[NP];
+            split_pair<NP>(g0, g1, q);
+#pragma unroll
+            for (int k = 0; k < NP; ++k) dr[k][c / 2] = q[k];
+          }
+          // with one piece, columns c0/2 .. c0/2 + 8 hold scores that are already in registers
+#pragma unroll
+          for (int k = 0; k < NP; ++k) {
+            // key side: P first, then dS; query side: dS first
+            tc::st8(lane_base + (MODE == kKeySide ? C::A1 : C::A0) + k * (BN / 2) + c0 / 2, dr[k]);
+            if constexpr (MODE == kKeySide || C::FIX)
+              tc::st8(lane_base + (MODE == kKeySide ? C::A0 : C::A1) + k * (BN / 2) + c0 / 2, pr[k]);
+          }
+        }
+        // tile sums into the row's sums: two levels keep the rounding of long rows small
+#pragma unroll
+        for (int k = 0; k < 10; ++k) {
+          float s0, s1;
+          tc::unpack(acc[k], s0, s1);
+          if constexpr (MODE == kQuerySide) sum[k] += s0 + s1;
+          else if (k < 3) sum[k] = fmaf(slope, s0 + s1, sum[k]);
+        }
+      }
+      tc::wait_st();
+      tc::fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(p_ready);
+    }
+
+    // ---- results
+    if (ok && total > 0) {
+      ok = tc::mbar_wait(empty((total - 1) % C::STAGES), ((total - 1) / C::STAGES) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+    }
+    if (ok) {
+      tc::fence_after();
+      const bool split = item.slot >= 0;
+      const int64_t at = row * heads + head;
+      float* part = split ? a.part + ((int64_t(item.slot) * heads + head) * kTileRows + tid) * C::PART : nullptr;
+      float f0 = 1.0f;
+      bool none = total == 0;
+      if constexpr (MODE == kForward) {
+        none = none || (m == -INFINITY && l == 0.0f);
+        f0 = split ? 1.0f : none ? 0.0f : 1.0f / l;
+      } else if constexpr (MODE == kQuerySide) {
+        f0 = split ? 1.0f : a.scale;
+      }
+      // query side: the sum of P is 1 up to the rounding of lse; dividing by it takes that out of delta
+      float inv = 0.0f, dl = 0.0f;
+      if constexpr (MODE == kQuerySide) {
+        inv = none ? 0.0f : 1.0f / sum[9];
+        dl = sum[0] * inv;
+      }
+#pragma unroll
+      for (int op = 0; op < C::OPS; ++op) {
+        const float f = MODE == kKeySide && op == 1 && !split ? a.scale : f0;
+        T* dst = static_cast<T*>(op ? a.out1 : a.out0) + at * a.D;
+        for (int d = 0; d < acc_n; d += 16) {
+          float o[16];
+          tc::ld16(lane_base + C::ACC + op * C::W + d, o);
+          if constexpr (C::SMALL > 0 || C::FIX) {
+            float e[16];
+            tc::ld16(lane_base + C::ACC + (C::OPS + op) * C::W + d, e);
+            tc::wait_ld();
+            const float fe = !C::FIX ? 1.0f : split ? 0.0f : delta0 - dl;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              if constexpr (C::FIX) {
+                if (split && valid) part[DP + 16 + d + k] = none ? 0.0f : e[k];
+              }
+              o[k] = fmaf(fe, e[k], o[k]);
+            }
+          } else {
+            tc::wait_ld();
+          }
+          if (valid) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) o[k] = none ? 0.0f : o[k] * f;
+            if (split) {
+#pragma unroll
+              for (int k = 0; k < 16; k += 4)
+                *reinterpret_cast<float4*>(part + op * DP + d_first + d + k) =
+                    make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+            } else {
+              store_row16<T>(dst, o, d_first + d, a.D, a.vec != 0);
+            }
+          }
+        }
+      }
+      if (valid) {
+        if constexpr (MODE == kForward) {
+          if (split) {
+            part[DP] = none ? -INFINITY : m;
+            part[DP + 1] = l;
+          } else {
+            a.lse[at] = none ? INFINITY : m + log2f(l);
+          }
+        } else if constexpr (MODE == kQuerySide) {
+          if (split) {
+#pragma unroll
+            for (int k = 0; k < 10; ++k) part[DP + k] = sum[k];
+            part[DP + 10] = delta0;
+          } else {
+            a.delta[at] = dl;
+            if constexpr (BIAS) {
+              a.slope_part[at] = -inv * (sum[1] - dl * sum[2]);
+#pragma unroll
+              for (int k = 0; k < 3; ++k) a.place_part[at * 3 + k] = -slope * inv * (sum[3 + k] - dl * sum[6 + k]);
+            }
+          }
+        } else if (BIAS && half == 0) {
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            if (split) part[2 * DP + k] = sum[k];
+            else a.place_part[at * 3 + k] = -sum[k];
+          }
+        }
+      }
+    } else {
+      s_abort = 1;
+    }
+  }
+  tc::fence_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc::fence_after();
+    tc::dealloc(tmem, C::COLUMNS);
+  }
+  if (tid == 0 && s_abort && a.status) atomicOr(a.status, Y3B_STATUS_TIMEOUT);
+}
+
+template <int MODE, int DP, int NP, bool BIAS>
+int launch_attention_tile(const AttTileArgs& a, int64_t items, cudaStream_t s) {
+  using C = AttCfg<MODE, DP, NP>;
+  const auto kernel = attention_tile_kernel<MODE, DP, NP, BIAS>;
+  Y3B_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+  const int64_t grid = items * (MODE == kKeySide ? a.Hk : a.H) * C::HALVES;
+  if (grid > INT32_MAX) return fail(Y3B_ERR_UNSUPPORTED, "structure_attention: %lld tiles", (long long)grid);
+  kernel<<<unsigned(grid), kTileThreads, C::SMEM, s>>>(a);
+  Y3B_LAUNCH_CHECK();
+  return Y3B_OK;
+}
+
+template <int MODE>
+int dispatch_attention_tile(int pieces, const AttTileArgs& a, int64_t items, cudaStream_t s) {
+  if (items == 0) return Y3B_OK;
+  const bool bias = a.slopes != nullptr, wide = a.D > 64;
+#define Y3B_TILE(DP, NP)                                                       \
+  return bias ? launch_attention_tile<MODE, DP, NP, true>(a, items, s)         \
+              : launch_attention_tile<MODE, DP, NP, false>(a, items, s)
+  if (pieces == 1) {
+    if (wide) { Y3B_TILE(128, 1); }
+    Y3B_TILE(64, 1);
+  }
+  if (wide) { Y3B_TILE(128, 3); }
+  Y3B_TILE(64, 3);
+#undef Y3B_TILE
+}
+
+// One mode a translation unit.
+int attention_forward_tiles(int pieces, const AttTileArgs& a, int64_t items, cudaStream_t s);
+int attention_query_tiles(int pieces, const AttTileArgs& a, int64_t items, cudaStream_t s);
+int attention_key_tiles(int pieces, const AttTileArgs& a, int64_t items, cudaStream_t s);
+
+}  // namespace y3b
+

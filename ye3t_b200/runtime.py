@@ -616,6 +616,43 @@ def _host_counts(counts, what):
     return c
 
 
+_TILE = 128       # rows of a tile
+_TILE_ROWS = 1    # structures with fewer rows are computed row by row
+
+
+def _work_tables(row_first, row_count, col_first, col_count, heads, tiled):
+    """Items, joins and single rows of one side (the layout of include/ye3t_b200.h)."""
+    r0, rn, c0, cn = row_first[tiled], row_count[tiled], col_first[tiled], col_count[tiled]
+    tiles = -(-rn // _TILE)
+    # columns are split so that every SM gets several CTAs
+    work = int((tiles * np.maximum(cn, 1)).sum()) * heads
+    chunk = max(512, -(-work // (148 * 16)))
+    parts = np.maximum(1, np.round(cn / chunk).astype(np.int64))
+    of = np.repeat(np.arange(rn.size), tiles)  # the structure of each tile
+    t = np.arange(of.size) - np.repeat(np.cumsum(tiles) - tiles, tiles)
+    row = r0[of] + t * _TILE
+    rows = np.minimum(rn[of] - t * _TILE, _TILE)
+    p = parts[of]
+    slot = np.where(p > 1, np.cumsum(np.where(p > 1, p, 0)) - p, -1)
+    ti = np.repeat(np.arange(of.size), p)
+    k = np.arange(ti.size) - np.repeat(np.cumsum(p) - p, p)
+    # parts begin at multiples of 64 columns
+    step = -(-(-(-cn[of] // p)) // 64) * 64
+    begin = np.minimum(k * step[ti], cn[of][ti])
+    end = np.minimum(begin + step[ti], cn[of][ti])
+    items = np.zeros((ti.size, 8), np.int64)
+    items[:, 0], items[:, 1], items[:, 2], items[:, 3] = row[ti], rows[ti], c0[of][ti] + begin, end - begin
+    items[:, 4] = np.where(slot[ti] >= 0, slot[ti] + k, -1)
+    items = items[np.argsort(-items[:, 3], kind="stable")]
+    split = p > 1
+    joins = np.stack([row, rows, slot, p], 1)[split]
+    single = np.flatnonzero(~tiled)
+    rest = np.repeat(row_first[single] - (np.cumsum(row_count[single]) - row_count[single]), row_count[single])
+    rest = rest + np.arange(rest.size)
+    return {"items": items, "joins": joins, "rows": rest, "item_count": len(items), "join_count": len(joins),
+            "slot_count": int(p[split].sum()), "row_count": rest.size}
+
+
 class StructureLayout:
     """Which rows of a packed batch belong to which structure, for :func:`structure_attention`.
 
@@ -643,14 +680,24 @@ class StructureLayout:
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
         number = np.arange(self.structure_count)
-        tables = [np.concatenate([[0], np.cumsum(queries)]), np.concatenate([[0], np.cumsum(keys)]),
+        q_first, k_first = np.cumsum(queries) - queries, np.cumsum(keys) - keys
+        # a single key has all the weight and no gradient through the softmax: the row kernels give exactly that
+        q_side = _work_tables(q_first, queries, k_first, keys, self.heads, (queries >= _TILE_ROWS) & (keys > 1))
+        k_side = _work_tables(k_first, keys, q_first, queries, self.key_heads, (keys >= _TILE_ROWS) & (keys > 1))
+        self._counts = tuple(int(side[name]) for side in (q_side, k_side) for name in
+                             ("item_count", "join_count", "slot_count", "row_count"))
+        # items and joins first: they are read as 32- and 16-byte records
+        tables = [q_side["items"], k_side["items"], q_side["joins"], k_side["joins"], q_side["rows"], k_side["rows"],
+                  np.concatenate([[0], np.cumsum(queries)]), np.concatenate([[0], np.cumsum(keys)]),
                   np.repeat(number, queries), np.repeat(number, keys)]
         # one copy to the device; it is complete when the constructor returns, so any stream may use it
-        packed = torch.as_tensor(np.concatenate(tables).astype(np.int32)).to(self.device)
+        packed = torch.as_tensor(np.concatenate([t.reshape(-1) for t in tables]).astype(np.int32)).to(self.device)
         self._stream = nat.stream_of(self.device)
         self._packed = packed
-        (self._query_offsets, self._key_offsets, self._query_structure, self._key_structure) = packed.split(
-            [t.size for t in tables])
+        first = np.cumsum([0] + [t.size for t in tables[:-1]]) * 4
+        (self._query_items, self._key_items, self._query_joins, self._key_joins, self._query_rows, self._key_rows,
+         self._query_offsets, self._key_offsets, self._query_structure, self._key_structure) = [
+            packed.data_ptr() + int(o) for o in first]
 
     def _use(self):
         """Keeps the tables' memory from reuse before the current stream is done with it."""
@@ -668,8 +715,12 @@ def _attention_args(query, key, value, x, y, slopes, layout, scale):
     a.key_row_stride, a.key_head_stride = key.stride(0), key.stride(1)
     a.value_row_stride, a.value_head_stride = value.stride(0), value.stride(1)
     a.positions, a.key_positions, a.slopes = nat.ptr(x), nat.ptr(y), nat.ptr(slopes)
-    a.query_offsets, a.key_offsets = layout._query_offsets.data_ptr(), layout._key_offsets.data_ptr()
-    a.query_structure, a.key_structure = layout._query_structure.data_ptr(), layout._key_structure.data_ptr()
+    a.query_offsets, a.key_offsets = layout._query_offsets, layout._key_offsets
+    a.query_structure, a.key_structure = layout._query_structure, layout._key_structure
+    (a.query_item_count, a.query_join_count, a.query_slot_count, a.query_row_count,
+     a.key_item_count, a.key_join_count, a.key_slot_count, a.key_row_count) = layout._counts
+    a.query_items, a.query_joins, a.query_rows = layout._query_items, layout._query_joins, layout._query_rows
+    a.key_items, a.key_joins, a.key_rows = layout._key_items, layout._key_joins, layout._key_rows
     a.scale = scale
     layout._use()
     return a
@@ -680,32 +731,44 @@ def _dense_rows(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _attention_forward(query, key, value, x, y, slopes, layout, scale):
+def _attention_workspace(args, adjoint, device):
+    need = int(nat.lib().y3b_structure_attention_workspace_bytes(ctypes.byref(args), adjoint))
+    if need < 0:
+        raise nat.NativeError("structure_attention: " + nat.lib().y3b_last_error().decode(errors="replace"))
+    return torch.empty(max(need, 1), dtype=torch.uint8, device=device), need
+
+
+def _attention_forward(query, key, value, x, y, slopes, layout, scale, validate):
     q, k, v = _dense_rows(query), _dense_rows(key), _dense_rows(value)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
     args = _attention_args(q, k, v, x, y, slopes, layout, scale)
-    nat.check(nat.lib().y3b_structure_attention(ctypes.byref(args), out.data_ptr(), lse.data_ptr(),
-                                                nat.stream_of(q.device)), "structure_attention")
+    ws, ws_bytes = _attention_workspace(args, 0, q.device)
+    status = _status(q.device) if validate else None
+    nat.check(nat.lib().y3b_structure_attention(ctypes.byref(args), ws.data_ptr(), ws_bytes, out.data_ptr(),
+                                                lse.data_ptr(), nat.ptr(status), nat.stream_of(q.device)),
+              "structure_attention")
+    if validate:
+        _raise_on_status(status, "structure_attention")
     return out, lse
 
 
 class _StructureAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, query, key, value, x, y, slopes, layout, scale):
+    def forward(ctx, query, key, value, x, y, slopes, layout, scale, validate):
         same = y is None
         x = None if x is None else x.contiguous()
         y = x if same else y.contiguous()
         slopes = None if slopes is None else slopes.contiguous()
-        out, lse = _attention_forward(query, key, value, x, y, slopes, layout, scale)
-        ctx.save_for_backward(query, key, value, x, y, slopes, lse)
-        ctx.layout, ctx.scale, ctx.same = layout, scale, same
+        out, lse = _attention_forward(query, key, value, x, y, slopes, layout, scale, validate)
+        ctx.save_for_backward(query, key, value, x, y, slopes, out, lse)
+        ctx.layout, ctx.scale, ctx.same, ctx.validate = layout, scale, same, validate
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        query, key, value, x, y, slopes, lse = ctx.saved_tensors
+        query, key, value, x, y, slopes, out, lse = ctx.saved_tensors
         layout, dev = ctx.layout, query.device
         q, k, v, g = _dense_rows(query), _dense_rows(key), _dense_rows(value), grad.contiguous()
         dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
@@ -715,16 +778,16 @@ class _StructureAttention(torch.autograd.Function):
         if slopes is not None:
             dx, dslopes = torch.empty_like(x), torch.empty_like(slopes)
             dy = None if ctx.same else torch.empty_like(y)
-        lib = nat.lib()
-        ws_bytes = int(lib.y3b_structure_attention_adjoint_workspace_bytes(q.shape[0], k.shape[0], q.shape[1],
-                                                                           k.shape[1]))
-        ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=dev)
         args = _attention_args(q, k, v, x, y, slopes, layout, ctx.scale)
-        nat.check(lib.y3b_structure_attention_adjoint(
-            ctypes.byref(args), g.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws_bytes, dq.data_ptr(), dk.data_ptr(),
-            dv.data_ptr(), nat.ptr(dx), nat.ptr(dy), nat.ptr(dslopes), nat.stream_of(dev)),
-            "structure_attention adjoint")
-        return dq, dk, dv, dx, dy, dslopes, None, None
+        ws, ws_bytes = _attention_workspace(args, 1, dev)
+        status = _status(dev) if ctx.validate else None
+        nat.check(nat.lib().y3b_structure_attention_adjoint(
+            ctypes.byref(args), out.data_ptr(), g.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws_bytes, dq.data_ptr(),
+            dk.data_ptr(), dv.data_ptr(), nat.ptr(dx), nat.ptr(dy), nat.ptr(dslopes), nat.ptr(status),
+            nat.stream_of(dev)), "structure_attention adjoint")
+        if ctx.validate:
+            _raise_on_status(status, "structure_attention adjoint")
+        return dq, dk, dv, dx, dy, dslopes, None, None, None
 
 
 def _check_positions(t, rows, what):
@@ -733,7 +796,7 @@ def _check_positions(t, rows, what):
 
 
 def structure_attention(query, key, value, layout, *, positions=None, key_positions=None, slopes=None, scale=None,
-                        backend="auto"):
+                        backend="auto", validate=None):
     """Softmax attention among the atoms of each structure of a packed batch, weaker with distance.
 
     ``s_ij = scale * q_i . k_j - slopes[h] * |positions_i - key_positions_j|`` over the keys ``j`` of query
@@ -783,12 +846,13 @@ def structure_attention(query, key, value, layout, *, positions=None, key_positi
         if slopes.dtype != torch.float32 or tuple(slopes.shape) != (layout.heads,):
             raise ValueError(f"slopes must be float32 [{layout.heads}], got {slopes.dtype} {tuple(slopes.shape)}")
     scale = float(query.shape[2]) ** -0.5 if scale is None else float(scale)
+    validate = _validate_default(validate)
     if torch.is_grad_enabled() and any(t.requires_grad for t in given):
-        return _StructureAttention.apply(query, key, value, positions, key_positions, slopes, layout, scale)
+        return _StructureAttention.apply(query, key, value, positions, key_positions, slopes, layout, scale, validate)
     x = None if positions is None else positions.contiguous()
     y = x if key_positions is None else key_positions.contiguous()
     return _attention_forward(query, key, value, x, y, None if slopes is None else slopes.contiguous(), layout,
-                              scale)[0]
+                              scale, validate)[0]
 
 
 def native_execution_plan_capabilities():
