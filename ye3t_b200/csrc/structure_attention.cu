@@ -559,7 +559,9 @@ struct AttPlan {
 };
 
 bool in_place(const y3b_structure_attention_args* p, const void* base, int64_t row, int64_t head) {
-  return p->dtype == Y3B_BF16 && p->width % 8 == 0 && row % 8 == 0 && head % 8 == 0 && on16(base);
+  // a tensor map takes positive strides below 2^40 bytes
+  const auto fits = [](int64_t v) { return v > 0 && v % 8 == 0 && v < (int64_t(1) << 39); };
+  return p->dtype == Y3B_BF16 && p->width % 8 == 0 && fits(row) && fits(head) && on16(base);
 }
 
 AttPlan make_plan(const y3b_structure_attention_args* p, bool adjoint) {
@@ -636,6 +638,8 @@ int operands(const y3b_structure_attention_args* p, const AttPlan& w, const void
 
 AttTileArgs tile_args(const y3b_structure_attention_args* p, const AttArgs& a, const AttPlan& w, int32_t* status) {
   AttTileArgs t{};
+  t.nq = a.nq;
+  t.nk = a.nk;
   t.H = a.H;
   t.Hk = a.Hk;
   t.D = a.D;
@@ -756,6 +760,36 @@ int backward(const y3b_structure_attention_args* p, const AttArgs& a, const AttP
 }  // namespace y3b
 
 using namespace y3b;
+
+namespace y3b {
+
+int encode_columns(CUtensorMap* map, const AttOperand& o, int D, int heads, int64_t rows, int pieces, int box_rows) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Encode encode = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult got;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &got) != cudaSuccess ||
+        got != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<Encode>(f);
+  }();
+  if (rows == 0) return Y3B_OK;  // no column is loaded
+  if (!encode) return fail(Y3B_ERR_CUDA, "structure_attention: the driver has no cuTensorMapEncodeTiled");
+  const int width = (D + 7) / 8 * 8;
+  const cuuint64_t size[4] = {cuuint64_t(width), cuuint64_t(heads), cuuint64_t(rows), cuuint64_t(pieces)};
+  const cuuint64_t stride[3] = {cuuint64_t(o.head) * 2, cuuint64_t(o.row) * 2,
+                                cuuint64_t(pieces > 1 ? o.piece : o.row) * 2};
+  const cuuint32_t box[4] = {64, 1, cuuint32_t(box_rows), 1}, step[4] = {1, 1, 1, 1};
+  const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<__nv_bfloat16*>(o.p), size, stride,
+                             box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rc != CUDA_SUCCESS) return fail(Y3B_ERR_CUDA, "structure_attention: tensor map refused (%d)", int(rc));
+  return Y3B_OK;
+}
+
+}  // namespace y3b
 
 extern "C" int64_t y3b_structure_attention_workspace_bytes(const y3b_structure_attention_args* args, int adjoint) {
   AttArgs a;

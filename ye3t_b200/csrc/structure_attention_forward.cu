@@ -3,7 +3,7 @@
 
 namespace y3b {
 
-int attention_forward_tiles(int pieces, const AttTileArgs& a, int64_t items, cudaStream_t s) {
+int attention_forward_tiles(int pieces, AttTileArgs& a, int64_t items, cudaStream_t s) {
   return dispatch_attention_tile<kForward>(pieces, a, items, s);
 }
 

@@ -3,7 +3,7 @@
 
 namespace y3b {
 
-int attention_key_tiles(int pieces, const AttTileArgs& a, int64_t items, cudaStream_t s) {
+int attention_key_tiles(int pieces, AttTileArgs& a, int64_t items, cudaStream_t s) {
   return dispatch_attention_tile<kKeySide>(pieces, a, items, s);
 }
 

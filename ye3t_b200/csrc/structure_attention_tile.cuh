@@ -22,6 +22,8 @@
 // product to about 2^-24, and P and dS are split likewise.
 #pragma once
 
+#include <cuda.h>
+
 #include <type_traits>
 
 #include "structure_attention.cuh"
@@ -49,7 +51,9 @@ struct AttOperand {
 };
 
 struct AttTileArgs {
+  CUtensorMap cols[2];  // the column operands (K, V or Q, G) in boxes of 64 values x 1 head x BN rows
   AttOperand q, k, v, g;
+  int64_t nq, nk;
   int H, Hk, D, group, chunks;  // chunks: 16-byte pieces of a row of an operand
   const float* x;
   const float* y;
@@ -74,7 +78,7 @@ struct AttCfg {
   static constexpr int BN = NP == 1 ? 64 : DP == 64 ? 32 : MODE == kForward ? 32 : 16;
   static constexpr int ROWOPS = MODE == kForward ? 1 : 2;
   static constexpr int PANELS = DP / 64;
-  static constexpr int STAGES = NP == 3 && DP == 128 && MODE != kForward ? 1 : 2;
+  static constexpr int STAGES = NP == 3 ? (DP == 128 && MODE != kForward ? 1 : 2) : DP == 128 ? 2 : 4;
   static constexpr int ROW_PIECE = kTileRows * DP * 2;
   static constexpr int COL_PIECE = BN * DP * 2;
   static constexpr int COL_STAGE = 2 * NP * COL_PIECE;
@@ -250,10 +254,11 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
   const uint32_t tmem = s_tmem;
 
   if (warp >= 5) {
-    // ---- loading warps: column tile t into stage t % STAGES, one tile ahead of its arrival
+    // ---- loading warps.  A full column tile comes by TMA; one cut short by the structure's end by
+    // cp.async, with zeros past it: rows of the next structure, whatever they hold, stay out.
     const int t = tid - 160;
     bool ok = true;
-    for (int j = 0; j < total && ok; ++j) {
+    for (int j = 0; j < total; ++j) {
       const int s = j % C::STAGES;
       if (j >= C::STAGES) ok = tc::mbar_wait(empty(s), ((j / C::STAGES) - 1) & 1);
       if (!ok) break;
@@ -262,9 +267,25 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
       const int64_t col = int64_t(item.col) + c0;
       const uint32_t dst = cols + s * C::COL_STAGE;
       const int ch = MODE == kKeySide ? head * a.group + sub : head / a.group;
-      load_tile<BN, DP, NP>(dst, MODE == kKeySide ? a.q : a.k, col, ch, n, a.chunks, t, kLoadThreads);
-      load_tile<BN, DP, NP>(dst + NP * C::COL_PIECE, MODE == kKeySide ? a.g : a.v, col, ch, n, a.chunks, t,
-                            kLoadThreads);
+      if (n == BN) {
+        if (t == 0) {
+          tc::mbar_expect(full(s), C::COL_STAGE);
+#pragma unroll
+          for (int op = 0; op < 2; ++op) {
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+#pragma unroll
+              for (int q = 0; q < C::PANELS; ++q)
+                tc::tma_load4(dst + (op * NP + p) * C::COL_PIECE + q * (BN * 128), &a.cols[op], full(s), q * 64, ch,
+                              int(col), p);
+            }
+          }
+        }
+      } else {
+        load_tile<BN, DP, NP>(dst, MODE == kKeySide ? a.q : a.k, col, ch, n, a.chunks, t, kLoadThreads);
+        load_tile<BN, DP, NP>(dst + NP * C::COL_PIECE, MODE == kKeySide ? a.g : a.v, col, ch, n, a.chunks, t,
+                              kLoadThreads);
+      }
       const uint32_t ex = tc::smem_addr(extra + s * C::EXTRA);
       if constexpr (BIAS) {
         const float* pos = MODE == kKeySide ? a.x : a.y;
@@ -281,22 +302,9 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
         }
       }
       tc::cp_commit();
-      if constexpr (C::STAGES == 1) {
-        tc::cp_wait<0>();
-        tc::fence_async_smem();
-        tc::mbar_arrive(full(s));
-      } else if (j > 0) {
-        tc::cp_wait<1>();
-        tc::fence_async_smem();
-        tc::mbar_arrive(full((j - 1) % C::STAGES));
-      }
-    }
-    tc::cp_wait<0>();
-    if constexpr (C::STAGES > 1) {
-      if (ok && total > 0) {
-        tc::fence_async_smem();
-        tc::mbar_arrive(full((total - 1) % C::STAGES));
-      }
+      tc::cp_wait<0>();
+      tc::fence_async_smem();
+      tc::mbar_arrive(full(s));
     }
     if (!ok) s_abort = 1;
   } else if (warp == 4) {
@@ -701,9 +709,18 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
   if (tid == 0 && s_abort && a.status) atomicOr(a.status, Y3B_STATUS_TIMEOUT);
 }
 
+// Encodes the tensor map of a column operand; its strides are positive multiples of 16 bytes.
+int encode_columns(CUtensorMap* map, const AttOperand& o, int D, int heads, int64_t rows, int pieces, int box_rows);
+
 template <int MODE, int DP, int NP, bool BIAS>
-int launch_attention_tile(const AttTileArgs& a, int64_t items, cudaStream_t s) {
+int launch_attention_tile(AttTileArgs& a, int64_t items, cudaStream_t s) {
   using C = AttCfg<MODE, DP, NP>;
+  int rc = encode_columns(&a.cols[0], MODE == kKeySide ? a.q : a.k, a.D, MODE == kKeySide ? a.H : a.Hk,
+                          MODE == kKeySide ? a.nq : a.nk, NP, C::BN);
+  if (!rc)
+    rc = encode_columns(&a.cols[1], MODE == kKeySide ? a.g : a.v, a.D, MODE == kKeySide ? a.H : a.Hk,
+                        MODE == kKeySide ? a.nq : a.nk, NP, C::BN);
+  if (rc) return rc;
   const auto kernel = attention_tile_kernel<MODE, DP, NP, BIAS>;
   Y3B_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
   const int64_t grid = items * (MODE == kKeySide ? a.Hk : a.H) * C::HALVES;
@@ -714,7 +731,7 @@ int launch_attention_tile(const AttTileArgs& a, int64_t items, cudaStream_t s) {
 }
 
 template <int MODE>
-int dispatch_attention_tile(int pieces, const AttTileArgs& a, int64_t items, cudaStream_t s) {
+int dispatch_attention_tile(int pieces, AttTileArgs& a, int64_t items, cudaStream_t s) {
   if (items == 0) return Y3B_OK;
   const bool bias = a.slopes != nullptr, wide = a.D > 64;
 #define Y3B_TILE(DP, NP)                                                       \
@@ -730,9 +747,9 @@ int dispatch_attention_tile(int pieces, const AttTileArgs& a, int64_t items, cud
 }
 
 // One mode a translation unit.
-int attention_forward_tiles(int pieces, const AttTileArgs& a, int64_t items, cudaStream_t s);
-int attention_query_tiles(int pieces, const AttTileArgs& a, int64_t items, cudaStream_t s);
-int attention_key_tiles(int pieces, const AttTileArgs& a, int64_t items, cudaStream_t s);
+int attention_forward_tiles(int pieces, AttTileArgs& a, int64_t items, cudaStream_t s);
+int attention_query_tiles(int pieces, AttTileArgs& a, int64_t items, cudaStream_t s);
+int attention_key_tiles(int pieces, AttTileArgs& a, int64_t items, cudaStream_t s);
 
 }  // namespace y3b
 
