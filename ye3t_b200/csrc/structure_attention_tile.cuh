@@ -8,8 +8,8 @@
 // (G = gradient of the output.)  Per tile of BN columns: tcgen05.mma forms the score products in
 // tensor memory; thread r of the four score warps reads row r, does the softmax arithmetic in fp32 and
 // writes P or dS back to tensor memory as bf16, where it is the A operand of the accumulating product
-// (B: the same shared-memory column tile, read MN-major).  One warp issues the MMAs, two
-// warps bring the next column tile with cp.async, rows outside the item as zeros; so
+// (B: the same shared-memory column tile, read MN-major).  One warp issues the MMAs, one
+// warp brings the column tiles (TMA; a tile cut by the structure's end with cp.async and zeros), so that
 // nothing of another structure enters a product.
 //
 // What bounds it: the score warps.  A score takes one exp2 and one square root on the special-function
@@ -34,8 +34,8 @@ namespace y3b {
 enum AttMode { kForward = 0, kQuerySide = 1, kKeySide = 2 };
 
 constexpr int kTileRows = 128;
-constexpr int kTileThreads = 224;  // 4 score warps, 1 MMA warp, 2 loading warps
-constexpr int kLoadThreads = 64;
+constexpr int kTileThreads = 192;  // 4 score warps, 1 MMA warp, 1 loading warp: 3 warps a scheduler with 2 CTAs
+constexpr int kLoadThreads = 32;
 
 struct AttItem {
   int row, rows, col, cols, slot, pad[3];
@@ -75,7 +75,7 @@ struct AttTileArgs {
 
 template <int MODE, int DP, int NP>
 struct AttCfg {
-  static constexpr int BN = NP == 1 ? 64 : DP == 64 ? 32 : MODE == kForward ? 32 : 16;
+  static constexpr int BN = NP == 1 ? (MODE == kForward ? 64 : 32) : DP == 64 || MODE == kForward ? 32 : 16;
   static constexpr int ROWOPS = MODE == kForward ? 1 : 2;
   static constexpr int PANELS = DP / 64;
   static constexpr int STAGES = NP == 3 ? (DP == 128 && MODE != kForward ? 1 : 2) : DP == 128 ? 2 : 4;
@@ -85,11 +85,15 @@ struct AttCfg {
   static constexpr int EXTRA = 5 * BN;  // floats a stage: x, y, z, -lse, delta of the columns
   static constexpr int SMEM = 1024 + ROWOPS * NP * ROW_PIECE + STAGES * (COL_STAGE + EXTRA * 4);
   // tensor memory columns; with one piece P and dS take the place of the scores they come from
-  static constexpr int S = 0;
-  static constexpr int T = BN;
-  static constexpr int SCORES = MODE == kForward ? BN : 2 * BN;
+  // Score buffers: with two, the products of tile j + 1 run under the arithmetic of tile j (a single
+  // stage of columns allows one).
+  static constexpr int BUFS = STAGES > 1 ? 2 : 1;
+  static constexpr int BUF = (MODE == kForward ? 1 : 2) * BN;  // columns of one buffer
+  static constexpr int T = BN;                                 // T within a buffer
+  static constexpr int SCORES = BUFS * BUF;
   static constexpr int A0 = NP == 1 ? 0 : SCORES;
   static constexpr int A1 = NP == 1 ? BN : SCORES + NP * BN / 2;
+  static constexpr int ABUF = NP == 1 ? BUF : 0;  // with one piece every buffer holds its own P and dS
   static constexpr int ACC = NP == 1 ? SCORES : SCORES + (MODE == kKeySide ? 2 : 1) * NP * BN / 2;
   // Accumulators.  OPS results (dV and dK on the key side); a second one of each for three pieces
   // takes all products but that of the leading pieces: the tensor cores truncate when they accumulate,
@@ -198,7 +202,7 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
   using T = typename std::conditional<NP == 1, __nv_bfloat16, float>::type;
   constexpr int BN = C::BN;
   extern __shared__ __align__(1024) unsigned char tile_smem[];
-  __shared__ __align__(8) uint64_t bars[2 * C::STAGES + 3];
+  __shared__ __align__(8) uint64_t bars[2 * C::STAGES + 2 * C::BUFS + 1];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
 
@@ -222,7 +226,9 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
   const uint32_t bar0 = tc::smem_addr(bars);
   const auto full = [&](int s) { return bar0 + 8 * s; };
   const auto empty = [&](int s) { return bar0 + 8 * (C::STAGES + s); };
-  const uint32_t s_ready = bar0 + 8 * (2 * C::STAGES), p_ready = s_ready + 8, drain = s_ready + 16;
+  const auto s_ready = [&](int j) { return bar0 + 8 * (2 * C::STAGES + j % C::BUFS); };
+  const auto p_ready = [&](int j) { return bar0 + 8 * (2 * C::STAGES + C::BUFS + j % C::BUFS); };
+  const uint32_t drain = bar0 + 8 * (2 * C::STAGES + 2 * C::BUFS);
 
   if (warp == 4) tc::alloc(tc::smem_addr(&s_tmem), C::COLUMNS);
   if (tid == 0) {
@@ -230,8 +236,10 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
       tc::mbar_init(full(s), kLoadThreads);
       tc::mbar_init(empty(s), 1);
     }
-    tc::mbar_init(s_ready, 1);
-    tc::mbar_init(p_ready, 4);
+    for (int k = 0; k < C::BUFS; ++k) {
+      tc::mbar_init(s_ready(k), 1);
+      tc::mbar_init(p_ready(k), 4);
+    }
     tc::mbar_init(drain, 1);
     tc::mbar_init_fence();
     s_abort = 0;
@@ -254,7 +262,7 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
   const uint32_t tmem = s_tmem;
 
   if (warp >= 5) {
-    // ---- loading warps.  A full column tile comes by TMA; one cut short by the structure's end by
+    // ---- loading warp.  A full column tile comes by TMA; one cut short by the structure's end by
     // cp.async, with zeros past it: rows of the next structure, whatever they hold, stay out.
     const int t = tid - 160;
     bool ok = true;
@@ -312,16 +320,15 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
     if (lane == 0) {
       const int ksteps = (a.D + 15) / 16;
       const uint32_t id_s = tc::idesc_bf16(kTileRows, BN, false), id_a = tc::idesc_bf16(kTileRows, acc_n, true);
-      bool ok = true;
-      for (int j = 0; j < total; ++j) {
+      const auto issue_scores = [&](int j) {
         const int s = j % C::STAGES;
-        ok = tc::mbar_wait(full(s), (j / C::STAGES) & 1);
-        if (!ok) break;
+        if (!tc::mbar_wait(full(s), (j / C::STAGES) & 1)) return false;
         tc::fence_after();
         const uint32_t c0 = cols + s * C::COL_STAGE, c1 = c0 + NP * C::COL_PIECE;
+        const uint32_t buf = tmem + (j % C::BUFS) * C::BUF;
 #pragma unroll
         for (int op = 0; op < C::ROWOPS; ++op) {
-          const uint32_t ra = op ? row1 : row0, cb = op ? c1 : c0, d = tmem + (op ? C::T : C::S);
+          const uint32_t ra = op ? row1 : row0, cb = op ? c1 : c0, d = buf + (op ? C::T : 0);
 #pragma unroll
           for (int n = 0; n < Pieces<NP>::N; ++n) {
             for (int ks = 0; ks < ksteps; ++ks) {
@@ -334,14 +341,22 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
             }
           }
         }
-        tc::commit(s_ready);
-        ok = tc::mbar_wait(p_ready, j & 1);
+        tc::commit(s_ready(j));
+        return true;
+      };
+      bool ok = total == 0 || issue_scores(0);
+      for (int j = 0; ok && j < total; ++j) {
+        const int s = j % C::STAGES;
+        const uint32_t c0 = cols + s * C::COL_STAGE, c1 = c0 + NP * C::COL_PIECE;
+        if (C::BUFS == 2 && j + 1 < total) ok = issue_scores(j + 1);
+        if (!ok) break;
+        ok = tc::mbar_wait(p_ready(j), (j / C::BUFS) & 1);
         if (!ok) break;
         tc::fence_after();
         // forward: P x V; query side: dS x K (and P x K); key side: P x G and dS x Q
 #pragma unroll
         for (int op = 0; op < C::OPS + (C::FIX ? 1 : 0); ++op) {
-          const uint32_t A = tmem + (op == 0 ? C::A0 : C::A1);
+          const uint32_t A = tmem + (j % C::BUFS) * C::ABUF + (op == 0 ? C::A0 : C::A1);
           const uint32_t cb = (MODE == kForward || (MODE == kKeySide && op == 0) ? c1 : c0) + half * (BN * 128);
 #pragma unroll
           for (int n = 0; n < Pieces<NP>::N; ++n) {
@@ -355,6 +370,7 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
           }
         }
         tc::commit(empty(s));
+        if (C::BUFS == 1 && j + 1 < total) ok = issue_scores(j + 1);
       }
       if (!ok) {
         s_abort = 1;
@@ -408,204 +424,237 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
     }
     const tc::f2 nL2 = tc::pack(nL, nL), delta02 = tc::pack(delta0, delta0);
 
+    tc::f2 acc[10];
+#pragma unroll
+    for (int k = 0; k < 10; ++k) acc[k] = tc::pack(0.0f, 0.0f);
+    // row sums go from pairs within a few tiles to the row's: two levels keep the rounding of long rows small
+    const auto fold = [&] {
+#pragma unroll
+      for (int k = 0; k < 10; ++k) {
+        float s0, s1;
+        tc::unpack(acc[k], s0, s1);
+        if constexpr (MODE == kQuerySide) sum[k] += s0 + s1;
+        else if (k < 3) sum[k] = fmaf(slope, s0 + s1, sum[k]);
+        acc[k] = tc::pack(0.0f, 0.0f);
+      }
+    };
+
+    // One tile's arithmetic; n < BN columns where CUT, all of them otherwise.
+    const auto forward_tile = [&](auto cut, int j, int n, const float* ex, uint32_t buf) {
+      constexpr bool CUT = decltype(cut)::value;
+      float v[BN];
+#pragma unroll
+      for (int c = 0; c < BN; c += 16) tc::ld16(buf + c, v + c);
+      tc::wait_ld();
+      float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < BN; c += 4) {
+        tc::f2 s0 = tc::mul2(tc::pack(v[c], v[c + 1]), scale2), s1 = tc::mul2(tc::pack(v[c + 2], v[c + 3]), scale2);
+        if constexpr (BIAS) {
+          const ulonglong2 xx = *reinterpret_cast<const ulonglong2*>(ex + c);
+          const ulonglong2 yy = *reinterpret_cast<const ulonglong2*>(ex + BN + c);
+          const ulonglong2 zz = *reinterpret_cast<const ulonglong2*>(ex + 2 * BN + c);
+          const tc::f2 dx0 = tc::sub2(px2, xx.x), dx1 = tc::sub2(px2, xx.y);
+          const tc::f2 dy0 = tc::sub2(py2, yy.x), dy1 = tc::sub2(py2, yy.y);
+          const tc::f2 dz0 = tc::sub2(pz2, zz.x), dz1 = tc::sub2(pz2, zz.y);
+          s0 = tc::fma2(distance(tc::fma2(dz0, dz0, tc::fma2(dy0, dy0, tc::fma2(dx0, dx0, tiny2)))).d, nslope2, s0);
+          s1 = tc::fma2(distance(tc::fma2(dz1, dz1, tc::fma2(dy1, dy1, tc::fma2(dx1, dx1, tiny2)))).d, nslope2, s1);
+        }
+        tc::unpack(s0, v[c], v[c + 1]);
+        tc::unpack(s1, v[c + 2], v[c + 3]);
+        if constexpr (CUT) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (c + k >= n) v[c + k] = -INFINITY;
+        }
+        t0 = tc::max3(t0, v[c], v[c + 1]);
+        t1 = tc::max3(t1, v[c + 2], v[c + 3]);
+      }
+      const float top = fmaxf(t0, t1);
+      // the reference maximum moves only when a row would pass 2^8 times it: P stays within 2^8
+      // and the accumulated rows are rescaled seldom
+      if (j == 0) {
+        m = top;
+      } else {
+        const bool move = top > m + 8.0f || (m == -INFINITY && top > m);
+        if (__any_sync(0xffffffffu, move)) {
+          const float f = move ? tc::ex2(m - top) : 1.0f;
+          if (move) m = top;
+          l *= f;
+          if (!__all_sync(0xffffffffu, tc::mbar_wait(empty((j - 1) % C::STAGES), ((j - 1) / C::STAGES) & 1))) return false;
+          tc::fence_after();
+#pragma unroll
+          for (int u = 0; u < C::OPS + C::SMALL; ++u) {
+            for (int d = 0; d < acc_n; d += 16) {
+              float o[16];
+              tc::ld16(lane_base + C::ACC + u * C::W + d, o);
+              tc::wait_ld();
+              uint32_t r[16];
+#pragma unroll
+              for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(o[k] * f);
+              tc::st16(lane_base + C::ACC + u * C::W + d, r);
+            }
+          }
+          tc::wait_st();
+        }
+      }
+      const float ref = m == -INFINITY ? 0.0f : m;
+      const tc::f2 nref = tc::pack(-ref, -ref);
+      tc::f2 l0 = tc::pack(0.0f, 0.0f), l1 = l0;
+      const uint32_t dst = lane_base + C::A0 + (j % C::BUFS) * C::ABUF;
+#pragma unroll
+      for (int c0 = 0; c0 < BN; c0 += 16) {
+        uint32_t pr[NP][8];
+#pragma unroll
+        for (int c = 0; c < 16; c += 2) {
+          float e0, e1;
+          tc::unpack(tc::add2(tc::pack(v[c0 + c], v[c0 + c + 1]), nref), e0, e1);
+          e0 = tc::ex2(e0);
+          e1 = tc::ex2(e1);
+          if (c & 2) l1 = tc::add2(l1, tc::pack(e0, e1));
+          else l0 = tc::add2(l0, tc::pack(e0, e1));
+          uint32_t r[NP];
+          split_pair<NP>(e0, e1, r);
+#pragma unroll
+          for (int p = 0; p < NP; ++p) pr[p][c / 2] = r[p];
+        }
+#pragma unroll
+        for (int p = 0; p < NP; ++p) tc::st8(dst + p * (BN / 2) + c0 / 2, pr[p]);
+      }
+      float s0, s1;
+      tc::unpack(tc::add2(l0, l1), s0, s1);
+      l += s0 + s1;
+      return true;
+    };
+
+    const auto backward_tile = [&](auto cut, int j, int n, const float* ex, uint32_t buf) {
+      constexpr bool CUT = decltype(cut)::value;
+      const uint32_t dst = lane_base + (j % C::BUFS) * C::ABUF;
+      float sv[2][16], tv[2][16];
+      tc::ld16(buf, sv[0]);
+      tc::ld16(buf + C::T, tv[0]);
+#pragma unroll
+      for (int c0 = 0; c0 < BN; c0 += 16) {
+        constexpr int kLast = BN - 16;
+        const int cur = (c0 / 16) & 1;
+        tc::wait_ld();
+        if (c0 < kLast) {
+          tc::ld16(buf + c0 + 16, sv[cur ^ 1]);
+          tc::ld16(buf + C::T + c0 + 16, tv[cur ^ 1]);
+        }
+        [[maybe_unused]] uint32_t pr[NP][8];
+        uint32_t dr[NP][8];
+#pragma unroll
+        for (int c = 0; c < 16; c += 2) {
+          const int cc = c0 + c;
+          [[maybe_unused]] tc::f2 dx, dy, dz, d, r;
+          tc::f2 score = tc::mul2(tc::pack(sv[cur][c], sv[cur][c + 1]), scale2);
+          if constexpr (BIAS) {
+            dx = tc::sub2(px2, *reinterpret_cast<const tc::f2*>(ex + cc));
+            dy = tc::sub2(py2, *reinterpret_cast<const tc::f2*>(ex + BN + cc));
+            dz = tc::sub2(pz2, *reinterpret_cast<const tc::f2*>(ex + 2 * BN + cc));
+            const Distance x = distance(tc::fma2(dz, dz, tc::fma2(dy, dy, tc::fma2(dx, dx, tiny2))));
+            d = x.d;
+            r = x.r;
+            score = tc::fma2(d, nslope2, score);
+          }
+          float p0, p1;
+          if constexpr (MODE == kQuerySide) tc::unpack(tc::add2(score, nL2), p0, p1);
+          else tc::unpack(tc::sub2(score, *reinterpret_cast<const tc::f2*>(ex + 3 * BN + cc)), p0, p1);
+          p0 = tc::ex2(p0);
+          p1 = tc::ex2(p1);
+          if constexpr (CUT) {
+            if (cc >= n) p0 = 0.0f;
+            if (cc + 1 >= n) p1 = 0.0f;
+          }
+          const tc::f2 p = tc::pack(p0, p1), tt = tc::pack(tv[cur][c], tv[cur][c + 1]);
+          float g0, g1;
+          if constexpr (MODE == kQuerySide) {
+            const tc::f2 pt = tc::mul2(p, tt);
+            tc::unpack(tc::mul2(p, tc::sub2(tt, delta02)), g0, g1);
+            acc[0] = tc::add2(acc[0], pt);
+            acc[9] = tc::add2(acc[9], p);
+            if constexpr (BIAS) {
+              acc[1] = tc::fma2(d, pt, acc[1]);
+              acc[2] = tc::fma2(d, p, acc[2]);
+              const tc::f2 u = tc::mul2(pt, r), w = tc::mul2(p, r);
+              acc[3] = tc::fma2(u, dx, acc[3]);
+              acc[4] = tc::fma2(u, dy, acc[4]);
+              acc[5] = tc::fma2(u, dz, acc[5]);
+              acc[6] = tc::fma2(w, dx, acc[6]);
+              acc[7] = tc::fma2(w, dy, acc[7]);
+              acc[8] = tc::fma2(w, dz, acc[8]);
+            }
+          } else {
+            const tc::f2 ds = tc::mul2(p, tc::sub2(tt, *reinterpret_cast<const tc::f2*>(ex + 4 * BN + cc)));
+            tc::unpack(ds, g0, g1);
+            if constexpr (BIAS) {
+              const tc::f2 u = tc::mul2(ds, r);
+              acc[0] = tc::fma2(u, dx, acc[0]);
+              acc[1] = tc::fma2(u, dy, acc[1]);
+              acc[2] = tc::fma2(u, dz, acc[2]);
+            }
+          }
+          if constexpr (MODE == kKeySide || C::FIX) {
+            uint32_t q[NP];
+            split_pair<NP>(p0, p1, q);
+#pragma unroll
+            for (int k = 0; k < NP; ++k) pr[k][c / 2] = q[k];
+          }
+          uint32_t q[NP];
+          split_pair<NP>(g0, g1, q);
+#pragma unroll
+          for (int k = 0; k < NP; ++k) dr[k][c / 2] = q[k];
+        }
+        // with one piece, columns c0 / 2 .. c0 / 2 + 8 hold scores that are already in registers
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+          // key side: P first, then dS; query side: dS first
+          tc::st8(dst + (MODE == kKeySide ? C::A1 : C::A0) + k * (BN / 2) + c0 / 2, dr[k]);
+          if constexpr (MODE == kKeySide || C::FIX)
+            tc::st8(dst + (MODE == kKeySide ? C::A0 : C::A1) + k * (BN / 2) + c0 / 2, pr[k]);
+        }
+      }
+      return true;
+    };
+
     for (int j = 0; j < total; ++j) {
       const int s = j % C::STAGES;
       const int sub = MODE == kKeySide ? j / ntiles : 0, jt = MODE == kKeySide ? j - sub * ntiles : j;
       const int n = item.cols - jt * BN;  // columns there are, BN or more in a full tile
-      ok = tc::mbar_wait(full(s), (j / C::STAGES) & 1) && tc::mbar_wait(s_ready, j & 1);
+      ok = tc::mbar_wait(full(s), (j / C::STAGES) & 1) && tc::mbar_wait(s_ready(j), (j / C::BUFS) & 1);
+      // several pieces have one place for P and dS: the product before must be done with it
+      if (NP > 1 && C::BUFS == 2 && j > 0 && ok)
+        ok = tc::mbar_wait(empty((j - 1) % C::STAGES), ((j - 1) / C::STAGES) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc::fence_after();
       const float* ex = extra + s * C::EXTRA;
-      if (32 * warp >= item.rows) {
-        // no row of the item in this warp: its lanes of P stay as they are and reach no result
-      } else if constexpr (MODE == kForward) {
-        float v[BN];
-#pragma unroll
-        for (int c = 0; c < BN; c += 16) tc::ld16(lane_base + C::S + c, v + c);
-        tc::wait_ld();
-        float top = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < BN; c += 4) {
-          tc::f2 s0 = tc::mul2(tc::pack(v[c], v[c + 1]), scale2), s1 = tc::mul2(tc::pack(v[c + 2], v[c + 3]), scale2);
-          if constexpr (BIAS) {
-            const ulonglong2 xx = *reinterpret_cast<const ulonglong2*>(ex + c);
-            const ulonglong2 yy = *reinterpret_cast<const ulonglong2*>(ex + BN + c);
-            const ulonglong2 zz = *reinterpret_cast<const ulonglong2*>(ex + 2 * BN + c);
-            const tc::f2 dx0 = tc::sub2(px2, xx.x), dx1 = tc::sub2(px2, xx.y);
-            const tc::f2 dy0 = tc::sub2(py2, yy.x), dy1 = tc::sub2(py2, yy.y);
-            const tc::f2 dz0 = tc::sub2(pz2, zz.x), dz1 = tc::sub2(pz2, zz.y);
-            s0 = tc::fma2(distance(tc::fma2(dz0, dz0, tc::fma2(dy0, dy0, tc::fma2(dx0, dx0, tiny2)))).d, nslope2, s0);
-            s1 = tc::fma2(distance(tc::fma2(dz1, dz1, tc::fma2(dy1, dy1, tc::fma2(dx1, dx1, tiny2)))).d, nslope2, s1);
-          }
-          tc::unpack(s0, v[c], v[c + 1]);
-          tc::unpack(s1, v[c + 2], v[c + 3]);
-        }
-        if (n < BN) {
-#pragma unroll
-          for (int c = 0; c < BN; ++c)
-            if (c >= n) v[c] = -INFINITY;
-        }
-#pragma unroll
-        for (int c = 0; c < BN; ++c) top = fmaxf(top, v[c]);
-        // the reference maximum moves only when a row would pass 2^8 times it: P stays within 2^8
-        // and the accumulated rows are rescaled seldom
-        if (j == 0) {
-          m = top;
+      const uint32_t buf = lane_base + (j % C::BUFS) * C::BUF;
+      // a warp without a row of the item only keeps the barriers going: its lanes of P reach no result
+      if (32 * warp < item.rows) {
+        if constexpr (MODE == kForward) {
+          ok = n >= BN ? forward_tile(std::false_type{}, j, n, ex, buf) : forward_tile(std::true_type{}, j, n, ex, buf);
+          if (!ok) break;
         } else {
-          const bool move = top > m + 8.0f || (m == -INFINITY && top > m);
-          if (__any_sync(0xffffffffu, move)) {
-            const float f = move ? tc::ex2(m - top) : 1.0f;
-            if (move) m = top;
-            l *= f;
-            ok = tc::mbar_wait(empty((j - 1) % C::STAGES), ((j - 1) / C::STAGES) & 1);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            tc::fence_after();
-#pragma unroll
-            for (int u = 0; u < C::OPS + C::SMALL; ++u) {
-              for (int d = 0; d < acc_n; d += 16) {
-                float o[16];
-                tc::ld16(lane_base + C::ACC + u * C::W + d, o);
-                tc::wait_ld();
-                uint32_t r[16];
-#pragma unroll
-                for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(o[k] * f);
-                tc::st16(lane_base + C::ACC + u * C::W + d, r);
-              }
+          if constexpr (MODE == kKeySide && BIAS) {
+            if (jt == 0) {
+              if (j > 0) fold();
+              slope = a.slopes[head * a.group + sub];
+              nslope2 = tc::pack(-slope * kLog2e, -slope * kLog2e);
             }
-            tc::wait_st();
           }
-        }
-        const float ref = m == -INFINITY ? 0.0f : m;
-        const tc::f2 nref = tc::pack(-ref, -ref);
-        tc::f2 l0 = tc::pack(0.0f, 0.0f), l1 = l0;
-#pragma unroll
-        for (int c0 = 0; c0 < BN; c0 += 16) {
-          uint32_t pr[NP][8];
-#pragma unroll
-          for (int c = 0; c < 16; c += 2) {
-            float e0, e1;
-            tc::unpack(tc::add2(tc::pack(v[c0 + c], v[c0 + c + 1]), nref), e0, e1);
-            e0 = tc::ex2(e0);
-            e1 = tc::ex2(e1);
-            if (c & 2) l1 = tc::add2(l1, tc::pack(e0, e1));
-            else l0 = tc::add2(l0, tc::pack(e0, e1));
-            uint32_t r[NP];
-            split_pair<NP>(e0, e1, r);
-#pragma unroll
-            for (int p = 0; p < NP; ++p) pr[p][c / 2] = r[p];
-          }
-#pragma unroll
-          for (int p = 0; p < NP; ++p) tc::st8(lane_base + C::A0 + p * (BN / 2) + c0 / 2, pr[p]);
-        }
-        float s0, s1;
-        tc::unpack(tc::add2(l0, l1), s0, s1);
-        l += s0 + s1;
-      } else {
-        if constexpr (MODE == kKeySide) {
-          if constexpr (BIAS) {
-            slope = a.slopes[head * a.group + sub];
-            nslope2 = tc::pack(-slope * kLog2e, -slope * kLog2e);
-          }
-        }
-        const tc::f2 zero2 = tc::pack(0.0f, 0.0f);
-        tc::f2 acc[10];
-#pragma unroll
-        for (int k = 0; k < 10; ++k) acc[k] = zero2;
-#pragma unroll
-        for (int c0 = 0; c0 < BN; c0 += 16) {
-          float sv[16], tv[16];
-          tc::ld16(lane_base + C::S + c0, sv);
-          tc::ld16(lane_base + C::T + c0, tv);
-          tc::wait_ld();
-          uint32_t pr[NP][8], dr[NP][8];
-#pragma unroll
-          for (int c = 0; c < 16; c += 2) {
-            const int cc = c0 + c;
-            tc::f2 e, dx, dy, dz, d, r, score = tc::mul2(tc::pack(sv[c], sv[c + 1]), scale2);
-            if constexpr (MODE == kQuerySide) e = nL2;
-            else e = *reinterpret_cast<const tc::f2*>(ex + 3 * BN + cc) ^ 0x8000000080000000ull;  // -lse
-            if constexpr (BIAS) {
-              dx = tc::sub2(px2, *reinterpret_cast<const tc::f2*>(ex + cc));
-              dy = tc::sub2(py2, *reinterpret_cast<const tc::f2*>(ex + BN + cc));
-              dz = tc::sub2(pz2, *reinterpret_cast<const tc::f2*>(ex + 2 * BN + cc));
-              const Distance x = distance(tc::fma2(dz, dz, tc::fma2(dy, dy, tc::fma2(dx, dx, tiny2))));
-              d = x.d;
-              r = x.r;
-              score = tc::fma2(d, nslope2, score);
-            }
-            e = tc::add2(score, e);
-            float p0, p1;
-            tc::unpack(e, p0, p1);
-            p0 = tc::ex2(p0);
-            p1 = tc::ex2(p1);
-            if (n < BN) {
-              if (cc >= n) p0 = 0.0f;
-              if (cc + 1 >= n) p1 = 0.0f;
-            }
-            const tc::f2 p = tc::pack(p0, p1), tt = tc::pack(tv[c], tv[c + 1]);
-            float g0, g1;
-            if constexpr (MODE == kQuerySide) {
-              const tc::f2 pt = tc::mul2(p, tt);
-              tc::unpack(tc::mul2(p, tc::sub2(tt, delta02)), g0, g1);
-              acc[0] = tc::add2(acc[0], pt);
-              acc[9] = tc::add2(acc[9], p);
-              if constexpr (BIAS) {
-                acc[1] = tc::fma2(d, pt, acc[1]);
-                acc[2] = tc::fma2(d, p, acc[2]);
-                const tc::f2 u = tc::mul2(pt, r), w = tc::mul2(p, r);
-                acc[3] = tc::fma2(u, dx, acc[3]);
-                acc[4] = tc::fma2(u, dy, acc[4]);
-                acc[5] = tc::fma2(u, dz, acc[5]);
-                acc[6] = tc::fma2(w, dx, acc[6]);
-                acc[7] = tc::fma2(w, dy, acc[7]);
-                acc[8] = tc::fma2(w, dz, acc[8]);
-              }
-            } else {
-              const tc::f2 ds = tc::mul2(p, tc::sub2(tt, *reinterpret_cast<const tc::f2*>(ex + 4 * BN + cc)));
-              tc::unpack(ds, g0, g1);
-              if constexpr (BIAS) {
-                const tc::f2 u = tc::mul2(ds, r);
-                acc[0] = tc::fma2(u, dx, acc[0]);
-                acc[1] = tc::fma2(u, dy, acc[1]);
-                acc[2] = tc::fma2(u, dz, acc[2]);
-              }
-            }
-            if constexpr (MODE == kKeySide || C::FIX) {
-              uint32_t q[NP];
-              split_pair<NP>(p0, p1, q);
-#pragma unroll
-              for (int k = 0; k < NP; ++k) pr[k][c / 2] = q[k];
-            }
-            uint32_t q[NP];
-            split_pair<NP>(g0, g1, q);
-#pragma unroll
-            for (int k = 0; k < NP; ++k) dr[k][c / 2] = q[k];
-          }
-          // with one piece, columns c0/2 .. c0/2 + 8 hold scores that are already in registers
-#pragma unroll
-          for (int k = 0; k < NP; ++k) {
-            // key side: P first, then dS; query side: dS first
-            tc::st8(lane_base + (MODE == kKeySide ? C::A1 : C::A0) + k * (BN / 2) + c0 / 2, dr[k]);
-            if constexpr (MODE == kKeySide || C::FIX)
-              tc::st8(lane_base + (MODE == kKeySide ? C::A0 : C::A1) + k * (BN / 2) + c0 / 2, pr[k]);
-          }
-        }
-        // tile sums into the row's sums: two levels keep the rounding of long rows small
-#pragma unroll
-        for (int k = 0; k < 10; ++k) {
-          float s0, s1;
-          tc::unpack(acc[k], s0, s1);
-          if constexpr (MODE == kQuerySide) sum[k] += s0 + s1;
-          else if (k < 3) sum[k] = fmaf(slope, s0 + s1, sum[k]);
+          if ((j & 3) == 3) fold();
+          if (n >= BN) backward_tile(std::false_type{}, j, n, ex, buf);
+          else backward_tile(std::true_type{}, j, n, ex, buf);
         }
       }
       tc::wait_st();
       tc::fence_before();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(p_ready);
+      if (lane == 0) tc::mbar_arrive(p_ready(j));
     }
+    if constexpr (MODE != kForward) fold();
 
     // ---- results
     if (ok && total > 0) {

@@ -191,6 +191,11 @@ __device__ __forceinline__ float sqrt_approx(float x) {
   asm("sqrt.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
   return r;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 // Two fp32 rounded to bf16: a in the low half.
 __device__ __forceinline__ uint32_t bf16x2(float a, float b) {
   uint32_t r;
