@@ -455,37 +455,40 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackA
   }
 }
 
-// Joins of split items, one CTA a (join, head), one warp a row; W = floats of a partial row.
+// Joins of split items, one warp a row; W = floats of a partial row.
+constexpr int kJoinCtas = kTileRows / 4;  // CTAs of four warps a tile
+
 template <typename T>
 __global__ void __launch_bounds__(128) join_forward_kernel(const AttJoin* __restrict__ joins,
                                                            const float* __restrict__ part, int W, int DP, int D,
                                                            int H, T* __restrict__ out, float* __restrict__ lse) {
-  const AttJoin jn = joins[blockIdx.x / unsigned(H)];
-  const int h = int(blockIdx.x % unsigned(H)), lane = threadIdx.x & 31;
+  const unsigned task = blockIdx.x / kJoinCtas;
+  const AttJoin jn = joins[task / unsigned(H)];
+  const int h = int(task % unsigned(H)), lane = threadIdx.x & 31;
+  const int r = int(blockIdx.x % kJoinCtas) * 4 + (threadIdx.x >> 5);
+  if (r >= jn.rows) return;
   const int64_t step = int64_t(H) * kTileRows * W;
-  for (int r = threadIdx.x >> 5; r < jn.rows; r += 4) {
-    const float* p = part + ((int64_t(jn.first) * H + h) * kTileRows + r) * W;
-    float m = -INFINITY;
-    for (int k = lane; k < jn.count; k += 32) m = fmaxf(m, p[k * step + DP]);
-    m = warp_max(m);
-    const float ref = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f;
-    for (int k = lane; k < jn.count; k += 32) l += p[k * step + DP + 1] * exp2f(p[k * step + DP] - ref);
-    l = warp_sum(l);
-    const bool none = m == -INFINITY && l == 0.0f;
-    const int64_t at = (int64_t(jn.row) + r) * H + h;
-    const float inv = none ? 0.0f : 1.0f / l;
-    for (int d = lane; d < D; d += 32) {
-      float o = 0.0f;
-      for (int k = 0; k < jn.count; ++k) {
-        // a part without any score above -inf holds no numbers
-        const float mk = p[k * step + DP];
-        if (!(mk == -INFINITY && p[k * step + DP + 1] == 0.0f)) o = fmaf(p[k * step + d], exp2f(mk - ref), o);
-      }
-      out[at * D + d] = from_float<T>(none ? 0.0f : o * inv);
+  const float* p = part + ((int64_t(jn.first) * H + h) * kTileRows + r) * W;
+  float m = -INFINITY;
+  for (int k = lane; k < jn.count; k += 32) m = fmaxf(m, p[k * step + DP]);
+  m = warp_max(m);
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f;
+  for (int k = lane; k < jn.count; k += 32) l += p[k * step + DP + 1] * exp2f(p[k * step + DP] - ref);
+  l = warp_sum(l);
+  const bool none = m == -INFINITY && l == 0.0f;
+  const int64_t at = (int64_t(jn.row) + r) * H + h;
+  const float inv = none ? 0.0f : 1.0f / l;
+  for (int d = lane; d < D; d += 32) {
+    float o = 0.0f;
+    for (int k = 0; k < jn.count; ++k) {
+      // a part without any score above -inf holds no numbers
+      const float mk = p[k * step + DP];
+      if (!(mk == -INFINITY && p[k * step + DP + 1] == 0.0f)) o = fmaf(p[k * step + d], exp2f(mk - ref), o);
     }
-    if (lane == 0) lse[at] = none ? INFINITY : m + log2f(l);
+    out[at * D + d] = from_float<T>(none ? 0.0f : o * inv);
   }
+  if (lane == 0) lse[at] = none ? INFINITY : m + log2f(l);
 }
 
 __device__ __forceinline__ float sum_parts(const float* p, int64_t step, int count) {
@@ -501,28 +504,29 @@ __global__ void __launch_bounds__(128) join_query_kernel(const AttJoin* __restri
                                                          T* __restrict__ dq, float* __restrict__ delta,
                                                          float* __restrict__ slope_part,
                                                          float* __restrict__ place_part) {
-  const AttJoin jn = joins[blockIdx.x / unsigned(H)];
-  const int h = int(blockIdx.x % unsigned(H)), lane = threadIdx.x & 31;
+  const unsigned task = blockIdx.x / kJoinCtas;
+  const AttJoin jn = joins[task / unsigned(H)];
+  const int h = int(task % unsigned(H)), lane = threadIdx.x & 31;
+  const int r = int(blockIdx.x % kJoinCtas) * 4 + (threadIdx.x >> 5);
+  if (r >= jn.rows) return;
   const int64_t step = int64_t(H) * kTileRows * W;
-  for (int r = threadIdx.x >> 5; r < jn.rows; r += 4) {
-    const float* p = part + ((int64_t(jn.first) * H + h) * kTileRows + r) * W;
-    const int64_t at = (int64_t(jn.row) + r) * H + h;
-    const float s = lane < 10 ? sum_parts(p + DP + lane, step, jn.count) : 0.0f;
-    const float all = __shfl_sync(0xffffffffu, s, 9), inv = all == 0.0f ? 0.0f : 1.0f / all;
-    const float dl = __shfl_sync(0xffffffffu, s, 0) * inv;
-    const float low = __shfl_sync(0xffffffffu, s, lane < 3 ? 6 + lane : 2);  // what delta multiplies
-    const float high = __shfl_sync(0xffffffffu, s, lane < 3 ? 3 + lane : 1);
-    if (lane == 0) delta[at] = dl;
-    for (int d = lane; d < D; d += 32) {
-      float x = sum_parts(p + d, step, jn.count);
-      // one piece: dS was formed with the forward's rounded delta, and P K follows the sums
-      if constexpr (sizeof(T) == 2) x = fmaf(p[DP + 10] - dl, sum_parts(p + DP + 16 + d, step, jn.count), x);
-      dq[at * D + d] = from_float<T>(scale * x);
-    }
-    if (slopes) {
-      if (lane < 3) place_part[at * 3 + lane] = -slopes[h] * inv * (high - dl * low);
-      if (lane == 3) slope_part[at] = -inv * (high - dl * low);
-    }
+  const float* p = part + ((int64_t(jn.first) * H + h) * kTileRows + r) * W;
+  const int64_t at = (int64_t(jn.row) + r) * H + h;
+  const float s = lane < 10 ? sum_parts(p + DP + lane, step, jn.count) : 0.0f;
+  const float all = __shfl_sync(0xffffffffu, s, 9), inv = all == 0.0f ? 0.0f : 1.0f / all;
+  const float dl = __shfl_sync(0xffffffffu, s, 0) * inv;
+  const float low = __shfl_sync(0xffffffffu, s, lane < 3 ? 6 + lane : 2);  // what delta multiplies
+  const float high = __shfl_sync(0xffffffffu, s, lane < 3 ? 3 + lane : 1);
+  if (lane == 0) delta[at] = dl;
+  for (int d = lane; d < D; d += 32) {
+    float x = sum_parts(p + d, step, jn.count);
+    // one piece: dS was formed with the forward's rounded delta, and P K follows the sums
+    if constexpr (sizeof(T) == 2) x = fmaf(p[DP + 10] - dl, sum_parts(p + DP + 16 + d, step, jn.count), x);
+    dq[at * D + d] = from_float<T>(scale * x);
+  }
+  if (slopes) {
+    if (lane < 3) place_part[at * 3 + lane] = -slopes[h] * inv * (high - dl * low);
+    if (lane == 3) slope_part[at] = -inv * (high - dl * low);
   }
 }
 
@@ -531,18 +535,19 @@ __global__ void __launch_bounds__(128) join_key_kernel(const AttJoin* __restrict
                                                        const float* __restrict__ part, int W, int DP, int D, int Hk,
                                                        float scale, T* __restrict__ dk, T* __restrict__ dv,
                                                        float* __restrict__ place_part) {
-  const AttJoin jn = joins[blockIdx.x / unsigned(Hk)];
-  const int h = int(blockIdx.x % unsigned(Hk)), lane = threadIdx.x & 31;
+  const unsigned task = blockIdx.x / kJoinCtas;
+  const AttJoin jn = joins[task / unsigned(Hk)];
+  const int h = int(task % unsigned(Hk)), lane = threadIdx.x & 31;
+  const int r = int(blockIdx.x % kJoinCtas) * 4 + (threadIdx.x >> 5);
+  if (r >= jn.rows) return;
   const int64_t step = int64_t(Hk) * kTileRows * W;
-  for (int r = threadIdx.x >> 5; r < jn.rows; r += 4) {
-    const float* p = part + ((int64_t(jn.first) * Hk + h) * kTileRows + r) * W;
-    const int64_t at = (int64_t(jn.row) + r) * Hk + h;
-    for (int d = lane; d < D; d += 32) {
-      dv[at * D + d] = from_float<T>(sum_parts(p + d, step, jn.count));
-      dk[at * D + d] = from_float<T>(scale * sum_parts(p + DP + d, step, jn.count));
-    }
-    if (place_part && lane < 3) place_part[at * 3 + lane] = -sum_parts(p + 2 * DP + lane, step, jn.count);
+  const float* p = part + ((int64_t(jn.first) * Hk + h) * kTileRows + r) * W;
+  const int64_t at = (int64_t(jn.row) + r) * Hk + h;
+  for (int d = lane; d < D; d += 32) {
+    dv[at * D + d] = from_float<T>(sum_parts(p + d, step, jn.count));
+    dk[at * D + d] = from_float<T>(scale * sum_parts(p + DP + d, step, jn.count));
   }
+  if (place_part && lane < 3) place_part[at * 3 + lane] = -sum_parts(p + 2 * DP + lane, step, jn.count);
 }
 
 // ---------------------------------------------------------------------------
@@ -674,7 +679,7 @@ int forward(const y3b_structure_attention_args* p, const AttArgs& a, const AttPl
     rc = attention_forward_tiles(w.pieces, t, p->query_item_count, s);
     if (rc) return rc;
     if (p->query_join_count > 0) {
-      join_forward_kernel<T><<<unsigned(p->query_join_count * a.H), 128, 0, s>>>(
+      join_forward_kernel<T><<<unsigned(p->query_join_count * a.H * kJoinCtas), 128, 0, s>>>(
           reinterpret_cast<const AttJoin*>(p->query_joins), t.part, w.Wf, w.DP, a.D, a.H, static_cast<T*>(out), lse);
       Y3B_LAUNCH_CHECK();
     }
@@ -716,7 +721,7 @@ int backward(const y3b_structure_attention_args* p, const AttArgs& a, const AttP
     const int rc = attention_query_tiles(w.pieces, t, p->query_item_count, s);
     if (rc) return rc;
     if (p->query_join_count > 0) {
-      join_query_kernel<T><<<unsigned(p->query_join_count * a.H), 128, 0, s>>>(
+      join_query_kernel<T><<<unsigned(p->query_join_count * a.H * kJoinCtas), 128, 0, s>>>(
           reinterpret_cast<const AttJoin*>(p->query_joins), t.part, w.Wq, w.DP, a.D, a.H, a.scale, a.slopes,
           static_cast<T*>(dq), delta, slope_part, dx_part);
       Y3B_LAUNCH_CHECK();
@@ -737,7 +742,7 @@ int backward(const y3b_structure_attention_args* p, const AttArgs& a, const AttP
     const int rc = attention_key_tiles(w.pieces, t, p->key_item_count, s);
     if (rc) return rc;
     if (p->key_join_count > 0) {
-      join_key_kernel<T><<<unsigned(p->key_join_count * a.Hk), 128, 0, s>>>(
+      join_key_kernel<T><<<unsigned(p->key_join_count * a.Hk * kJoinCtas), 128, 0, s>>>(
           reinterpret_cast<const AttJoin*>(p->key_joins), t.part, w.Wk, w.DP, a.D, a.Hk, a.scale,
           static_cast<T*>(dk), static_cast<T*>(dv), a.slopes ? dy_part : nullptr);
       Y3B_LAUNCH_CHECK();

@@ -34,7 +34,6 @@ namespace y3b {
 enum AttMode { kForward = 0, kQuerySide = 1, kKeySide = 2 };
 
 constexpr int kTileRows = 128;
-constexpr int kTileThreads = 192;  // 4 score warps, 1 MMA warp, 1 loading warp: 3 warps a scheduler with 2 CTAs
 constexpr int kLoadThreads = 32;
 
 struct AttItem {
@@ -75,7 +74,12 @@ struct AttTileArgs {
 
 template <int MODE, int DP, int NP>
 struct AttCfg {
-  static constexpr int BN = NP == 1 ? (MODE == kForward ? 64 : 32) : DP == 64 || MODE == kForward ? 32 : 16;
+  static constexpr int BN = NP == 1 && MODE == kForward ? 64 : NP == 1 || DP == 64 || MODE == kForward ? 32 : 16;
+  // Score groups of four warps; with two, each takes every other column tile.  The backward with one piece is
+  // 14 % faster with two (8,192 atoms, 8 heads of 64); the forward, which needs more registers, 10 % slower.
+  static constexpr int GROUPS = NP == 1 && MODE != kForward ? 2 : 1;
+  static constexpr int MMA_WARP = 4 * GROUPS, LOAD_WARP = MMA_WARP + 1;
+  static constexpr int THREADS = 32 * (LOAD_WARP + 1);
   static constexpr int ROWOPS = MODE == kForward ? 1 : 2;
   static constexpr int PANELS = DP / 64;
   static constexpr int STAGES = NP == 3 ? (DP == 128 && MODE != kForward ? 1 : 2) : DP == 128 ? 2 : 4;
@@ -196,7 +200,7 @@ __device__ __forceinline__ Distance distance(tc::f2 squares) {
 }
 
 template <int MODE, int DP, int NP, bool BIAS>
-__global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) attention_tile_kernel(
+__global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP, NP>::PER_SM) attention_tile_kernel(
     const __grid_constant__ AttTileArgs a) {
   using C = AttCfg<MODE, DP, NP>;
   using T = typename std::conditional<NP == 1, __nv_bfloat16, float>::type;
@@ -230,7 +234,7 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
   const auto p_ready = [&](int j) { return bar0 + 8 * (2 * C::STAGES + C::BUFS + j % C::BUFS); };
   const uint32_t drain = bar0 + 8 * (2 * C::STAGES + 2 * C::BUFS);
 
-  if (warp == 4) tc::alloc(tc::smem_addr(&s_tmem), C::COLUMNS);
+  if (warp == C::MMA_WARP) tc::alloc(tc::smem_addr(&s_tmem), C::COLUMNS);
   if (tid == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
       tc::mbar_init(full(s), kLoadThreads);
@@ -247,10 +251,10 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
   // row operands, by all threads
   {
     const AttOperand& r0 = MODE == kKeySide ? a.k : a.q;
-    load_tile<kTileRows, DP, NP>(row0, r0, item.row, head, item.rows, a.chunks, tid, kTileThreads);
+    load_tile<kTileRows, DP, NP>(row0, r0, item.row, head, item.rows, a.chunks, tid, C::THREADS);
     if constexpr (MODE != kForward) {
       const AttOperand& r1 = MODE == kKeySide ? a.v : a.g;
-      load_tile<kTileRows, DP, NP>(row1, r1, item.row, head, item.rows, a.chunks, tid, kTileThreads);
+      load_tile<kTileRows, DP, NP>(row1, r1, item.row, head, item.rows, a.chunks, tid, C::THREADS);
     }
     tc::cp_commit();
     tc::cp_wait<0>();
@@ -261,10 +265,10 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
   tc::fence_after();
   const uint32_t tmem = s_tmem;
 
-  if (warp >= 5) {
+  if (warp == C::LOAD_WARP) {
     // ---- loading warp.  A full column tile comes by TMA; one cut short by the structure's end by
     // cp.async, with zeros past it: rows of the next structure, whatever they hold, stay out.
-    const int t = tid - 160;
+    const int t = lane;
     bool ok = true;
     for (int j = 0; j < total; ++j) {
       const int s = j % C::STAGES;
@@ -315,7 +319,7 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
       tc::mbar_arrive(full(s));
     }
     if (!ok) s_abort = 1;
-  } else if (warp == 4) {
+  } else if (warp == C::MMA_WARP) {
     // ---- MMA issue: scores of tile j, then (when P is back) its accumulating product
     if (lane == 0) {
       const int ksteps = (a.D + 15) / 16;
@@ -380,10 +384,11 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
     }
     __syncwarp();
   } else {
-    // ---- score warps: thread = row
-    const bool valid = tid < item.rows;
-    const int64_t row = int64_t(item.row) + (valid ? tid : 0);
-    const uint32_t lane_base = tmem + (uint32_t(32 * warp) << 16);
+    // ---- score warps: thread = row, in each group
+    const int r_tile = tid & (kTileRows - 1), group = C::GROUPS == 1 ? 0 : tid / kTileRows;
+    const bool valid = r_tile < item.rows;
+    const int64_t row = int64_t(item.row) + (valid ? r_tile : 0);
+    const uint32_t lane_base = tmem + (uint32_t(32 * (warp & 3)) << 16);
     float px = 0.0f, py = 0.0f, pz = 0.0f, slope = 0.0f;
     if constexpr (BIAS) {
       const float* pos = (MODE == kKeySide ? a.y : a.x) + 3 * row;
@@ -481,7 +486,8 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
           const float f = move ? tc::ex2(m - top) : 1.0f;
           if (move) m = top;
           l *= f;
-          if (!__all_sync(0xffffffffu, tc::mbar_wait(empty((j - 1) % C::STAGES), ((j - 1) / C::STAGES) & 1))) return false;
+          if (!__all_sync(0xffffffffu, tc::mbar_wait(empty((j - 1) % C::STAGES), ((j - 1) / C::STAGES) & 1)))
+            return false;
           tc::fence_after();
 #pragma unroll
           for (int u = 0; u < C::OPS + C::SMALL; ++u) {
@@ -618,7 +624,8 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
       return true;
     };
 
-    for (int j = 0; j < total; ++j) {
+    [[maybe_unused]] int last_sub = -1;
+    for (int j = group; j < total; j += C::GROUPS) {
       const int s = j % C::STAGES;
       const int sub = MODE == kKeySide ? j / ntiles : 0, jt = MODE == kKeySide ? j - sub * ntiles : j;
       const int n = item.cols - jt * BN;  // columns there are, BN or more in a full tile
@@ -632,19 +639,20 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
       const float* ex = extra + s * C::EXTRA;
       const uint32_t buf = lane_base + (j % C::BUFS) * C::BUF;
       // a warp without a row of the item only keeps the barriers going: its lanes of P reach no result
-      if (32 * warp < item.rows) {
+      if (32 * (warp & 3) < item.rows) {
         if constexpr (MODE == kForward) {
           ok = n >= BN ? forward_tile(std::false_type{}, j, n, ex, buf) : forward_tile(std::true_type{}, j, n, ex, buf);
           if (!ok) break;
         } else {
           if constexpr (MODE == kKeySide && BIAS) {
-            if (jt == 0) {
-              if (j > 0) fold();
+            if (sub != last_sub) {
+              fold();
+              last_sub = sub;
               slope = a.slopes[head * a.group + sub];
               nslope2 = tc::pack(-slope * kLog2e, -slope * kLog2e);
             }
           }
-          if ((j & 3) == 3) fold();
+          if (((j / C::GROUPS) & 3) == 3) fold();
           if (n >= BN) backward_tile(std::false_type{}, j, n, ex, buf);
           else backward_tile(std::true_type{}, j, n, ex, buf);
         }
@@ -661,11 +669,27 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
       ok = tc::mbar_wait(empty((total - 1) % C::STAGES), ((total - 1) / C::STAGES) & 1);
       ok = __all_sync(0xffffffffu, ok);
     }
+    // the groups' sums: every thread gets the other group's of its row, through the stages' memory
+    if constexpr (C::GROUPS == 2) {
+      float* shared = reinterpret_cast<float*>(tile_smem + (cols - tc::smem_addr(tile_smem)));
+      constexpr int N = MODE == kQuerySide ? 10 : 3;
+      asm volatile("bar.sync 1, 256;\n" ::: "memory");
+      if (ok) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) shared[(group * N + k) * kTileRows + r_tile] = sum[k];
+      }
+      asm volatile("bar.sync 1, 256;\n" ::: "memory");
+      if (ok) {
+        const float* other = shared + (1 - group) * N * kTileRows + r_tile;
+#pragma unroll
+        for (int k = 0; k < N; ++k) sum[k] += other[k * kTileRows];
+      }
+    }
     if (ok) {
       tc::fence_after();
       const bool split = item.slot >= 0;
       const int64_t at = row * heads + head;
-      float* part = split ? a.part + ((int64_t(item.slot) * heads + head) * kTileRows + tid) * C::PART : nullptr;
+      float* part = split ? a.part + ((int64_t(item.slot) * heads + head) * kTileRows + r_tile) * C::PART : nullptr;
       float f0 = 1.0f;
       bool none = total == 0;
       if constexpr (MODE == kForward) {
@@ -684,7 +708,7 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
       for (int op = 0; op < C::OPS; ++op) {
         const float f = MODE == kKeySide && op == 1 && !split ? a.scale : f0;
         T* dst = static_cast<T*>(op ? a.out1 : a.out0) + at * a.D;
-        for (int d = 0; d < acc_n; d += 16) {
+        for (int d = 16 * group; d < acc_n; d += 16 * C::GROUPS) {
           float o[16];
           tc::ld16(lane_base + C::ACC + op * C::W + d, o);
           if constexpr (C::SMALL > 0 || C::FIX) {
@@ -716,7 +740,7 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
           }
         }
       }
-      if (valid) {
+      if (valid && group == 0) {
         if constexpr (MODE == kForward) {
           if (split) {
             part[DP] = none ? -INFINITY : m;
@@ -751,7 +775,7 @@ __global__ void __launch_bounds__(kTileThreads, AttCfg<MODE, DP, NP>::PER_SM) at
   }
   tc::fence_before();
   __syncthreads();
-  if (warp == 4) {
+  if (warp == C::MMA_WARP) {
     tc::fence_after();
     tc::dealloc(tmem, C::COLUMNS);
   }
@@ -774,7 +798,7 @@ int launch_attention_tile(AttTileArgs& a, int64_t items, cudaStream_t s) {
   Y3B_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
   const int64_t grid = items * (MODE == kKeySide ? a.Hk : a.H) * C::HALVES;
   if (grid > INT32_MAX) return fail(Y3B_ERR_UNSUPPORTED, "structure_attention: %lld tiles", (long long)grid);
-  kernel<<<unsigned(grid), kTileThreads, C::SMEM, s>>>(a);
+  kernel<<<unsigned(grid), C::THREADS, C::SMEM, s>>>(a);
   Y3B_LAUNCH_CHECK();
   return Y3B_OK;
 }

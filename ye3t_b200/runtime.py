@@ -624,9 +624,9 @@ def _work_tables(row_first, row_count, col_first, col_count, heads, tiled):
     """Items, joins and single rows of one side (the layout of include/ye3t_b200.h)."""
     r0, rn, c0, cn = row_first[tiled], row_count[tiled], col_first[tiled], col_count[tiled]
     tiles = -(-rn // _TILE)
-    # columns are split so that every SM gets several CTAs
+    # columns are split where the tiles alone would not give every SM its two CTAs
     work = int((tiles * np.maximum(cn, 1)).sum()) * heads
-    chunk = max(512, -(-work // (148 * 16)))
+    chunk = max(256, work // (148 * 2))
     parts = np.maximum(1, np.round(cn / chunk).astype(np.int64))
     of = np.repeat(np.arange(rn.size), tiles)  # the structure of each tile
     t = np.arange(of.size) - np.repeat(np.cumsum(tiles) - tiles, tiles)
