@@ -24,6 +24,7 @@ STATUS_TABLE = 4
 STATUS_TIMEOUT = 8
 
 _DTYPE_CODE = {torch.float32: F32, torch.float64: F64, torch.complex64: C64, torch.complex128: C128}
+_LEARNED_CODE = {torch.float32: F32, torch.float64: F64, torch.bfloat16: BF16}
 
 I64 = ctypes.c_int64
 I32 = ctypes.c_int32
@@ -224,7 +225,7 @@ def dtype_code(dtype: torch.dtype) -> int:
 
 def learned_dtype_code(dtype: torch.dtype) -> int:
     """Code of a dtype of the learned operators, which also take bfloat16 but nothing complex."""
-    code = {torch.float32: F32, torch.float64: F64, torch.bfloat16: BF16}.get(dtype)
+    code = _LEARNED_CODE.get(dtype)
     if code is None:
         raise TypeError(f"unsupported dtype {dtype}")
     return code

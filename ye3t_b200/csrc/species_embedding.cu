@@ -3,9 +3,10 @@
 //   out[i, c]   = scale * table[z_i, c]
 //   dtable[v, c] = scale * sum_{i : z_i = v} grad[i, c]
 //
-// The lookup is one pass over the output; the gradient orders the atoms by species
-// (stable radix sort of the indices) and sums runs of equal species, so that no
-// floating-point atomics are needed and results are bitwise repeatable.
+// The lookup is one pass over the output.  The gradient of a small table (a few hundred species) is summed
+// in copies of the table in shared memory; that of a larger one orders the atoms by species (stable
+// radix sort of the indices) and sums runs of equal species.  Neither needs floating-point atomics, and
+// results are bitwise repeatable.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -32,41 +33,162 @@ __device__ __forceinline__ int64_t species_at(const I* z, int64_t i, int64_t V) 
   return s >= 0 && s < V ? s : -1;
 }
 
-// One thread per VEC consecutive channels of one atom; consecutive threads write
-// consecutive addresses.  Bound by the output's store: the table stays in L2.
-template <typename T, typename I, int VEC>
+// A thread writes VEC consecutive channels of kLookups atoms, consecutive threads consecutive addresses.  Bound
+// by the output's store (the table stays in L2); U is 32 bits wide where the element count allows, for the
+// division.
+constexpr int kLookups = 4;
+
+template <typename T, typename I, int VEC, typename U>
 __global__ void __launch_bounds__(256) embedding_kernel(const T* __restrict__ table, int64_t V, int C,
                                                         const I* __restrict__ z, int64_t N,
                                                         typename Acc<T>::type scale, T* __restrict__ out,
                                                         int32_t* status) {
   using P = Pack<T, VEC>;
-  const int per_row = C / VEC;
-  const int64_t total = N * per_row;
-  for (int64_t t = blockIdx.x * int64_t(blockDim.x) + threadIdx.x; t < total; t += int64_t(gridDim.x) * blockDim.x) {
-    const int64_t i = t / per_row;
-    const int p = int(t - i * per_row);
-    const int64_t s = species_at(z, i, V);
-    P r;
-    if (s >= 0) {
-      r = *reinterpret_cast<const P*>(table + s * C + p * VEC);
+  const U per_row = U(C / VEC), total = U(N) * per_row;
+  const U step = U(gridDim.x) * 256;
+  U t = U(blockIdx.x) * 256 + threadIdx.x;
+  P r[kLookups];
+  int64_t s[kLookups];
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) r.v[k] = narrow<T>(scale * widen<T>(r.v[k]));
-    } else {
-      if (status && p == 0) atomicOr(status, Y3B_STATUS_INDEX_RANGE);
+  for (int k = 0; k < kLookups; ++k) {
+    const U u = t + U(k) * step;
+    s[k] = -2;
+    if (u < total) s[k] = species_at(z, int64_t(u / per_row), V);
+  }
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) r.v[k] = narrow<T>(0);
-    }
-    *reinterpret_cast<P*>(out + t * VEC) = r;
+  for (int k = 0; k < kLookups; ++k) {
+    const U p = (t + U(k) * step) % per_row;
+    if (s[k] >= 0) r[k] = *reinterpret_cast<const P*>(table + s[k] * C + int64_t(p) * VEC);
+    if (s[k] == -1 && status && p == 0) atomicOr(status, Y3B_STATUS_INDEX_RANGE);
+  }
+#pragma unroll
+  for (int k = 0; k < kLookups; ++k) {
+    if (s[k] == -2) continue;
+#pragma unroll
+    for (int q = 0; q < VEC; ++q) r[k].v[q] = s[k] >= 0 ? narrow<T>(scale * widen<T>(r[k].v[q])) : narrow<T>(0);
+    *reinterpret_cast<P*>(out + (int64_t(t) + int64_t(k) * step) * VEC) = r[k];
   }
 }
 
 // ---------------------------------------------------------------------------
-// Stable radix sort of (species, atom index), 8 bits a pass.  A tile is 4096 keys:
-// 8 warps of 512, warp w's element e at tile * 4096 + w * 512 + e, so that the order
-// (warp, step, lane) is the order of the keys.
+// Gradient of a small table.  A unit of L lanes has a copy of L * VEC of the table's channels in shared
+// memory (and one row more, for atoms without a species) and adds its rows to it, in order; lanes are
+// channels, so nothing is shared between lanes.  The copies are added in order of the units, and the CTAs' sums
+// (one part each) by part_sum_kernel.  Bound by reading the gradients once: a unit keeps eight rows in flight while
+// it adds the eight before, and adds four at a time (their table rows are loaded together, equal species among
+// them taken from registers).
+constexpr int kTableRows = 8;
+constexpr int kTableThreads = 256;
+
+template <typename T, typename I, int VEC, int L>
+__global__ void __launch_bounds__(kTableThreads) table_sum_kernel(
+    const T* __restrict__ grad, const I* __restrict__ z, int64_t N, int V, int C, int64_t rows_per_unit,
+    typename Acc<T>::type scale, T* __restrict__ dtable, typename Acc<T>::type* __restrict__ part, int32_t* status) {
+  using A = typename Acc<T>::type;
+  using P = Pack<T, VEC>;
+  using PA = Pack<A, VEC>;
+  extern __shared__ __align__(32) unsigned char table_smem[];
+  A* copies = reinterpret_cast<A*>(table_smem);  // [unit][V + 1][L * VEC]
+  constexpr int S = L * VEC, kUnits = kTableThreads / L;
+  const int lane = threadIdx.x % L, unit = threadIdx.x / L;
+  const int copy = (V + 1) * S;
+  for (int u = threadIdx.x; u < kUnits * copy; u += kTableThreads) copies[u] = A(0);
+  __syncthreads();
+  A* mine = copies + unit * copy + lane * VEC;
+  const int c = int(blockIdx.y) * S + lane * VEC;
+  const bool there = c < C;
+  const int64_t b = (blockIdx.x * int64_t(kUnits) + unit) * rows_per_unit;
+  const int64_t e = b + rows_per_unit < N ? b + rows_per_unit : N;
+  const auto species = [&](int64_t r) {  // of the unit's row r + lane, by its first lanes
+    if (lane >= kTableRows || r + lane >= e) return V;
+    const int64_t s = species_at(z, r + lane, V);
+    if (s < 0 && status && blockIdx.y == 0) atomicOr(status, Y3B_STATUS_INDEX_RANGE);
+    return s < 0 ? V : int(s);
+  };
+  const auto fetch = [&](int64_t r, P (&g)[kTableRows]) {
+#pragma unroll
+    for (int j = 0; j < kTableRows; ++j) {
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) g[j].v[q] = narrow<T>(0);
+      if (r + j < e && there) g[j] = *reinterpret_cast<const P*>(grad + (r + j) * C + c);
+    }
+  };
+  const auto add_rows = [&](const P (&g)[kTableRows], int zs) {
+#pragma unroll
+    for (int j = 0; j < kTableRows; j += 4) {
+      int k[4];
+      PA r[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        k[u] = __shfl_sync(0xffffffffu, zs, j + u, L);
+        r[u] = *reinterpret_cast<const PA*>(mine + k[u] * S);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+#pragma unroll
+        for (int w = 0; w < u; ++w)
+          if (k[w] == k[u]) r[u] = r[w];  // the latest of the equal ones stays
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) r[u].v[q] += widen<T>(g[j + u].v[q]);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) *reinterpret_cast<PA*>(mine + k[u] * S) = r[u];
+    }
+  };
+  // every unit takes the same number of steps, so that the shuffles find all lanes
+  P g0[kTableRows], g1[kTableRows];
+  int z0 = species(b), z1;
+  fetch(b, g0);
+  for (int64_t r = 0; r < rows_per_unit; r += 2 * kTableRows) {
+    z1 = species(b + r + kTableRows);
+    fetch(b + r + kTableRows, g1);
+    add_rows(g0, z0);
+    z0 = species(b + r + 2 * kTableRows);
+    fetch(b + r + 2 * kTableRows, g0);
+    add_rows(g1, z1);
+  }
+  __syncthreads();
+  for (int u = threadIdx.x; u < V * S; u += kTableThreads) {
+    const int v = u / S, cc = int(blockIdx.y) * S + u - v * S;
+    if (cc >= C) continue;
+    A sum = copies[u];
+    for (int w = 1; w < kUnits; ++w) sum += copies[w * copy + u];
+    if (part) part[(int64_t(blockIdx.x) * V + v) * C + cc] = sum;
+    else dtable[int64_t(v) * C + cc] = narrow<T>(scale * sum);
+  }
+}
+
+// dtable = scale * the parts' sums: 32 entries a CTA, every 32nd part a warp, the warps in order.
+template <typename T>
+__global__ void __launch_bounds__(1024) part_sum_kernel(const typename Acc<T>::type* __restrict__ part, int64_t parts,
+                                                        int64_t entries, typename Acc<T>::type scale,
+                                                        T* __restrict__ dtable) {
+  using A = typename Acc<T>::type;
+  __shared__ A sums[32][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t u = blockIdx.x * int64_t(32) + lane;
+  A sum = A(0);
+  if (u < entries) {
+#pragma unroll 4
+    for (int64_t p = warp; p < parts; p += 32) sum += part[p * entries + u];
+  }
+  sums[warp][lane] = sum;
+  __syncthreads();
+  if (warp == 0 && u < entries) {
+    A all = sums[0][lane];
+#pragma unroll
+    for (int w = 1; w < 32; ++w) all += sums[w][lane];
+    dtable[u] = narrow<T>(scale * all);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Stable radix sort of (species, atom index), 8 bits a pass.  A tile is 1024 keys: 8 warps of
+// 128, warp w's element e at tile * 1024 + w * 128 + e, so that the order (warp, step, lane) is the
+// order of the keys.
 constexpr int kSortThreads = 256;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortSteps = 16;
+constexpr int kSortSteps = 4;
 constexpr int kSortTile = kSortThreads * kSortSteps;
 
 // The first pass reads the caller's species; an invalid one sorts last, as key V.
@@ -201,13 +323,89 @@ __global__ void __launch_bounds__(kSortThreads) sort_move_kernel(
   }
 }
 
+// The whole sort in one CTA for up to kOneSort atoms, where the launches of a pass would cost more than its work.
+constexpr int kOneSort = 4096;
+constexpr int kOneWarps = 32;
+constexpr int kOneSmem = kOneSort * 8 + kOneWarps * 256 * 2;
+
+template <typename I>
+__global__ void __launch_bounds__(32 * kOneWarps) one_sort_kernel(const I* __restrict__ z, int N, int64_t V, int passes,
+                                                                 uint32_t* __restrict__ keys_out,
+                                                                 uint32_t* __restrict__ values_out, int32_t* status) {
+  extern __shared__ __align__(16) unsigned char sort_smem[];
+  uint32_t* s_key = reinterpret_cast<uint32_t*>(sort_smem);
+  uint32_t* s_val = s_key + kOneSort;
+  uint16_t* place = reinterpret_cast<uint16_t*>(s_val + kOneSort);  // [warp][256]
+  __shared__ uint32_t warp_sums[kOneWarps];
+  constexpr int STEPS = kOneSort / (32 * kOneWarps);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, base = warp * (32 * STEPS) + lane;
+  for (int e = 0; e < STEPS; ++e) {
+    const int i = base + e * 32;
+    if (i < N) {
+      s_key[i] = first_key(z, i, V, status);
+      s_val[i] = uint32_t(i);
+    }
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    for (int u = tid; u < kOneWarps * 256; u += blockDim.x) place[u] = 0;
+    __syncthreads();
+    uint32_t key[STEPS], value[STEPS], rank[STEPS];
+#pragma unroll
+    for (int e = 0; e < STEPS; ++e) {
+      const int i = base + e * 32;
+      const bool there = i < N;
+      key[e] = there ? s_key[i] : 0u;
+      value[e] = there ? s_val[i] : 0u;
+      const uint32_t digit = there ? (key[e] >> (8 * pass)) & 255u : 256u;
+      const uint32_t same = __match_any_sync(0xffffffffu, digit);
+      const int leader = __ffs(int(same)) - 1;
+      uint32_t before = 0;
+      if (lane == leader && there) {
+        before = place[warp * 256 + digit];
+        place[warp * 256 + digit] = uint16_t(before + __popc(same));
+      }
+      before = __shfl_sync(0xffffffffu, before, leader);
+      rank[e] = before + __popc(same & ((1u << lane) - 1u));
+      __syncwarp();
+    }
+    __syncthreads();
+    // exclusive prefix of each digit over the warps, then over the digits
+    uint32_t total = 0;
+    if (tid < 256) {
+      for (int w = 0; w < kOneWarps; ++w) {
+        const uint32_t c = place[w * 256 + tid];
+        place[w * 256 + tid] = uint16_t(total);
+        total += c;
+      }
+    }
+    uint32_t all;
+    const uint32_t start = block_scan(total, warp_sums, &all);
+    if (tid < 256) {
+      for (int w = 0; w < kOneWarps; ++w) place[w * 256 + tid] = uint16_t(place[w * 256 + tid] + start);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < STEPS; ++e) {
+      if (base + e * 32 < N) {
+        const uint32_t to = place[warp * 256 + ((key[e] >> (8 * pass)) & 255u)] + rank[e];
+        s_key[to] = key[e];
+        s_val[to] = value[e];
+      }
+    }
+    __syncthreads();
+  }
+  for (int i = tid; i < N; i += blockDim.x) {
+    keys_out[i] = s_key[i];
+    values_out[i] = s_val[i];
+  }
+}
+
 // ---------------------------------------------------------------------------
-// Sums over runs of equal species.  A warp takes one chunk of the sorted atoms and 32 *
+// Sums over runs of equal species.  A unit of L lanes takes one chunk of the sorted atoms and L *
 // VEC channels.  A run inside the chunk is written to its table row; the part of a run
 // that began in an earlier chunk goes to head[chunk], the part of one that goes on
-// into the next chunk to tail[chunk].  Eight gradient rows are loaded ahead of
-// their sums.
-template <typename T, int VEC>
+// into the next chunk to tail[chunk].  Eight gradient rows load while the eight before are added.
+template <typename T, int VEC, int L>
 __global__ void __launch_bounds__(128) run_sum_kernel(const T* __restrict__ grad, const uint32_t* __restrict__ keys,
                                                       const uint32_t* __restrict__ order, int64_t N, int64_t V,
                                                       int C, int chunk_rows, int64_t chunks,
@@ -217,73 +415,89 @@ __global__ void __launch_bounds__(128) run_sum_kernel(const T* __restrict__ grad
   using A = typename Acc<T>::type;
   using P = Pack<T, VEC>;
   using PA = Pack<A, VEC>;
-  const int lane = threadIdx.x & 31;
-  const int64_t chunk = blockIdx.x * int64_t(4) + (threadIdx.x >> 5);
-  const int c = int(blockIdx.y) * 32 * VEC + lane * VEC;
-  if (chunk >= chunks) return;
-  const bool mine = c < C;
-  const int64_t b = chunk * chunk_rows, e = b + chunk_rows < N ? b + chunk_rows : N;
+  constexpr int kRows = 8;
+  const int lane = threadIdx.x % L;
+  const int64_t chunk = blockIdx.x * int64_t(128 / L) + threadIdx.x / L;
+  const int c = (int(blockIdx.y) * L + lane) * VEC;
+  const bool mine = c < C && chunk < chunks;
+  const int64_t b = chunk * chunk_rows < N ? chunk * chunk_rows : N, e = b + chunk_rows < N ? b + chunk_rows : N;
   const uint32_t none = 0xffffffffu;
-  const uint32_t before = b > 0 ? keys[b - 1] : none, after = e < N ? keys[e] : none;
+  const uint32_t before = b > 0 && b < N ? keys[b - 1] : none, after = e < N ? keys[e] : none;
   A acc[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) acc[k] = A(0);
-  uint32_t current = keys[b];
+  uint32_t current = b < e ? keys[b] : none;
   bool at_begin = true;  // the run holds the chunk's first row
-  auto store = [&](uint32_t key, bool begins, bool ends) {
-    if (!mine || key >= V) return;  // key V: atoms whose species is out of range
-    if (begins && before == key) {
+  auto store = [&](bool ends) {
+    if (!mine || current >= V) return;  // key V: atoms whose species is out of range
+    A* to = at_begin && before == current ? head : ends && after == current ? tail : nullptr;
+    if (to) {
       PA p;
 #pragma unroll
       for (int k = 0; k < VEC; ++k) p.v[k] = acc[k];
-      *reinterpret_cast<PA*>(head + chunk * C + c) = p;
-    } else if (ends && after == key) {
-      PA p;
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) p.v[k] = acc[k];
-      *reinterpret_cast<PA*>(tail + chunk * C + c) = p;
+      *reinterpret_cast<PA*>(to + chunk * C + c) = p;
     } else {
       P p;
 #pragma unroll
       for (int k = 0; k < VEC; ++k) p.v[k] = narrow<T>(scale * acc[k]);
-      *reinterpret_cast<P*>(dtable + int64_t(key) * C + c) = p;
+      *reinterpret_cast<P*>(dtable + int64_t(current) * C + c) = p;
     }
   };
-  for (int64_t r0 = b; r0 < e; r0 += 32) {
-    const int n = e - r0 < 32 ? int(e - r0) : 32;
-    const uint32_t my_key = lane < n ? keys[r0 + lane] : none, my_row = lane < n ? order[r0 + lane] : 0u;
-    for (int j0 = 0; j0 < n; j0 += 8) {
-      P g[8];
+  uint32_t key = none, row = 0u;
+  const auto index = [&](int64_t r) {  // of the unit's row r + lane, by its first lanes
+    const bool ok = lane < kRows && r + lane < e;
+    key = ok ? keys[r + lane] : none;
+    row = ok ? order[r + lane] : 0u;
+  };
+  const auto fetch = [&](P (&g)[kRows]) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t row = __shfl_sync(0xffffffffu, my_row, (j0 + j) & 31);
-        if (j0 + j < n && mine) g[j] = *reinterpret_cast<const P*>(grad + int64_t(row) * C + c);
+    for (int j = 0; j < kRows; ++j) {
+      const uint32_t from = __shfl_sync(0xffffffffu, row, j, L);
+      if (mine) g[j] = *reinterpret_cast<const P*>(grad + int64_t(from) * C + c);  // row 0 past the end
+    }
+  };
+  const auto add_rows = [&](uint32_t keys_of, const P (&g)[kRows]) {
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      const uint32_t k = __shfl_sync(0xffffffffu, keys_of, j, L);
+      if (k == none) continue;  // past the chunk's end
+      if (k != current) {
+        store(false);
+        at_begin = false;
+        current = k;
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) acc[q] = A(0);
       }
+      if (mine) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t key = __shfl_sync(0xffffffffu, my_key, (j0 + j) & 31);
-        if (j0 + j < n) {  // uniform over the warp
-          if (key != current) {
-            store(current, at_begin, false);
-            at_begin = false;
-            current = key;
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) acc[k] = A(0);
-          }
-          if (mine) {
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) acc[k] += widen<T>(g[j].v[k]);
-          }
-        }
+        for (int q = 0; q < VEC; ++q) acc[q] += widen<T>(g[j].v[q]);
       }
     }
+  };
+  // the indices run two steps ahead of the sums, the gradients one
+  P g0[kRows], g1[kRows];
+  index(b);
+  uint32_t k0 = key, k1;
+  fetch(g0);
+  index(b + kRows);
+  for (int r = 0; r < chunk_rows; r += 2 * kRows) {
+    k1 = key;
+    fetch(g1);
+    index(b + r + 2 * kRows);
+    add_rows(k0, g0);
+    k0 = key;
+    fetch(g0);
+    index(b + r + 3 * kRows);
+    add_rows(k1, g1);
   }
-  store(current, at_begin, true);
+  store(true);
 }
 
 // Joins the runs that cross chunks: the chunk in which such a run begins adds its own
-// part and those of the chunks that follow.  Warp w takes every 8th chunk and the
-// warps' sums are added in order; lanes are channels.
+// part and those of the chunks that follow.  A CTA looks at 8 chunks, one after the other; warp w takes
+// every 8th of a run's chunks and the warps' sums are added in order; lanes are channels.
+constexpr int kJoinChunks = 8;
+
 template <typename T>
 __global__ void __launch_bounds__(256) run_join_kernel(const uint32_t* __restrict__ keys, int64_t N, int64_t V, int C,
                                                        int chunk_rows, int64_t chunks, typename Acc<T>::type scale,
@@ -292,48 +506,80 @@ __global__ void __launch_bounds__(256) run_join_kernel(const uint32_t* __restric
                                                        const typename Acc<T>::type* __restrict__ tail) {
   using A = typename Acc<T>::type;
   __shared__ A part[8][32];
-  const int64_t chunk = blockIdx.x;
-  const int64_t e = (chunk + 1) * chunk_rows;
-  if (e >= N) return;  // the last chunk has no run that goes on
-  const uint32_t key = keys[e - 1];
-  if (key >= V || keys[e] != key) return;
-  const int64_t b = chunk * chunk_rows;
-  if (b > 0 && keys[b - 1] == key && keys[b] == key) return;  // the run began earlier
-  // the run's last chunk: chunks whose first key is still this one (keys are sorted)
-  int64_t lo = chunk + 1, hi = chunks;
-  while (hi - lo > 1) {
-    const int64_t mid = (lo + hi) / 2;
-    if (keys[mid * chunk_rows] == key) lo = mid;
-    else hi = mid;
-  }
+  __shared__ uint32_t run_key[kJoinChunks];
+  __shared__ int64_t run_last[kJoinChunks];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int c0 = int(blockIdx.y) * 32; c0 < C; c0 += int(gridDim.y) * 32) {
-    const int c = c0 + lane;
-    A sum = A(0);
-    if (c < C) {
-      int64_t q = chunk + 1 + warp;
-      for (; q + 24 <= lo; q += 32) {
-        const A a0 = head[q * C + c], a1 = head[(q + 8) * C + c];
-        const A a2 = head[(q + 16) * C + c], a3 = head[(q + 24) * C + c];
-        sum += (a0 + a1) + (a2 + a3);
+  // each warp looks at one chunk: does a run begin in it and go on, and up to which chunk?
+  {
+    const int64_t chunk = blockIdx.x * int64_t(kJoinChunks) + warp, b = chunk * chunk_rows, e = b + chunk_rows;
+    uint32_t key = 0xffffffffu;
+    int64_t lo = chunk;
+    if (e < N) {
+      key = keys[e - 1];
+      const bool earlier = b > 0 && keys[b - 1] == key && keys[b] == key;
+      if (key >= V || keys[e] != key || earlier) key = 0xffffffffu;
+    }
+    if (key != 0xffffffffu) {
+      // keys are sorted: the last chunk whose first key is still this one, by 32 probes a round
+      lo = chunk + 1;
+      int64_t hi = chunks;  // first chunk known to begin with another key
+      while (hi - lo > 1) {
+        const int64_t step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step;
+        const bool same = at < hi && keys[at * chunk_rows] == key;
+        const int n = __popc(__ballot_sync(0xffffffffu, same));
+        const int64_t up = lo + int64_t(n + 1) * step;
+        lo += n * step;
+        hi = up < hi ? up : hi;
       }
-      for (; q <= lo; q += 8) sum += head[q * C + c];
     }
-    part[warp][lane] = sum;
-    __syncthreads();
-    if (warp == 0 && c < C) {
-      A all = tail[chunk * C + c];
+    // a short run is the warp's own work, a long one the CTA's
+    const bool brief = key != 0xffffffffu && lo - chunk <= 16;
+    if (brief) {
+      for (int c = int(blockIdx.y) * 32 + lane; c < C; c += int(gridDim.y) * 32) {
+        A sum = tail[chunk * C + c];
+#pragma unroll 4
+        for (int64_t q = chunk + 1; q <= lo; ++q) sum += head[q * C + c];
+        dtable[int64_t(key) * C + c] = narrow<T>(scale * sum);
+      }
+    }
+    if (lane == 0) {
+      run_key[warp] = brief ? 0xffffffffu : key;
+      run_last[warp] = lo;
+    }
+  }
+  __syncthreads();
+  for (int k = 0; k < kJoinChunks; ++k) {
+    const uint32_t key = run_key[k];
+    if (key == 0xffffffffu) continue;
+    const int64_t chunk = blockIdx.x * int64_t(kJoinChunks) + k, last = run_last[k];
+    for (int c0 = int(blockIdx.y) * 32; c0 < C; c0 += int(gridDim.y) * 32) {
+      const int c = c0 + lane;
+      A sum = A(0);
+      if (c < C) {
+#pragma unroll 4
+        for (int64_t q = chunk + 1 + warp; q <= last; q += 8) sum += head[q * C + c];
+      }
+      part[warp][lane] = sum;
+      __syncthreads();
+      if (warp == 0 && c < C) {
+        A all = tail[chunk * C + c];
 #pragma unroll
-      for (int w = 0; w < 8; ++w) all += part[w][lane];
-      dtable[int64_t(key) * C + c] = narrow<T>(scale * all);
+        for (int w = 0; w < 8; ++w) all += part[w][lane];
+        dtable[int64_t(key) * C + c] = narrow<T>(scale * all);
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
 }
 
-// Workspace: two pairs of (key, index) arrays, the tiles' digit counts, the digits'
-// totals and the chunks' head and tail sums; every part 32-byte aligned.
+// How the gradient of one call is formed.  A table is small where an SM holds a copy of lanes * vec of its
+// channels for each unit of two CTAs (26 species in fp32): fewer warps do not keep the memory busy.
+// Workspace: the parts of the small path; of the other two pairs of (key, index) arrays, the
+// tiles' digit counts, the digits' totals and the chunks' head and tail sums; 32-byte aligned.
 struct AdjointPlan {
+  bool small;
+  int vec, lanes;  // of the small path
+  int64_t parts, rows_per_unit;
   int64_t tiles, chunks;
   int chunk_rows, passes;
   int64_t keys[2], order[2], hist, totals, head, tail, bytes;
@@ -341,26 +587,46 @@ struct AdjointPlan {
 
 int64_t align32(int64_t v) { return (v + 31) / 32 * 32; }
 
+// Lanes of a unit: the fewest of 8, 16 and 32 that hold C channels by VEC.
+int unit_lanes(int64_t C, int vec) { return C <= 8 * vec ? 8 : C <= 16 * vec ? 16 : 32; }
+
 AdjointPlan adjoint_plan(int dtype, int64_t N, int64_t V, int64_t C) {
-  AdjointPlan p;
-  p.tiles = (N + kSortTile - 1) / kSortTile;
-  p.chunk_rows = N < (int64_t(1) << 18) ? 32 : 128;
-  p.chunks = (N + p.chunk_rows - 1) / p.chunk_rows;
-  p.passes = 1;
-  while (p.passes < 4 && (V >> (8 * p.passes)) != 0) ++p.passes;
+  AdjointPlan p{};
+  const int64_t real = dtype == Y3B_F64 ? 8 : 4;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t here = at;
     at += align32(bytes);
     return here;
   };
+  // an odd number of bf16 channels has no aligned pairs
+  const int wide = dtype == Y3B_F64 ? 2 : 4;
+  p.vec = C % wide == 0 ? wide : 1;
+  p.lanes = unit_lanes(C, p.vec);
+  const int64_t units = kTableThreads / p.lanes, copies = units * (V + 1) * p.lanes * p.vec * real;
+  p.small = 2 * (copies + 1024) <= 220 * 1024;
+  if (p.small) {
+    const int64_t slabs = (C + p.lanes * p.vec - 1) / (p.lanes * p.vec);
+    const int64_t per_sm = std::min<int64_t>(2048 / kTableThreads, 220 * 1024 / (copies + 1024));
+    const int64_t most = std::max<int64_t>(1, kSMs * per_sm / slabs);
+    // at least 64 rows a unit: fewer do not pay for another part
+    p.parts = std::min(most, std::max<int64_t>(1, (N + units * 64 - 1) / (units * 64)));
+    p.rows_per_unit = (N + p.parts * units - 1) / (p.parts * units);
+    p.head = take(p.parts > 1 ? p.parts * V * C * real : 0);
+    p.bytes = at;
+    return p;
+  }
+  p.tiles = (N + kSortTile - 1) / kSortTile;
+  p.chunk_rows = N < (int64_t(1) << 18) ? 32 : 128;
+  p.chunks = (N + p.chunk_rows - 1) / p.chunk_rows;
+  p.passes = 1;
+  while (p.passes < 4 && (V >> (8 * p.passes)) != 0) ++p.passes;
   for (int k = 0; k < 2; ++k) {
     p.keys[k] = take(N * 4);
     p.order[k] = take(N * 4);
   }
   p.hist = take(256 * p.tiles * 4);
   p.totals = take(256 * 4);
-  const int64_t real = dtype == Y3B_F64 ? 8 : 4;
   p.head = take(p.chunks * C * real);
   p.tail = take(p.chunks * C * real);
   p.bytes = at;
@@ -371,16 +637,36 @@ bool embedding_dtype(int dtype) { return dtype == Y3B_F32 || dtype == Y3B_F64 ||
 
 bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
-template <typename T, typename I>
+template <typename T, typename I, int VEC>
 int lookup(const T* table, int64_t V, int C, const I* z, int64_t N, double scale, T* out, int32_t* status,
            cudaStream_t s) {
   using A = typename Acc<T>::type;
+  const int64_t total = N * (C / VEC), ctas = (total + 256 * kLookups - 1) / (256 * kLookups);
+  if (ctas > INT32_MAX) return fail(Y3B_ERR_UNSUPPORTED, "species_embedding: %lld values", (long long)(N * C));
+  // past 2^31 - (the grid's reach) elements the index needs 64 bits
+  if (total < (int64_t(1) << 31))
+    embedding_kernel<T, I, VEC, uint32_t><<<unsigned(ctas), 256, 0, s>>>(table, V, C, z, N, A(scale), out, status);
+  else
+    embedding_kernel<T, I, VEC, uint64_t><<<unsigned(ctas), 256, 0, s>>>(table, V, C, z, N, A(scale), out, status);
+  Y3B_LAUNCH_CHECK();
+  return Y3B_OK;
+}
+
+template <typename T, typename I>
+int lookup(const T* table, int64_t V, int C, const I* z, int64_t N, double scale, T* out, int32_t* status,
+           cudaStream_t s) {
   constexpr int W = 16 / int(sizeof(T));
-  if (C % W == 0 && aligned(table, 16) && aligned(out, 16)) {
-    embedding_kernel<T, I, W><<<grid_for(N * (C / W), 256), 256, 0, s>>>(table, V, C, z, N, A(scale), out, status);
-  } else {
-    embedding_kernel<T, I, 1><<<grid_for(N * C, 256), 256, 0, s>>>(table, V, C, z, N, A(scale), out, status);
-  }
+  if (C % W == 0 && aligned(table, 16) && aligned(out, 16)) return lookup<T, I, W>(table, V, C, z, N, scale, out, status, s);
+  return lookup<T, I, 1>(table, V, C, z, N, scale, out, status, s);
+}
+
+template <typename T, int VEC, int L>
+int run_sums(const T* grad, const AdjointPlan& p, const uint32_t* keys, const uint32_t* order, int64_t N, int64_t V,
+             int C, double scale, T* dtable, void* head, void* tail, cudaStream_t s) {
+  using A = typename Acc<T>::type;
+  const dim3 grid(unsigned((p.chunks * L + 127) / 128), unsigned((C + L * VEC - 1) / (L * VEC)));
+  run_sum_kernel<T, VEC, L><<<grid, 128, 0, s>>>(grad, keys, order, N, V, C, p.chunk_rows, p.chunks, A(scale), dtable,
+                                                 static_cast<A*>(head), static_cast<A*>(tail));
   Y3B_LAUNCH_CHECK();
   return Y3B_OK;
 }
@@ -388,12 +674,44 @@ int lookup(const T* table, int64_t V, int C, const I* z, int64_t N, double scale
 template <typename T, int VEC>
 int run_sums(const T* grad, const AdjointPlan& p, const uint32_t* keys, const uint32_t* order, int64_t N, int64_t V,
              int C, double scale, T* dtable, void* head, void* tail, cudaStream_t s) {
+  const int lanes = unit_lanes(C, VEC);
+  if (lanes == 8) return run_sums<T, VEC, 8>(grad, p, keys, order, N, V, C, scale, dtable, head, tail, s);
+  if (lanes == 16) return run_sums<T, VEC, 16>(grad, p, keys, order, N, V, C, scale, dtable, head, tail, s);
+  return run_sums<T, VEC, 32>(grad, p, keys, order, N, V, C, scale, dtable, head, tail, s);
+}
+
+template <typename T, typename I, int VEC, int L>
+int table_sums(const AdjointPlan& p, const T* grad, const I* z, int64_t N, int64_t V, int C, double scale,
+               unsigned char* ws, T* dtable, int32_t* status, cudaStream_t s) {
   using A = typename Acc<T>::type;
-  const dim3 grid(unsigned((p.chunks + 3) / 4), unsigned((C + 32 * VEC - 1) / (32 * VEC)));
-  run_sum_kernel<T, VEC><<<grid, 128, 0, s>>>(grad, keys, order, N, V, C, p.chunk_rows, p.chunks, A(scale), dtable,
-                                              static_cast<A*>(head), static_cast<A*>(tail));
+  const auto kernel = table_sum_kernel<T, I, VEC, L>;
+  const int smem = int(kTableThreads * (V + 1) * VEC * int64_t(sizeof(A))), slabs = (C + L * VEC - 1) / (L * VEC);
+  Y3B_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  A* part = p.parts > 1 ? reinterpret_cast<A*>(ws + p.head) : nullptr;
+  kernel<<<dim3(unsigned(p.parts), unsigned(slabs)), kTableThreads, smem, s>>>(grad, z, N, int(V), C, p.rows_per_unit,
+                                                                              A(scale), dtable, part, status);
   Y3B_LAUNCH_CHECK();
+  if (part) {
+    part_sum_kernel<T><<<unsigned((V * C + 31) / 32), 1024, 0, s>>>(part, p.parts, V * C, A(scale), dtable);
+    Y3B_LAUNCH_CHECK();
+  }
   return Y3B_OK;
+}
+
+// The lanes follow from the plan's; a gradient off the vectors' alignment is read value by value by as many
+// lanes, in more slabs.
+template <typename T, typename I>
+int table_sums(const AdjointPlan& p, const T* grad, const I* z, int64_t N, int64_t V, int C, double scale,
+               unsigned char* ws, T* dtable, int32_t* status, cudaStream_t s) {
+  constexpr int W = sizeof(T) == 8 ? 2 : 4;
+  const bool wide = p.vec == W && aligned(grad, sizeof(T) * W);
+#define Y3B_TABLE(L)                                                                              \
+  return wide ? table_sums<T, I, W, L>(p, grad, z, N, V, C, scale, ws, dtable, status, s)         \
+              : table_sums<T, I, 1, L>(p, grad, z, N, V, C, scale, ws, dtable, status, s)
+  if (p.lanes == 8) { Y3B_TABLE(8); }
+  if (p.lanes == 16) { Y3B_TABLE(16); }
+  Y3B_TABLE(32);
+#undef Y3B_TABLE
 }
 
 template <typename T, typename I>
@@ -401,10 +719,20 @@ int adjoint(int dtype, const T* grad, const I* z, int64_t N, int64_t V, int C, d
             T* dtable, int32_t* status, cudaStream_t s) {
   using A = typename Acc<T>::type;
   const AdjointPlan p = adjoint_plan(dtype, N, V, C);
+  if (p.small) return table_sums<T, I>(p, grad, z, N, V, C, scale, ws, dtable, status, s);
   uint32_t* hist = reinterpret_cast<uint32_t*>(ws + p.hist);
   uint32_t* totals = reinterpret_cast<uint32_t*>(ws + p.totals);
   const unsigned tiles = unsigned(p.tiles);
-  for (int pass = 0; pass < p.passes; ++pass) {
+  const bool one = N <= kOneSort;
+  if (one) {
+    Y3B_CUDA_TRY(cudaFuncSetAttribute(one_sort_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, kOneSmem));
+    const int to = (p.passes - 1) & 1;
+    one_sort_kernel<I><<<1, 32 * kOneWarps, kOneSmem, s>>>(z, int(N), V, p.passes,
+                                                           reinterpret_cast<uint32_t*>(ws + p.keys[to]),
+                                                           reinterpret_cast<uint32_t*>(ws + p.order[to]), status);
+    Y3B_LAUNCH_CHECK();
+  }
+  for (int pass = 0; !one && pass < p.passes; ++pass) {
     const uint32_t* ki = reinterpret_cast<const uint32_t*>(ws + p.keys[(pass + 1) & 1]);
     const uint32_t* vi = reinterpret_cast<const uint32_t*>(ws + p.order[(pass + 1) & 1]);
     uint32_t* ko = reinterpret_cast<uint32_t*>(ws + p.keys[pass & 1]);
@@ -425,17 +753,13 @@ int adjoint(int dtype, const T* grad, const I* z, int64_t N, int64_t V, int C, d
   const uint32_t* keys = reinterpret_cast<const uint32_t*>(ws + p.keys[(p.passes - 1) & 1]);
   const uint32_t* order = reinterpret_cast<const uint32_t*>(ws + p.order[(p.passes - 1) & 1]);
   Y3B_CUDA_TRY(cudaMemsetAsync(dtable, 0, size_t(V) * C * sizeof(T), s));
-  // the widest load that still gives most lanes a channel
-  constexpr int W = 16 / int(sizeof(T));
-  int rc;
-  if (C >= 16 * W && C % W == 0 && aligned(grad, 16) && aligned(dtable, 16))
-    rc = run_sums<T, W>(grad, p, keys, order, N, V, C, scale, dtable, ws + p.head, ws + p.tail, s);
-  else if (C >= 48 && C % 2 == 0 && aligned(grad, 2 * sizeof(T)) && aligned(dtable, 2 * sizeof(T)))
-    rc = run_sums<T, 2>(grad, p, keys, order, N, V, C, scale, dtable, ws + p.head, ws + p.tail, s);
-  else
-    rc = run_sums<T, 1>(grad, p, keys, order, N, V, C, scale, dtable, ws + p.head, ws + p.tail, s);
+  constexpr int W = sizeof(T) == 8 ? 2 : 4;
+  const bool wide = C % W == 0 && aligned(grad, W * sizeof(T)) && aligned(dtable, W * sizeof(T));
+  const int rc = wide ? run_sums<T, W>(grad, p, keys, order, N, V, C, scale, dtable, ws + p.head, ws + p.tail, s)
+                      : run_sums<T, 1>(grad, p, keys, order, N, V, C, scale, dtable, ws + p.head, ws + p.tail, s);
   if (rc) return rc;
-  const dim3 grid(unsigned(p.chunks), unsigned(std::min((C + 31) / 32, 64)));
+  if (p.chunks == 1) return Y3B_OK;
+  const dim3 grid(unsigned((p.chunks + kJoinChunks - 1) / kJoinChunks), unsigned(std::min((C + 31) / 32, 64)));
   run_join_kernel<T><<<grid, 256, 0, s>>>(keys, N, V, C, p.chunk_rows, p.chunks, A(scale), dtable,
                                           reinterpret_cast<const A*>(ws + p.head),
                                           reinterpret_cast<const A*>(ws + p.tail));

@@ -532,21 +532,25 @@ def pace_radial_channel_contraction_with_derivative(values, derivatives, coeffic
 
 
 # -- learned per-atom operators ----------------------------------------------------------------
+def _raw_stream(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def _embedding_forward(table, species, scale, validate):
-    dev = nat.require_cuda(table, species, what="species_embedding")
+    dev = table.device
     t, z = table.contiguous(), species.contiguous()
-    out = torch.empty(tuple(species.shape) + (t.shape[1],), dtype=t.dtype, device=dev)
+    out = torch.empty(z.shape + (t.shape[1],), dtype=t.dtype, device=dev)
     status = _status(dev) if validate else None
     nat.check(nat.lib().y3b_species_embedding(nat.learned_dtype_code(t.dtype), t.data_ptr(), t.shape[0], t.shape[1],
                                               z.data_ptr(), z.element_size(), z.numel(), scale, out.data_ptr(),
-                                              nat.ptr(status), nat.stream_of(dev)), "species_embedding")
+                                              nat.ptr(status), _raw_stream(dev)), "species_embedding")
     if validate:
         _raise_on_status(status, "species_embedding")
     return out
 
 
 def _embedding_adjoint(grad, species, species_count, scale):
-    dev = nat.require_cuda(grad, species, what="species_embedding adjoint")
+    dev = grad.device
     g, z = grad.contiguous(), species.contiguous()
     C = g.shape[-1]
     code = nat.learned_dtype_code(g.dtype)
@@ -558,7 +562,7 @@ def _embedding_adjoint(grad, species, species_count, scale):
     ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=dev)
     nat.check(lib.y3b_species_embedding_adjoint(code, g.data_ptr(), z.data_ptr(), z.element_size(), z.numel(),
                                                 species_count, C, scale, ws.data_ptr(), ws_bytes, out.data_ptr(), 0,
-                                                nat.stream_of(dev)), "species_embedding adjoint")
+                                                _raw_stream(dev)), "species_embedding adjoint")
     return out
 
 
@@ -588,8 +592,10 @@ def species_embedding(table, species, *, scale=1.0, backend="auto", validate=Non
     in a fixed order, so the gradient is bitwise repeatable.
     """
     _check_backend(backend)
-    table = torch.as_tensor(table)
-    species = torch.as_tensor(species, device=table.device)
+    if not isinstance(table, torch.Tensor):
+        table = torch.as_tensor(table)
+    if not isinstance(species, torch.Tensor):
+        species = torch.as_tensor(species, device=table.device)
     nat.require_cuda(table, species, what="species_embedding")
     nat.learned_dtype_code(table.dtype)
     if table.ndim != 2 or table.shape[1] < 1:
