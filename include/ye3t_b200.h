@@ -667,13 +667,17 @@ typedef struct {
   const int32_t* key_offsets;     /* [structure_count + 1] */
   const int32_t* query_structure; /* [query_count], in [0, structure_count) */
   const int32_t* key_structure;   /* [key_count], in [0, structure_count) */
-  /* Work tables.  Every query is in query_rows (one warp computes it) or in exactly one tile
-   * of up to 128 queries of one structure; a tile is one item, or several items with consecutive slots
-   * that split its keys and one join.  Keys likewise, with queries as the columns.
+  /* Work tables.  A structure of up to 64 queries and 64 keys is in small (those of up to 32 of each first).
+   * Every query of the others is in query_rows (one warp computes it) or in exactly one tile of up to 128 queries
+   * of one structure; a tile is one item, or several items with consecutive slots that split its keys and
+   * one join.  Keys likewise, with queries as the columns.
+   *   small (first query, queries, first key, keys)
    *   item  (first row, rows, first column, columns, slot or -1, 0, 0, 0)
    *   join  (first row, rows, first slot, slots) */
+  int64_t small_32_count, small_64_count;
   int64_t query_item_count, query_join_count, query_slot_count, query_row_count;
   int64_t key_item_count, key_join_count, key_slot_count, key_row_count;
+  const int32_t* small;       /* 16-byte aligned */
   const int32_t* query_items; /* 32-byte aligned */
   const int32_t* query_joins; /* 16-byte aligned */
   const int32_t* query_rows;

@@ -103,9 +103,10 @@ class StructureAttentionArgs(ctypes.Structure):
         ("value_row_stride", I64), ("value_head_stride", I64),
         ("positions", VP), ("key_positions", VP), ("slopes", VP),
         ("query_offsets", VP), ("key_offsets", VP), ("query_structure", VP), ("key_structure", VP),
+        ("small_32_count", I64), ("small_64_count", I64),
         ("query_item_count", I64), ("query_join_count", I64), ("query_slot_count", I64), ("query_row_count", I64),
         ("key_item_count", I64), ("key_join_count", I64), ("key_slot_count", I64), ("key_row_count", I64),
-        ("query_items", VP), ("query_joins", VP), ("query_rows", VP), ("key_items", VP), ("key_joins", VP),
+        ("small", VP), ("query_items", VP), ("query_joins", VP), ("query_rows", VP), ("key_items", VP), ("key_joins", VP),
         ("key_rows", VP), ("scale", ctypes.c_float),
     ]
 

@@ -16,6 +16,7 @@
 // then the D components for the sums.
 #include <algorithm>
 
+#include "structure_attention_small.cuh"
 #include "structure_attention_tile.cuh"
 
 namespace y3b {
@@ -373,6 +374,9 @@ int unpack(const y3b_structure_attention_args* p, const char* what, AttArgs* a) 
     Y3B_CHECK_ARG(p->query_count == 0 || p->positions, "%s: slopes without positions", what);
     Y3B_CHECK_ARG(p->key_count == 0 || p->key_positions, "%s: slopes without key positions", what);
   }
+  Y3B_CHECK_ARG(p->small_32_count >= 0 && p->small_64_count >= 0 &&
+                    (p->small_32_count + p->small_64_count == 0 || p->small),
+                "%s: bad table of small structures", what);
   Y3B_CHECK_ARG(p->query_item_count >= 0 && p->query_join_count >= 0 && p->query_slot_count >= 0 &&
                     p->query_row_count >= 0 && p->key_item_count >= 0 && p->key_join_count >= 0 &&
                     p->key_slot_count >= 0 && p->key_row_count >= 0,
@@ -662,6 +666,11 @@ AttTileArgs tile_args(const y3b_structure_attention_args* p, const AttArgs& a, c
 template <typename T>
 int forward(const y3b_structure_attention_args* p, const AttArgs& a, const AttPlan& w, unsigned char* ws, void* out,
             float* lse, int32_t* status, cudaStream_t s) {
+  if (p->small_32_count + p->small_64_count > 0) {
+    const int rc = attention_small_forward<T>(a, reinterpret_cast<const AttSmall*>(p->small), p->small_32_count,
+                                              p->small_64_count, static_cast<T*>(out), s);
+    if (rc) return rc;
+  }
   if (p->query_row_count > 0) {
     row_forward_kernel<T><<<row_grid(p->query_row_count * a.H), 32 * kRowWarps, 0, s>>>(
         a, p->query_rows, p->query_row_count, static_cast<T*>(out), lse);
@@ -704,6 +713,12 @@ int backward(const y3b_structure_attention_args* p, const AttArgs& a, const AttP
   t.lse = const_cast<float*>(lse);
   t.delta = delta;
   t.slope_part = slope_part;
+  if (p->small_32_count + p->small_64_count > 0) {
+    const int rc = attention_small_backward<T>(a, reinterpret_cast<const AttSmall*>(p->small), p->small_32_count,
+                                               p->small_64_count, g, static_cast<T*>(dq), static_cast<T*>(dk),
+                                               static_cast<T*>(dv), slope_part, dx_part, dy_part, s);
+    if (rc) return rc;
+  }
   // query side: it also gives delta, which the key side reads
   if (p->query_row_count > 0) {
     row_backward_query_kernel<T><<<row_grid(p->query_row_count * a.H), 32 * kRowWarps, 0, s>>>(

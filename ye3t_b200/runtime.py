@@ -623,10 +623,10 @@ def _host_counts(counts, what):
 
 
 _TILE = 128       # rows of a tile
-_TILE_ROWS = 1    # structures with fewer rows are computed row by row
+_SMALL = 64       # structures of up to so many queries and keys take the small-structure kernels
 
 
-def _work_tables(row_first, row_count, col_first, col_count, heads, tiled):
+def _work_tables(row_first, row_count, col_first, col_count, heads, tiled, by_row):
     """Items, joins and single rows of one side (the layout of include/ye3t_b200.h)."""
     r0, rn, c0, cn = row_first[tiled], row_count[tiled], col_first[tiled], col_count[tiled]
     tiles = -(-rn // _TILE)
@@ -652,7 +652,7 @@ def _work_tables(row_first, row_count, col_first, col_count, heads, tiled):
     items = items[np.argsort(-items[:, 3], kind="stable")]
     split = p > 1
     joins = np.stack([row, rows, slot, p], 1)[split]
-    single = np.flatnonzero(~tiled)
+    single = np.flatnonzero(by_row)
     rest = np.repeat(row_first[single] - (np.cumsum(row_count[single]) - row_count[single]), row_count[single])
     rest = rest + np.arange(rest.size)
     return {"items": items, "joins": joins, "rows": rest, "item_count": len(items), "join_count": len(joins),
@@ -687,13 +687,22 @@ class StructureLayout:
             self.device = torch.device("cuda", torch.cuda.current_device())
         number = np.arange(self.structure_count)
         q_first, k_first = np.cumsum(queries) - queries, np.cumsum(keys) - keys
+        small = (queries <= _SMALL) & (keys <= _SMALL)
+        # beside larger structures, a launch of their own has to fill the SMs
+        if not small.all() and int(small.sum()) * self.key_heads < 2 * 148:
+            small &= queries + keys < 0
+        tiny = small & (queries <= _SMALL // 2) & (keys <= _SMALL // 2)
+        order = np.concatenate([np.flatnonzero(tiny & (queries + keys > 0)), np.flatnonzero(small & ~tiny)])
+        structures = np.stack([q_first, queries, k_first, keys], 1)[order]
         # a single key has all the weight and no gradient through the softmax: the row kernels give exactly that
-        q_side = _work_tables(q_first, queries, k_first, keys, self.heads, (queries >= _TILE_ROWS) & (keys > 1))
-        k_side = _work_tables(k_first, keys, q_first, queries, self.key_heads, (keys >= _TILE_ROWS) & (keys > 1))
+        q_side = _work_tables(q_first, queries, k_first, keys, self.heads, ~small & (keys > 1), ~small & (keys <= 1))
+        k_side = _work_tables(k_first, keys, q_first, queries, self.key_heads, ~small & (keys > 1),
+                              ~small & (keys <= 1))
+        self._small_counts = int((tiny & (queries + keys > 0)).sum()), int((small & ~tiny).sum())
         self._counts = tuple(int(side[name]) for side in (q_side, k_side) for name in
                              ("item_count", "join_count", "slot_count", "row_count"))
-        # items and joins first: they are read as 32- and 16-byte records
-        tables = [q_side["items"], k_side["items"], q_side["joins"], k_side["joins"], q_side["rows"], k_side["rows"],
+        # items, then joins and structures: they are read as 32- and 16-byte records
+        tables = [q_side["items"], k_side["items"], q_side["joins"], k_side["joins"], structures, q_side["rows"], k_side["rows"],
                   np.concatenate([[0], np.cumsum(queries)]), np.concatenate([[0], np.cumsum(keys)]),
                   np.repeat(number, queries), np.repeat(number, keys)]
         # one copy to the device; it is complete when the constructor returns, so any stream may use it
@@ -701,8 +710,8 @@ class StructureLayout:
         self._stream = nat.stream_of(self.device)
         self._packed = packed
         first = np.cumsum([0] + [t.size for t in tables[:-1]]) * 4
-        (self._query_items, self._key_items, self._query_joins, self._key_joins, self._query_rows, self._key_rows,
-         self._query_offsets, self._key_offsets, self._query_structure, self._key_structure) = [
+        (self._query_items, self._key_items, self._query_joins, self._key_joins, self._small, self._query_rows,
+         self._key_rows, self._query_offsets, self._key_offsets, self._query_structure, self._key_structure) = [
             packed.data_ptr() + int(o) for o in first]
 
     def _use(self):
@@ -725,6 +734,7 @@ def _attention_args(query, key, value, x, y, slopes, layout, scale):
     a.query_structure, a.key_structure = layout._query_structure, layout._key_structure
     (a.query_item_count, a.query_join_count, a.query_slot_count, a.query_row_count,
      a.key_item_count, a.key_join_count, a.key_slot_count, a.key_row_count) = layout._counts
+    (a.small_32_count, a.small_64_count), a.small = layout._small_counts, layout._small
     a.query_items, a.query_joins, a.query_rows = layout._query_items, layout._query_joins, layout._query_rows
     a.key_items, a.key_joins, a.key_rows = layout._key_items, layout._key_joins, layout._key_rows
     a.scale = scale
