@@ -645,7 +645,7 @@ int y3b_species_embedding_adjoint(int dtype, const void* grad, const void* speci
  * keys gives zeros.  The last dimension is dense; rows and heads have strides in elements.
  * positions [query_count, 3], key_positions [key_count, 3] and slopes [heads] are fp32 and null
  * together.  Structure s holds queries query_offsets[s] .. query_offsets[s + 1] and keys
- * key_offsets[s] .. key_offsets[s + 1]; *_structure names each row's structure. */
+ * key_offsets[s] .. key_offsets[s + 1]. */
 typedef struct {
   int32_t dtype; /* Y3B_F32 or Y3B_BF16 */
   int32_t heads;
@@ -663,14 +663,13 @@ typedef struct {
   const float* positions;
   const float* key_positions;
   const float* slopes;
-  const int32_t* query_offsets;   /* [structure_count + 1] */
-  const int32_t* key_offsets;     /* [structure_count + 1] */
-  const int32_t* query_structure; /* [query_count], in [0, structure_count) */
-  const int32_t* key_structure;   /* [key_count], in [0, structure_count) */
+  const int32_t* query_offsets; /* [structure_count + 1] */
+  const int32_t* key_offsets;   /* [structure_count + 1] */
   /* Work tables.  A structure of up to 64 queries and 64 keys is in small (those of up to 32 of each first).
    * Every query of the others is in query_rows (one warp computes it) or in exactly one tile of up to 128 queries
    * of one structure; a tile is one item, or several items with consecutive slots that split its keys and
    * one join.  Keys likewise, with queries as the columns.
+   *   row   (query or key, its structure)
    *   small (first query, queries, first key, keys)
    *   item  (first row, rows, first column, columns, slot or -1, 0, 0, 0)
    *   join  (first row, rows, first slot, slots) */

@@ -102,7 +102,7 @@ class StructureAttentionArgs(ctypes.Structure):
         ("query_row_stride", I64), ("query_head_stride", I64), ("key_row_stride", I64), ("key_head_stride", I64),
         ("value_row_stride", I64), ("value_head_stride", I64),
         ("positions", VP), ("key_positions", VP), ("slopes", VP),
-        ("query_offsets", VP), ("key_offsets", VP), ("query_structure", VP), ("key_structure", VP),
+        ("query_offsets", VP), ("key_offsets", VP),
         ("small_32_count", I64), ("small_64_count", I64),
         ("query_item_count", I64), ("query_join_count", I64), ("query_slot_count", I64), ("query_row_count", I64),
         ("key_item_count", I64), ("key_join_count", I64), ("key_slot_count", I64), ("key_row_count", I64),

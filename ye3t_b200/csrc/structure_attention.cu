@@ -29,19 +29,11 @@ struct Range {
   int64_t b, e;
 };
 
-__device__ __forceinline__ Range keys_of(const AttArgs& a, int64_t i) {
-  const int s = a.q_struct[i];
-  Range r{a.k_off[s], a.k_off[s + 1]};
+// Rows of a structure, within the array whatever the offsets hold.
+__device__ __forceinline__ Range rows_of(const int32_t* off, int structure, int64_t n) {
+  Range r{off[structure], off[structure + 1]};
   if (r.b < 0) r.b = 0;
-  if (r.e > a.nk) r.e = a.nk;
-  return r;
-}
-
-__device__ __forceinline__ Range queries_of(const AttArgs& a, int64_t j) {
-  const int s = a.k_struct[j];
-  Range r{a.q_off[s], a.q_off[s + 1]};
-  if (r.b < 0) r.b = 0;
-  if (r.e > a.nq) r.e = a.nq;
+  if (r.e > n) r.e = n;
   return r;
 }
 
@@ -66,7 +58,7 @@ __device__ __forceinline__ Apart apart(float ax, float ay, float az, const float
 }
 
 template <typename T>
-__global__ void __launch_bounds__(32 * kRowWarps) row_forward_kernel(AttArgs a, const int32_t* __restrict__ rows,
+__global__ void __launch_bounds__(32 * kRowWarps) row_forward_kernel(AttArgs a, const int2* __restrict__ rows,
                                                                      int64_t row_count, T* __restrict__ out,
                                                                      float* __restrict__ lse) {
   __shared__ float s_q[kRowWarps][kAttMaxWidth];
@@ -74,7 +66,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) row_forward_kernel(AttArgs a, 
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t task = blockIdx.x * int64_t(kRowWarps) + w;
   if (task >= row_count * a.H) return;
-  const int64_t i = rows[task / a.H];
+  const int2 of = rows[task / a.H];  // (row, structure)
+  const int64_t i = of.x;
   const int h = int(task % a.H), hk = h / a.group;
   const T* q = static_cast<const T*>(a.q) + i * a.q_row + h * a.q_head;
   const T* k = static_cast<const T*>(a.k) + hk * a.k_head;
@@ -88,7 +81,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) row_forward_kernel(AttArgs a, 
     pz = a.x[3 * i + 2];
   }
   __syncwarp();
-  const Range r = keys_of(a, i);
+  const Range r = rows_of(a.k_off, of.y, a.nk);
   float m = -INFINITY, l = 0.0f, acc[kRowAcc];
 #pragma unroll
   for (int t = 0; t < kRowAcc; ++t) acc[t] = 0.0f;
@@ -133,7 +126,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) row_forward_kernel(AttArgs a, 
 // Query side of the backward: delta, dq and this row's parts of dslope and dx.
 template <typename T>
 __global__ void __launch_bounds__(32 * kRowWarps) row_backward_query_kernel(
-    AttArgs a, const int32_t* __restrict__ rows, int64_t row_count, const T* __restrict__ grad,
+    AttArgs a, const int2* __restrict__ rows, int64_t row_count, const T* __restrict__ grad,
     const float* __restrict__ lse, float* __restrict__ delta, T* __restrict__ dq, float* __restrict__ dslope_part, float* __restrict__ dx_part) {
   __shared__ float s_q[kRowWarps][kAttMaxWidth];
   __shared__ float s_g[kRowWarps][kAttMaxWidth];
@@ -141,7 +134,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) row_backward_query_kernel(
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t task = blockIdx.x * int64_t(kRowWarps) + w;
   if (task >= row_count * a.H) return;
-  const int64_t i = rows[task / a.H];
+  const int2 of = rows[task / a.H];  // (row, structure)
+  const int64_t i = of.x;
   const int h = int(task % a.H), hk = h / a.group;
   const T* q = static_cast<const T*>(a.q) + i * a.q_row + h * a.q_head;
   const T* k = static_cast<const T*>(a.k) + hk * a.k_head;
@@ -159,7 +153,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) row_backward_query_kernel(
   }
   const float slope2 = slope * kLog2e;
   __syncwarp();
-  const Range r = keys_of(a, i);
+  const Range r = rows_of(a.k_off, of.y, a.nk);
   const float L = lse[i * a.H + h];
   float dl = 0.0f;
   for (int64_t j = r.b + lane; j < r.e; j += 32) {
@@ -227,7 +221,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) row_backward_query_kernel(
 // Key side: dk, dv and dy of one (key, key head), over the query heads that share it.
 template <typename T>
 __global__ void __launch_bounds__(32 * kRowWarps) row_backward_key_kernel(
-    AttArgs a, const int32_t* __restrict__ rows, int64_t row_count, const T* __restrict__ grad,
+    AttArgs a, const int2* __restrict__ rows, int64_t row_count, const T* __restrict__ grad,
     const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ dy_part) {
   __shared__ float s_k[kRowWarps][kAttMaxWidth];
   __shared__ float s_v[kRowWarps][kAttMaxWidth];
@@ -236,7 +230,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) row_backward_key_kernel(
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t task = blockIdx.x * int64_t(kRowWarps) + w;
   if (task >= row_count * a.Hk) return;
-  const int64_t j = rows[task / a.Hk];
+  const int2 of = rows[task / a.Hk];  // (row, structure)
+  const int64_t j = of.x;
   const int hk = int(task % a.Hk);
   const T* k = static_cast<const T*>(a.k) + j * a.k_row + hk * a.k_head;
   const T* v = static_cast<const T*>(a.v) + j * a.v_row + hk * a.v_head;
@@ -245,7 +240,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) row_backward_key_kernel(
     s_v[w][d] = to_float(v[d]);
   }
   __syncwarp();
-  const Range r = queries_of(a, j);
+  const Range r = rows_of(a.q_off, of.y, a.nq);
   float acc_k[kRowAcc], acc_v[kRowAcc], fx = 0.0f, fy = 0.0f, fz = 0.0f;
 #pragma unroll
   for (int t = 0; t < kRowAcc; ++t) acc_k[t] = acc_v[t] = 0.0f;
@@ -367,8 +362,8 @@ int unpack(const y3b_structure_attention_args* p, const char* what, AttArgs* a) 
     Y3B_CHECK_ARG(p->structure_count >= 1, "%s: atoms without a structure", what);
     Y3B_CHECK_ARG(p->query_offsets && p->key_offsets, "%s: null offsets", what);
   }
-  Y3B_CHECK_ARG(p->query_count == 0 || (p->query && p->query_structure), "%s: null query argument", what);
-  Y3B_CHECK_ARG(p->key_count == 0 || (p->key && p->value && p->key_structure), "%s: null key or value", what);
+  Y3B_CHECK_ARG(p->query_count == 0 || p->query, "%s: null query argument", what);
+  Y3B_CHECK_ARG(p->key_count == 0 || (p->key && p->value), "%s: null key or value", what);
   Y3B_CHECK_ARG((p->slopes != nullptr) || (!p->positions && !p->key_positions), "%s: positions without slopes", what);
   if (p->slopes) {
     Y3B_CHECK_ARG(p->query_count == 0 || p->positions, "%s: slopes without positions", what);
@@ -407,8 +402,6 @@ int unpack(const y3b_structure_attention_args* p, const char* what, AttArgs* a) 
   a->scale2 = p->scale * kLog2e;
   a->q_off = p->query_offsets;
   a->k_off = p->key_offsets;
-  a->q_struct = p->query_structure;
-  a->k_struct = p->key_structure;
   return Y3B_OK;
 }
 
@@ -673,7 +666,7 @@ int forward(const y3b_structure_attention_args* p, const AttArgs& a, const AttPl
   }
   if (p->query_row_count > 0) {
     row_forward_kernel<T><<<row_grid(p->query_row_count * a.H), 32 * kRowWarps, 0, s>>>(
-        a, p->query_rows, p->query_row_count, static_cast<T*>(out), lse);
+        a, reinterpret_cast<const int2*>(p->query_rows), p->query_row_count, static_cast<T*>(out), lse);
     Y3B_LAUNCH_CHECK();
   }
   if (p->query_item_count > 0) {
@@ -722,7 +715,7 @@ int backward(const y3b_structure_attention_args* p, const AttArgs& a, const AttP
   // query side: it also gives delta, which the key side reads
   if (p->query_row_count > 0) {
     row_backward_query_kernel<T><<<row_grid(p->query_row_count * a.H), 32 * kRowWarps, 0, s>>>(
-        a, p->query_rows, p->query_row_count, g, lse, delta, static_cast<T*>(dq), slope_part, dx_part);
+        a, reinterpret_cast<const int2*>(p->query_rows), p->query_row_count, g, lse, delta, static_cast<T*>(dq), slope_part, dx_part);
     Y3B_LAUNCH_CHECK();
   }
   if (p->query_item_count > 0) {
@@ -744,7 +737,7 @@ int backward(const y3b_structure_attention_args* p, const AttArgs& a, const AttP
   }
   if (p->key_row_count > 0) {
     row_backward_key_kernel<T><<<row_grid(p->key_row_count * a.Hk), 32 * kRowWarps, 0, s>>>(
-        a, p->key_rows, p->key_row_count, g, lse, delta, static_cast<T*>(dk), static_cast<T*>(dv), dy_part);
+        a, reinterpret_cast<const int2*>(p->key_rows), p->key_row_count, g, lse, delta, static_cast<T*>(dk), static_cast<T*>(dv), dy_part);
     Y3B_LAUNCH_CHECK();
   }
   if (p->key_item_count > 0) {

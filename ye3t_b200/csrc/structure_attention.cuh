@@ -23,10 +23,8 @@ struct AttArgs {
   const float* slopes;  // [H]
   float scale2;         // scale * log2(e)
   float scale;
-  const int32_t* q_off;     // [S + 1]
-  const int32_t* k_off;     // [S + 1]
-  const int32_t* q_struct;  // [nq]
-  const int32_t* k_struct;  // [nk]
+  const int32_t* q_off;  // [S + 1]
+  const int32_t* k_off;  // [S + 1]
 };
 
 __device__ __forceinline__ float to_float(float v) { return v; }

@@ -653,10 +653,11 @@ def _work_tables(row_first, row_count, col_first, col_count, heads, tiled, by_ro
     split = p > 1
     joins = np.stack([row, rows, slot, p], 1)[split]
     single = np.flatnonzero(by_row)
-    rest = np.repeat(row_first[single] - (np.cumsum(row_count[single]) - row_count[single]), row_count[single])
-    rest = rest + np.arange(rest.size)
+    n = row_count[single]
+    rest = np.repeat(row_first[single] - (np.cumsum(n) - n), n) + np.arange(n.sum())
+    rest = np.stack([rest, np.repeat(single, n)], 1)
     return {"items": items, "joins": joins, "rows": rest, "item_count": len(items), "join_count": len(joins),
-            "slot_count": int(p[split].sum()), "row_count": rest.size}
+            "slot_count": int(p[split].sum()), "row_count": len(rest)}
 
 
 class StructureLayout:
@@ -685,7 +686,6 @@ class StructureLayout:
             raise ValueError(f"StructureLayout: ye3t_b200 evaluates on CUDA devices only, not on {self.device}")
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
-        number = np.arange(self.structure_count)
         q_first, k_first = np.cumsum(queries) - queries, np.cumsum(keys) - keys
         small = (queries <= _SMALL) & (keys <= _SMALL)
         # beside larger structures, a launch of their own has to fill the SMs
@@ -698,47 +698,39 @@ class StructureLayout:
         q_side = _work_tables(q_first, queries, k_first, keys, self.heads, ~small & (keys > 1), ~small & (keys <= 1))
         k_side = _work_tables(k_first, keys, q_first, queries, self.key_heads, ~small & (keys > 1),
                               ~small & (keys <= 1))
-        self._small_counts = int((tiny & (queries + keys > 0)).sum()), int((small & ~tiny).sum())
-        self._counts = tuple(int(side[name]) for side in (q_side, k_side) for name in
-                             ("item_count", "join_count", "slot_count", "row_count"))
         # items, then joins and structures: they are read as 32- and 16-byte records
-        tables = [q_side["items"], k_side["items"], q_side["joins"], k_side["joins"], structures, q_side["rows"], k_side["rows"],
-                  np.concatenate([[0], np.cumsum(queries)]), np.concatenate([[0], np.cumsum(keys)]),
-                  np.repeat(number, queries), np.repeat(number, keys)]
+        tables = [q_side["items"], k_side["items"], q_side["joins"], k_side["joins"], structures, q_side["rows"],
+                  k_side["rows"], np.concatenate([[0], np.cumsum(queries)]), np.concatenate([[0], np.cumsum(keys)])]
         # one copy to the device; it is complete when the constructor returns, so any stream may use it
-        packed = torch.as_tensor(np.concatenate([t.reshape(-1) for t in tables]).astype(np.int32)).to(self.device)
-        self._stream = nat.stream_of(self.device)
-        self._packed = packed
-        first = np.cumsum([0] + [t.size for t in tables[:-1]]) * 4
-        (self._query_items, self._key_items, self._query_joins, self._key_joins, self._small, self._query_rows,
-         self._key_rows, self._query_offsets, self._key_offsets, self._query_structure, self._key_structure) = [
-            packed.data_ptr() + int(o) for o in first]
-
-    def _use(self):
-        """Keeps the tables' memory from reuse before the current stream is done with it."""
-        if nat.stream_of(self.device) != self._stream:
-            self._packed.record_stream(torch.cuda.current_stream(self.device))
+        self._packed = torch.as_tensor(np.concatenate([t.reshape(-1) for t in tables]).astype(np.int32)).to(self.device)
+        self._stream = _raw_stream(self.device)
+        first = self._packed.data_ptr() + 4 * np.cumsum([0] + [t.size for t in tables[:-1]])
+        a = self._args = nat.StructureAttentionArgs()
+        a.heads, a.key_heads = self.heads, self.key_heads
+        a.query_count, a.key_count, a.structure_count = self.query_count, self.key_count, self.structure_count
+        a.small_32_count, a.small_64_count = int((tiny & (queries + keys > 0)).sum()), int((small & ~tiny).sum())
+        for name, side in (("query", q_side), ("key", k_side)):
+            for what in ("item_count", "join_count", "slot_count", "row_count"):
+                setattr(a, f"{name}_{what}", int(side[what]))
+        for name, at in zip(("query_items", "key_items", "query_joins", "key_joins", "small", "query_rows", "key_rows",
+                             "query_offsets", "key_offsets"), first):
+            setattr(a, name, int(at))
 
 
 def _attention_args(query, key, value, x, y, slopes, layout, scale):
-    a = nat.StructureAttentionArgs()
+    a = nat.StructureAttentionArgs.from_buffer_copy(layout._args)
     a.dtype = nat.learned_dtype_code(query.dtype)
-    a.heads, a.key_heads, a.width = query.shape[1], key.shape[1], query.shape[2]
-    a.query_count, a.key_count, a.structure_count = query.shape[0], key.shape[0], layout.structure_count
+    a.width = query.shape[2]
     a.query, a.key, a.value = query.data_ptr(), key.data_ptr(), value.data_ptr()
-    a.query_row_stride, a.query_head_stride = query.stride(0), query.stride(1)
-    a.key_row_stride, a.key_head_stride = key.stride(0), key.stride(1)
-    a.value_row_stride, a.value_head_stride = value.stride(0), value.stride(1)
-    a.positions, a.key_positions, a.slopes = nat.ptr(x), nat.ptr(y), nat.ptr(slopes)
-    a.query_offsets, a.key_offsets = layout._query_offsets, layout._key_offsets
-    a.query_structure, a.key_structure = layout._query_structure, layout._key_structure
-    (a.query_item_count, a.query_join_count, a.query_slot_count, a.query_row_count,
-     a.key_item_count, a.key_join_count, a.key_slot_count, a.key_row_count) = layout._counts
-    (a.small_32_count, a.small_64_count), a.small = layout._small_counts, layout._small
-    a.query_items, a.query_joins, a.query_rows = layout._query_items, layout._query_joins, layout._query_rows
-    a.key_items, a.key_joins, a.key_rows = layout._key_items, layout._key_joins, layout._key_rows
+    a.query_row_stride, a.query_head_stride, _ = query.stride()
+    a.key_row_stride, a.key_head_stride, _ = key.stride()
+    a.value_row_stride, a.value_head_stride, _ = value.stride()
+    if slopes is not None:
+        a.positions, a.key_positions, a.slopes = x.data_ptr(), y.data_ptr(), slopes.data_ptr()
     a.scale = scale
-    layout._use()
+    if _raw_stream(layout.device) != layout._stream:
+        # keeps the tables' memory from reuse before the current stream is done with it
+        layout._packed.record_stream(torch.cuda.current_stream(layout.device))
     return a
 
 
@@ -762,7 +754,7 @@ def _attention_forward(query, key, value, x, y, slopes, layout, scale, validate)
     ws, ws_bytes = _attention_workspace(args, 0, q.device)
     status = _status(q.device) if validate else None
     nat.check(nat.lib().y3b_structure_attention(ctypes.byref(args), ws.data_ptr(), ws_bytes, out.data_ptr(),
-                                                lse.data_ptr(), nat.ptr(status), nat.stream_of(q.device)),
+                                                lse.data_ptr(), nat.ptr(status), _raw_stream(q.device)),
               "structure_attention")
     if validate:
         _raise_on_status(status, "structure_attention")
