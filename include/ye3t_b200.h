@@ -666,7 +666,8 @@ typedef struct {
   const int32_t* query_offsets; /* [structure_count + 1] */
   const int32_t* key_offsets;   /* [structure_count + 1] */
   /* Work tables.  A structure of up to 64 queries and 64 keys is in small (those of up to 32 of each first).
-   * Every query of the others is in query_rows (one warp computes it) or in exactly one tile of up to 128 queries
+   * One or two queries of a larger structure are the rows of an item in few_items, its keys split over items that one
+   * few_joins entry joins.  Every other query is in query_rows (one warp computes it) or in exactly one tile of up to 128 queries
    * of one structure; a tile is one item, or several items with consecutive slots that split its keys and
    * one join.  Keys likewise, with queries as the columns.
    *   row   (query or key, its structure)
@@ -674,9 +675,12 @@ typedef struct {
    *   item  (first row, rows, first column, columns, slot or -1, 0, 0, 0)
    *   join  (first row, rows, first slot, slots) */
   int64_t small_32_count, small_64_count;
+  int64_t few_item_count, few_join_count, few_slot_count;
   int64_t query_item_count, query_join_count, query_slot_count, query_row_count;
   int64_t key_item_count, key_join_count, key_slot_count, key_row_count;
   const int32_t* small;       /* 16-byte aligned */
+  const int32_t* few_items;   /* 32-byte aligned */
+  const int32_t* few_joins;   /* 16-byte aligned */
   const int32_t* query_items; /* 32-byte aligned */
   const int32_t* query_joins; /* 16-byte aligned */
   const int32_t* query_rows;

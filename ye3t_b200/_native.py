@@ -104,9 +104,10 @@ class StructureAttentionArgs(ctypes.Structure):
         ("positions", VP), ("key_positions", VP), ("slopes", VP),
         ("query_offsets", VP), ("key_offsets", VP),
         ("small_32_count", I64), ("small_64_count", I64),
+        ("few_item_count", I64), ("few_join_count", I64), ("few_slot_count", I64),
         ("query_item_count", I64), ("query_join_count", I64), ("query_slot_count", I64), ("query_row_count", I64),
         ("key_item_count", I64), ("key_join_count", I64), ("key_slot_count", I64), ("key_row_count", I64),
-        ("small", VP), ("query_items", VP), ("query_joins", VP), ("query_rows", VP), ("key_items", VP), ("key_joins", VP),
+        ("small", VP), ("few_items", VP), ("few_joins", VP), ("query_items", VP), ("query_joins", VP), ("query_rows", VP), ("key_items", VP), ("key_joins", VP),
         ("key_rows", VP), ("scale", ctypes.c_float),
     ]
 

@@ -16,6 +16,7 @@
 // then the D components for the sums.
 #include <algorithm>
 
+#include "structure_attention_few.cuh"
 #include "structure_attention_small.cuh"
 #include "structure_attention_tile.cuh"
 
@@ -372,6 +373,9 @@ int unpack(const y3b_structure_attention_args* p, const char* what, AttArgs* a) 
   Y3B_CHECK_ARG(p->small_32_count >= 0 && p->small_64_count >= 0 &&
                     (p->small_32_count + p->small_64_count == 0 || p->small),
                 "%s: bad table of small structures", what);
+  Y3B_CHECK_ARG(p->few_item_count >= 0 && p->few_join_count >= 0 && p->few_slot_count >= 0 &&
+                    (p->few_item_count == 0 || (p->few_items && p->few_joins && p->few_join_count > 0)),
+                "%s: bad table of few-query structures", what);
   Y3B_CHECK_ARG(p->query_item_count >= 0 && p->query_join_count >= 0 && p->query_slot_count >= 0 &&
                     p->query_row_count >= 0 && p->key_item_count >= 0 && p->key_join_count >= 0 &&
                     p->key_slot_count >= 0 && p->key_row_count >= 0,
@@ -452,20 +456,20 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackA
   }
 }
 
-// Joins of split items, one warp a row; W = floats of a partial row.
-constexpr int kJoinCtas = kTileRows / 4;  // CTAs of four warps a tile
+// Joins of split items, one warp a row, four a CTA.  Partial results lie at ((slot * heads + head) * RS + row) * W
+// floats: RS is kTileRows, or kFewQueries for the few-query kernels.
 
 template <typename T>
 __global__ void __launch_bounds__(128) join_forward_kernel(const AttJoin* __restrict__ joins,
-                                                           const float* __restrict__ part, int W, int DP, int D,
+                                                           const float* __restrict__ part, int RS, int W, int DP, int D,
                                                            int H, T* __restrict__ out, float* __restrict__ lse) {
-  const unsigned task = blockIdx.x / kJoinCtas;
+  const unsigned ctas = unsigned(RS + 3) / 4, task = blockIdx.x / ctas;
   const AttJoin jn = joins[task / unsigned(H)];
   const int h = int(task % unsigned(H)), lane = threadIdx.x & 31;
-  const int r = int(blockIdx.x % kJoinCtas) * 4 + (threadIdx.x >> 5);
+  const int r = int(blockIdx.x % ctas) * 4 + (threadIdx.x >> 5);
   if (r >= jn.rows) return;
-  const int64_t step = int64_t(H) * kTileRows * W;
-  const float* p = part + ((int64_t(jn.first) * H + h) * kTileRows + r) * W;
+  const int64_t step = int64_t(H) * RS * W;
+  const float* p = part + ((int64_t(jn.first) * H + h) * RS + r) * W;
   float m = -INFINITY;
   for (int k = lane; k < jn.count; k += 32) m = fmaxf(m, p[k * step + DP]);
   m = warp_max(m);
@@ -476,38 +480,57 @@ __global__ void __launch_bounds__(128) join_forward_kernel(const AttJoin* __rest
   const bool none = m == -INFINITY && l == 0.0f;
   const int64_t at = (int64_t(jn.row) + r) * H + h;
   const float inv = none ? 0.0f : 1.0f / l;
-  for (int d = lane; d < D; d += 32) {
-    float o = 0.0f;
-    for (int k = 0; k < jn.count; ++k) {
-      // a part without any score above -inf holds no numbers
-      const float mk = p[k * step + DP];
-      if (!(mk == -INFINITY && p[k * step + DP + 1] == 0.0f)) o = fmaf(p[k * step + d], exp2f(mk - ref), o);
+  float o[kAttMaxWidth / 32] = {};
+  for (int k0 = 0; k0 < jn.count; k0 += 32) {
+    // lane k weighs part k0 + k; a part without any score above -inf holds no numbers
+    float weight = 0.0f;
+    if (k0 + lane < jn.count) {
+      const float mk = p[(k0 + lane) * step + DP];
+      if (!(mk == -INFINITY && p[(k0 + lane) * step + DP + 1] == 0.0f)) weight = exp2f(mk - ref);
     }
-    out[at * D + d] = from_float<T>(none ? 0.0f : o * inv);
+    const int n = jn.count - k0 < 32 ? jn.count - k0 : 32;
+#pragma unroll 8
+    for (int k = 0; k < n; ++k) {
+      const float f = __shfl_sync(0xffffffffu, weight, k);
+#pragma unroll
+      for (int t = 0; t < kAttMaxWidth / 32; ++t) {
+        const int d = lane + 32 * t;
+        if (d < D) {
+          const float x = p[(k0 + k) * step + d];
+          o[t] = f == 0.0f ? o[t] : fmaf(x, f, o[t]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < kAttMaxWidth / 32; ++t) {
+    const int d = lane + 32 * t;
+    if (d < D) out[at * D + d] = from_float<T>(none ? 0.0f : o[t] * inv);
   }
   if (lane == 0) lse[at] = none ? INFINITY : m + log2f(l);
 }
 
 __device__ __forceinline__ float sum_parts(const float* p, int64_t step, int count) {
   float s = 0.0f;
+#pragma unroll 8
   for (int k = 0; k < count; ++k) s += p[k * step];
   return s;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(128) join_query_kernel(const AttJoin* __restrict__ joins,
-                                                         const float* __restrict__ part, int W, int DP, int D, int H,
-                                                         float scale, const float* __restrict__ slopes,
+                                                         const float* __restrict__ part, int RS, int W, int DP, int D, int H,
+                                                         float scale, bool fix, const float* __restrict__ slopes,
                                                          T* __restrict__ dq, float* __restrict__ delta,
                                                          float* __restrict__ slope_part,
                                                          float* __restrict__ place_part) {
-  const unsigned task = blockIdx.x / kJoinCtas;
+  const unsigned ctas = unsigned(RS + 3) / 4, task = blockIdx.x / ctas;
   const AttJoin jn = joins[task / unsigned(H)];
   const int h = int(task % unsigned(H)), lane = threadIdx.x & 31;
-  const int r = int(blockIdx.x % kJoinCtas) * 4 + (threadIdx.x >> 5);
+  const int r = int(blockIdx.x % ctas) * 4 + (threadIdx.x >> 5);
   if (r >= jn.rows) return;
-  const int64_t step = int64_t(H) * kTileRows * W;
-  const float* p = part + ((int64_t(jn.first) * H + h) * kTileRows + r) * W;
+  const int64_t step = int64_t(H) * RS * W;
+  const float* p = part + ((int64_t(jn.first) * H + h) * RS + r) * W;
   const int64_t at = (int64_t(jn.row) + r) * H + h;
   const float s = lane < 10 ? sum_parts(p + DP + lane, step, jn.count) : 0.0f;
   const float all = __shfl_sync(0xffffffffu, s, 9), inv = all == 0.0f ? 0.0f : 1.0f / all;
@@ -517,8 +540,8 @@ __global__ void __launch_bounds__(128) join_query_kernel(const AttJoin* __restri
   if (lane == 0) delta[at] = dl;
   for (int d = lane; d < D; d += 32) {
     float x = sum_parts(p + d, step, jn.count);
-    // one piece: dS was formed with the forward's rounded delta, and P K follows the sums
-    if constexpr (sizeof(T) == 2) x = fmaf(p[DP + 10] - dl, sum_parts(p + DP + 16 + d, step, jn.count), x);
+    // fix: dS was formed with delta from the rounded result, and P K follows the sums
+    if (fix) x = fmaf(p[DP + 10] - dl, sum_parts(p + DP + 16 + d, step, jn.count), x);
     dq[at * D + d] = from_float<T>(scale * x);
   }
   if (slopes) {
@@ -529,16 +552,16 @@ __global__ void __launch_bounds__(128) join_query_kernel(const AttJoin* __restri
 
 template <typename T>
 __global__ void __launch_bounds__(128) join_key_kernel(const AttJoin* __restrict__ joins,
-                                                       const float* __restrict__ part, int W, int DP, int D, int Hk,
+                                                       const float* __restrict__ part, int RS, int W, int DP, int D, int Hk,
                                                        float scale, T* __restrict__ dk, T* __restrict__ dv,
                                                        float* __restrict__ place_part) {
-  const unsigned task = blockIdx.x / kJoinCtas;
+  const unsigned ctas = unsigned(RS + 3) / 4, task = blockIdx.x / ctas;
   const AttJoin jn = joins[task / unsigned(Hk)];
   const int h = int(task % unsigned(Hk)), lane = threadIdx.x & 31;
-  const int r = int(blockIdx.x % kJoinCtas) * 4 + (threadIdx.x >> 5);
+  const int r = int(blockIdx.x % ctas) * 4 + (threadIdx.x >> 5);
   if (r >= jn.rows) return;
-  const int64_t step = int64_t(Hk) * kTileRows * W;
-  const float* p = part + ((int64_t(jn.first) * Hk + h) * kTileRows + r) * W;
+  const int64_t step = int64_t(Hk) * RS * W;
+  const float* p = part + ((int64_t(jn.first) * Hk + h) * RS + r) * W;
   const int64_t at = (int64_t(jn.row) + r) * Hk + h;
   for (int d = lane; d < D; d += 32) {
     dv[at * D + d] = from_float<T>(sum_parts(p + d, step, jn.count));
@@ -557,7 +580,7 @@ struct AttPlan {
   int pieces, DP, chunks, Wf, Wq, Wk;
   bool tiles;
   bool direct[3];  // query, key, value are read in place
-  int64_t packed[4], delta, slope, dx, dy, part_q, part_k, bytes;
+  int64_t packed[4], delta, slope, dx, dy, part_q, part_k, part_few, bytes;
 };
 
 bool in_place(const y3b_structure_attention_args* p, const void* base, int64_t row, int64_t head) {
@@ -596,6 +619,7 @@ AttPlan make_plan(const y3b_structure_attention_args* p, bool adjoint) {
   w.dy = take(adjoint ? nk * Hk * 12 : 0);
   w.part_q = take(p->query_slot_count * H * kTileRows * w.Wq * 4);
   w.part_k = take(adjoint ? p->key_slot_count * Hk * kTileRows * w.Wk * 4 : 0);
+  w.part_few = take(p->few_slot_count * H * kFewQueries * ((adjoint ? 2 : 1) * w.DP + 16) * 4);
   w.bytes = at;
   return w;
 }
@@ -669,6 +693,16 @@ int forward(const y3b_structure_attention_args* p, const AttArgs& a, const AttPl
         a, reinterpret_cast<const int2*>(p->query_rows), p->query_row_count, static_cast<T*>(out), lse);
     Y3B_LAUNCH_CHECK();
   }
+  if (p->few_item_count > 0) {
+    float* part = reinterpret_cast<float*>(ws + w.part_few);
+    const int rc = attention_few_forward<T>(a, reinterpret_cast<const AttItem*>(p->few_items), p->few_item_count, w.DP,
+                                            w.DP + 16, part, s);
+    if (rc) return rc;
+    join_forward_kernel<T><<<unsigned(p->few_join_count * a.H), 128, 0, s>>>(
+        reinterpret_cast<const AttJoin*>(p->few_joins), part, kFewQueries, w.DP + 16, w.DP, a.D, a.H,
+        static_cast<T*>(out), lse);
+    Y3B_LAUNCH_CHECK();
+  }
   if (p->query_item_count > 0) {
     AttTileArgs t = tile_args(p, a, w, status);
     int rc = operands(p, w, nullptr, ws, &t, s);
@@ -681,8 +715,8 @@ int forward(const y3b_structure_attention_args* p, const AttArgs& a, const AttPl
     rc = attention_forward_tiles(w.pieces, t, p->query_item_count, s);
     if (rc) return rc;
     if (p->query_join_count > 0) {
-      join_forward_kernel<T><<<unsigned(p->query_join_count * a.H * kJoinCtas), 128, 0, s>>>(
-          reinterpret_cast<const AttJoin*>(p->query_joins), t.part, w.Wf, w.DP, a.D, a.H, static_cast<T*>(out), lse);
+      join_forward_kernel<T><<<unsigned(p->query_join_count * a.H * (kTileRows / 4)), 128, 0, s>>>(
+          reinterpret_cast<const AttJoin*>(p->query_joins), t.part, kTileRows, w.Wf, w.DP, a.D, a.H, static_cast<T*>(out), lse);
       Y3B_LAUNCH_CHECK();
     }
   }
@@ -718,6 +752,16 @@ int backward(const y3b_structure_attention_args* p, const AttArgs& a, const AttP
         a, reinterpret_cast<const int2*>(p->query_rows), p->query_row_count, g, lse, delta, static_cast<T*>(dq), slope_part, dx_part);
     Y3B_LAUNCH_CHECK();
   }
+  if (p->few_item_count > 0) {
+    float* part = reinterpret_cast<float*>(ws + w.part_few);
+    const int rc = attention_few_query<T>(a, reinterpret_cast<const AttItem*>(p->few_items), p->few_item_count, w.DP,
+                                          2 * w.DP + 16, static_cast<const T*>(out), g, lse, part, s);
+    if (rc) return rc;
+    join_query_kernel<T><<<unsigned(p->few_join_count * a.H), 128, 0, s>>>(
+        reinterpret_cast<const AttJoin*>(p->few_joins), part, kFewQueries, 2 * w.DP + 16, w.DP, a.D, a.H, a.scale, true,
+        a.slopes, static_cast<T*>(dq), delta, slope_part, dx_part);
+    Y3B_LAUNCH_CHECK();
+  }
   if (p->query_item_count > 0) {
     t.items = reinterpret_cast<const AttItem*>(p->query_items);
     t.out_in = out;
@@ -729,8 +773,9 @@ int backward(const y3b_structure_attention_args* p, const AttArgs& a, const AttP
     const int rc = attention_query_tiles(w.pieces, t, p->query_item_count, s);
     if (rc) return rc;
     if (p->query_join_count > 0) {
-      join_query_kernel<T><<<unsigned(p->query_join_count * a.H * kJoinCtas), 128, 0, s>>>(
-          reinterpret_cast<const AttJoin*>(p->query_joins), t.part, w.Wq, w.DP, a.D, a.H, a.scale, a.slopes,
+      join_query_kernel<T><<<unsigned(p->query_join_count * a.H * (kTileRows / 4)), 128, 0, s>>>(
+          reinterpret_cast<const AttJoin*>(p->query_joins), t.part, kTileRows, w.Wq, w.DP, a.D, a.H, a.scale,
+          w.pieces == 1, a.slopes,
           static_cast<T*>(dq), delta, slope_part, dx_part);
       Y3B_LAUNCH_CHECK();
     }
@@ -750,8 +795,8 @@ int backward(const y3b_structure_attention_args* p, const AttArgs& a, const AttP
     const int rc = attention_key_tiles(w.pieces, t, p->key_item_count, s);
     if (rc) return rc;
     if (p->key_join_count > 0) {
-      join_key_kernel<T><<<unsigned(p->key_join_count * a.Hk * kJoinCtas), 128, 0, s>>>(
-          reinterpret_cast<const AttJoin*>(p->key_joins), t.part, w.Wk, w.DP, a.D, a.Hk, a.scale,
+      join_key_kernel<T><<<unsigned(p->key_join_count * a.Hk * (kTileRows / 4)), 128, 0, s>>>(
+          reinterpret_cast<const AttJoin*>(p->key_joins), t.part, kTileRows, w.Wk, w.DP, a.D, a.Hk, a.scale,
           static_cast<T*>(dk), static_cast<T*>(dv), a.slopes ? dy_part : nullptr);
       Y3B_LAUNCH_CHECK();
     }

@@ -623,23 +623,27 @@ def _host_counts(counts, what):
 
 
 _TILE = 128       # rows of a tile
+_FEW = 2          # structures of up to so many queries take the few-query kernels
 _SMALL = 64       # structures of up to so many queries and keys take the small-structure kernels
 
 
-def _work_tables(row_first, row_count, col_first, col_count, heads, tiled, by_row):
-    """Items, joins and single rows of one side (the layout of include/ye3t_b200.h)."""
+def _work_tables(row_first, row_count, col_first, col_count, heads, tiled, by_row, always=False):
+    """Items, joins and single rows of one side (the layout of include/ye3t_b200.h); ``always``: every tile is
+    joined, also one that is not split."""
     r0, rn, c0, cn = row_first[tiled], row_count[tiled], col_first[tiled], col_count[tiled]
     tiles = -(-rn // _TILE)
-    # columns are split where the tiles alone would not give every SM its two CTAs
+    # columns are split where the tiles alone would not give every SM its CTAs: two of the tile kernels', four
+    # of the few-query kernels'
     work = int((tiles * np.maximum(cn, 1)).sum()) * heads
-    chunk = max(256, work // (148 * 2))
+    chunk = max(128, work // (148 * 4)) if always else max(256, work // (148 * 2))
     parts = np.maximum(1, np.round(cn / chunk).astype(np.int64))
     of = np.repeat(np.arange(rn.size), tiles)  # the structure of each tile
     t = np.arange(of.size) - np.repeat(np.cumsum(tiles) - tiles, tiles)
     row = r0[of] + t * _TILE
     rows = np.minimum(rn[of] - t * _TILE, _TILE)
     p = parts[of]
-    slot = np.where(p > 1, np.cumsum(np.where(p > 1, p, 0)) - p, -1)
+    split = (p > 1) | always
+    slot = np.where(split, np.cumsum(np.where(split, p, 0)) - p, -1)
     ti = np.repeat(np.arange(of.size), p)
     k = np.arange(ti.size) - np.repeat(np.cumsum(p) - p, p)
     # parts begin at multiples of 64 columns
@@ -650,7 +654,6 @@ def _work_tables(row_first, row_count, col_first, col_count, heads, tiled, by_ro
     items[:, 0], items[:, 1], items[:, 2], items[:, 3] = row[ti], rows[ti], c0[of][ti] + begin, end - begin
     items[:, 4] = np.where(slot[ti] >= 0, slot[ti] + k, -1)
     items = items[np.argsort(-items[:, 3], kind="stable")]
-    split = p > 1
     joins = np.stack([row, rows, slot, p], 1)[split]
     single = np.flatnonzero(by_row)
     n = row_count[single]
@@ -695,12 +698,16 @@ class StructureLayout:
         order = np.concatenate([np.flatnonzero(tiny & (queries + keys > 0)), np.flatnonzero(small & ~tiny)])
         structures = np.stack([q_first, queries, k_first, keys], 1)[order]
         # a single key has all the weight and no gradient through the softmax: the row kernels give exactly that
-        q_side = _work_tables(q_first, queries, k_first, keys, self.heads, ~small & (keys > 1), ~small & (keys <= 1))
+        few = ~small & (keys > 1) & (queries <= _FEW)
+        q_side = _work_tables(q_first, queries, k_first, keys, self.heads, ~small & (keys > 1) & ~few,
+                              ~small & (keys <= 1))
+        f_side = _work_tables(q_first, queries, k_first, keys, self.key_heads, few & (queries > 0), small & ~small,
+                              always=True)
         k_side = _work_tables(k_first, keys, q_first, queries, self.key_heads, ~small & (keys > 1),
                               ~small & (keys <= 1))
         # items, then joins and structures: they are read as 32- and 16-byte records
-        tables = [q_side["items"], k_side["items"], q_side["joins"], k_side["joins"], structures, q_side["rows"],
-                  k_side["rows"], np.concatenate([[0], np.cumsum(queries)]), np.concatenate([[0], np.cumsum(keys)])]
+        tables = [q_side["items"], k_side["items"], f_side["items"], q_side["joins"], k_side["joins"], f_side["joins"],
+                  structures, q_side["rows"], k_side["rows"], np.concatenate([[0], np.cumsum(queries)]), np.concatenate([[0], np.cumsum(keys)])]
         # one copy to the device; it is complete when the constructor returns, so any stream may use it
         self._packed = torch.as_tensor(np.concatenate([t.reshape(-1) for t in tables]).astype(np.int32)).to(self.device)
         self._stream = _raw_stream(self.device)
@@ -709,10 +716,10 @@ class StructureLayout:
         a.heads, a.key_heads = self.heads, self.key_heads
         a.query_count, a.key_count, a.structure_count = self.query_count, self.key_count, self.structure_count
         a.small_32_count, a.small_64_count = int((tiny & (queries + keys > 0)).sum()), int((small & ~tiny).sum())
-        for name, side in (("query", q_side), ("key", k_side)):
-            for what in ("item_count", "join_count", "slot_count", "row_count"):
+        for name, side in (("query", q_side), ("key", k_side), ("few", f_side)):
+            for what in ("item_count", "join_count", "slot_count") + (() if name == "few" else ("row_count",)):
                 setattr(a, f"{name}_{what}", int(side[what]))
-        for name, at in zip(("query_items", "key_items", "query_joins", "key_joins", "small", "query_rows", "key_rows",
+        for name, at in zip(("query_items", "key_items", "few_items", "query_joins", "key_joins", "few_joins", "small", "query_rows", "key_rows",
                              "query_offsets", "key_offsets"), first):
             setattr(a, name, int(at))
 
