@@ -99,16 +99,17 @@ struct AttCfg {
   static constexpr int A1 = NP == 1 ? BN : SCORES + NP * BN / 2;
   static constexpr int ABUF = NP == 1 ? BUF : 0;  // with one piece every buffer holds its own P and dS
   static constexpr int ACC = NP == 1 ? SCORES : SCORES + (MODE == kKeySide ? 2 : 1) * NP * BN / 2;
-  // Accumulators.  OPS results (dV and dK on the key side); a second one of each for three pieces
-  // takes all products but that of the leading pieces: the tensor cores truncate when they accumulate,
-  // once a product, and the sum of the leading pieces then sees a sixth as many.  With one piece the
+  // Accumulators: OPS results (dV and dK on the key side).  The tensor cores truncate when they accumulate; three
+  // pieces are six products, each of which truncates the long sum.  The score warps therefore add the accumulator
+  // to a total in fp32, also in tensor memory, every FLUSH tiles, and it starts again.  With one piece the
   // query side also accumulates P K, to correct dQ for the rounding of delta.
   static constexpr int OPS = MODE == kKeySide ? 2 : 1;
-  static constexpr int SMALL = NP == 3 ? OPS : 0;
+  static constexpr int FLUSH = 2;
+  static constexpr int TOTALS = NP == 3 ? OPS : 0;
   static constexpr bool FIX = MODE == kQuerySide && NP == 1;
   static constexpr int HALVES = MODE == kKeySide && NP == 3 && DP == 128 ? 2 : 1;  // CTAs that share a width
   static constexpr int W = DP / HALVES;  // columns of one accumulator
-  static constexpr int NEED = ACC + (OPS + SMALL + (FIX ? 1 : 0)) * W;
+  static constexpr int NEED = ACC + (OPS + TOTALS + (FIX ? 1 : 0)) * W;
   static constexpr int COLUMNS = NEED <= 128 ? 128 : NEED <= 256 ? 256 : 512;
   static constexpr int PER_SM_TMEM = 512 / COLUMNS;
   static constexpr int PER_SM_SMEM = (227 * 1024) / (SMEM + 2048);
@@ -364,13 +365,12 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
           const uint32_t cb = (MODE == kForward || (MODE == kKeySide && op == 0) ? c1 : c0) + half * (BN * 128);
 #pragma unroll
           for (int n = 0; n < Pieces<NP>::N; ++n) {
-            const bool small = NP == 3 && n < Pieces<NP>::N - 1;
-            const uint32_t d = tmem + C::ACC + (op + (small ? C::OPS : 0)) * C::W;
+            const uint32_t d = tmem + C::ACC + op * C::W;
 #pragma unroll
             for (int ks = 0; ks < BN / 16; ++ks)
               tc::mma_ts(d, A + Pieces<NP>::a(n) * (BN / 2) + ks * 8,
                          tc::desc_sw128(cb + Pieces<NP>::b(n) * C::COL_PIECE + ks * 2048, BN * 128, 1024), id_a,
-                         j > 0 || ks > 0 || (small && n > 0));
+                         (C::TOTALS ? j % C::FLUSH > 0 : j > 0) || n > 0 || ks > 0);
           }
         }
         tc::commit(empty(s));
@@ -444,6 +444,21 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
       }
     };
 
+    // The accumulators of the tiles before j into the totals.
+    const auto flush = [&](int j) {
+      for (int d = 0; d < C::OPS * C::W; d += 16) {
+        float o[16], e[16];
+        tc::ld16(lane_base + C::ACC + d, o);
+        if (j > C::FLUSH) tc::ld16(lane_base + C::ACC + C::OPS * C::W + d, e);
+        tc::wait_ld();
+        uint32_t r[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(j > C::FLUSH ? e[k] + o[k] : o[k]);
+        tc::st16(lane_base + C::ACC + C::OPS * C::W + d, r);
+      }
+      tc::wait_st();
+    };
+
     // One tile's arithmetic; n < BN columns where CUT, all of them otherwise.
     const auto forward_tile = [&](auto cut, int j, int n, const float* ex, uint32_t buf) {
       constexpr bool CUT = decltype(cut)::value;
@@ -490,7 +505,7 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
             return false;
           tc::fence_after();
 #pragma unroll
-          for (int u = 0; u < C::OPS + C::SMALL; ++u) {
+          for (int u = 0; u < C::OPS + C::TOTALS; ++u) {
             for (int d = 0; d < acc_n; d += 16) {
               float o[16];
               tc::ld16(lane_base + C::ACC + u * C::W + d, o);
@@ -631,7 +646,7 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
       const int n = item.cols - jt * BN;  // columns there are, BN or more in a full tile
       ok = tc::mbar_wait(full(s), (j / C::STAGES) & 1) && tc::mbar_wait(s_ready(j), (j / C::BUFS) & 1);
       // several pieces have one place for P and dS: the product before must be done with it
-      if (NP > 1 && C::BUFS == 2 && j > 0 && ok)
+      if (NP > 1 && j > 0 && ok && (C::BUFS == 2 || j % C::FLUSH == 0))
         ok = tc::mbar_wait(empty((j - 1) % C::STAGES), ((j - 1) / C::STAGES) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -640,6 +655,9 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
       const uint32_t buf = lane_base + (j % C::BUFS) * C::BUF;
       // a warp without a row of the item only keeps the barriers going: its lanes of P reach no result
       if (32 * (warp & 3) < item.rows) {
+        if constexpr (C::TOTALS > 0) {
+          if (j > 0 && j % C::FLUSH == 0) flush(j);
+        }
         if constexpr (MODE == kForward) {
           ok = n >= BN ? forward_tile(std::false_type{}, j, n, ex, buf) : forward_tile(std::true_type{}, j, n, ex, buf);
           if (!ok) break;
@@ -711,10 +729,15 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
         for (int d = 16 * group; d < acc_n; d += 16 * C::GROUPS) {
           float o[16];
           tc::ld16(lane_base + C::ACC + op * C::W + d, o);
-          if constexpr (C::SMALL > 0 || C::FIX) {
+          if constexpr (C::TOTALS > 0 || C::FIX) {
             float e[16];
             tc::ld16(lane_base + C::ACC + (C::OPS + op) * C::W + d, e);
             tc::wait_ld();
+            const bool whole = C::TOTALS > 0 && total <= C::FLUSH;  // nothing went into the total
+            if (whole) {
+#pragma unroll
+              for (int k = 0; k < 16; ++k) e[k] = 0.0f;
+            }
             const float fe = !C::FIX ? 1.0f : split ? 0.0f : delta0 - dl;
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
