@@ -75,30 +75,34 @@ struct AttTileArgs {
 template <int MODE, int DP, int NP>
 struct AttCfg {
   static constexpr int BN = NP == 1 && MODE == kForward ? 64 : NP == 1 || DP == 64 || MODE == kForward ? 32 : 16;
+  static constexpr int STAGES = NP == 3 ? (DP == 128 && MODE != kForward ? 1 : 2) : DP == 128 ? 2 : 4;
   // Score groups of four warps; with two, each takes every other column tile.  The backward with one piece is
   // 14 % faster with two (8,192 atoms, 8 heads of 64); the forward, which needs more registers, 10 % slower.
-  static constexpr int GROUPS = NP == 1 && MODE != kForward ? 2 : 1;
+  static constexpr int GROUPS = STAGES > 1 && MODE != kForward ? 2 : 1;
   static constexpr int MMA_WARP = 4 * GROUPS, LOAD_WARP = MMA_WARP + 1;
   static constexpr int THREADS = 32 * (LOAD_WARP + 1);
   static constexpr int ROWOPS = MODE == kForward ? 1 : 2;
   static constexpr int PANELS = DP / 64;
-  static constexpr int STAGES = NP == 3 ? (DP == 128 && MODE != kForward ? 1 : 2) : DP == 128 ? 2 : 4;
   static constexpr int ROW_PIECE = kTileRows * DP * 2;
   static constexpr int COL_PIECE = BN * DP * 2;
   static constexpr int COL_STAGE = 2 * NP * COL_PIECE;
   static constexpr int EXTRA = 5 * BN;  // floats a stage: x, y, z, -lse, delta of the columns
-  static constexpr int SMEM = 1024 + ROWOPS * NP * ROW_PIECE + STAGES * (COL_STAGE + EXTRA * 4);
-  // tensor memory columns; with one piece P and dS take the place of the scores they come from
+  // Three pieces: the row operands lie in tensor memory where they fit.  A product of 128 rows and 32 columns reads
+  // 4 KB of rows from shared memory for 1 KB of columns, and six products of pieces make that the bound
+  // (4,096 atoms, 4 heads of 64: query side 578 us, key side 650, without the products 189 and 207).
+  static constexpr bool ROWS_TMEM = NP == 3 && (DP == 64 || MODE == kForward);
+  static constexpr int ROW_BYTES = ROWS_TMEM ? 0 : ROWOPS * NP * ROW_PIECE;
+  // Tensor memory columns.  P and dS (NP * BN / 2 columns each) take the place of the scores they come from.
   // Score buffers: with two, the products of tile j + 1 run under the arithmetic of tile j (a single
   // stage of columns allows one).
   static constexpr int BUFS = STAGES > 1 ? 2 : 1;
-  static constexpr int BUF = (MODE == kForward ? 1 : 2) * BN;  // columns of one buffer
-  static constexpr int T = BN;                                 // T within a buffer
-  static constexpr int SCORES = BUFS * BUF;
-  static constexpr int A0 = NP == 1 ? 0 : SCORES;
-  static constexpr int A1 = NP == 1 ? BN : SCORES + NP * BN / 2;
-  static constexpr int ABUF = NP == 1 ? BUF : 0;  // with one piece every buffer holds its own P and dS
-  static constexpr int ACC = NP == 1 ? SCORES : SCORES + (MODE == kKeySide ? 2 : 1) * NP * BN / 2;
+  static constexpr int T = BN;  // T within a buffer
+  static constexpr int A0 = 0;
+  static constexpr int A1 = NP == 1 ? BN : NP * BN / 2;
+  static constexpr int BUF = MODE == kForward ? (NP == 1 ? BN : NP * BN / 2)
+                             : MODE == kKeySide ? (NP == 1 ? 2 * BN : NP * BN)
+                                                : 2 * BN;
+  static constexpr int ACC = BUFS * BUF;
   // Accumulators: OPS results (dV and dK on the key side).  The tensor cores truncate when they accumulate; three
   // pieces are six products, each of which truncates the long sum.  The score warps therefore add the accumulator
   // to a total in fp32, also in tensor memory, every FLUSH tiles, and it starts again.  With one piece the
@@ -109,7 +113,12 @@ struct AttCfg {
   static constexpr bool FIX = MODE == kQuerySide && NP == 1;
   static constexpr int HALVES = MODE == kKeySide && NP == 3 && DP == 128 ? 2 : 1;  // CTAs that share a width
   static constexpr int W = DP / HALVES;  // columns of one accumulator
-  static constexpr int NEED = ACC + (OPS + TOTALS + (FIX ? 1 : 0)) * W;
+  // the totals lie in shared memory, [component][row], where the row operands leave it free
+  static constexpr bool TOTALS_SMEM = ROWS_TMEM;
+  static constexpr int ROWS = ACC + (OPS + (TOTALS_SMEM ? 0 : TOTALS) + (FIX ? 1 : 0)) * W;  // row operands
+  static constexpr int NEED = ROWS + (ROWS_TMEM ? ROWOPS * NP * DP / 2 : 0);
+  static constexpr int SMEM = 1024 + ROW_BYTES + STAGES * (COL_STAGE + EXTRA * 4) +
+                              (TOTALS_SMEM ? TOTALS * W * kTileRows * 4 : 0);
   static constexpr int COLUMNS = NEED <= 128 ? 128 : NEED <= 256 ? 256 : 512;
   static constexpr int PER_SM_TMEM = 512 / COLUMNS;
   static constexpr int PER_SM_SMEM = (227 * 1024) / (SMEM + 2048);
@@ -225,9 +234,9 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
 
   const uint32_t smem = (tc::smem_addr(tile_smem) + 1023u) & ~1023u;
   const uint32_t row0 = smem, row1 = smem + NP * C::ROW_PIECE;
-  const uint32_t cols = smem + C::ROWOPS * NP * C::ROW_PIECE;
-  float* extra = reinterpret_cast<float*>(tile_smem + (smem - tc::smem_addr(tile_smem)) + C::ROWOPS * NP * C::ROW_PIECE +
-                                          C::STAGES * C::COL_STAGE);
+  const uint32_t cols = smem + C::ROW_BYTES;
+  float* extra = reinterpret_cast<float*>(tile_smem + (cols - tc::smem_addr(tile_smem)) + C::STAGES * C::COL_STAGE);
+  [[maybe_unused]] float* totals = extra + C::STAGES * C::EXTRA;
   const uint32_t bar0 = tc::smem_addr(bars);
   const auto full = [&](int s) { return bar0 + 8 * s; };
   const auto empty = [&](int s) { return bar0 + 8 * (C::STAGES + s); };
@@ -250,7 +259,7 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
     s_abort = 0;
   }
   // row operands, by all threads
-  {
+  if constexpr (!C::ROWS_TMEM) {
     const AttOperand& r0 = MODE == kKeySide ? a.k : a.q;
     load_tile<kTileRows, DP, NP>(row0, r0, item.row, head, item.rows, a.chunks, tid, C::THREADS);
     if constexpr (MODE != kForward) {
@@ -265,6 +274,37 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = s_tmem;
+  if constexpr (C::ROWS_TMEM) {
+    // or into tensor memory, a thread its row: two values a column, DP / 2 columns a piece
+    if (warp < C::MMA_WARP) {
+      const int r = tid & (kTileRows - 1);
+      const uint32_t dst = tmem + (uint32_t(32 * (warp & 3)) << 16) + C::ROWS;
+#pragma unroll 1
+      for (int u = tid / kTileRows; u < C::ROWOPS * NP; u += C::GROUPS) {
+        const int op = u / NP, piece = u - op * NP;
+        const AttOperand& o = MODE == kKeySide ? (op ? a.v : a.k) : op ? a.g : a.q;
+        const __nv_bfloat16* src = o.p + piece * o.piece + (int64_t(item.row) + r) * o.row + head * o.head;
+#pragma unroll
+        for (int c = 0; c < DP / 8; c += 4) {
+          uint32_t w[16];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint4 x = make_uint4(0u, 0u, 0u, 0u);
+            if (r < item.rows && c + k < a.chunks) x = *reinterpret_cast<const uint4*>(src + (c + k) * 8);
+            w[4 * k] = x.x;
+            w[4 * k + 1] = x.y;
+            w[4 * k + 2] = x.z;
+            w[4 * k + 3] = x.w;
+          }
+          tc::st16(dst + u * (DP / 2) + c * 4, w);
+        }
+      }
+      tc::wait_st();
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+  }
 
   if (warp == C::LOAD_WARP) {
     // ---- loading warp.  A full column tile comes by TMA; one cut short by the structure's end by
@@ -325,24 +365,36 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
     if (lane == 0) {
       const int ksteps = (a.D + 15) / 16;
       const uint32_t id_s = tc::idesc_bf16(kTileRows, BN, false), id_a = tc::idesc_bf16(kTileRows, acc_n, true);
+      // One thread issues every MMA, some 70 a tile with three pieces, so its own arithmetic counts: descriptors are
+      // formed once, and each MMA adds a constant to their address field (16-byte units).
+      [[maybe_unused]] const uint64_t rows_desc = tc::desc_sw128(row0, 16, 1024);
+      const uint64_t cols_k = tc::desc_sw128(cols, 16, 1024), cols_mn = tc::desc_sw128(cols, BN * 128, 1024);
       const auto issue_scores = [&](int j) {
         const int s = j % C::STAGES;
         if (!tc::mbar_wait(full(s), (j / C::STAGES) & 1)) return false;
         tc::fence_after();
-        const uint32_t c0 = cols + s * C::COL_STAGE, c1 = c0 + NP * C::COL_PIECE;
+        const uint64_t b0 = cols_k + uint64_t(s * (C::COL_STAGE / 16));
         const uint32_t buf = tmem + (j % C::BUFS) * C::BUF;
 #pragma unroll
-        for (int op = 0; op < C::ROWOPS; ++op) {
-          const uint32_t ra = op ? row1 : row0, cb = op ? c1 : c0, d = buf + (op ? C::T : 0);
+        for (int n = 0; n < Pieces<NP>::N; ++n) {
 #pragma unroll
-          for (int n = 0; n < Pieces<NP>::N; ++n) {
-            for (int ks = 0; ks < ksteps; ++ks) {
-              const uint32_t off = (ks & 3) * 32;
-              tc::mma_ss(d,
-                         tc::desc_sw128(ra + Pieces<NP>::a(n) * C::ROW_PIECE + (ks >> 2) * (kTileRows * 128) + off, 16,
-                                        1024),
-                         tc::desc_sw128(cb + Pieces<NP>::b(n) * C::COL_PIECE + (ks >> 2) * (BN * 128) + off, 16, 1024),
-                         id_s, n > 0 || ks > 0);
+          for (int ks = 0; ks < DP / 16; ++ks) {
+            if (ks < ksteps) {
+#pragma unroll
+              for (int op = 0; op < C::ROWOPS; ++op) {
+                const int off = (ks & 3) * 32;
+                const uint64_t b =
+                    b0 + uint64_t(((op * NP + Pieces<NP>::b(n)) * C::COL_PIECE + (ks >> 2) * (BN * 128) + off) / 16);
+                const uint32_t d = buf + (op ? C::T : 0);
+                if constexpr (C::ROWS_TMEM) {
+                  tc::mma_ts(d, tmem + C::ROWS + (op * NP + Pieces<NP>::a(n)) * (DP / 2) + ks * 8, b, id_s,
+                             n > 0 || ks > 0);
+                } else {
+                  const uint64_t r = rows_desc + uint64_t(((op * NP + Pieces<NP>::a(n)) * C::ROW_PIECE +
+                                                           (ks >> 2) * (kTileRows * 128) + off) / 16);
+                  tc::mma_ss(d, r, b, id_s, n > 0 || ks > 0);
+                }
+              }
             }
           }
         }
@@ -352,25 +404,27 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
       bool ok = total == 0 || issue_scores(0);
       for (int j = 0; ok && j < total; ++j) {
         const int s = j % C::STAGES;
-        const uint32_t c0 = cols + s * C::COL_STAGE, c1 = c0 + NP * C::COL_PIECE;
         if (C::BUFS == 2 && j + 1 < total) ok = issue_scores(j + 1);
         if (!ok) break;
         ok = tc::mbar_wait(p_ready(j), (j / C::BUFS) & 1);
         if (!ok) break;
         tc::fence_after();
         // forward: P x V; query side: dS x K (and P x K); key side: P x G and dS x Q
+        const uint64_t b0 = cols_mn + uint64_t(s * (C::COL_STAGE / 16) + half * (BN * 128 / 16));
+        const uint32_t buf = tmem + (j % C::BUFS) * C::BUF;
+        const uint32_t go_on = C::TOTALS ? j % C::FLUSH > 0 : j > 0;
 #pragma unroll
-        for (int op = 0; op < C::OPS + (C::FIX ? 1 : 0); ++op) {
-          const uint32_t A = tmem + (j % C::BUFS) * C::ABUF + (op == 0 ? C::A0 : C::A1);
-          const uint32_t cb = (MODE == kForward || (MODE == kKeySide && op == 0) ? c1 : c0) + half * (BN * 128);
+        for (int n = 0; n < Pieces<NP>::N; ++n) {
 #pragma unroll
-          for (int n = 0; n < Pieces<NP>::N; ++n) {
-            const uint32_t d = tmem + C::ACC + op * C::W;
+          for (int ks = 0; ks < BN / 16; ++ks) {
 #pragma unroll
-            for (int ks = 0; ks < BN / 16; ++ks)
-              tc::mma_ts(d, A + Pieces<NP>::a(n) * (BN / 2) + ks * 8,
-                         tc::desc_sw128(cb + Pieces<NP>::b(n) * C::COL_PIECE + ks * 2048, BN * 128, 1024), id_a,
-                         (C::TOTALS ? j % C::FLUSH > 0 : j > 0) || n > 0 || ks > 0);
+            for (int op = 0; op < C::OPS + (C::FIX ? 1 : 0); ++op) {
+              const int second = MODE == kForward || (MODE == kKeySide && op == 0) ? 1 : 0;  // V or G
+              tc::mma_ts(tmem + C::ACC + op * C::W,
+                         buf + (op == 0 ? C::A0 : C::A1) + Pieces<NP>::a(n) * (BN / 2) + ks * 8,
+                         b0 + uint64_t(((second * NP + Pieces<NP>::b(n)) * C::COL_PIECE + ks * 2048) / 16), id_a,
+                         n > 0 || ks > 0 ? 1u : go_on);
+            }
           }
         }
         tc::commit(empty(s));
@@ -446,17 +500,29 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
 
     // The accumulators of the tiles before j into the totals.
     const auto flush = [&](int j) {
+      const bool first = j == C::FLUSH;
       for (int d = 0; d < C::OPS * C::W; d += 16) {
         float o[16], e[16];
         tc::ld16(lane_base + C::ACC + d, o);
-        if (j > C::FLUSH) tc::ld16(lane_base + C::ACC + C::OPS * C::W + d, e);
-        tc::wait_ld();
-        uint32_t r[16];
+        if (!C::TOTALS_SMEM && !first) tc::ld16(lane_base + C::ACC + C::OPS * C::W + d, e);
+        if (C::TOTALS_SMEM && !first) {
 #pragma unroll
-        for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(j > C::FLUSH ? e[k] + o[k] : o[k]);
-        tc::st16(lane_base + C::ACC + C::OPS * C::W + d, r);
+          for (int k = 0; k < 16; ++k) e[k] = totals[(d + k) * kTileRows + r_tile];
+        }
+        tc::wait_ld();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) o[k] = first ? o[k] : e[k] + o[k];
+        if constexpr (C::TOTALS_SMEM) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) totals[(d + k) * kTileRows + r_tile] = o[k];
+        } else {
+          uint32_t r[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(o[k]);
+          tc::st16(lane_base + C::ACC + C::OPS * C::W + d, r);
+        }
       }
-      tc::wait_st();
+      if constexpr (!C::TOTALS_SMEM) tc::wait_st();
     };
 
     // One tile's arithmetic; n < BN columns where CUT, all of them otherwise.
@@ -505,7 +571,7 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
             return false;
           tc::fence_after();
 #pragma unroll
-          for (int u = 0; u < C::OPS + C::TOTALS; ++u) {
+          for (int u = 0; u < C::OPS + (C::TOTALS_SMEM ? 0 : C::TOTALS); ++u) {
             for (int d = 0; d < acc_n; d += 16) {
               float o[16];
               tc::ld16(lane_base + C::ACC + u * C::W + d, o);
@@ -517,12 +583,17 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
             }
           }
           tc::wait_st();
+          if constexpr (C::TOTALS_SMEM) {
+            if (j > C::FLUSH) {
+              for (int d = 0; d < acc_n; ++d) totals[d * kTileRows + r_tile] *= f;
+            }
+          }
         }
       }
       const float ref = m == -INFINITY ? 0.0f : m;
       const tc::f2 nref = tc::pack(-ref, -ref);
       tc::f2 l0 = tc::pack(0.0f, 0.0f), l1 = l0;
-      const uint32_t dst = lane_base + C::A0 + (j % C::BUFS) * C::ABUF;
+      const uint32_t dst = lane_base + C::A0 + (j % C::BUFS) * C::BUF;
 #pragma unroll
       for (int c0 = 0; c0 < BN; c0 += 16) {
         uint32_t pr[NP][8];
@@ -550,16 +621,22 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
 
     const auto backward_tile = [&](auto cut, int j, int n, const float* ex, uint32_t buf) {
       constexpr bool CUT = decltype(cut)::value;
-      const uint32_t dst = lane_base + (j % C::BUFS) * C::ABUF;
-      float sv[2][16], tv[2][16];
-      tc::ld16(buf, sv[0]);
-      tc::ld16(buf + C::T, tv[0]);
+      const uint32_t dst = lane_base + (j % C::BUFS) * C::BUF;
+      // One piece: the next 16 columns load under these; P and dS of columns c0 .. take half of the columns that were
+      // read.  Several pieces take more than that: all scores come to registers first.
+      constexpr int HOLD = NP == 1 ? 2 : BN / 16;
+      float sv[HOLD][16], tv[HOLD][16];
+#pragma unroll
+      for (int k = 0; k < (NP == 1 ? 1 : HOLD); ++k) {
+        tc::ld16(buf + 16 * k, sv[k]);
+        tc::ld16(buf + C::T + 16 * k, tv[k]);
+      }
 #pragma unroll
       for (int c0 = 0; c0 < BN; c0 += 16) {
         constexpr int kLast = BN - 16;
-        const int cur = (c0 / 16) & 1;
-        tc::wait_ld();
-        if (c0 < kLast) {
+        const int cur = (c0 / 16) % HOLD;
+        if (NP == 1 || c0 == 0) tc::wait_ld();
+        if (NP == 1 && c0 < kLast) {
           tc::ld16(buf + c0 + 16, sv[cur ^ 1]);
           tc::ld16(buf + C::T + c0 + 16, tv[cur ^ 1]);
         }
@@ -627,7 +704,6 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
 #pragma unroll
           for (int k = 0; k < NP; ++k) dr[k][c / 2] = q[k];
         }
-        // with one piece, columns c0 / 2 .. c0 / 2 + 8 hold scores that are already in registers
 #pragma unroll
         for (int k = 0; k < NP; ++k) {
           // key side: P first, then dS; query side: dS first
@@ -645,9 +721,6 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
       const int sub = MODE == kKeySide ? j / ntiles : 0, jt = MODE == kKeySide ? j - sub * ntiles : j;
       const int n = item.cols - jt * BN;  // columns there are, BN or more in a full tile
       ok = tc::mbar_wait(full(s), (j / C::STAGES) & 1) && tc::mbar_wait(s_ready(j), (j / C::BUFS) & 1);
-      // several pieces have one place for P and dS: the product before must be done with it
-      if (NP > 1 && j > 0 && ok && (C::BUFS == 2 || j % C::FLUSH == 0))
-        ok = tc::mbar_wait(empty((j - 1) % C::STAGES), ((j - 1) / C::STAGES) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc::fence_after();
@@ -655,9 +728,6 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
       const uint32_t buf = lane_base + (j % C::BUFS) * C::BUF;
       // a warp without a row of the item only keeps the barriers going: its lanes of P reach no result
       if (32 * (warp & 3) < item.rows) {
-        if constexpr (C::TOTALS > 0) {
-          if (j > 0 && j % C::FLUSH == 0) flush(j);
-        }
         if constexpr (MODE == kForward) {
           ok = n >= BN ? forward_tile(std::false_type{}, j, n, ex, buf) : forward_tile(std::true_type{}, j, n, ex, buf);
           if (!ok) break;
@@ -676,6 +746,15 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
         }
       }
       tc::wait_st();
+      if constexpr (C::TOTALS > 0) {
+        // the product of this tile starts the accumulators again: what they hold goes to the totals
+        if (j > 0 && j % C::FLUSH == 0) {
+          ok = __all_sync(0xffffffffu, tc::mbar_wait(empty((j - 1) % C::STAGES), ((j - 1) / C::STAGES) & 1));
+          if (!ok) break;
+          tc::fence_after();
+          flush(j);
+        }
+      }
       tc::fence_before();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(p_ready(j));
@@ -731,7 +810,12 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
           tc::ld16(lane_base + C::ACC + op * C::W + d, o);
           if constexpr (C::TOTALS > 0 || C::FIX) {
             float e[16];
-            tc::ld16(lane_base + C::ACC + (C::OPS + op) * C::W + d, e);
+            if constexpr (C::TOTALS_SMEM) {
+#pragma unroll
+              for (int k = 0; k < 16; ++k) e[k] = totals[(op * C::W + d + k) * kTileRows + r_tile];
+            } else {
+              tc::ld16(lane_base + C::ACC + (C::OPS + op) * C::W + d, e);
+            }
             tc::wait_ld();
             const bool whole = C::TOTALS > 0 && total <= C::FLUSH;  // nothing went into the total
             if (whole) {
