@@ -362,19 +362,25 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
     if (!ok) s_abort = 1;
   } else if (warp == C::MMA_WARP) {
     // ---- MMA issue: scores of tile j, then (when P is back) its accumulating product
-    if (lane == 0) {
+    {
+      const bool lead = tc::elect();
       const int ksteps = (a.D + 15) / 16;
       const uint32_t id_s = tc::idesc_bf16(kTileRows, BN, false), id_a = tc::idesc_bf16(kTileRows, acc_n, true);
-      // One thread issues every MMA, some 70 a tile with three pieces, so its own arithmetic counts: descriptors are
-      // formed once, and each MMA adds a constant to their address field (16-byte units).
+      // every lane waits, one issues
+      const auto wait = [&](uint32_t bar, uint32_t parity) {
+        const bool done = __all_sync(0xffffffffu, tc::mbar_wait(bar, parity));
+        tc::fence_after();
+        return done;
+      };
+      // Descriptors are formed once, and each MMA adds a constant to their address field (16-byte units).
       [[maybe_unused]] const uint64_t rows_desc = tc::desc_sw128(row0, 16, 1024);
       const uint64_t cols_k = tc::desc_sw128(cols, 16, 1024), cols_mn = tc::desc_sw128(cols, BN * 128, 1024);
       const auto issue_scores = [&](int j) {
         const int s = j % C::STAGES;
-        if (!tc::mbar_wait(full(s), (j / C::STAGES) & 1)) return false;
-        tc::fence_after();
+        if (!wait(full(s), (j / C::STAGES) & 1)) return false;
         const uint64_t b0 = cols_k + uint64_t(s * (C::COL_STAGE / 16));
         const uint32_t buf = tmem + (j % C::BUFS) * C::BUF;
+        if (lead) {
 #pragma unroll
         for (int n = 0; n < Pieces<NP>::N; ++n) {
 #pragma unroll
@@ -399,6 +405,8 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
           }
         }
         tc::commit(s_ready(j));
+        }
+        __syncwarp();
         return true;
       };
       bool ok = total == 0 || issue_scores(0);
@@ -406,13 +414,13 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
         const int s = j % C::STAGES;
         if (C::BUFS == 2 && j + 1 < total) ok = issue_scores(j + 1);
         if (!ok) break;
-        ok = tc::mbar_wait(p_ready(j), (j / C::BUFS) & 1);
+        ok = wait(p_ready(j), (j / C::BUFS) & 1);
         if (!ok) break;
-        tc::fence_after();
         // forward: P x V; query side: dS x K (and P x K); key side: P x G and dS x Q
         const uint64_t b0 = cols_mn + uint64_t(s * (C::COL_STAGE / 16) + half * (BN * 128 / 16));
         const uint32_t buf = tmem + (j % C::BUFS) * C::BUF;
         const uint32_t go_on = C::TOTALS ? j % C::FLUSH > 0 : j > 0;
+        if (lead) {
 #pragma unroll
         for (int n = 0; n < Pieces<NP>::N; ++n) {
 #pragma unroll
@@ -428,11 +436,13 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
           }
         }
         tc::commit(empty(s));
+        }
+        __syncwarp();
         if (C::BUFS == 1 && j + 1 < total) ok = issue_scores(j + 1);
       }
       if (!ok) {
         s_abort = 1;
-        tc::commit(drain);
+        if (lead) tc::commit(drain);
         tc::mbar_wait(drain, 0);
       }
     }
