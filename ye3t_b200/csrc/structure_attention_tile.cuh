@@ -74,11 +74,17 @@ struct AttTileArgs {
 
 template <int MODE, int DP, int NP>
 struct AttCfg {
-  static constexpr int BN = NP == 1 && MODE == kForward ? 64 : NP == 1 || DP == 64 || MODE == kForward ? 32 : 16;
+  static constexpr bool KEY_BF16 = MODE == kKeySide && NP == 1 && DP == 64;
+  // Columns a tile: as many as tensor and shared memory hold.  Twice the columns are 23 and 26 % faster on the
+  // backward of 128-wide heads in bf16 and 14 % on the fp32 query side (4,096 atoms, 4 heads).
+  static constexpr int BN = NP == 1 ? (MODE == kQuerySide && DP == 64 ? 32 : 64)
+                            : DP == 64 ? (MODE == kQuerySide ? 64 : 32)
+                                       : (MODE == kForward ? 32 : 16);
   static constexpr int STAGES = NP == 3 ? (DP == 128 && MODE != kForward ? 1 : 2) : DP == 128 ? 2 : 4;
-  // Score groups of four warps; with two, each takes every other column tile.  The backward with one piece is
-  // 14 % faster with two (8,192 atoms, 8 heads of 64); the forward, which needs more registers, 10 % slower.
-  static constexpr int GROUPS = STAGES > 1 && MODE != kForward ? 2 : 1;
+  // Score groups of four warps; with two, each takes every other column tile: for what leaves an SM a single CTA.
+  // Two CTAs of one group with 64 columns a tile and one buffer (key side), or 32 and two (query side), are 6 and 7 %
+  // faster than two of two groups (8,192 atoms, 8 heads of 64: 636 against 677 us, 777 against 837).
+  static constexpr int GROUPS = MODE != kForward && STAGES > 1 && (NP == 3 || DP == 128) ? 2 : 1;
   static constexpr int MMA_WARP = 4 * GROUPS, LOAD_WARP = MMA_WARP + 1;
   static constexpr int THREADS = 32 * (LOAD_WARP + 1);
   static constexpr int ROWOPS = MODE == kForward ? 1 : 2;
@@ -95,7 +101,7 @@ struct AttCfg {
   // Tensor memory columns.  P and dS (NP * BN / 2 columns each) take the place of the scores they come from.
   // Score buffers: with two, the products of tile j + 1 run under the arithmetic of tile j (a single
   // stage of columns allows one).
-  static constexpr int BUFS = STAGES > 1 ? 2 : 1;
+  static constexpr int BUFS = STAGES > 1 && !KEY_BF16 ? 2 : 1;
   static constexpr int T = BN;  // T within a buffer
   static constexpr int A0 = 0;
   static constexpr int A1 = NP == 1 ? BN : NP * BN / 2;
@@ -105,7 +111,7 @@ struct AttCfg {
   static constexpr int ACC = BUFS * BUF;
   // Accumulators: OPS results (dV and dK on the key side).  The tensor cores truncate when they accumulate; three
   // pieces are six products, each of which truncates the long sum.  The score warps therefore add the accumulator
-  // to a total in fp32, also in tensor memory, every FLUSH tiles, and it starts again.  With one piece the
+  // to a total in fp32 every FLUSH tiles, and it starts again.  With one piece the
   // query side also accumulates P K, to correct dQ for the rounding of delta.
   static constexpr int OPS = MODE == kKeySide ? 2 : 1;
   static constexpr int FLUSH = 2;
@@ -120,6 +126,7 @@ struct AttCfg {
   static constexpr int SMEM = 1024 + ROW_BYTES + STAGES * (COL_STAGE + EXTRA * 4) +
                               (TOTALS_SMEM ? TOTALS * W * kTileRows * 4 : 0);
   static constexpr int COLUMNS = NEED <= 128 ? 128 : NEED <= 256 ? 256 : 512;
+  static_assert(NEED <= 512 && SMEM <= 227 * 1024 && ACC % 16 == 0 && FLUSH % GROUPS == 0, "tile shape");
   static constexpr int PER_SM_TMEM = 512 / COLUMNS;
   static constexpr int PER_SM_SMEM = (227 * 1024) / (SMEM + 2048);
   static constexpr int PER_SM_MIN = PER_SM_TMEM < PER_SM_SMEM ? PER_SM_TMEM : PER_SM_SMEM;
