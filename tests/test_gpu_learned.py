@@ -320,6 +320,31 @@ def test_attention_on_another_stream():
     assert torch.equal(want[0], got[0]) and all(torch.equal(s, t) for s, t in zip(want[1], got[1]))
 
 
+def test_attention_from_a_thread_of_its_own():
+    """A thread's first CUDA work is the call itself: no context is current there yet."""
+    import threading
+    from ye3t_b200 import runtime as rt
+    n = [300, 200]
+    q, k, v, grad, x, _, sl = _inputs(n, n, 2, 2, 64, torch.bfloat16, 4)
+    layout = rt.StructureLayout(n, heads=2, device=DEV)
+    want = rt.structure_attention(q, k, v, layout, positions=x, slopes=sl)
+    torch.cuda.synchronize()
+    got = []
+
+    def work():
+        try:
+            got.append(rt.structure_attention(q, k, v, layout, positions=x, slopes=sl))
+        except Exception as exc:  # noqa: BLE001 - shown by the assertion
+            got.append(exc)
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert isinstance(got[0], torch.Tensor), got[0]
+    assert torch.equal(got[0], want)
+
+
 def test_attention_empty_batches():
     from ye3t_b200 import runtime as rt
     for queries, keys in (([], []), ([0, 0], [0, 0]), ([0, 0], [3, 4]), ([3, 4], [0, 0])):

@@ -316,36 +316,57 @@ __global__ void __launch_bounds__(32 * kRowWarps) row_backward_key_kernel(
   }
 }
 
-// dx[i] = sum over heads of dx_part (and of dy_part where queries and keys are the same
-// atoms); dy[j] likewise.  One thread per component.
-__global__ void __launch_bounds__(256) position_grad_kernel(const float* __restrict__ part, int64_t n, int heads,
-                                                            const float* __restrict__ other, int other_heads,
-                                                            float* __restrict__ out) {
-  const int64_t t = blockIdx.x * int64_t(blockDim.x) + threadIdx.x;
-  if (t >= n * 3) return;
-  const int64_t i = t / 3;
-  const int c = int(t - 3 * i);
+// What the parts add up to, in one launch: dx[i] = sum over heads of dx_part (and of dy_part where queries and keys
+// are the same atoms), dy[j] likewise, one thread a component; then dslope[h] = sum over rows, one CTA a head,
+// in fp64 and a fixed order.
+struct FinishArgs {
+  const float* dx_part;
+  const float* dy_part;
+  const float* slope_part;
+  float* dx;
+  float* dy;  // null: dx takes both sums
+  float* dslopes;
+  int64_t nq, nk;
+  int H, Hk;
+  unsigned x_ctas, y_ctas;
+};
+constexpr int kFinishThreads = 512;
+
+__device__ __forceinline__ float head_sum(const float* part, int64_t i, int c, int heads) {
   float sum = 0.0f;
+#pragma unroll 4
   for (int h = 0; h < heads; ++h) sum += part[(i * heads + h) * 3 + c];
-  if (other)
-    for (int h = 0; h < other_heads; ++h) sum += other[(i * other_heads + h) * 3 + c];
-  out[t] = sum;
+  return sum;
 }
 
-// dslope[h] = sum over rows, one CTA a head, summed in fp64 in a fixed order.
-__global__ void __launch_bounds__(256) slope_grad_kernel(const float* __restrict__ part, int64_t n, int H,
-                                                         float* __restrict__ out) {
-  __shared__ double s[256];
-  const int h = blockIdx.x;
+__global__ void __launch_bounds__(kFinishThreads) finish_kernel(const __grid_constant__ FinishArgs a) {
+  __shared__ double s[kFinishThreads];
+  if (blockIdx.x < a.x_ctas + a.y_ctas) {
+    const bool keys = blockIdx.x >= a.x_ctas;
+    const int64_t t = (blockIdx.x - (keys ? a.x_ctas : 0u)) * int64_t(kFinishThreads) + threadIdx.x;
+    if (t >= (keys ? a.nk : a.nq) * 3) return;
+    const int64_t i = t / 3;
+    const int c = int(t - 3 * i);
+    if (keys) {
+      a.dy[t] = head_sum(a.dy_part, i, c, a.Hk);
+    } else {
+      float sum = head_sum(a.dx_part, i, c, a.H);
+      if (a.dy == nullptr && a.nk > 0) sum += head_sum(a.dy_part, i, c, a.Hk);
+      a.dx[t] = sum;
+    }
+    return;
+  }
+  const int h = int(blockIdx.x - a.x_ctas - a.y_ctas);
   double sum = 0.0;
-  for (int64_t i = threadIdx.x; i < n; i += 256) sum += double(part[i * H + h]);
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < a.nq; i += kFinishThreads) sum += double(a.slope_part[i * a.H + h]);
   s[threadIdx.x] = sum;
   __syncthreads();
-  for (int o = 128; o > 0; o >>= 1) {
+  for (int o = kFinishThreads / 2; o > 0; o >>= 1) {
     if (int(threadIdx.x) < o) s[threadIdx.x] += s[threadIdx.x + o];
     __syncthreads();
   }
-  if (threadIdx.x == 0) out[h] = float(s[0]);
+  if (threadIdx.x == 0) a.dslopes[h] = float(s[0]);
 }
 
 int unpack(const y3b_structure_attention_args* p, const char* what, AttArgs* a) {
@@ -571,7 +592,19 @@ __global__ void __launch_bounds__(128) join_key_kernel(const AttJoin* __restrict
 }
 
 // ---------------------------------------------------------------------------
+constexpr int kJoinCtas = kTileRows / 4;  // CTAs of a tile's join
+
 unsigned row_grid(int64_t tasks) { return unsigned((tasks + kRowWarps - 1) / kRowWarps); }
+
+// Launch grids that the tables ask for stay within 2^31 - 1 CTAs.
+int check_grids(const y3b_structure_attention_args* p, const char* what) {
+  const int64_t most = int64_t(INT32_MAX) / kJoinCtas;
+  if (p->query_row_count * p->heads > INT32_MAX || p->key_row_count * p->key_heads > INT32_MAX ||
+      p->query_join_count * p->heads > most || p->few_join_count * p->heads > most ||
+      p->key_join_count * p->key_heads > most)
+    return fail(Y3B_ERR_UNSUPPORTED, "%s: the batch's tables ask for more than 2^31 - 1 CTAs", what);
+  return Y3B_OK;
+}
 
 bool on16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
@@ -715,7 +748,7 @@ int forward(const y3b_structure_attention_args* p, const AttArgs& a, const AttPl
     rc = attention_forward_tiles(w.pieces, t, p->query_item_count, s);
     if (rc) return rc;
     if (p->query_join_count > 0) {
-      join_forward_kernel<T><<<unsigned(p->query_join_count * a.H * (kTileRows / 4)), 128, 0, s>>>(
+      join_forward_kernel<T><<<unsigned(p->query_join_count * a.H * kJoinCtas), 128, 0, s>>>(
           reinterpret_cast<const AttJoin*>(p->query_joins), t.part, kTileRows, w.Wf, w.DP, a.D, a.H, static_cast<T*>(out), lse);
       Y3B_LAUNCH_CHECK();
     }
@@ -773,7 +806,7 @@ int backward(const y3b_structure_attention_args* p, const AttArgs& a, const AttP
     const int rc = attention_query_tiles(w.pieces, t, p->query_item_count, s);
     if (rc) return rc;
     if (p->query_join_count > 0) {
-      join_query_kernel<T><<<unsigned(p->query_join_count * a.H * (kTileRows / 4)), 128, 0, s>>>(
+      join_query_kernel<T><<<unsigned(p->query_join_count * a.H * kJoinCtas), 128, 0, s>>>(
           reinterpret_cast<const AttJoin*>(p->query_joins), t.part, kTileRows, w.Wq, w.DP, a.D, a.H, a.scale,
           w.pieces == 1, a.slopes,
           static_cast<T*>(dq), delta, slope_part, dx_part);
@@ -795,20 +828,17 @@ int backward(const y3b_structure_attention_args* p, const AttArgs& a, const AttP
     const int rc = attention_key_tiles(w.pieces, t, p->key_item_count, s);
     if (rc) return rc;
     if (p->key_join_count > 0) {
-      join_key_kernel<T><<<unsigned(p->key_join_count * a.Hk * (kTileRows / 4)), 128, 0, s>>>(
+      join_key_kernel<T><<<unsigned(p->key_join_count * a.Hk * kJoinCtas), 128, 0, s>>>(
           reinterpret_cast<const AttJoin*>(p->key_joins), t.part, kTileRows, w.Wk, w.DP, a.D, a.Hk, a.scale,
           static_cast<T*>(dk), static_cast<T*>(dv), a.slopes ? dy_part : nullptr);
       Y3B_LAUNCH_CHECK();
     }
   }
   if (a.slopes) {
-    // dy == null: queries and keys are the same atoms and dx takes both sums
-    if (a.nq > 0)
-      position_grad_kernel<<<unsigned((a.nq * 3 + 255) / 256), 256, 0, s>>>(
-          dx_part, a.nq, a.H, dy == nullptr && a.nk > 0 ? dy_part : nullptr, a.Hk, dx);
-    if (dy && a.nk > 0)
-      position_grad_kernel<<<unsigned((a.nk * 3 + 255) / 256), 256, 0, s>>>(dy_part, a.nk, a.Hk, nullptr, 0, dy);
-    slope_grad_kernel<<<a.H, 256, 0, s>>>(slope_part, a.nq, a.H, dslopes);
+    const auto ctas = [](int64_t n) { return unsigned((n * 3 + kFinishThreads - 1) / kFinishThreads); };
+    const FinishArgs f{dx_part, dy_part, slope_part, dx, dy, dslopes, a.nq, a.nk, a.H, a.Hk, ctas(a.nq),
+                       dy ? ctas(a.nk) : 0u};
+    finish_kernel<<<f.x_ctas + f.y_ctas + unsigned(a.H), kFinishThreads, 0, s>>>(f);
     Y3B_LAUNCH_CHECK();
   }
   return Y3B_OK;
@@ -835,6 +865,10 @@ int encode_columns(CUtensorMap* map, const AttOperand& o, int D, int heads, int6
   }();
   if (rows == 0) return Y3B_OK;  // no column is loaded
   if (!encode) return fail(Y3B_ERR_CUDA, "structure_attention: the driver has no cuTensorMapEncodeTiled");
+  // the encoder is a driver call: a thread that has not used the runtime yet (as autograd's) has no context current
+  int device = 0;
+  Y3B_CUDA_TRY(cudaGetDevice(&device));
+  Y3B_CUDA_TRY(cudaSetDevice(device));
   const int width = (D + 7) / 8 * 8;
   const cuuint64_t size[4] = {cuuint64_t(width), cuuint64_t(heads), cuuint64_t(rows), cuuint64_t(pieces)};
   const cuuint64_t stride[3] = {cuuint64_t(o.head) * 2, cuuint64_t(o.row) * 2,
@@ -873,6 +907,8 @@ extern "C" int y3b_structure_attention(const y3b_structure_attention_args* args,
   int rc = unpack(args, "structure_attention", &a);
   if (rc) return rc;
   if (a.nq == 0) return Y3B_OK;
+  rc = check_grids(args, "structure_attention");
+  if (rc) return rc;
   Y3B_CHECK_ARG(out && lse, "structure_attention: null output");
   const AttPlan w = make_plan(args, false);
   rc = check_workspace(w, workspace, workspace_bytes, "structure_attention");
@@ -897,6 +933,8 @@ extern "C" int y3b_structure_attention_adjoint(const y3b_structure_attention_arg
                 "structure_attention_adjoint: null position or slope gradient");
   Y3B_CHECK_ARG(!a.slopes || key_positions_grad || a.nk == 0 || a.nq == a.nk,
                 "structure_attention_adjoint: one position gradient needs as many queries as keys");
+  rc = check_grids(args, "structure_attention_adjoint");
+  if (rc) return rc;
   const AttPlan w = make_plan(args, true);
   rc = check_workspace(w, workspace, workspace_bytes, "structure_attention_adjoint");
   if (rc) return rc;

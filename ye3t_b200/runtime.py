@@ -755,8 +755,8 @@ def _attention_workspace(args, adjoint, device):
 
 def _attention_forward(query, key, value, x, y, slopes, layout, scale, validate):
     q, k, v = _dense_rows(query), _dense_rows(key), _dense_rows(value)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+    out = q.new_empty(q.shape)
+    lse = q.new_empty(q.shape[:2], dtype=torch.float32)
     args = _attention_args(q, k, v, x, y, slopes, layout, scale)
     ws, ws_bytes = _attention_workspace(args, 0, q.device)
     status = _status(q.device) if validate else None
@@ -786,9 +786,7 @@ class _StructureAttention(torch.autograd.Function):
         query, key, value, x, y, slopes, out, lse = ctx.saved_tensors
         layout, dev = ctx.layout, query.device
         q, k, v, g = _dense_rows(query), _dense_rows(key), _dense_rows(value), grad.contiguous()
-        dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=dev)
-        dv = torch.empty(v.shape, dtype=v.dtype, device=dev)
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
         dx = dy = dslopes = None
         if slopes is not None:
             dx, dslopes = torch.empty_like(x), torch.empty_like(slopes)
