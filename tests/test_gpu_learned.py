@@ -320,6 +320,125 @@ def test_attention_on_another_stream():
     assert torch.equal(want[0], got[0]) and all(torch.equal(s, t) for s, t in zip(want[1], got[1]))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_attention_mixed_batch(dtype):
+    """Every kind of structure in one batch: none, single atoms and keys, molecules, one or two queries over many
+    keys, and structures of several tiles."""
+    queries = [0, 1, 5, 1, 2, 200, 300, 64, 65, 3] + [20] * 300
+    keys = [3, 1, 0, 500, 900, 200, 1, 64, 65, 70] + [20] * 300
+    _check(queries, keys, 4, 2, 64, dtype, seed=17)
+    _check([20] * 80 + [500, 1, 0, 64], [20] * 80 + [500, 1, 0, 64], 4, 4, 40, dtype, same=True, seed=18)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_attention_long_and_split(dtype):
+    """Columns split over several CTAs and joined on both sides, many tiles of rescaled rows."""
+    _check([130, 2], [2100, 9], 2, 1, 64, dtype, seed=31)
+    _check([1500], [140], 2, 1, 128, dtype, seed=32)
+    from ye3t_b200 import runtime as rt
+    q, k, v, grad, x, y, sl = _inputs([150], [1300], 2, 2, 64, dtype, 33)
+    # scores that rise along the keys: the running maximum moves at every tile
+    ramp = torch.linspace(0, 30, 1300, device=DEV)[:, None, None]
+    k = (k * 0.1 + ramp * q.float().mean(0) / q.float().mean(0).norm(dim=-1, keepdim=True) ** 2).to(dtype)
+    out, grads, _ = _run(rt, q, k, v, grad, x, y, sl, [150], [1300], 1.0, False)
+    ref = _plain(q, k, v, x, y, sl, 1.0, [150], [1300], grad)
+    # scores of some hundreds carry 2^-24 of themselves
+    _close(out, ref[0], 1e-4 if dtype == torch.float32 else 6e-3, "out")
+
+
+def test_attention_offsets_past_32_bits():
+    """Rows so far apart that their offsets pass 2^32 elements."""
+    from ye3t_b200 import runtime as rt
+    n, far = 2200, 1 << 21
+    base = torch.zeros(n * far, dtype=torch.bfloat16, device=DEV)
+    for queries in ([n], [1]):
+        q, k, v, _, x, y, sl = _inputs(queries, [n], 1, 1, 32, torch.bfloat16, 5)
+        wide = base.as_strided((n, 2, 1, 32), (far, 1 << 20, 32, 1))
+        wide[:, 0], wide[:, 1] = k, v
+        layout = rt.StructureLayout(queries, [n], heads=1, device=DEV)
+        near = rt.structure_attention(q, k, v, layout, positions=x, key_positions=y, slopes=sl)
+        got = rt.structure_attention(q, wide[:, 0], wide[:, 1], layout, positions=x, key_positions=y, slopes=sl)
+        assert torch.equal(near, got)
+
+
+def test_embedding_past_32_bits():
+    from ye3t_b200 import runtime as rt
+    n, c = (1 << 21) + 5, 1025
+    table = torch.randn(7, c, device=DEV).bfloat16()
+    z = torch.arange(n, device=DEV) % 7
+    out = rt.species_embedding(table, z)
+    rows = torch.tensor([0, 1, (1 << 20) + 3, n - 2, n - 1], device=DEV)
+    assert torch.equal(out[rows], table[z[rows]])
+    dt = rt._embedding_adjoint(out, z, 7, 1.0)
+    # bf16 inputs summed in fp32: each species' sum is its row times its count
+    want = table.double() * torch.bincount(z).double()[:, None]
+    _close(dt, want, TOL[torch.bfloat16])
+
+
+def test_learned_in_a_cuda_graph():
+    from ye3t_b200 import runtime as rt
+    n = [300, 20, 1]
+    q, k, v, _, x, _, sl = _inputs(n, n, 2, 2, 64, torch.bfloat16, 4)
+    layout = rt.StructureLayout(n, heads=2, device=DEV)
+    table, z = torch.randn(5, 64, device=DEV), torch.randint(0, 5, (321,), device=DEV)
+
+    def step():
+        return rt.structure_attention(q, k, v, layout, positions=x, slopes=sl), rt.species_embedding(table, z)
+
+    want = step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    q.add_(1.0)
+    z.add_(1).remainder_(5)
+    graph.replay()
+    again = step()
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+    assert not torch.equal(got[0], want[0])
+
+
+def test_learned_torch_ops():
+    """torch.ops.ye3t_b200.* give the runtime functions' results and gradients."""
+    import ye3t_b200.torch_ops  # noqa: F401
+    from ye3t_b200 import runtime as rt
+    ops = torch.ops.ye3t_b200
+    n = [70, 1, 0, 30]
+    q, k, v, grad, x, _, sl = _inputs(n, n, 4, 2, 48, torch.float32, 6)
+    layout = rt.StructureLayout(n, heads=4, key_heads=2, device=DEV)
+    want, grads, _ = _run(rt, q, k, v, grad, x, x, sl, n, n, 0.3, True)
+    args = [t.detach().requires_grad_(True) for t in (q, k, v, x, sl)]
+    out, _ = ops.structure_attention(args[0], args[1], args[2], layout.tables, layout.counts, args[3], None, args[4], 0.3)
+    assert torch.equal(out, want)
+    for a, b in zip(torch.autograd.grad(out, args, grad), grads):
+        assert torch.equal(a, b)
+    out, _ = ops.structure_attention(q, k, v, layout.tables, layout.counts, None, None, None, 0.3)
+    assert torch.equal(out, rt.structure_attention(q, k, v, layout, scale=0.3))
+    table = torch.randn(9, 20, device=DEV, requires_grad=True)
+    z = torch.randint(0, 9, (100,), device=DEV)
+    g = torch.randn(100, 20, device=DEV)
+    a, b = ops.species_embedding(table, z, 2.0), rt.species_embedding(table, z, scale=2.0)
+    assert torch.equal(a, b)
+    assert torch.equal(torch.autograd.grad(a, table, g)[0], torch.autograd.grad(b, table, g)[0])
+    with pytest.raises(ValueError):
+        rt.StructureLayout.from_tensors(layout.tables[:-1], layout.counts)
+    with pytest.raises(ValueError):
+        rt.StructureLayout.from_tensors(layout.tables, layout.counts[:-1])
+
+
+def test_attention_energies_example():
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples",
+                        "attention_energies.py")
+    spec = importlib.util.spec_from_file_location("attention_energies", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    losses, forces = example.train(25, log=None)
+    assert losses[-1] < 0.5 * losses[0]
+    assert torch.isfinite(forces).all() and float(forces.norm()) > 0
+
+
 def test_attention_from_a_thread_of_its_own():
     """A thread's first CUDA work is the call itself: no context is current there yet."""
     import threading

@@ -2,6 +2,8 @@
 
 import ctypes
 
+
+import numpy as np
 import pytest
 import torch
 
@@ -81,3 +83,68 @@ def test_argument_struct_layout(tmp_path):
     out = [int(v) for v in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
     assert out[0] == ctypes.sizeof(cls)
     assert out[1:] == [getattr(cls, f).offset for f in fields]
+
+
+def _random_counts(rng):
+    n = int(rng.integers(1, 30))
+    big = int(rng.choice([3, 40, 200, 3000]))
+    queries, keys = rng.integers(0, big, n), rng.integers(0, big, n)
+    if rng.random() < 0.3:
+        queries = np.minimum(queries, 2)
+    return queries, keys
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_layout_tables_hold_every_row_once(seed):
+    """Every query (and key) of a batch is in exactly one small structure, row entry, few-query item set or tile; a
+    tile's items are its structure's columns, each once; slots are joined once."""
+    from ye3t_b200 import runtime as rt
+    rng = np.random.default_rng(seed)
+    queries, keys = _random_counts(rng)
+    heads, key_heads = ((8, 2), (4, 4), (1, 1))[seed % 3]
+    tables, counts = rt._layout_tables(queries, keys, heads, key_heads)
+    q_off, k_off = tables["query_offsets"], tables["key_offsets"]
+    small = {tuple(r) for r in tables["small"]}
+    assert len(small) == len(tables["small"]) == counts["small_32_count"] + counts["small_64_count"]
+    for k, (a, n, b, m) in enumerate(tables["small"]):
+        most = 32 if k < counts["small_32_count"] else 64
+        assert n <= most and m <= most
+    for side, off, other, number in (("query", q_off, k_off, queries), ("key", k_off, q_off, keys)):
+        seen = np.zeros(off[-1], int)
+        for a, n, b, m in small:
+            first, count = (a, n) if side == "query" else (b, m)
+            seen[first:first + count] += 1
+        for row, structure in tables[f"{side}_rows"]:
+            assert off[structure] <= row < off[structure + 1]
+            seen[row] += 1
+        kinds = ("query", "few") if side == "query" else ("key",)
+        for kind in kinds:
+            items, joins = tables[f"{kind}_items"], tables[f"{kind}_joins"]
+            columns, slots = {}, {}
+            for row, rows, col, cols, slot, *rest in items:
+                structure = int(np.searchsorted(off, row, side="right")) - 1
+                assert 1 <= rows <= 128 and off[structure] <= row and row + rows <= off[structure + 1]
+                assert not any(rest)
+                columns.setdefault((row, rows), []).append((col, cols, structure))
+                if slot >= 0:
+                    assert slot not in slots
+                    slots[slot] = (row, rows)
+                else:
+                    assert kind != "few"
+            assert sorted(slots) == list(range(counts[f"{kind}_slot_count"]))
+            for (row, rows), parts in columns.items():
+                seen[row:row + rows] += 1
+                structure = parts[0][2]
+                at = other[structure]
+                for col, cols, _ in sorted(p for p in parts if p[1]):
+                    assert col == at
+                    at += cols
+                assert at == other[structure + 1]
+            joined = []
+            for row, rows, first, count in joins:
+                assert all(slots[first + k] == (row, rows) for k in range(count))
+                joined += list(range(first, first + count))
+            assert sorted(joined) == sorted(slots)
+            if kind == "few":
+                assert all(i[1] <= 2 for i in items)
+        assert (seen == 1).all()

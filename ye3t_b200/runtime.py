@@ -663,6 +663,47 @@ def _work_tables(row_first, row_count, col_first, col_count, heads, tiled, by_ro
             "slot_count": int(p[split].sum()), "row_count": len(rest)}
 
 
+# the counts of a layout, in the order of StructureLayout.counts
+_LAYOUT_COUNTS = ("heads", "key_heads", "query_count", "key_count", "structure_count", "shared", "small_32_count",
+                  "small_64_count", "few_item_count", "few_join_count", "few_slot_count", "query_item_count",
+                  "query_join_count", "query_slot_count", "query_row_count", "key_item_count", "key_join_count",
+                  "key_slot_count", "key_row_count")
+# its tables in their order, with the integers of an entry and the count they go by: 32-byte records first, then
+# 16-byte ones
+_LAYOUT_TABLES = (("query_items", 8, "query_item_count"), ("key_items", 8, "key_item_count"),
+                  ("few_items", 8, "few_item_count"), ("query_joins", 4, "query_join_count"),
+                  ("key_joins", 4, "key_join_count"), ("few_joins", 4, "few_join_count"),
+                  ("small", 4, None), ("query_rows", 2, "query_row_count"), ("key_rows", 2, "key_row_count"),
+                  ("query_offsets", 1, "structure_count"), ("key_offsets", 1, "structure_count"))
+
+
+def _layout_tables(queries, keys, heads, key_heads):
+    """A layout's tables by name and its counts, on the host."""
+    q_first, k_first = np.cumsum(queries) - queries, np.cumsum(keys) - keys
+    small = (queries <= _SMALL) & (keys <= _SMALL)
+    # beside larger structures, a launch of their own has to fill the SMs
+    if not small.all() and int(small.sum()) * key_heads < 2 * 148:
+        small = np.zeros_like(small)
+    tiny = small & (queries <= _SMALL // 2) & (keys <= _SMALL // 2)
+    low, high = np.flatnonzero(tiny & (queries + keys > 0)), np.flatnonzero(small & ~tiny)
+    # a single key has all the weight and no gradient through the softmax: the row kernels give exactly that
+    by_row, rest = ~small & (keys <= 1), ~small & (keys > 1)
+    few = rest & (queries <= _FEW)
+    none = np.zeros_like(small)
+    sides = {"query": _work_tables(q_first, queries, k_first, keys, heads, rest & ~few, by_row),
+             "key": _work_tables(k_first, keys, q_first, queries, key_heads, rest, by_row),
+             "few": _work_tables(q_first, queries, k_first, keys, key_heads, few & (queries > 0), none, always=True)}
+    tables = {f"{name}_{what}": side[what] for name, side in sides.items() for what in ("items", "joins", "rows")}
+    tables["small"] = np.stack([q_first, queries, k_first, keys], 1)[np.concatenate([low, high])]
+    tables["query_offsets"] = np.concatenate([[0], np.cumsum(queries)])
+    tables["key_offsets"] = np.concatenate([[0], np.cumsum(keys)])
+    counts = {f"{name}_{what}": int(side[what]) for name, side in sides.items()
+              for what in ("item_count", "join_count", "slot_count", "row_count")}
+    counts.update(heads=heads, key_heads=key_heads, query_count=int(queries.sum()), key_count=int(keys.sum()),
+                  structure_count=int(queries.size), small_32_count=low.size, small_64_count=high.size)
+    return tables, counts
+
+
 class StructureLayout:
     """Which rows of a packed batch belong to which structure, for :func:`structure_attention`.
 
@@ -670,6 +711,9 @@ class StructureLayout:
     by structure; with ``key_counts`` None the queries and the keys are the same atoms.  Counts are host
     integers and may be zero.  A layout is built once per batch and used for every layer and head width with
     its numbers of heads; it holds index tables only.
+
+    ``tables`` (int32, on the device) and ``counts`` (host integers) are the whole of it, as the registered
+    operators take them.
     """
 
     def __init__(self, query_counts, key_counts=None, *, heads, key_heads=None, device="cuda"):
@@ -677,51 +721,47 @@ class StructureLayout:
         keys = queries if key_counts is None else _host_counts(key_counts, "key_counts")
         if keys.size != queries.size:
             raise ValueError(f"{queries.size} structures of queries, but {keys.size} of keys")
-        self.heads = int(heads)
-        self.key_heads = self.heads if key_heads is None else int(key_heads)
-        if self.heads < 1 or self.key_heads < 1 or self.heads % self.key_heads:
-            raise ValueError(f"heads ({self.heads}) must be a positive multiple of key_heads ({self.key_heads})")
-        self.shared = key_counts is None
-        self.structure_count = int(queries.size)
-        self.query_count, self.key_count = int(queries.sum()), int(keys.sum())
-        self.device = torch.device(device)
-        if self.device.type != "cuda":
-            raise ValueError(f"StructureLayout: ye3t_b200 evaluates on CUDA devices only, not on {self.device}")
-        if self.device.index is None:
-            self.device = torch.device("cuda", torch.cuda.current_device())
-        q_first, k_first = np.cumsum(queries) - queries, np.cumsum(keys) - keys
-        small = (queries <= _SMALL) & (keys <= _SMALL)
-        # beside larger structures, a launch of their own has to fill the SMs
-        if not small.all() and int(small.sum()) * self.key_heads < 2 * 148:
-            small &= queries + keys < 0
-        tiny = small & (queries <= _SMALL // 2) & (keys <= _SMALL // 2)
-        order = np.concatenate([np.flatnonzero(tiny & (queries + keys > 0)), np.flatnonzero(small & ~tiny)])
-        structures = np.stack([q_first, queries, k_first, keys], 1)[order]
-        # a single key has all the weight and no gradient through the softmax: the row kernels give exactly that
-        few = ~small & (keys > 1) & (queries <= _FEW)
-        q_side = _work_tables(q_first, queries, k_first, keys, self.heads, ~small & (keys > 1) & ~few,
-                              ~small & (keys <= 1))
-        f_side = _work_tables(q_first, queries, k_first, keys, self.key_heads, few & (queries > 0), small & ~small,
-                              always=True)
-        k_side = _work_tables(k_first, keys, q_first, queries, self.key_heads, ~small & (keys > 1),
-                              ~small & (keys <= 1))
-        # items, then joins and structures: they are read as 32- and 16-byte records
-        tables = [q_side["items"], k_side["items"], f_side["items"], q_side["joins"], k_side["joins"], f_side["joins"],
-                  structures, q_side["rows"], k_side["rows"], np.concatenate([[0], np.cumsum(queries)]), np.concatenate([[0], np.cumsum(keys)])]
+        heads = int(heads)
+        key_heads = heads if key_heads is None else int(key_heads)
+        if heads < 1 or key_heads < 1 or heads % key_heads:
+            raise ValueError(f"heads ({heads}) must be a positive multiple of key_heads ({key_heads})")
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError(f"StructureLayout: ye3t_b200 evaluates on CUDA devices only, not on {device}")
+        tables, counts = _layout_tables(queries, keys, heads, key_heads)
+        counts["shared"] = int(key_counts is None)
+        packed = np.concatenate([tables[name].reshape(-1) for name, _, _ in _LAYOUT_TABLES]).astype(np.int32)
         # one copy to the device; it is complete when the constructor returns, so any stream may use it
-        self._packed = torch.as_tensor(np.concatenate([t.reshape(-1) for t in tables]).astype(np.int32)).to(self.device)
+        self._set(torch.as_tensor(packed).to(device), [counts[name] for name in _LAYOUT_COUNTS])
+
+    def _set(self, tables, counts):
+        self.tables, self.counts = tables, [int(c) for c in counts]
+        c = dict(zip(_LAYOUT_COUNTS, self.counts))
+        self.heads, self.key_heads, self.shared = c["heads"], c["key_heads"], bool(c["shared"])
+        self.query_count, self.key_count = c["query_count"], c["key_count"]
+        self.structure_count, self.device = c["structure_count"], tables.device
         self._stream = _raw_stream(self.device)
-        first = self._packed.data_ptr() + 4 * np.cumsum([0] + [t.size for t in tables[:-1]])
         a = self._args = nat.StructureAttentionArgs()
-        a.heads, a.key_heads = self.heads, self.key_heads
-        a.query_count, a.key_count, a.structure_count = self.query_count, self.key_count, self.structure_count
-        a.small_32_count, a.small_64_count = int((tiny & (queries + keys > 0)).sum()), int((small & ~tiny).sum())
-        for name, side in (("query", q_side), ("key", k_side), ("few", f_side)):
-            for what in ("item_count", "join_count", "slot_count") + (() if name == "few" else ("row_count",)):
-                setattr(a, f"{name}_{what}", int(side[what]))
-        for name, at in zip(("query_items", "key_items", "few_items", "query_joins", "key_joins", "few_joins", "small", "query_rows", "key_rows",
-                             "query_offsets", "key_offsets"), first):
-            setattr(a, name, int(at))
+        for name in _LAYOUT_COUNTS:
+            if name != "shared":
+                setattr(a, name, c[name])
+        at = 0
+        for name, width, count in _LAYOUT_TABLES:
+            setattr(a, name, tables.data_ptr() + 4 * at)
+            n = c["small_32_count"] + c["small_64_count"] if count is None else c[count]
+            at += width * (n + (1 if name.endswith("offsets") else 0))
+        if tables.dtype != torch.int32 or not tables.is_contiguous() or tables.numel() != at:
+            raise ValueError(f"layout tables must be {at} contiguous int32 values")
+
+    @classmethod
+    def from_tensors(cls, tables, counts):
+        """The layout whose ``tables`` and ``counts`` these are."""
+        nat.require_cuda(tables, what="StructureLayout")
+        if len(counts) != len(_LAYOUT_COUNTS):
+            raise ValueError(f"a layout has {len(_LAYOUT_COUNTS)} counts, got {len(counts)}")
+        layout = cls.__new__(cls)
+        layout._set(tables, counts)
+        return layout
 
 
 def _attention_args(query, key, value, x, y, slopes, layout, scale):
@@ -737,7 +777,7 @@ def _attention_args(query, key, value, x, y, slopes, layout, scale):
     a.scale = scale
     if _raw_stream(layout.device) != layout._stream:
         # keeps the tables' memory from reuse before the current stream is done with it
-        layout._packed.record_stream(torch.cuda.current_stream(layout.device))
+        layout.tables.record_stream(torch.cuda.current_stream(layout.device))
     return a
 
 
@@ -768,6 +808,26 @@ def _attention_forward(query, key, value, x, y, slopes, layout, scale, validate)
     return out, lse
 
 
+def _attention_adjoint(grad, query, key, value, x, y, slopes, out, lse, layout, scale, same, validate):
+    dev = query.device
+    q, k, v, g = _dense_rows(query), _dense_rows(key), _dense_rows(value), grad.contiguous()
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    dx = dy = dslopes = None
+    if slopes is not None:
+        dx, dslopes = torch.empty_like(x), torch.empty_like(slopes)
+        dy = None if same else torch.empty_like(y)
+    args = _attention_args(q, k, v, x, y, slopes, layout, scale)
+    ws, ws_bytes = _attention_workspace(args, 1, dev)
+    status = _status(dev) if validate else None
+    nat.check(nat.lib().y3b_structure_attention_adjoint(
+        ctypes.byref(args), out.data_ptr(), g.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws_bytes, dq.data_ptr(),
+        dk.data_ptr(), dv.data_ptr(), nat.ptr(dx), nat.ptr(dy), nat.ptr(dslopes), nat.ptr(status), _raw_stream(dev)),
+        "structure_attention adjoint")
+    if validate:
+        _raise_on_status(status, "structure_attention adjoint")
+    return dq, dk, dv, dx, dy, dslopes
+
+
 class _StructureAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, key, value, x, y, slopes, layout, scale, validate):
@@ -783,24 +843,8 @@ class _StructureAttention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        query, key, value, x, y, slopes, out, lse = ctx.saved_tensors
-        layout, dev = ctx.layout, query.device
-        q, k, v, g = _dense_rows(query), _dense_rows(key), _dense_rows(value), grad.contiguous()
-        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-        dx = dy = dslopes = None
-        if slopes is not None:
-            dx, dslopes = torch.empty_like(x), torch.empty_like(slopes)
-            dy = None if ctx.same else torch.empty_like(y)
-        args = _attention_args(q, k, v, x, y, slopes, layout, ctx.scale)
-        ws, ws_bytes = _attention_workspace(args, 1, dev)
-        status = _status(dev) if ctx.validate else None
-        nat.check(nat.lib().y3b_structure_attention_adjoint(
-            ctypes.byref(args), out.data_ptr(), g.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws_bytes, dq.data_ptr(),
-            dk.data_ptr(), dv.data_ptr(), nat.ptr(dx), nat.ptr(dy), nat.ptr(dslopes), nat.ptr(status),
-            nat.stream_of(dev)), "structure_attention adjoint")
-        if ctx.validate:
-            _raise_on_status(status, "structure_attention adjoint")
-        return dq, dk, dv, dx, dy, dslopes, None, None, None
+        return _attention_adjoint(grad, *ctx.saved_tensors, ctx.layout, ctx.scale, ctx.same,
+                                  ctx.validate) + (None, None, None)
 
 
 def _check_positions(t, rows, what):
@@ -808,24 +852,7 @@ def _check_positions(t, rows, what):
         raise ValueError(f"{what} must be float32 [{rows}, 3], got {t.dtype} {tuple(t.shape)}")
 
 
-def structure_attention(query, key, value, layout, *, positions=None, key_positions=None, slopes=None, scale=None,
-                        backend="auto", validate=None):
-    """Softmax attention among the atoms of each structure of a packed batch, weaker with distance.
-
-    ``s_ij = scale * q_i . k_j - slopes[h] * |positions_i - key_positions_j|`` over the keys ``j`` of query
-    ``i``'s own structure, ``out_i = sum_j softmax_j(s_ij) v_j``.  ``query`` is ``[queries, heads, width]``,
-    ``key`` and ``value`` ``[keys, key_heads, width]`` (float32 or bfloat16, width 1 to 128); key head
-    ``h // (heads // key_heads)`` serves query head ``h``.  ``layout`` is the batch's
-    :class:`StructureLayout`; one query per structure makes a pooled readout.  ``positions`` and ``slopes``
-    (float32, both or neither) give the distance term; ``key_positions`` is left out where queries and keys
-    are the same atoms.  ``scale`` defaults to ``width ** -0.5``.  A query whose structure has no keys gives
-    zeros.
-
-    Scores, softmax statistics and sums are held in float32.  Differentiable once in query, key, value,
-    positions, key_positions and slopes (a pair at distance zero gives no position gradient); results and
-    gradients are bitwise repeatable.
-    """
-    _check_backend(backend)
+def _check_attention(query, key, value, layout, positions, key_positions, slopes):
     given = [t for t in (query, key, value, positions, key_positions, slopes) if t is not None]
     dev = nat.require_cuda(*given, what="structure_attention")
     if not isinstance(layout, StructureLayout):
@@ -858,9 +885,31 @@ def structure_attention(query, key, value, layout, *, positions=None, key_positi
             raise ValueError("the layout has keys of its own: give key_positions")
         if slopes.dtype != torch.float32 or tuple(slopes.shape) != (layout.heads,):
             raise ValueError(f"slopes must be float32 [{layout.heads}], got {slopes.dtype} {tuple(slopes.shape)}")
+
+
+def structure_attention(query, key, value, layout, *, positions=None, key_positions=None, slopes=None, scale=None,
+                        backend="auto", validate=None):
+    """Softmax attention among the atoms of each structure of a packed batch, weaker with distance.
+
+    ``s_ij = scale * q_i . k_j - slopes[h] * |positions_i - key_positions_j|`` over the keys ``j`` of query
+    ``i``'s own structure, ``out_i = sum_j softmax_j(s_ij) v_j``.  ``query`` is ``[queries, heads, width]``,
+    ``key`` and ``value`` ``[keys, key_heads, width]`` (float32 or bfloat16, width 1 to 128); key head
+    ``h // (heads // key_heads)`` serves query head ``h``.  ``layout`` is the batch's
+    :class:`StructureLayout`; one query per structure makes a pooled readout.  ``positions`` and ``slopes``
+    (float32, both or neither) give the distance term; ``key_positions`` is left out where queries and keys
+    are the same atoms.  ``scale`` defaults to ``width ** -0.5``.  A query whose structure has no keys gives
+    zeros.
+
+    Scores, softmax statistics and sums are held in float32.  Differentiable once in query, key, value,
+    positions, key_positions and slopes (a pair at distance zero gives no position gradient); results and
+    gradients are bitwise repeatable.
+    """
+    _check_backend(backend)
+    _check_attention(query, key, value, layout, positions, key_positions, slopes)
     scale = float(query.shape[2]) ** -0.5 if scale is None else float(scale)
     validate = _validate_default(validate)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
+    given = (query, key, value, positions, key_positions, slopes)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in given):
         return _StructureAttention.apply(query, key, value, positions, key_positions, slopes, layout, scale, validate)
     x = None if positions is None else positions.contiguous()
     y = x if key_positions is None else key_positions.contiguous()

@@ -11,12 +11,14 @@ and grouped symmetric power carry first-order autograd through their GPU
 adjoints.  ``factorized_schedule`` is the schedule evaluator over raw table
 tensors (the reference's ``evaluate_factorized_schedule_cpu`` arguments,
 core/csrc/factorized_runtime.cpp:426); its autograd lives in
-``ye3t_b200.couplings.evaluate_factorized_schedule_torch``.
+``ye3t_b200.couplings.evaluate_factorized_schedule_torch``.  The learned per-atom operators
+(``species_embedding``, ``structure_attention``) have no counterpart in the reference; they carry first-order
+autograd, and ``structure_attention`` takes a ``StructureLayout`` as its ``tables`` and ``counts``.
 """
 
 from __future__ import annotations
 
-from typing import Tuple
+from typing import List, Optional, Tuple
 
 import torch
 from torch import Tensor
@@ -213,3 +215,99 @@ def factorized_schedule(block_values: Tensor, component_offsets: Tensor, compone
 @factorized_schedule.register_fake
 def _(block_values, component_offsets, component_label_index, block_m_indices, coeffs):
     return block_values.new_empty((block_values.shape[0], component_offsets.reshape(-1).shape[0] - 1))
+
+
+# -- learned per-atom operators (runtime.species_embedding, runtime.structure_attention) ---------
+@custom_op("ye3t_b200::species_embedding", mutates_args=())
+def species_embedding(table: Tensor, species: Tensor, scale: float) -> Tensor:
+    with torch.no_grad():
+        return rt.species_embedding(table, species, scale=scale)
+
+
+@species_embedding.register_fake
+def _(table, species, scale):
+    return table.new_empty(tuple(species.shape) + (table.shape[1],))
+
+
+@custom_op("ye3t_b200::species_embedding_adjoint", mutates_args=())
+def species_embedding_adjoint(grad: Tensor, species: Tensor, species_count: int, scale: float) -> Tensor:
+    nat.require_cuda(grad, species, what="species_embedding_adjoint")
+    return rt._embedding_adjoint(grad, species, species_count, scale)
+
+
+@species_embedding_adjoint.register_fake
+def _(grad, species, species_count, scale):
+    return grad.new_empty((species_count, grad.shape[-1]))
+
+
+def _embedding_setup(ctx, inputs, output):
+    ctx.save_for_backward(inputs[1])
+    ctx.species_count, ctx.scale = inputs[0].shape[0], inputs[2]
+
+
+def _embedding_backward(ctx, grad):
+    (species,) = ctx.saved_tensors
+    return (torch.ops.ye3t_b200.species_embedding_adjoint(grad.contiguous(), species, ctx.species_count, ctx.scale),
+            None, None)
+
+
+species_embedding.register_autograd(_embedding_backward, setup_context=_embedding_setup)
+
+
+# ``tables`` and ``counts`` are a runtime.StructureLayout's; the second result (log-sum-exp) serves the adjoint
+@custom_op("ye3t_b200::structure_attention", mutates_args=())
+def structure_attention(query: Tensor, key: Tensor, value: Tensor, tables: Tensor, counts: List[int],
+                        positions: Optional[Tensor], key_positions: Optional[Tensor], slopes: Optional[Tensor],
+                        scale: float) -> Tuple[Tensor, Tensor]:
+    layout = rt.StructureLayout.from_tensors(tables, counts)
+    rt._check_attention(query, key, value, layout, positions, key_positions, slopes)
+    x, y, slopes = _places(positions, key_positions, slopes)
+    return rt._attention_forward(query, key, value, x, y, slopes, layout, scale, False)
+
+
+def _places(positions, key_positions, slopes):
+    if slopes is None:
+        return None, None, None
+    x = positions.contiguous()
+    return x, x if key_positions is None else key_positions.contiguous(), slopes.contiguous()
+
+
+@structure_attention.register_fake
+def _(query, key, value, tables, counts, positions, key_positions, slopes, scale):
+    return query.new_empty(query.shape), query.new_empty(query.shape[:2], dtype=torch.float32)
+
+
+@custom_op("ye3t_b200::structure_attention_adjoint", mutates_args=())
+def structure_attention_adjoint(grad: Tensor, query: Tensor, key: Tensor, value: Tensor, tables: Tensor,
+                                counts: List[int], positions: Optional[Tensor], key_positions: Optional[Tensor],
+                                slopes: Optional[Tensor], out: Tensor, lse: Tensor,
+                                scale: float) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    layout = rt.StructureLayout.from_tensors(tables, counts)
+    rt._check_attention(query, key, value, layout, positions, key_positions, slopes)
+    x, y, slopes = _places(positions, key_positions, slopes)
+    grads = rt._attention_adjoint(grad, query, key, value, x, y, slopes, out, lse, layout, scale,
+                                  key_positions is None, False)
+    # an absent argument's gradient is an empty tensor
+    return tuple(lse.new_empty(0) if g is None else g for g in grads)
+
+
+@structure_attention_adjoint.register_fake
+def _(grad, query, key, value, tables, counts, positions, key_positions, slopes, out, lse, scale):
+    return tuple(lse.new_empty(0) if t is None else t.new_empty(t.shape)
+                 for t in (query, key, value, positions, key_positions, slopes))
+
+
+def _attention_setup(ctx, inputs, output):
+    query, key, value, tables, ctx.counts, positions, key_positions, slopes, ctx.scale = inputs
+    ctx.save_for_backward(query, key, value, tables, positions, key_positions, slopes, *output)
+
+
+def _attention_backward(ctx, grad, _):
+    query, key, value, tables, positions, key_positions, slopes, out, lse = ctx.saved_tensors
+    g = torch.ops.ye3t_b200.structure_attention_adjoint(grad.contiguous(), query, key, value, tables, ctx.counts,
+                                                        positions, key_positions, slopes, out, lse, ctx.scale)
+    dx, dy, ds = (None if t is None else d for t, d in zip((positions, key_positions, slopes), g[3:]))
+    return g[0], g[1], g[2], None, None, dx, dy, ds, None
+
+
+structure_attention.register_autograd(_attention_backward, setup_context=_attention_setup)
