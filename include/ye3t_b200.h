@@ -690,6 +690,14 @@ typedef struct {
   float scale;
 } y3b_structure_attention_args;
 
+/* Work tables of a batch (host arrays): query_counts[s] queries and key_counts[s] keys of structure s, one after the
+ * other.  counts takes the thirteen table sizes from small_32_count to key_row_count in the order of the struct;
+ * tables takes query_items, key_items, few_items, query_joins, key_joins, few_joins, small, query_rows, key_rows,
+ * query_offsets and key_offsets one after the other, if capacity holds them.  Returns their number of int32 values, or
+ * a negative error code. */
+int64_t y3b_structure_layout(const int64_t* query_counts, const int64_t* key_counts, int64_t structure_count,
+                             int64_t heads, int64_t key_heads, int64_t* counts, int32_t* tables, int64_t capacity);
+
 /* Bytes of workspace (16-byte aligned) of the call below, or with adjoint != 0 of its adjoint; -1 for bad
  * arguments.  The tables must be filled in. */
 int64_t y3b_structure_attention_workspace_bytes(const y3b_structure_attention_args* args, int adjoint);

@@ -49,6 +49,13 @@ def test_entry_points_refuse_bad_arguments():
     assert lib.y3b_species_embedding_adjoint_workspace_bytes(nat.F32, 1 << 31, 1, 1) == -1
     assert lib.y3b_species_embedding_adjoint_workspace_bytes(nat.F32, 1000, 1000, 8) > 0
     assert lib.y3b_species_embedding_adjoint(nat.F32, 0, 0, 8, 10, 3, 4, 1.0, 0, 0, 0, 0, 0) == -1
+    one, minus = np.array([5], np.int64), np.array([-1], np.int64)
+    sizes = np.zeros(13, np.int64)
+    layout = lambda q, k, h=4, hk=2: lib.y3b_structure_layout(  # noqa: E731
+        q.ctypes.data, k.ctypes.data, 1, h, hk, sizes.ctypes.data, 0, 0)
+    assert layout(one, one) > 0
+    assert layout(minus, one) == -1 and layout(one, minus) == -1 and layout(one, one, 4, 3) == -1
+    assert lib.y3b_structure_layout(0, 0, 1, 1, 1, sizes.ctypes.data, 0, 0) == -1
     assert lib.y3b_structure_attention(None, 0, 0, 0, 0, 0, 0) == -1
     a = nat.StructureAttentionArgs()
     a.dtype, a.heads, a.key_heads, a.width = nat.F32, 4, 2, 32
@@ -102,7 +109,15 @@ def test_layout_tables_hold_every_row_once(seed):
     rng = np.random.default_rng(seed)
     queries, keys = _random_counts(rng)
     heads, key_heads = ((8, 2), (4, 4), (1, 1))[seed % 3]
-    tables, counts = rt._layout_tables(queries, keys, heads, key_heads)
+    packed, sizes = rt._layout_tables(queries, keys, heads, key_heads)
+    counts = dict(zip(rt._LAYOUT_COUNTS[6:], sizes), structure_count=len(queries))
+    tables, at = {}, 0
+    for name, width, count in rt._LAYOUT_TABLES:
+        n = counts["small_32_count"] + counts["small_64_count"] if count is None else counts[count]
+        n = n + 1 if name.endswith("offsets") else n
+        tables[name] = packed[at:at + width * n].reshape((n, width) if width > 1 else n)
+        at += width * n
+    assert at == packed.size
     q_off, k_off = tables["query_offsets"], tables["key_offsets"]
     small = {tuple(r) for r in tables["small"]}
     assert len(small) == len(tables["small"]) == counts["small_32_count"] + counts["small_64_count"]

@@ -177,6 +177,7 @@ _SIGS = {
     "y3b_species_embedding_adjoint_workspace_bytes": (I64, [ctypes.c_int, I64, I64, I64]),
     "y3b_species_embedding_adjoint": (ctypes.c_int, [ctypes.c_int, VP, VP, ctypes.c_int, I64, I64, I64, DBL, VP, I64,
                                                      VP, VP, VP]),
+    "y3b_structure_layout": (I64, [VP, VP, I64, I64, I64, VP, VP, I64]),
     "y3b_structure_attention_workspace_bytes": (I64, [ctypes.POINTER(StructureAttentionArgs), ctypes.c_int]),
     "y3b_structure_attention": (ctypes.c_int, [ctypes.POINTER(StructureAttentionArgs), VP, I64, VP, VP, VP, VP]),
     "y3b_structure_attention_adjoint": (ctypes.c_int, [ctypes.POINTER(StructureAttentionArgs), VP, VP, VP, VP, I64,

@@ -1,0 +1,168 @@
+// Work tables of a batch for structure attention, built on the host (the layout in include/ye3t_b200.h).
+//
+// Which kernel computes which structure:
+//   small   up to 64 queries and 64 keys, where all structures are small or the small ones fill the SMs by
+//           themselves (a tile of 128 rows would be mostly empty, but a launch for a few structures costs more than it
+//           saves: 4 molecules beside 12 clusters of some hundred atoms, 362 us against 201 in a training step);
+//   row     no or a single key: its weight is exactly 1 and its gradients through the softmax exactly 0, which the
+//           row kernels keep;
+//   few     up to two queries: a tile would hold 2 rows of 128 (8 structures of 16,384 keys, 8 heads: 111 us on tiles,
+//           64 on the few-query kernels); their keys keep to the tile kernels;
+//   tile    the rest.
+// A tile's columns are split where the tiles alone would not give every SM its two CTAs, and joined.
+#include <algorithm>
+#include <iterator>
+#include <new>
+#include <vector>
+
+#include "common.cuh"
+
+namespace y3b {
+namespace {
+
+constexpr int64_t kTile = 128, kSmall = 64, kFew = 2;
+
+struct Side {
+  std::vector<int32_t> items, joins, rows;
+  int64_t slots = 0;
+};
+
+struct Range {
+  int64_t first, count;
+};
+
+struct Part {
+  int32_t row, rows, col, cols, slot;
+};
+
+// Tiles of the structures in `which`: rows [row] and columns [col] of each; `always` joins every tile.
+void add_tiles(Side* side, const std::vector<Range>& row, const std::vector<Range>& col,
+               const std::vector<int64_t>& which, int64_t heads, bool always) {
+  int64_t work = 0;
+  for (const int64_t s : which) work += (row[s].count + kTile - 1) / kTile * std::max<int64_t>(col[s].count, 1);
+  work *= heads;
+  // two CTAs an SM of the tile kernels, four of the few-query kernels
+  const int64_t chunk = always ? std::max<int64_t>(128, work / (kSMs * 4)) : std::max<int64_t>(256, work / (kSMs * 2));
+  std::vector<Part> parts;
+  for (const int64_t s : which) {
+    const int64_t n = std::max<int64_t>(1, (2 * col[s].count + chunk) / (2 * chunk));
+    const int64_t step = ((col[s].count + n - 1) / n + 63) / 64 * 64;  // parts begin at multiples of 64 columns
+    for (int64_t r = 0; r < row[s].count; r += kTile) {
+      const int32_t first = int32_t(row[s].first + r), rows = int32_t(std::min(kTile, row[s].count - r));
+      const bool split = n > 1 || always;
+      if (split) {
+        const int32_t join[4] = {first, rows, int32_t(side->slots), int32_t(n)};
+        side->joins.insert(side->joins.end(), join, join + 4);
+      }
+      for (int64_t k = 0; k < n; ++k) {
+        const int64_t b = std::min(k * step, col[s].count), e = std::min(b + step, col[s].count);
+        parts.push_back({first, rows, int32_t(col[s].first + b), int32_t(e - b),
+                         split ? int32_t(side->slots + k) : -1});
+      }
+      if (split) side->slots += n;
+    }
+  }
+  // the longest first: the last CTAs to start are short
+  std::stable_sort(parts.begin(), parts.end(), [](const Part& a, const Part& b) { return a.cols > b.cols; });
+  side->items.reserve(parts.size() * 8);
+  for (const Part& p : parts) {
+    const int32_t item[8] = {p.row, p.rows, p.col, p.cols, p.slot, 0, 0, 0};
+    side->items.insert(side->items.end(), item, item + 8);
+  }
+}
+
+void add_rows(Side* side, const std::vector<Range>& row, const std::vector<int64_t>& which) {
+  for (const int64_t s : which) {
+    for (int64_t r = 0; r < row[s].count; ++r) {
+      side->rows.push_back(int32_t(row[s].first + r));
+      side->rows.push_back(int32_t(s));
+    }
+  }
+}
+
+int64_t build(const int64_t* queries, const int64_t* keys, int64_t n, int64_t heads, int64_t key_heads,
+              int64_t* counts, int32_t* out, int64_t capacity) {
+  std::vector<Range> q(n), k(n);
+  int64_t nq = 0, nk = 0;
+  for (int64_t s = 0; s < n; ++s) {
+    q[s] = {nq, queries[s]};
+    k[s] = {nk, keys[s]};
+    nq += queries[s];
+    nk += keys[s];
+  }
+  int64_t small_count = 0;
+  for (int64_t s = 0; s < n; ++s) small_count += queries[s] <= kSmall && keys[s] <= kSmall;
+  const bool use_small = small_count == n || small_count * key_heads >= 2 * kSMs;
+  std::vector<int64_t> low, high, by_row, few, tiled, key_tiled;
+  for (int64_t s = 0; s < n; ++s) {
+    if (use_small && queries[s] <= kSmall && keys[s] <= kSmall) {
+      if (queries[s] > kSmall / 2 || keys[s] > kSmall / 2) high.push_back(s);
+      else if (queries[s] + keys[s] > 0) low.push_back(s);
+    } else if (keys[s] <= 1) {
+      by_row.push_back(s);
+    } else {
+      key_tiled.push_back(s);
+      if (queries[s] > kFew) tiled.push_back(s);
+      else if (queries[s] > 0) few.push_back(s);
+    }
+  }
+  Side query, key, one;
+  add_tiles(&query, q, k, tiled, heads, false);
+  add_tiles(&key, k, q, key_tiled, key_heads, false);
+  add_tiles(&one, q, k, few, key_heads, true);
+  add_rows(&query, q, by_row);
+  add_rows(&key, k, by_row);
+  const auto entries = [](const std::vector<int32_t>& v, int width) { return int64_t(v.size()) / width; };
+  const int64_t all[] = {int64_t(low.size()),      int64_t(high.size()),     entries(one.items, 8),
+                         entries(one.joins, 4),    one.slots,                entries(query.items, 8),
+                         entries(query.joins, 4),  query.slots,              entries(query.rows, 2),
+                         entries(key.items, 8),    entries(key.joins, 4),    key.slots,
+                         entries(key.rows, 2)};
+  std::copy(std::begin(all), std::end(all), counts);
+  const std::vector<int32_t>* const tables[] = {&query.items, &key.items, &one.items, &query.joins, &key.joins,
+                                                &one.joins};
+  int64_t need = 4 * int64_t(low.size() + high.size()) + int64_t(query.rows.size() + key.rows.size()) + 2 * (n + 1);
+  for (const auto* t : tables) need += int64_t(t->size());
+  if (!out || capacity < need) return need;
+  for (const auto* t : tables) out = std::copy(t->begin(), t->end(), out);
+  for (const auto* list : {&low, &high}) {
+    for (const int64_t s : *list) {
+      const int64_t entry[4] = {q[s].first, q[s].count, k[s].first, k[s].count};
+      for (const int64_t v : entry) *out++ = int32_t(v);
+    }
+  }
+  out = std::copy(query.rows.begin(), query.rows.end(), out);
+  out = std::copy(key.rows.begin(), key.rows.end(), out);
+  for (int64_t s = 0; s < n; ++s) *out++ = int32_t(q[s].first);
+  *out++ = int32_t(nq);
+  for (int64_t s = 0; s < n; ++s) *out++ = int32_t(k[s].first);
+  *out++ = int32_t(nk);
+  return need;
+}
+
+}  // namespace
+}  // namespace y3b
+
+using namespace y3b;
+
+extern "C" int64_t y3b_structure_layout(const int64_t* query_counts, const int64_t* key_counts, int64_t structure_count,
+                                        int64_t heads, int64_t key_heads, int64_t* counts, int32_t* tables,
+                                        int64_t capacity) {
+  Y3B_CHECK_ARG(structure_count >= 0 && structure_count < INT32_MAX, "structure_layout: bad structure count");
+  Y3B_CHECK_ARG(counts && (structure_count == 0 || (query_counts && key_counts)), "structure_layout: null argument");
+  Y3B_CHECK_ARG(heads >= 1 && key_heads >= 1 && heads % key_heads == 0 && heads <= 1024,
+                "structure_layout: the query heads must be a multiple of the key heads, 1024 at most");
+  int64_t nq = 0, nk = 0;
+  for (int64_t s = 0; s < structure_count; ++s) {
+    Y3B_CHECK_ARG(query_counts[s] >= 0 && key_counts[s] >= 0, "structure_layout: negative count");
+    Y3B_CHECK_ARG(query_counts[s] <= INT32_MAX - nq && key_counts[s] <= INT32_MAX - nk,
+                  "structure_layout: at most 2^31 - 1 atoms in a batch");
+    nq += query_counts[s];
+    nk += key_counts[s];
+  }
+  try {
+    return build(query_counts, key_counts, structure_count, heads, key_heads, counts, tables, capacity);
+  } catch (const std::bad_alloc&) {
+    return fail(Y3B_ERR_ARGUMENT, "structure_layout: out of host memory");
+  }
+}

@@ -614,53 +614,12 @@ def _host_counts(counts, what):
     c = np.asarray(counts)
     if c.ndim != 1 or (c.size and c.dtype.kind not in "iu"):
         raise ValueError(f"{what} must be a one-dimensional list of integers")
-    c = c.astype(np.int64)
+    c = np.ascontiguousarray(c, np.int64)
     if c.size and int(c.min()) < 0:
         raise ValueError(f"{what} must not be negative")
     if int(c.sum()) > 2**31 - 1:
         raise ValueError(f"{what}: at most 2^31 - 1 atoms in a batch")
     return c
-
-
-_TILE = 128       # rows of a tile
-_FEW = 2          # structures of up to so many queries take the few-query kernels
-_SMALL = 64       # structures of up to so many queries and keys take the small-structure kernels
-
-
-def _work_tables(row_first, row_count, col_first, col_count, heads, tiled, by_row, always=False):
-    """Items, joins and single rows of one side (the layout of include/ye3t_b200.h); ``always``: every tile is
-    joined, also one that is not split."""
-    r0, rn, c0, cn = row_first[tiled], row_count[tiled], col_first[tiled], col_count[tiled]
-    tiles = -(-rn // _TILE)
-    # columns are split where the tiles alone would not give every SM its CTAs: two of the tile kernels', four
-    # of the few-query kernels'
-    work = int((tiles * np.maximum(cn, 1)).sum()) * heads
-    chunk = max(128, work // (148 * 4)) if always else max(256, work // (148 * 2))
-    parts = np.maximum(1, np.round(cn / chunk).astype(np.int64))
-    of = np.repeat(np.arange(rn.size), tiles)  # the structure of each tile
-    t = np.arange(of.size) - np.repeat(np.cumsum(tiles) - tiles, tiles)
-    row = r0[of] + t * _TILE
-    rows = np.minimum(rn[of] - t * _TILE, _TILE)
-    p = parts[of]
-    split = (p > 1) | always
-    slot = np.where(split, np.cumsum(np.where(split, p, 0)) - p, -1)
-    ti = np.repeat(np.arange(of.size), p)
-    k = np.arange(ti.size) - np.repeat(np.cumsum(p) - p, p)
-    # parts begin at multiples of 64 columns
-    step = -(-(-(-cn[of] // p)) // 64) * 64
-    begin = np.minimum(k * step[ti], cn[of][ti])
-    end = np.minimum(begin + step[ti], cn[of][ti])
-    items = np.zeros((ti.size, 8), np.int64)
-    items[:, 0], items[:, 1], items[:, 2], items[:, 3] = row[ti], rows[ti], c0[of][ti] + begin, end - begin
-    items[:, 4] = np.where(slot[ti] >= 0, slot[ti] + k, -1)
-    items = items[np.argsort(-items[:, 3], kind="stable")]
-    joins = np.stack([row, rows, slot, p], 1)[split]
-    single = np.flatnonzero(by_row)
-    n = row_count[single]
-    rest = np.repeat(row_first[single] - (np.cumsum(n) - n), n) + np.arange(n.sum())
-    rest = np.stack([rest, np.repeat(single, n)], 1)
-    return {"items": items, "joins": joins, "rows": rest, "item_count": len(items), "join_count": len(joins),
-            "slot_count": int(p[split].sum()), "row_count": len(rest)}
 
 
 # the counts of a layout, in the order of StructureLayout.counts
@@ -678,30 +637,19 @@ _LAYOUT_TABLES = (("query_items", 8, "query_item_count"), ("key_items", 8, "key_
 
 
 def _layout_tables(queries, keys, heads, key_heads):
-    """A layout's tables by name and its counts, on the host."""
-    q_first, k_first = np.cumsum(queries) - queries, np.cumsum(keys) - keys
-    small = (queries <= _SMALL) & (keys <= _SMALL)
-    # beside larger structures, a launch of their own has to fill the SMs
-    if not small.all() and int(small.sum()) * key_heads < 2 * 148:
-        small = np.zeros_like(small)
-    tiny = small & (queries <= _SMALL // 2) & (keys <= _SMALL // 2)
-    low, high = np.flatnonzero(tiny & (queries + keys > 0)), np.flatnonzero(small & ~tiny)
-    # a single key has all the weight and no gradient through the softmax: the row kernels give exactly that
-    by_row, rest = ~small & (keys <= 1), ~small & (keys > 1)
-    few = rest & (queries <= _FEW)
-    none = np.zeros_like(small)
-    sides = {"query": _work_tables(q_first, queries, k_first, keys, heads, rest & ~few, by_row),
-             "key": _work_tables(k_first, keys, q_first, queries, key_heads, rest, by_row),
-             "few": _work_tables(q_first, queries, k_first, keys, key_heads, few & (queries > 0), none, always=True)}
-    tables = {f"{name}_{what}": side[what] for name, side in sides.items() for what in ("items", "joins", "rows")}
-    tables["small"] = np.stack([q_first, queries, k_first, keys], 1)[np.concatenate([low, high])]
-    tables["query_offsets"] = np.concatenate([[0], np.cumsum(queries)])
-    tables["key_offsets"] = np.concatenate([[0], np.cumsum(keys)])
-    counts = {f"{name}_{what}": int(side[what]) for name, side in sides.items()
-              for what in ("item_count", "join_count", "slot_count", "row_count")}
-    counts.update(heads=heads, key_heads=key_heads, query_count=int(queries.sum()), key_count=int(keys.sum()),
-                  structure_count=int(queries.size), small_32_count=low.size, small_64_count=high.size)
-    return tables, counts
+    """A layout's tables, one after the other, and the counts of their entries (``small_32_count`` on)."""
+    lib, counts = nat.lib(), np.empty(13, np.int64)
+    # room for a few entries a structure; a batch that needs more says how much
+    tables = np.empty(16 * queries.size + 256, np.int32)
+    for _ in range(2):
+        n = int(lib.y3b_structure_layout(queries.ctypes.data, keys.ctypes.data, queries.size, heads, key_heads,
+                                         counts.ctypes.data, tables.ctypes.data, tables.size))
+        if n < 0:
+            raise ValueError(lib.y3b_last_error().decode(errors="replace"))
+        if n <= tables.size:
+            break
+        tables = np.empty(n, np.int32)
+    return tables[:n], counts.tolist()
 
 
 class StructureLayout:
@@ -728,11 +676,10 @@ class StructureLayout:
         device = torch.device(device)
         if device.type != "cuda":
             raise ValueError(f"StructureLayout: ye3t_b200 evaluates on CUDA devices only, not on {device}")
-        tables, counts = _layout_tables(queries, keys, heads, key_heads)
-        counts["shared"] = int(key_counts is None)
-        packed = np.concatenate([tables[name].reshape(-1) for name, _, _ in _LAYOUT_TABLES]).astype(np.int32)
+        packed, counts = _layout_tables(queries, keys, heads, key_heads)
         # one copy to the device; it is complete when the constructor returns, so any stream may use it
-        self._set(torch.as_tensor(packed).to(device), [counts[name] for name in _LAYOUT_COUNTS])
+        self._set(torch.from_numpy(packed).to(device), [heads, key_heads, int(queries.sum()), int(keys.sum()),
+                                                        queries.size, int(key_counts is None)] + counts)
 
     def _set(self, tables, counts):
         self.tables, self.counts = tables, [int(c) for c in counts]
