@@ -72,12 +72,17 @@ struct AttTileArgs {
   int vec;              // 16-byte stores to out0 / out1 and loads of out_in / grad_in
 };
 
-template <int MODE, int DP, int NP>
+// HP: heads of a CTA.  Two heads see the same distances, so that the forward in bf16 shares the differences, squares and
+// reciprocal square roots of a pair of atoms among two: 8,192 atoms, 8 heads of 64: 384 us against 459.  The backward
+// gains nothing by it: its accumulators then fill the tensor memory, one CTA an SM is left (775 against 777 us, 649
+// against 638).
+template <int MODE, int DP, int NP, int HP>
 struct AttCfg {
   static constexpr bool KEY_BF16 = MODE == kKeySide && NP == 1 && DP == 64;
   // Columns a tile: as many as tensor and shared memory hold.  Twice the columns are 23 and 26 % faster on the
   // backward of 128-wide heads in bf16 and 14 % on the fp32 query side (4,096 atoms, 4 heads).
-  static constexpr int BN = NP == 1 ? (MODE == kQuerySide && DP == 64 ? 32 : 64)
+  static constexpr int BN = HP == 2   ? 32
+                            : NP == 1 ? (MODE == kQuerySide && DP == 64 ? 32 : 64)
                             : DP == 64 ? (MODE == kQuerySide ? 64 : 32)
                                        : (MODE == kForward ? 32 : 16);
   static constexpr int STAGES = NP == 3 ? (DP == 128 && MODE != kForward ? 1 : 2) : DP == 128 ? 2 : 4;
@@ -91,13 +96,14 @@ struct AttCfg {
   static constexpr int PANELS = DP / 64;
   static constexpr int ROW_PIECE = kTileRows * DP * 2;
   static constexpr int COL_PIECE = BN * DP * 2;
-  static constexpr int COL_STAGE = 2 * NP * COL_PIECE;
-  static constexpr int EXTRA = 5 * BN;  // floats a stage: x, y, z, -lse, delta of the columns
+  static constexpr int COL_HEAD = 2 * NP * COL_PIECE;
+  static constexpr int COL_STAGE = HP * COL_HEAD;
+  static constexpr int EXTRA = 5 * BN;  // floats a stage: x, y, z, lse, delta of the columns
   // Three pieces: the row operands lie in tensor memory where they fit.  A product of 128 rows and 32 columns reads
   // 4 KB of rows from shared memory for 1 KB of columns, and six products of pieces make that the bound
   // (4,096 atoms, 4 heads of 64: query side 578 us, key side 650, without the products 189 and 207).
   static constexpr bool ROWS_TMEM = NP == 3 && (DP == 64 || MODE == kForward);
-  static constexpr int ROW_BYTES = ROWS_TMEM ? 0 : ROWOPS * NP * ROW_PIECE;
+  static constexpr int ROW_BYTES = ROWS_TMEM ? 0 : HP * ROWOPS * NP * ROW_PIECE;
   // Tensor memory columns.  P and dS (NP * BN / 2 columns each) take the place of the scores they come from.
   // Score buffers: with two, the products of tile j + 1 run under the arithmetic of tile j (a single
   // stage of columns allows one).
@@ -107,8 +113,8 @@ struct AttCfg {
   static constexpr int A1 = NP == 1 ? BN : NP * BN / 2;
   static constexpr int BUF = MODE == kForward ? (NP == 1 ? BN : NP * BN / 2)
                              : MODE == kKeySide ? (NP == 1 ? 2 * BN : NP * BN)
-                                                : 2 * BN;
-  static constexpr int ACC = BUFS * BUF;
+                                                : 2 * BN;  // of one head
+  static constexpr int ACC = BUFS * HP * BUF;
   // Accumulators: OPS results (dV and dK on the key side).  The tensor cores truncate when they accumulate; three
   // pieces are six products, each of which truncates the long sum.  The score warps therefore add the accumulator
   // to a total in fp32 every FLUSH tiles, and it starts again.  With one piece the
@@ -121,7 +127,8 @@ struct AttCfg {
   static constexpr int W = DP / HALVES;  // columns of one accumulator
   // the totals lie in shared memory, [component][row], where the row operands leave it free
   static constexpr bool TOTALS_SMEM = ROWS_TMEM;
-  static constexpr int ROWS = ACC + (OPS + (TOTALS_SMEM ? 0 : TOTALS) + (FIX ? 1 : 0)) * W;  // row operands
+  static constexpr int NACC = OPS + (TOTALS_SMEM ? 0 : TOTALS) + (FIX ? 1 : 0);  // accumulators of one head
+  static constexpr int ROWS = ACC + HP * NACC * W;                                // row operands
   static constexpr int NEED = ROWS + (ROWS_TMEM ? ROWOPS * NP * DP / 2 : 0);
   static constexpr int SMEM = 1024 + ROW_BYTES + STAGES * (COL_STAGE + EXTRA * 4) +
                               (TOTALS_SMEM ? TOTALS * W * kTileRows * 4 : 0);
@@ -216,10 +223,10 @@ __device__ __forceinline__ Distance distance(tc::f2 squares) {
   return x;
 }
 
-template <int MODE, int DP, int NP, bool BIAS>
-__global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP, NP>::PER_SM) attention_tile_kernel(
-    const __grid_constant__ AttTileArgs a) {
-  using C = AttCfg<MODE, DP, NP>;
+template <int MODE, int DP, int NP, int HP, bool BIAS>
+__global__ void __launch_bounds__(AttCfg<MODE, DP, NP, HP>::THREADS, AttCfg<MODE, DP, NP, HP>::PER_SM)
+    attention_tile_kernel(const __grid_constant__ AttTileArgs a) {
+  using C = AttCfg<MODE, DP, NP, HP>;
   using T = typename std::conditional<NP == 1, __nv_bfloat16, float>::type;
   constexpr int BN = C::BN;
   extern __shared__ __align__(1024) unsigned char tile_smem[];
@@ -231,8 +238,9 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
   const int heads = MODE == kKeySide ? a.Hk : a.H;
   const int half = C::HALVES == 1 ? 0 : int(blockIdx.x % C::HALVES);
   const unsigned task = blockIdx.x / C::HALVES;
-  const int head = int(task % unsigned(heads));
-  const AttItem item = a.items[task / unsigned(heads)];
+  const unsigned head_blocks = unsigned(heads) / HP;
+  const int head0 = int(task % head_blocks) * HP;  // heads head0 .. head0 + HP
+  const AttItem item = a.items[task / head_blocks];
   const int d_first = half * C::W;                                            // accumulated components: d_first ..
   const int d_count = C::HALVES == 1 ? a.D : min(a.D - d_first, int(C::W));   // .. d_first + d_count (D > 64 with halves)
   const int acc_n = (d_count + 15) / 16 * 16;
@@ -240,7 +248,7 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
   const int total = MODE == kKeySide ? ntiles * a.group : ntiles;
 
   const uint32_t smem = (tc::smem_addr(tile_smem) + 1023u) & ~1023u;
-  const uint32_t row0 = smem, row1 = smem + NP * C::ROW_PIECE;
+  const uint32_t rows_at = smem;  // (head, operand) one after the other
   const uint32_t cols = smem + C::ROW_BYTES;
   float* extra = reinterpret_cast<float*>(tile_smem + (cols - tc::smem_addr(tile_smem)) + C::STAGES * C::COL_STAGE);
   [[maybe_unused]] float* totals = extra + C::STAGES * C::EXTRA;
@@ -267,11 +275,11 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
   }
   // row operands, by all threads
   if constexpr (!C::ROWS_TMEM) {
-    const AttOperand& r0 = MODE == kKeySide ? a.k : a.q;
-    load_tile<kTileRows, DP, NP>(row0, r0, item.row, head, item.rows, a.chunks, tid, C::THREADS);
-    if constexpr (MODE != kForward) {
-      const AttOperand& r1 = MODE == kKeySide ? a.v : a.g;
-      load_tile<kTileRows, DP, NP>(row1, r1, item.row, head, item.rows, a.chunks, tid, C::THREADS);
+#pragma unroll
+    for (int u = 0; u < HP * C::ROWOPS; ++u) {
+      const int h = u / C::ROWOPS, op = u % C::ROWOPS;
+      load_tile<kTileRows, DP, NP>(rows_at + u * NP * C::ROW_PIECE, MODE == kKeySide ? (op ? a.v : a.k) : op ? a.g : a.q,
+                                   item.row, head0 + h, item.rows, a.chunks, tid, C::THREADS);
     }
     tc::cp_commit();
     tc::cp_wait<0>();
@@ -290,7 +298,7 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
       for (int u = tid / kTileRows; u < C::ROWOPS * NP; u += C::GROUPS) {
         const int op = u / NP, piece = u - op * NP;
         const AttOperand& o = MODE == kKeySide ? (op ? a.v : a.k) : op ? a.g : a.q;
-        const __nv_bfloat16* src = o.p + piece * o.piece + (int64_t(item.row) + r) * o.row + head * o.head;
+        const __nv_bfloat16* src = o.p + piece * o.piece + (int64_t(item.row) + r) * o.row + head0 * o.head;
 #pragma unroll
         for (int c = 0; c < DP / 8; c += 4) {
           uint32_t w[16];
@@ -326,25 +334,24 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
       const int c0 = jt * BN, n = item.cols - c0 < BN ? item.cols - c0 : BN;
       const int64_t col = int64_t(item.col) + c0;
       const uint32_t dst = cols + s * C::COL_STAGE;
-      const int ch = MODE == kKeySide ? head * a.group + sub : head / a.group;
+      const auto head_of = [&](int h) { return MODE == kKeySide ? (head0 + h) * a.group + sub : (head0 + h) / a.group; };
       if (n == BN) {
         if (t == 0) {
           tc::mbar_expect(full(s), C::COL_STAGE);
 #pragma unroll
-          for (int op = 0; op < 2; ++op) {
+          for (int u = 0; u < HP * 2 * NP; ++u) {
+            const int h = u / (2 * NP), op = u / NP % 2, p = u % NP;
 #pragma unroll
-            for (int p = 0; p < NP; ++p) {
-#pragma unroll
-              for (int q = 0; q < C::PANELS; ++q)
-                tc::tma_load4(dst + (op * NP + p) * C::COL_PIECE + q * (BN * 128), &a.cols[op], full(s), q * 64, ch,
-                              int(col), p);
-            }
+            for (int q = 0; q < C::PANELS; ++q)
+              tc::tma_load4(dst + u * C::COL_PIECE + q * (BN * 128), &a.cols[op], full(s), q * 64, head_of(h), int(col), p);
           }
         }
       } else {
-        load_tile<BN, DP, NP>(dst, MODE == kKeySide ? a.q : a.k, col, ch, n, a.chunks, t, kLoadThreads);
-        load_tile<BN, DP, NP>(dst + NP * C::COL_PIECE, MODE == kKeySide ? a.g : a.v, col, ch, n, a.chunks, t,
-                              kLoadThreads);
+#pragma unroll
+        for (int u = 0; u < HP * 2; ++u) {
+          load_tile<BN, DP, NP>(dst + u * NP * C::COL_PIECE, MODE == kKeySide ? (u % 2 ? a.g : a.q) : u % 2 ? a.v : a.k,
+                                col, head_of(u / 2), n, a.chunks, t, kLoadThreads);
+        }
       }
       const uint32_t ex = tc::smem_addr(extra + s * C::EXTRA);
       if constexpr (BIAS) {
@@ -356,9 +363,9 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
       }
       if constexpr (MODE == kKeySide) {
         for (int u = t; u < 2 * BN; u += kLoadThreads) {
-          const int r = u >> 1, c = u & 1;
+          const int c = u / BN, r = u % BN;
           const float* src = c ? a.delta : a.lse;
-          tc::cp4(ex + ((3 + c) * BN + r) * 4, r < n ? src + (col + r) * a.H + ch : src, r < n);
+          tc::cp4(ex + (3 * BN + u) * 4, r < n ? src + (col + r) * a.H + head_of(0) : src, r < n);
         }
       }
       tc::cp_commit();
@@ -380,38 +387,37 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
         return done;
       };
       // Descriptors are formed once, and each MMA adds a constant to their address field (16-byte units).
-      [[maybe_unused]] const uint64_t rows_desc = tc::desc_sw128(row0, 16, 1024);
+      [[maybe_unused]] const uint64_t rows_desc = tc::desc_sw128(rows_at, 16, 1024);
       const uint64_t cols_k = tc::desc_sw128(cols, 16, 1024), cols_mn = tc::desc_sw128(cols, BN * 128, 1024);
       const auto issue_scores = [&](int j) {
         const int s = j % C::STAGES;
         if (!wait(full(s), (j / C::STAGES) & 1)) return false;
         const uint64_t b0 = cols_k + uint64_t(s * (C::COL_STAGE / 16));
-        const uint32_t buf = tmem + (j % C::BUFS) * C::BUF;
+        const uint32_t buf = tmem + (j % C::BUFS) * (HP * C::BUF);
         if (lead) {
 #pragma unroll
-        for (int n = 0; n < Pieces<NP>::N; ++n) {
+          for (int n = 0; n < Pieces<NP>::N; ++n) {
 #pragma unroll
-          for (int ks = 0; ks < DP / 16; ++ks) {
-            if (ks < ksteps) {
+            for (int ks = 0; ks < DP / 16; ++ks) {
+              if (ks >= ksteps) continue;
 #pragma unroll
-              for (int op = 0; op < C::ROWOPS; ++op) {
-                const int off = (ks & 3) * 32;
-                const uint64_t b =
-                    b0 + uint64_t(((op * NP + Pieces<NP>::b(n)) * C::COL_PIECE + (ks >> 2) * (BN * 128) + off) / 16);
-                const uint32_t d = buf + (op ? C::T : 0);
+              for (int u = 0; u < HP * C::ROWOPS; ++u) {
+                const int h = u / C::ROWOPS, op = u % C::ROWOPS, off = (ks & 3) * 32;
+                const uint64_t b = b0 + uint64_t((h * C::COL_HEAD + (op * NP + Pieces<NP>::b(n)) * C::COL_PIECE +
+                                                  (ks >> 2) * (BN * 128) + off) / 16);
+                const uint32_t d = buf + h * C::BUF + (op ? C::T : 0);
                 if constexpr (C::ROWS_TMEM) {
                   tc::mma_ts(d, tmem + C::ROWS + (op * NP + Pieces<NP>::a(n)) * (DP / 2) + ks * 8, b, id_s,
                              n > 0 || ks > 0);
                 } else {
-                  const uint64_t r = rows_desc + uint64_t(((op * NP + Pieces<NP>::a(n)) * C::ROW_PIECE +
+                  const uint64_t r = rows_desc + uint64_t(((u * NP + Pieces<NP>::a(n)) * C::ROW_PIECE +
                                                            (ks >> 2) * (kTileRows * 128) + off) / 16);
                   tc::mma_ss(d, r, b, id_s, n > 0 || ks > 0);
                 }
               }
             }
           }
-        }
-        tc::commit(s_ready(j));
+          tc::commit(s_ready(j));
         }
         __syncwarp();
         return true;
@@ -425,24 +431,27 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
         if (!ok) break;
         // forward: P x V; query side: dS x K (and P x K); key side: P x G and dS x Q
         const uint64_t b0 = cols_mn + uint64_t(s * (C::COL_STAGE / 16) + half * (BN * 128 / 16));
-        const uint32_t buf = tmem + (j % C::BUFS) * C::BUF;
+        const uint32_t buf = tmem + (j % C::BUFS) * (HP * C::BUF);
         const uint32_t go_on = C::TOTALS ? j % C::FLUSH > 0 : j > 0;
         if (lead) {
+          constexpr int kOps = C::OPS + (C::FIX ? 1 : 0);
 #pragma unroll
-        for (int n = 0; n < Pieces<NP>::N; ++n) {
+          for (int n = 0; n < Pieces<NP>::N; ++n) {
 #pragma unroll
-          for (int ks = 0; ks < BN / 16; ++ks) {
+            for (int ks = 0; ks < BN / 16; ++ks) {
 #pragma unroll
-            for (int op = 0; op < C::OPS + (C::FIX ? 1 : 0); ++op) {
-              const int second = MODE == kForward || (MODE == kKeySide && op == 0) ? 1 : 0;  // V or G
-              tc::mma_ts(tmem + C::ACC + op * C::W,
-                         buf + (op == 0 ? C::A0 : C::A1) + Pieces<NP>::a(n) * (BN / 2) + ks * 8,
-                         b0 + uint64_t(((second * NP + Pieces<NP>::b(n)) * C::COL_PIECE + ks * 2048) / 16), id_a,
-                         n > 0 || ks > 0 ? 1u : go_on);
+              for (int u = 0; u < HP * kOps; ++u) {
+                const int h = u / kOps, op = u % kOps;
+                const int second = MODE == kForward || (MODE == kKeySide && op == 0) ? 1 : 0;  // V or G
+                tc::mma_ts(tmem + C::ACC + (h * C::NACC + op) * C::W,
+                           buf + h * C::BUF + (op == 0 ? C::A0 : C::A1) + Pieces<NP>::a(n) * (BN / 2) + ks * 8,
+                           b0 + uint64_t((h * C::COL_HEAD + (second * NP + Pieces<NP>::b(n)) * C::COL_PIECE + ks * 2048) /
+                                         16),
+                           id_a, n > 0 || ks > 0 ? 1u : go_on);
+              }
             }
           }
-        }
-        tc::commit(empty(s));
+          tc::commit(empty(s));
         }
         __syncwarp();
         if (C::BUFS == 1 && j + 1 < total) ok = issue_scores(j + 1);
@@ -460,30 +469,50 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
     const bool valid = r_tile < item.rows;
     const int64_t row = int64_t(item.row) + (valid ? r_tile : 0);
     const uint32_t lane_base = tmem + (uint32_t(32 * (warp & 3)) << 16);
-    float px = 0.0f, py = 0.0f, pz = 0.0f, slope = 0.0f;
+    float px = 0.0f, py = 0.0f, pz = 0.0f, slope[HP];
+    tc::f2 nslope2[HP];
+    const auto set_slopes = [&](int sub) {
+#pragma unroll
+      for (int h = 0; h < HP; ++h) {
+        slope[h] = 0.0f;
+        if (BIAS) slope[h] = a.slopes[MODE == kKeySide ? (head0 + h) * a.group + sub : head0 + h];
+        nslope2[h] = tc::pack(-slope[h] * kLog2e, -slope[h] * kLog2e);
+      }
+    };
+    set_slopes(0);
     if constexpr (BIAS) {
       const float* pos = (MODE == kKeySide ? a.y : a.x) + 3 * row;
       px = pos[0];
       py = pos[1];
       pz = pos[2];
-      slope = MODE == kKeySide ? 0.0f : a.slopes[head];
     }
     const tc::f2 px2 = tc::pack(px, px), py2 = tc::pack(py, py), pz2 = tc::pack(pz, pz);
     const tc::f2 scale2 = tc::pack(a.scale2, a.scale2), tiny2 = tc::pack(1e-30f, 1e-30f);
-    tc::f2 nslope2 = tc::pack(-slope * kLog2e, -slope * kLog2e);
     bool ok = true;
 
-    // state of the forward: reference maximum and sum; of the query side: the ten sums
-    float m = -INFINITY, l = 0.0f;
-    float nL = 0.0f, delta0 = 0.0f;
-    float sum[10];
+    // state of the forward: each head's reference maximum and sum; of the query side: the ten sums; of the key side: the
+    // force
+    float m[HP], l[HP];
 #pragma unroll
-    for (int k = 0; k < 10; ++k) sum[k] = 0.0f;
+    for (int h = 0; h < HP; ++h) {
+      m[h] = -INFINITY;
+      l[h] = 0.0f;
+    }
+    float nL = 0.0f, delta0 = 0.0f;
+    constexpr int SUMS = MODE == kQuerySide ? 10 : 3;
+    float sum[SUMS];
+    tc::f2 acc[SUMS];
+#pragma unroll
+    for (int k = 0; k < SUMS; ++k) {
+      sum[k] = 0.0f;
+      acc[k] = tc::pack(0.0f, 0.0f);
+    }
     if constexpr (MODE == kQuerySide) {
       if (valid) {
-        nL = -a.lse[row * a.H + head];
-        const T* o = static_cast<const T*>(a.out_in) + (row * a.H + head) * a.D;
-        const T* g = static_cast<const T*>(a.grad_in) + (row * a.H + head) * a.D;
+        const int64_t at = row * a.H + head0;
+        nL = -a.lse[at];
+        const T* o = static_cast<const T*>(a.out_in) + at * a.D;
+        const T* g = static_cast<const T*>(a.grad_in) + at * a.D;
         constexpr int W = 16 / int(sizeof(T));
         int d = 0;
         if (a.vec) {
@@ -500,17 +529,14 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
     }
     const tc::f2 nL2 = tc::pack(nL, nL), delta02 = tc::pack(delta0, delta0);
 
-    tc::f2 acc[10];
-#pragma unroll
-    for (int k = 0; k < 10; ++k) acc[k] = tc::pack(0.0f, 0.0f);
     // row sums go from pairs within a few tiles to the row's: two levels keep the rounding of long rows small
     const auto fold = [&] {
 #pragma unroll
-      for (int k = 0; k < 10; ++k) {
+      for (int k = 0; k < SUMS; ++k) {
         float s0, s1;
         tc::unpack(acc[k], s0, s1);
-        if constexpr (MODE == kQuerySide) sum[k] += s0 + s1;
-        else if (k < 3) sum[k] = fmaf(slope, s0 + s1, sum[k]);
+        if constexpr (MODE == kKeySide) sum[k] = fmaf(slope[0], s0 + s1, sum[k]);
+        else sum[k] += s0 + s1;
         acc[k] = tc::pack(0.0f, 0.0f);
       }
     };
@@ -545,14 +571,18 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
     // One tile's arithmetic; n < BN columns where CUT, all of them otherwise.
     const auto forward_tile = [&](auto cut, int j, int n, const float* ex, uint32_t buf) {
       constexpr bool CUT = decltype(cut)::value;
-      float v[BN];
+      float v[HP][BN];
 #pragma unroll
-      for (int c = 0; c < BN; c += 16) tc::ld16(buf + c, v + c);
+      for (int h = 0; h < HP; ++h)
+#pragma unroll
+        for (int c = 0; c < BN; c += 16) tc::ld16(buf + h * C::BUF + c, v[h] + c);
       tc::wait_ld();
-      float t0 = -INFINITY, t1 = -INFINITY;
+      float top[HP];
+#pragma unroll
+      for (int h = 0; h < HP; ++h) top[h] = -INFINITY;
 #pragma unroll
       for (int c = 0; c < BN; c += 4) {
-        tc::f2 s0 = tc::mul2(tc::pack(v[c], v[c + 1]), scale2), s1 = tc::mul2(tc::pack(v[c + 2], v[c + 3]), scale2);
+        [[maybe_unused]] tc::f2 d0, d1;
         if constexpr (BIAS) {
           const ulonglong2 xx = *reinterpret_cast<const ulonglong2*>(ex + c);
           const ulonglong2 yy = *reinterpret_cast<const ulonglong2*>(ex + BN + c);
@@ -560,79 +590,98 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
           const tc::f2 dx0 = tc::sub2(px2, xx.x), dx1 = tc::sub2(px2, xx.y);
           const tc::f2 dy0 = tc::sub2(py2, yy.x), dy1 = tc::sub2(py2, yy.y);
           const tc::f2 dz0 = tc::sub2(pz2, zz.x), dz1 = tc::sub2(pz2, zz.y);
-          s0 = tc::fma2(distance(tc::fma2(dz0, dz0, tc::fma2(dy0, dy0, tc::fma2(dx0, dx0, tiny2)))).d, nslope2, s0);
-          s1 = tc::fma2(distance(tc::fma2(dz1, dz1, tc::fma2(dy1, dy1, tc::fma2(dx1, dx1, tiny2)))).d, nslope2, s1);
+          d0 = distance(tc::fma2(dz0, dz0, tc::fma2(dy0, dy0, tc::fma2(dx0, dx0, tiny2)))).d;
+          d1 = distance(tc::fma2(dz1, dz1, tc::fma2(dy1, dy1, tc::fma2(dx1, dx1, tiny2)))).d;
         }
-        tc::unpack(s0, v[c], v[c + 1]);
-        tc::unpack(s1, v[c + 2], v[c + 3]);
-        if constexpr (CUT) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (c + k >= n) v[c + k] = -INFINITY;
+        for (int h = 0; h < HP; ++h) {
+          float* w = v[h] + c;
+          tc::f2 s0 = tc::mul2(tc::pack(w[0], w[1]), scale2), s1 = tc::mul2(tc::pack(w[2], w[3]), scale2);
+          if constexpr (BIAS) {
+            s0 = tc::fma2(d0, nslope2[h], s0);
+            s1 = tc::fma2(d1, nslope2[h], s1);
+          }
+          tc::unpack(s0, w[0], w[1]);
+          tc::unpack(s1, w[2], w[3]);
+          if constexpr (CUT) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (c + k >= n) w[k] = -INFINITY;
+          }
+          top[h] = tc::max3(tc::max3(top[h], w[0], w[1]), w[2], w[3]);
         }
-        t0 = tc::max3(t0, v[c], v[c + 1]);
-        t1 = tc::max3(t1, v[c + 2], v[c + 3]);
       }
-      const float top = fmaxf(t0, t1);
       // the reference maximum moves only when a row would pass 2^8 times it: P stays within 2^8
       // and the accumulated rows are rescaled seldom
       if (j == 0) {
-        m = top;
+#pragma unroll
+        for (int h = 0; h < HP; ++h) m[h] = top[h];
       } else {
-        const bool move = top > m + 8.0f || (m == -INFINITY && top > m);
-        if (__any_sync(0xffffffffu, move)) {
-          const float f = move ? tc::ex2(m - top) : 1.0f;
-          if (move) m = top;
-          l *= f;
+        bool move[HP], any = false;
+#pragma unroll
+        for (int h = 0; h < HP; ++h) {
+          move[h] = top[h] > m[h] + 8.0f || (m[h] == -INFINITY && top[h] > m[h]);
+          any = any || move[h];
+        }
+        if (__any_sync(0xffffffffu, any)) {
           if (!__all_sync(0xffffffffu, tc::mbar_wait(empty((j - 1) % C::STAGES), ((j - 1) / C::STAGES) & 1)))
             return false;
           tc::fence_after();
 #pragma unroll
-          for (int u = 0; u < C::OPS + (C::TOTALS_SMEM ? 0 : C::TOTALS); ++u) {
-            for (int d = 0; d < acc_n; d += 16) {
-              float o[16];
-              tc::ld16(lane_base + C::ACC + u * C::W + d, o);
-              tc::wait_ld();
-              uint32_t r[16];
+          for (int h = 0; h < HP; ++h) {
+            const float f = move[h] ? tc::ex2(m[h] - top[h]) : 1.0f;
+            if (move[h]) m[h] = top[h];
+            l[h] *= f;
 #pragma unroll
-              for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(o[k] * f);
-              tc::st16(lane_base + C::ACC + u * C::W + d, r);
+            for (int u = 0; u < C::NACC; ++u) {
+              for (int d = 0; d < acc_n; d += 16) {
+                float o[16];
+                tc::ld16(lane_base + C::ACC + (h * C::NACC + u) * C::W + d, o);
+                tc::wait_ld();
+                uint32_t r[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(o[k] * f);
+                tc::st16(lane_base + C::ACC + (h * C::NACC + u) * C::W + d, r);
+              }
+            }
+            if constexpr (C::TOTALS_SMEM) {
+              if (j > C::FLUSH) {
+                for (int d = 0; d < acc_n; ++d) totals[d * kTileRows + r_tile] *= f;
+              }
             }
           }
           tc::wait_st();
-          if constexpr (C::TOTALS_SMEM) {
-            if (j > C::FLUSH) {
-              for (int d = 0; d < acc_n; ++d) totals[d * kTileRows + r_tile] *= f;
-            }
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < HP; ++h) {
+        const float ref = m[h] == -INFINITY ? 0.0f : m[h];
+        const tc::f2 nref = tc::pack(-ref, -ref);
+        tc::f2 l0 = tc::pack(0.0f, 0.0f), l1 = l0;
+        const uint32_t dst = lane_base + C::A0 + ((j % C::BUFS) * HP + h) * C::BUF;
+#pragma unroll
+        for (int c0 = 0; c0 < BN; c0 += 16) {
+          uint32_t pr[NP][8];
+#pragma unroll
+          for (int c = 0; c < 16; c += 2) {
+            float e0, e1;
+            tc::unpack(tc::add2(tc::pack(v[h][c0 + c], v[h][c0 + c + 1]), nref), e0, e1);
+            e0 = tc::ex2(e0);
+            e1 = tc::ex2(e1);
+            if (c & 2) l1 = tc::add2(l1, tc::pack(e0, e1));
+            else l0 = tc::add2(l0, tc::pack(e0, e1));
+            uint32_t r[NP];
+            split_pair<NP>(e0, e1, r);
+#pragma unroll
+            for (int p = 0; p < NP; ++p) pr[p][c / 2] = r[p];
           }
+#pragma unroll
+          for (int p = 0; p < NP; ++p) tc::st8(dst + p * (BN / 2) + c0 / 2, pr[p]);
         }
+        float s0, s1;
+        tc::unpack(tc::add2(l0, l1), s0, s1);
+        l[h] += s0 + s1;
       }
-      const float ref = m == -INFINITY ? 0.0f : m;
-      const tc::f2 nref = tc::pack(-ref, -ref);
-      tc::f2 l0 = tc::pack(0.0f, 0.0f), l1 = l0;
-      const uint32_t dst = lane_base + C::A0 + (j % C::BUFS) * C::BUF;
-#pragma unroll
-      for (int c0 = 0; c0 < BN; c0 += 16) {
-        uint32_t pr[NP][8];
-#pragma unroll
-        for (int c = 0; c < 16; c += 2) {
-          float e0, e1;
-          tc::unpack(tc::add2(tc::pack(v[c0 + c], v[c0 + c + 1]), nref), e0, e1);
-          e0 = tc::ex2(e0);
-          e1 = tc::ex2(e1);
-          if (c & 2) l1 = tc::add2(l1, tc::pack(e0, e1));
-          else l0 = tc::add2(l0, tc::pack(e0, e1));
-          uint32_t r[NP];
-          split_pair<NP>(e0, e1, r);
-#pragma unroll
-          for (int p = 0; p < NP; ++p) pr[p][c / 2] = r[p];
-        }
-#pragma unroll
-        for (int p = 0; p < NP; ++p) tc::st8(dst + p * (BN / 2) + c0 / 2, pr[p]);
-      }
-      float s0, s1;
-      tc::unpack(tc::add2(l0, l1), s0, s1);
-      l += s0 + s1;
       return true;
     };
 
@@ -671,7 +720,7 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
             const Distance x = distance(tc::fma2(dz, dz, tc::fma2(dy, dy, tc::fma2(dx, dx, tiny2))));
             d = x.d;
             r = x.r;
-            score = tc::fma2(d, nslope2, score);
+            score = tc::fma2(d, nslope2[0], score);
           }
           float p0, p1;
           if constexpr (MODE == kQuerySide) tc::unpack(tc::add2(score, nL2), p0, p1);
@@ -742,7 +791,7 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
       if (!ok) break;
       tc::fence_after();
       const float* ex = extra + s * C::EXTRA;
-      const uint32_t buf = lane_base + (j % C::BUFS) * C::BUF;
+      const uint32_t buf = lane_base + (j % C::BUFS) * (HP * C::BUF);
       // a warp without a row of the item only keeps the barriers going: its lanes of P reach no result
       if (32 * (warp & 3) < item.rows) {
         if constexpr (MODE == kForward) {
@@ -753,8 +802,7 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
             if (sub != last_sub) {
               fold();
               last_sub = sub;
-              slope = a.slopes[head * a.group + sub];
-              nslope2 = tc::pack(-slope * kLog2e, -slope * kLog2e);
+              set_slopes(sub);
             }
           }
           if (((j / C::GROUPS) & 3) == 3) fold();
@@ -786,110 +834,112 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
     // the groups' sums: every thread gets the other group's of its row, through the stages' memory
     if constexpr (C::GROUPS == 2) {
       float* shared = reinterpret_cast<float*>(tile_smem + (cols - tc::smem_addr(tile_smem)));
-      constexpr int N = MODE == kQuerySide ? 10 : 3;
       asm volatile("bar.sync 1, 256;\n" ::: "memory");
       if (ok) {
 #pragma unroll
-        for (int k = 0; k < N; ++k) shared[(group * N + k) * kTileRows + r_tile] = sum[k];
+        for (int k = 0; k < SUMS; ++k) shared[(group * SUMS + k) * kTileRows + r_tile] = sum[k];
       }
       asm volatile("bar.sync 1, 256;\n" ::: "memory");
       if (ok) {
-        const float* other = shared + (1 - group) * N * kTileRows + r_tile;
+        const float* other = shared + (1 - group) * SUMS * kTileRows + r_tile;
 #pragma unroll
-        for (int k = 0; k < N; ++k) sum[k] += other[k * kTileRows];
+        for (int k = 0; k < SUMS; ++k) sum[k] += other[k * kTileRows];
       }
     }
     if (ok) {
       tc::fence_after();
       const bool split = item.slot >= 0;
-      const int64_t at = row * heads + head;
-      float* part = split ? a.part + ((int64_t(item.slot) * heads + head) * kTileRows + r_tile) * C::PART : nullptr;
-      float f0 = 1.0f;
-      bool none = total == 0;
-      if constexpr (MODE == kForward) {
-        none = none || (m == -INFINITY && l == 0.0f);
-        f0 = split ? 1.0f : none ? 0.0f : 1.0f / l;
-      } else if constexpr (MODE == kQuerySide) {
-        f0 = split ? 1.0f : a.scale;
-      }
-      // query side: the sum of P is 1 up to the rounding of lse; dividing by it takes that out of delta
-      float inv = 0.0f, dl = 0.0f;
-      if constexpr (MODE == kQuerySide) {
-        inv = none ? 0.0f : 1.0f / sum[9];
-        dl = sum[0] * inv;
-      }
 #pragma unroll
-      for (int op = 0; op < C::OPS; ++op) {
-        const float f = MODE == kKeySide && op == 1 && !split ? a.scale : f0;
-        T* dst = static_cast<T*>(op ? a.out1 : a.out0) + at * a.D;
-        for (int d = 16 * group; d < acc_n; d += 16 * C::GROUPS) {
-          float o[16];
-          tc::ld16(lane_base + C::ACC + op * C::W + d, o);
-          if constexpr (C::TOTALS > 0 || C::FIX) {
-            float e[16];
-            if constexpr (C::TOTALS_SMEM) {
+      for (int h = 0; h < HP; ++h) {
+        const int64_t at = row * heads + head0 + h;
+        float* part = split ? a.part + ((int64_t(item.slot) * heads + head0 + h) * kTileRows + r_tile) * C::PART : nullptr;
+          float f0 = 1.0f;
+        bool none = total == 0;
+        if constexpr (MODE == kForward) {
+          none = none || (m[h] == -INFINITY && l[h] == 0.0f);
+          f0 = split ? 1.0f : none ? 0.0f : 1.0f / l[h];
+        } else if constexpr (MODE == kQuerySide) {
+          f0 = split ? 1.0f : a.scale;
+        }
+        // query side: the sum of P is 1 up to the rounding of lse; dividing by it takes that out of delta
+        float inv = 0.0f, dl = 0.0f;
+        if constexpr (MODE == kQuerySide) {
+          inv = none ? 0.0f : 1.0f / sum[9];
+          dl = sum[0] * inv;
+        }
 #pragma unroll
-              for (int k = 0; k < 16; ++k) e[k] = totals[(op * C::W + d + k) * kTileRows + r_tile];
-            } else {
-              tc::ld16(lane_base + C::ACC + (C::OPS + op) * C::W + d, e);
-            }
-            tc::wait_ld();
-            const bool whole = C::TOTALS > 0 && total <= C::FLUSH;  // nothing went into the total
-            if (whole) {
+        for (int op = 0; op < C::OPS; ++op) {
+          const float f = MODE == kKeySide && op == 1 && !split ? a.scale : f0;
+          T* dst = static_cast<T*>(op ? a.out1 : a.out0) + at * a.D;
+          for (int d = 16 * group; d < acc_n; d += 16 * C::GROUPS) {
+            float o[16];
+            tc::ld16(lane_base + C::ACC + (h * C::NACC + op) * C::W + d, o);
+            if constexpr (C::TOTALS > 0 || C::FIX) {
+              float e[16];
+              if constexpr (C::TOTALS_SMEM) {
 #pragma unroll
-              for (int k = 0; k < 16; ++k) e[k] = 0.0f;
-            }
-            const float fe = !C::FIX ? 1.0f : split ? 0.0f : delta0 - dl;
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              if constexpr (C::FIX) {
-                if (split && valid) part[DP + 16 + d + k] = none ? 0.0f : e[k];
+                for (int k = 0; k < 16; ++k) e[k] = totals[(op * C::W + d + k) * kTileRows + r_tile];
+              } else {
+                tc::ld16(lane_base + C::ACC + (h * C::NACC + C::OPS + op) * C::W + d, e);
               }
-              o[k] = fmaf(fe, e[k], o[k]);
-            }
-          } else {
-            tc::wait_ld();
-          }
-          if (valid) {
+              tc::wait_ld();
+              const bool whole = C::TOTALS > 0 && total <= C::FLUSH;  // nothing went into the total
+              if (whole) {
 #pragma unroll
-            for (int k = 0; k < 16; ++k) o[k] = none ? 0.0f : o[k] * f;
-            if (split) {
+                for (int k = 0; k < 16; ++k) e[k] = 0.0f;
+              }
+              const float fe = !C::FIX ? 1.0f : split ? 0.0f : delta0 - dl;
 #pragma unroll
-              for (int k = 0; k < 16; k += 4)
-                *reinterpret_cast<float4*>(part + op * DP + d_first + d + k) =
-                    make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+              for (int k = 0; k < 16; ++k) {
+                if constexpr (C::FIX) {
+                  if (split && valid) part[DP + 16 + d + k] = none ? 0.0f : e[k];
+                }
+                o[k] = fmaf(fe, e[k], o[k]);
+              }
             } else {
-              store_row16<T>(dst, o, d_first + d, a.D, a.vec != 0);
+              tc::wait_ld();
+            }
+            if (valid) {
+#pragma unroll
+              for (int k = 0; k < 16; ++k) o[k] = none ? 0.0f : o[k] * f;
+              if (split) {
+#pragma unroll
+                for (int k = 0; k < 16; k += 4)
+                  *reinterpret_cast<float4*>(part + op * DP + d_first + d + k) =
+                      make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+              } else {
+                store_row16<T>(dst, o, d_first + d, a.D, a.vec != 0);
+              }
             }
           }
         }
-      }
-      if (valid && group == 0) {
-        if constexpr (MODE == kForward) {
-          if (split) {
-            part[DP] = none ? -INFINITY : m;
-            part[DP + 1] = l;
-          } else {
-            a.lse[at] = none ? INFINITY : m + log2f(l);
-          }
-        } else if constexpr (MODE == kQuerySide) {
-          if (split) {
-#pragma unroll
-            for (int k = 0; k < 10; ++k) part[DP + k] = sum[k];
-            part[DP + 10] = delta0;
-          } else {
-            a.delta[at] = dl;
-            if constexpr (BIAS) {
-              a.slope_part[at] = -inv * (sum[1] - dl * sum[2]);
-#pragma unroll
-              for (int k = 0; k < 3; ++k) a.place_part[at * 3 + k] = -slope * inv * (sum[3 + k] - dl * sum[6 + k]);
+        if (valid && group == 0) {
+          if constexpr (MODE == kForward) {
+            if (split) {
+              part[DP] = none ? -INFINITY : m[h];
+              part[DP + 1] = l[h];
+            } else {
+              a.lse[at] = none ? INFINITY : m[h] + log2f(l[h]);
             }
-          }
-        } else if (BIAS && half == 0) {
+          } else if constexpr (MODE == kQuerySide) {
+            if (split) {
 #pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            if (split) part[2 * DP + k] = sum[k];
-            else a.place_part[at * 3 + k] = -sum[k];
+              for (int k = 0; k < 10; ++k) part[DP + k] = sum[k];
+              part[DP + 10] = delta0;
+            } else {
+              a.delta[at] = dl;
+              if constexpr (BIAS) {
+                a.slope_part[at] = -inv * (sum[1] - dl * sum[2]);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) a.place_part[at * 3 + k] = -slope[0] * inv * (sum[3 + k] - dl * sum[6 + k]);
+              }
+            }
+          } else if (BIAS && half == 0) {
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+              if (split) part[2 * DP + k] = sum[k];
+              else a.place_part[at * 3 + k] = -sum[k];
+            }
           }
         }
       }
@@ -909,18 +959,18 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP>::THREADS, AttCfg<MODE, DP
 // Encodes the tensor map of a column operand; its strides are positive multiples of 16 bytes.
 int encode_columns(CUtensorMap* map, const AttOperand& o, int D, int heads, int64_t rows, int pieces, int box_rows);
 
-template <int MODE, int DP, int NP, bool BIAS>
+template <int MODE, int DP, int NP, int HP, bool BIAS>
 int launch_attention_tile(AttTileArgs& a, int64_t items, cudaStream_t s) {
-  using C = AttCfg<MODE, DP, NP>;
+  using C = AttCfg<MODE, DP, NP, HP>;
   int rc = encode_columns(&a.cols[0], MODE == kKeySide ? a.q : a.k, a.D, MODE == kKeySide ? a.H : a.Hk,
                           MODE == kKeySide ? a.nq : a.nk, NP, C::BN);
   if (!rc)
     rc = encode_columns(&a.cols[1], MODE == kKeySide ? a.g : a.v, a.D, MODE == kKeySide ? a.H : a.Hk,
                         MODE == kKeySide ? a.nq : a.nk, NP, C::BN);
   if (rc) return rc;
-  const auto kernel = attention_tile_kernel<MODE, DP, NP, BIAS>;
+  const auto kernel = attention_tile_kernel<MODE, DP, NP, HP, BIAS>;
   Y3B_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-  const int64_t grid = items * (MODE == kKeySide ? a.Hk : a.H) * C::HALVES;
+  const int64_t grid = items * ((MODE == kKeySide ? a.Hk : a.H) / HP) * C::HALVES;
   if (grid > INT32_MAX) return fail(Y3B_ERR_UNSUPPORTED, "structure_attention: %lld tiles", (long long)grid);
   kernel<<<unsigned(grid), C::THREADS, C::SMEM, s>>>(a);
   Y3B_LAUNCH_CHECK();
@@ -932,9 +982,12 @@ int dispatch_attention_tile(int pieces, AttTileArgs& a, int64_t items, cudaStrea
   if (items == 0) return Y3B_OK;
   const bool bias = a.slopes != nullptr, wide = a.D > 64;
 #define Y3B_TILE(DP, NP)                                                       \
-  return bias ? launch_attention_tile<MODE, DP, NP, true>(a, items, s)         \
-              : launch_attention_tile<MODE, DP, NP, false>(a, items, s)
+  return bias ? launch_attention_tile<MODE, DP, NP, 1, true>(a, items, s)      \
+              : launch_attention_tile<MODE, DP, NP, 1, false>(a, items, s)
   if (pieces == 1) {
+    if constexpr (MODE == kForward) {
+      if (bias && !wide && a.H % 2 == 0) return launch_attention_tile<MODE, 64, 1, 2, true>(a, items, s);
+    }
     if (wide) { Y3B_TILE(128, 1); }
     Y3B_TILE(64, 1);
   }
