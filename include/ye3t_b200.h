@@ -669,19 +669,23 @@ typedef struct {
    * One or two queries of a larger structure are the rows of an item in few_items, its keys split over items that one
    * few_joins entry joins.  Every other query is in query_rows (one warp computes it) or in exactly one tile of up to 128 queries
    * of one structure; a tile is one item, or several items with consecutive slots that split its keys and
-   * one join.  Keys likewise, with queries as the columns.
+   * one join: in forward_items and forward_joins for the call, in query_items and query_joins for its
+   * adjoint.  Keys likewise, with queries as the columns.
    *   row   (query or key, its structure)
    *   small (first query, queries, first key, keys)
    *   item  (first row, rows, first column, columns, slot or -1, 0, 0, 0)
    *   join  (first row, rows, first slot, slots) */
   int64_t small_32_count, small_64_count;
   int64_t few_item_count, few_join_count, few_slot_count;
+  int64_t forward_item_count, forward_join_count, forward_slot_count;
   int64_t query_item_count, query_join_count, query_slot_count, query_row_count;
   int64_t key_item_count, key_join_count, key_slot_count, key_row_count;
   const int32_t* small;       /* 16-byte aligned */
   const int32_t* few_items;   /* 32-byte aligned */
   const int32_t* few_joins;   /* 16-byte aligned */
-  const int32_t* query_items; /* 32-byte aligned */
+  const int32_t* forward_items; /* 32-byte aligned */
+  const int32_t* forward_joins; /* 16-byte aligned */
+  const int32_t* query_items;   /* 32-byte aligned */
   const int32_t* query_joins; /* 16-byte aligned */
   const int32_t* query_rows;
   const int32_t* key_items;
@@ -691,8 +695,8 @@ typedef struct {
 } y3b_structure_attention_args;
 
 /* Work tables of a batch (host arrays): query_counts[s] queries and key_counts[s] keys of structure s, one after the
- * other.  counts takes the thirteen table sizes from small_32_count to key_row_count in the order of the struct;
- * tables takes query_items, key_items, few_items, query_joins, key_joins, few_joins, small, query_rows, key_rows,
+ * other.  counts takes the sixteen table sizes from small_32_count to key_row_count in the order of the struct;
+ * tables takes forward_items, query_items, key_items, few_items, forward_joins, query_joins, key_joins, few_joins, small, query_rows, key_rows,
  * query_offsets and key_offsets one after the other, if capacity holds them.  Returns their number of int32 values, or
  * a negative error code. */
 int64_t y3b_structure_layout(const int64_t* query_counts, const int64_t* key_counts, int64_t structure_count,

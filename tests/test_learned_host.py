@@ -50,7 +50,7 @@ def test_entry_points_refuse_bad_arguments():
     assert lib.y3b_species_embedding_adjoint_workspace_bytes(nat.F32, 1000, 1000, 8) > 0
     assert lib.y3b_species_embedding_adjoint(nat.F32, 0, 0, 8, 10, 3, 4, 1.0, 0, 0, 0, 0, 0) == -1
     one, minus = np.array([5], np.int64), np.array([-1], np.int64)
-    sizes = np.zeros(13, np.int64)
+    sizes = np.zeros(16, np.int64)
     layout = lambda q, k, h=4, hk=2: lib.y3b_structure_layout(  # noqa: E731
         q.ctypes.data, k.ctypes.data, 1, h, hk, sizes.ctypes.data, 0, 0)
     assert layout(one, one) > 0
@@ -102,12 +102,12 @@ def _random_counts(rng):
 
 
 @pytest.mark.parametrize("seed", range(40))
-def test_layout_tables_hold_every_row_once(seed):
+def test_layout_tables_hold_every_row_once(seed, counts=None):
     """Every query (and key) of a batch is in exactly one small structure, row entry, few-query item set or tile; a
     tile's items are its structure's columns, each once; slots are joined once."""
     from ye3t_b200 import runtime as rt
     rng = np.random.default_rng(seed)
-    queries, keys = _random_counts(rng)
+    queries, keys = _random_counts(rng) if counts is None else (np.array(counts), np.array(counts))
     heads, key_heads = ((8, 2), (4, 4), (1, 1))[seed % 3]
     packed, sizes = rt._layout_tables(queries, keys, heads, key_heads)
     counts = dict(zip(rt._LAYOUT_COUNTS[6:], sizes), structure_count=len(queries))
@@ -124,15 +124,15 @@ def test_layout_tables_hold_every_row_once(seed):
     for k, (a, n, b, m) in enumerate(tables["small"]):
         most = 32 if k < counts["small_32_count"] else 64
         assert n <= most and m <= most
-    for side, off, other, number in (("query", q_off, k_off, queries), ("key", k_off, q_off, keys)):
+    for side, off, other in (("query", q_off, k_off), ("forward", q_off, k_off), ("key", k_off, q_off)):
         seen = np.zeros(off[-1], int)
         for a, n, b, m in small:
-            first, count = (a, n) if side == "query" else (b, m)
+            first, count = (b, m) if side == "key" else (a, n)
             seen[first:first + count] += 1
-        for row, structure in tables[f"{side}_rows"]:
+        for row, structure in tables["key_rows" if side == "key" else "query_rows"]:
             assert off[structure] <= row < off[structure + 1]
             seen[row] += 1
-        kinds = ("query", "few") if side == "query" else ("key",)
+        kinds = ("key",) if side == "key" else (side, "few")
         for kind in kinds:
             items, joins = tables[f"{kind}_items"], tables[f"{kind}_joins"]
             columns, slots = {}, {}
@@ -163,3 +163,10 @@ def test_layout_tables_hold_every_row_once(seed):
             if kind == "few":
                 assert all(i[1] <= 2 for i in items)
         assert (seen == 1).all()
+
+
+@pytest.mark.parametrize("atoms", [129, 1000, 2048, 5000, 8192, 16384, 20000])
+def test_layout_tables_of_one_structure(atoms):
+    """The same for one structure, whose tiles are cut by waves."""
+    for seed in range(3):
+        test_layout_tables_hold_every_row_once(seed, [atoms])

@@ -105,9 +105,11 @@ class StructureAttentionArgs(ctypes.Structure):
         ("query_offsets", VP), ("key_offsets", VP),
         ("small_32_count", I64), ("small_64_count", I64),
         ("few_item_count", I64), ("few_join_count", I64), ("few_slot_count", I64),
+        ("forward_item_count", I64), ("forward_join_count", I64), ("forward_slot_count", I64),
         ("query_item_count", I64), ("query_join_count", I64), ("query_slot_count", I64), ("query_row_count", I64),
         ("key_item_count", I64), ("key_join_count", I64), ("key_slot_count", I64), ("key_row_count", I64),
-        ("small", VP), ("few_items", VP), ("few_joins", VP), ("query_items", VP), ("query_joins", VP), ("query_rows", VP), ("key_items", VP), ("key_joins", VP),
+        ("small", VP), ("few_items", VP), ("few_joins", VP), ("forward_items", VP),
+        ("forward_joins", VP), ("query_items", VP), ("query_joins", VP), ("query_rows", VP), ("key_items", VP), ("key_joins", VP),
         ("key_rows", VP), ("scale", ctypes.c_float),
     ]
 

@@ -397,6 +397,9 @@ int unpack(const y3b_structure_attention_args* p, const char* what, AttArgs* a) 
   Y3B_CHECK_ARG(p->few_item_count >= 0 && p->few_join_count >= 0 && p->few_slot_count >= 0 &&
                     (p->few_item_count == 0 || (p->few_items && p->few_joins && p->few_join_count > 0)),
                 "%s: bad table of few-query structures", what);
+  Y3B_CHECK_ARG(p->forward_item_count >= 0 && p->forward_join_count >= 0 && p->forward_slot_count >= 0 &&
+                    (p->forward_item_count == 0 || p->forward_items) && (p->forward_join_count == 0 || p->forward_joins),
+                "%s: bad table of the forward", what);
   Y3B_CHECK_ARG(p->query_item_count >= 0 && p->query_join_count >= 0 && p->query_slot_count >= 0 &&
                     p->query_row_count >= 0 && p->key_item_count >= 0 && p->key_join_count >= 0 &&
                     p->key_slot_count >= 0 && p->key_row_count >= 0,
@@ -600,7 +603,7 @@ unsigned row_grid(int64_t tasks) { return unsigned((tasks + kRowWarps - 1) / kRo
 int check_grids(const y3b_structure_attention_args* p, const char* what) {
   const int64_t most = int64_t(INT32_MAX) / kJoinCtas;
   if (p->query_row_count * p->heads > INT32_MAX || p->key_row_count * p->key_heads > INT32_MAX ||
-      p->query_join_count * p->heads > most || p->few_join_count * p->heads > most ||
+      p->query_join_count * p->heads > most || p->forward_join_count * p->heads > most || p->few_join_count * p->heads > most ||
       p->key_join_count * p->key_heads > most)
     return fail(Y3B_ERR_UNSUPPORTED, "%s: the batch's tables ask for more than 2^31 - 1 CTAs", what);
   return Y3B_OK;
@@ -631,7 +634,7 @@ AttPlan make_plan(const y3b_structure_attention_args* p, bool adjoint) {
   w.Wf = w.DP + 16;
   w.Wq = (w.pieces == 1 ? 2 : 1) * w.DP + 16;
   w.Wk = 2 * w.DP + 16;
-  w.tiles = p->query_item_count > 0 || (adjoint && p->key_item_count > 0);
+  w.tiles = adjoint ? p->query_item_count > 0 || p->key_item_count > 0 : p->forward_item_count > 0;
   w.direct[0] = in_place(p, p->query, p->query_row_stride, p->query_head_stride);
   w.direct[1] = in_place(p, p->key, p->key_row_stride, p->key_head_stride);
   w.direct[2] = in_place(p, p->value, p->value_row_stride, p->value_head_stride);
@@ -650,7 +653,8 @@ AttPlan make_plan(const y3b_structure_attention_args* p, bool adjoint) {
   w.slope = take(adjoint ? nq * H * 4 : 0);
   w.dx = take(adjoint ? nq * H * 12 : 0);
   w.dy = take(adjoint ? nk * Hk * 12 : 0);
-  w.part_q = take(p->query_slot_count * H * kTileRows * w.Wq * 4);
+  w.part_q = take(adjoint ? p->query_slot_count * H * kTileRows * w.Wq * 4
+                          : p->forward_slot_count * H * kTileRows * w.Wf * 4);
   w.part_k = take(adjoint ? p->key_slot_count * Hk * kTileRows * w.Wk * 4 : 0);
   w.part_few = take(p->few_slot_count * H * kFewQueries * ((adjoint ? 2 : 1) * w.DP + 16) * 4);
   w.bytes = at;
@@ -736,20 +740,20 @@ int forward(const y3b_structure_attention_args* p, const AttArgs& a, const AttPl
         static_cast<T*>(out), lse);
     Y3B_LAUNCH_CHECK();
   }
-  if (p->query_item_count > 0) {
+  if (p->forward_item_count > 0) {
     AttTileArgs t = tile_args(p, a, w, status);
     int rc = operands(p, w, nullptr, ws, &t, s);
     if (rc) return rc;
-    t.items = reinterpret_cast<const AttItem*>(p->query_items);
+    t.items = reinterpret_cast<const AttItem*>(p->forward_items);
     t.out0 = out;
     t.lse = lse;
     t.part = reinterpret_cast<float*>(ws + w.part_q);
     t.vec = a.D * sizeof(T) % 16 == 0 && on16(out);
-    rc = attention_forward_tiles(w.pieces, t, p->query_item_count, s);
+    rc = attention_forward_tiles(w.pieces, t, p->forward_item_count, s);
     if (rc) return rc;
-    if (p->query_join_count > 0) {
-      join_forward_kernel<T><<<unsigned(p->query_join_count * a.H * kJoinCtas), 128, 0, s>>>(
-          reinterpret_cast<const AttJoin*>(p->query_joins), t.part, kTileRows, w.Wf, w.DP, a.D, a.H, static_cast<T*>(out), lse);
+    if (p->forward_join_count > 0) {
+      join_forward_kernel<T><<<unsigned(p->forward_join_count * a.H * kJoinCtas), 128, 0, s>>>(
+          reinterpret_cast<const AttJoin*>(p->forward_joins), t.part, kTileRows, w.Wf, w.DP, a.D, a.H, static_cast<T*>(out), lse);
       Y3B_LAUNCH_CHECK();
     }
   }

@@ -9,7 +9,8 @@
 //   few     up to two queries: a tile would hold 2 rows of 128 (8 structures of 16,384 keys, 8 heads: 111 us on tiles,
 //           64 on the few-query kernels); their keys keep to the tile kernels;
 //   tile    the rest.
-// A tile's columns are split where the tiles alone would not give every SM its two CTAs, and joined.
+// A tile's columns are cut into parts, which are joined, where that makes the last wave of CTAs shorter (16,384 atoms, 8
+// heads: forward 1,273 us and 39 to join against 1,431 uncut).
 #include <algorithm>
 #include <iterator>
 #include <new>
@@ -35,19 +36,61 @@ struct Part {
   int32_t row, rows, col, cols, slot;
 };
 
-// Tiles of the structures in `which`: rows [row] and columns [col] of each; `always` joins every tile.
+// How many parts a tile of `cols` columns is cut into: all alike, or only those past the last full wave.  CTAs cost
+// kStart columns of time to start and finish, and a part kJoin more to be joined.
+constexpr int64_t kStart = 96, kJoin = 64, kMostParts = 8;
+
+struct Cut {
+  int64_t all = 1, last = 1, from = 0;  // tiles from number `from` on are cut into `last` parts, those before into `all`
+};
+
+// Tiles of equal length on `slots` places for a tile (over all heads): the cheapest number of waves.
+Cut cut_evenly(int64_t tiles, int64_t cols, int64_t slots) {
+  Cut best;
+  best.from = tiles;
+  const auto waves = [&](int64_t n) { return (n + slots - 1) / slots; };
+  int64_t least = waves(tiles) * (cols + kStart);
+  for (int64_t n = 2; n <= kMostParts && cols / n >= 256; ++n) {
+    const int64_t part = cols / n + kStart + kJoin;
+    if (waves(tiles * n) * part < least) {
+      least = waves(tiles * n) * part;
+      best.all = best.last = n;
+      best.from = tiles;
+    }
+    const int64_t full = tiles / slots * slots;
+    const int64_t cost = full / slots * (cols + kStart) + waves((tiles - full) * n) * part;
+    if (full > 0 && cost < least) {
+      least = cost;
+      best.all = 1;
+      best.last = n;
+      best.from = full;
+    }
+  }
+  return best;
+}
+
+// Tiles of the structures in `which`: rows [row] and columns [col] of each, on `slots` places over all heads; `always`
+// joins every tile.
 void add_tiles(Side* side, const std::vector<Range>& row, const std::vector<Range>& col,
-               const std::vector<int64_t>& which, int64_t heads, bool always) {
-  int64_t work = 0;
-  for (const int64_t s : which) work += (row[s].count + kTile - 1) / kTile * std::max<int64_t>(col[s].count, 1);
-  work *= heads;
-  // two CTAs an SM of the tile kernels, four of the few-query kernels
-  const int64_t chunk = always ? std::max<int64_t>(128, work / (kSMs * 4)) : std::max<int64_t>(256, work / (kSMs * 2));
-  std::vector<Part> parts;
+               const std::vector<int64_t>& which, int64_t heads, int64_t slots, bool always) {
+  int64_t work = 0, tiles = 0;
+  bool even = !which.empty() && !always;
   for (const int64_t s : which) {
-    const int64_t n = std::max<int64_t>(1, (2 * col[s].count + chunk) / (2 * chunk));
-    const int64_t step = ((col[s].count + n - 1) / n + 63) / 64 * 64;  // parts begin at multiples of 64 columns
-    for (int64_t r = 0; r < row[s].count; r += kTile) {
+    const int64_t n = (row[s].count + kTile - 1) / kTile;
+    tiles += n;
+    work += n * std::max<int64_t>(col[s].count, 1);
+    even = even && col[s].count == col[which[0]].count;
+  }
+  // parts of tiles of many lengths: no longer than what a place would get of the whole
+  const int64_t chunk = std::max<int64_t>(always ? 128 : 256, work * heads / slots);
+  const Cut cut = even ? cut_evenly(tiles * heads, col[which[0]].count, slots) : Cut{};
+  std::vector<Part> parts;
+  int64_t tile = 0;
+  for (const int64_t s : which) {
+    for (int64_t r = 0; r < row[s].count; r += kTile, ++tile) {
+      const int64_t n = even ? (tile * heads >= cut.from ? cut.last : cut.all)
+                             : std::max<int64_t>(1, (2 * col[s].count + chunk) / (2 * chunk));
+      const int64_t step = ((col[s].count + n - 1) / n + 63) / 64 * 64;  // parts begin at multiples of 64 columns
       const int32_t first = int32_t(row[s].first + r), rows = int32_t(std::min(kTile, row[s].count - r));
       const bool split = n > 1 || always;
       if (split) {
@@ -106,21 +149,25 @@ int64_t build(const int64_t* queries, const int64_t* keys, int64_t n, int64_t he
       else if (queries[s] > 0) few.push_back(s);
     }
   }
-  Side query, key, one;
-  add_tiles(&query, q, k, tiled, heads, false);
-  add_tiles(&key, k, q, key_tiled, key_heads, false);
-  add_tiles(&one, q, k, few, key_heads, true);
+  // Places: two CTAs an SM of the tile kernels, and the forward's take two heads where their number is even; four of
+  // the few-query kernels.
+  Side forward, query, key, one;
+  add_tiles(&forward, q, k, tiled, heads, kSMs * (heads % 2 == 0 ? 4 : 2), false);
+  add_tiles(&query, q, k, tiled, heads, kSMs * 2, false);
+  add_tiles(&key, k, q, key_tiled, key_heads, kSMs * 2, false);
+  add_tiles(&one, q, k, few, key_heads, kSMs * 4, true);
   add_rows(&query, q, by_row);
   add_rows(&key, k, by_row);
   const auto entries = [](const std::vector<int32_t>& v, int width) { return int64_t(v.size()) / width; };
   const int64_t all[] = {int64_t(low.size()),      int64_t(high.size()),     entries(one.items, 8),
-                         entries(one.joins, 4),    one.slots,                entries(query.items, 8),
+                         entries(one.joins, 4),    one.slots,                entries(forward.items, 8),
+                         entries(forward.joins, 4), forward.slots,           entries(query.items, 8),
                          entries(query.joins, 4),  query.slots,              entries(query.rows, 2),
                          entries(key.items, 8),    entries(key.joins, 4),    key.slots,
                          entries(key.rows, 2)};
   std::copy(std::begin(all), std::end(all), counts);
-  const std::vector<int32_t>* const tables[] = {&query.items, &key.items, &one.items, &query.joins, &key.joins,
-                                                &one.joins};
+  const std::vector<int32_t>* const tables[] = {&forward.items, &query.items, &key.items, &one.items,
+                                                &forward.joins, &query.joins, &key.joins, &one.joins};
   int64_t need = 4 * int64_t(low.size() + high.size()) + int64_t(query.rows.size() + key.rows.size()) + 2 * (n + 1);
   for (const auto* t : tables) need += int64_t(t->size());
   if (!out || capacity < need) return need;

@@ -624,13 +624,15 @@ def _host_counts(counts, what):
 
 # the counts of a layout, in the order of StructureLayout.counts
 _LAYOUT_COUNTS = ("heads", "key_heads", "query_count", "key_count", "structure_count", "shared", "small_32_count",
-                  "small_64_count", "few_item_count", "few_join_count", "few_slot_count", "query_item_count",
+                  "small_64_count", "few_item_count", "few_join_count", "few_slot_count", "forward_item_count",
+                  "forward_join_count", "forward_slot_count", "query_item_count",
                   "query_join_count", "query_slot_count", "query_row_count", "key_item_count", "key_join_count",
                   "key_slot_count", "key_row_count")
 # its tables in their order, with the integers of an entry and the count they go by: 32-byte records first, then
 # 16-byte ones
-_LAYOUT_TABLES = (("query_items", 8, "query_item_count"), ("key_items", 8, "key_item_count"),
-                  ("few_items", 8, "few_item_count"), ("query_joins", 4, "query_join_count"),
+_LAYOUT_TABLES = (("forward_items", 8, "forward_item_count"), ("query_items", 8, "query_item_count"), ("key_items", 8, "key_item_count"),
+                  ("few_items", 8, "few_item_count"), ("forward_joins", 4, "forward_join_count"),
+                  ("query_joins", 4, "query_join_count"),
                   ("key_joins", 4, "key_join_count"), ("few_joins", 4, "few_join_count"),
                   ("small", 4, None), ("query_rows", 2, "query_row_count"), ("key_rows", 2, "key_row_count"),
                   ("query_offsets", 1, "structure_count"), ("key_offsets", 1, "structure_count"))
@@ -638,7 +640,7 @@ _LAYOUT_TABLES = (("query_items", 8, "query_item_count"), ("key_items", 8, "key_
 
 def _layout_tables(queries, keys, heads, key_heads):
     """A layout's tables, one after the other, and the counts of their entries (``small_32_count`` on)."""
-    lib, counts = nat.lib(), np.empty(13, np.int64)
+    lib, counts = nat.lib(), np.empty(16, np.int64)
     # room for a few entries a structure; a batch that needs more says how much
     tables = np.empty(16 * queries.size + 256, np.int32)
     for _ in range(2):
