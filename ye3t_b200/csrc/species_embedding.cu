@@ -33,40 +33,36 @@ __device__ __forceinline__ int64_t species_at(const I* z, int64_t i, int64_t V) 
   return s >= 0 && s < V ? s : -1;
 }
 
-// A thread writes VEC consecutive channels of kLookups atoms, consecutive threads consecutive addresses.  Bound
-// by the output's store (the table stays in L2); U is 32 bits wide where the element count allows, for the
-// division.
+// A CTA is X threads along the channels by 256 / X along the atoms; a thread writes VEC channels of kLookups atoms.
+// Bound by the output's store: the table stays in L2.
 constexpr int kLookups = 4;
 
-template <typename T, typename I, int VEC, typename U>
+template <typename T, typename I, int VEC>
 __global__ void __launch_bounds__(256) embedding_kernel(const T* __restrict__ table, int64_t V, int C,
                                                         const I* __restrict__ z, int64_t N,
                                                         typename Acc<T>::type scale, T* __restrict__ out,
                                                         int32_t* status) {
   using P = Pack<T, VEC>;
-  const U per_row = U(C / VEC), total = U(N) * per_row;
-  const U step = U(gridDim.x) * 256;
-  U t = U(blockIdx.x) * 256 + threadIdx.x;
-  P r[kLookups];
+  const int64_t first = blockIdx.x * int64_t(blockDim.y * kLookups) + threadIdx.y;
   int64_t s[kLookups];
 #pragma unroll
   for (int k = 0; k < kLookups; ++k) {
-    const U u = t + U(k) * step;
-    s[k] = -2;
-    if (u < total) s[k] = species_at(z, int64_t(u / per_row), V);
+    const int64_t i = first + k * blockDim.y;
+    s[k] = i < N ? species_at(z, i, V) : -2;
+    if (s[k] == -1 && status && threadIdx.x == 0 && blockIdx.y == 0) atomicOr(status, Y3B_STATUS_INDEX_RANGE);
   }
+  const int c = int(blockIdx.y * blockDim.x + threadIdx.x) * VEC;
+  if (c >= C) return;
+  P r[kLookups];
 #pragma unroll
-  for (int k = 0; k < kLookups; ++k) {
-    const U p = (t + U(k) * step) % per_row;
-    if (s[k] >= 0) r[k] = *reinterpret_cast<const P*>(table + s[k] * C + int64_t(p) * VEC);
-    if (s[k] == -1 && status && p == 0) atomicOr(status, Y3B_STATUS_INDEX_RANGE);
-  }
+  for (int k = 0; k < kLookups; ++k)
+    if (s[k] >= 0) r[k] = *reinterpret_cast<const P*>(table + s[k] * C + c);
 #pragma unroll
   for (int k = 0; k < kLookups; ++k) {
     if (s[k] == -2) continue;
 #pragma unroll
     for (int q = 0; q < VEC; ++q) r[k].v[q] = s[k] >= 0 ? narrow<T>(scale * widen<T>(r[k].v[q])) : narrow<T>(0);
-    *reinterpret_cast<P*>(out + (int64_t(t) + int64_t(k) * step) * VEC) = r[k];
+    *reinterpret_cast<P*>(out + (first + k * blockDim.y) * C + c) = r[k];
   }
 }
 
@@ -641,13 +637,15 @@ template <typename T, typename I, int VEC>
 int lookup(const T* table, int64_t V, int C, const I* z, int64_t N, double scale, T* out, int32_t* status,
            cudaStream_t s) {
   using A = typename Acc<T>::type;
-  const int64_t total = N * (C / VEC), ctas = (total + 256 * kLookups - 1) / (256 * kLookups);
-  if (ctas > INT32_MAX) return fail(Y3B_ERR_UNSUPPORTED, "species_embedding: %lld values", (long long)(N * C));
-  // past 2^31 - (the grid's reach) elements the index needs 64 bits
-  if (total < (int64_t(1) << 31))
-    embedding_kernel<T, I, VEC, uint32_t><<<unsigned(ctas), 256, 0, s>>>(table, V, C, z, N, A(scale), out, status);
-  else
-    embedding_kernel<T, I, VEC, uint64_t><<<unsigned(ctas), 256, 0, s>>>(table, V, C, z, N, A(scale), out, status);
+  const int per_row = C / VEC;
+  unsigned x = 1;
+  while (x < 256 && int(x) < per_row) x *= 2;
+  const unsigned y = 256 / x;
+  const int64_t ctas = (N + y * kLookups - 1) / (y * kLookups), slabs = (per_row + x - 1) / x;
+  if (ctas > INT32_MAX || slabs > 65535)
+    return fail(Y3B_ERR_UNSUPPORTED, "species_embedding: %lld atoms of %d channels", (long long)N, C);
+  embedding_kernel<T, I, VEC><<<dim3(unsigned(ctas), unsigned(slabs)), dim3(x, y), 0, s>>>(table, V, C, z, N, A(scale),
+                                                                                          out, status);
   Y3B_LAUNCH_CHECK();
   return Y3B_OK;
 }

@@ -485,8 +485,9 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackA
 
 template <typename T>
 __global__ void __launch_bounds__(128) join_forward_kernel(const AttJoin* __restrict__ joins,
-                                                           const float* __restrict__ part, int RS, int W, int DP, int D,
-                                                           int H, T* __restrict__ out, float* __restrict__ lse) {
+                                                           const float* __restrict__ part, int W, int DP, int D, int H,
+                                                           T* __restrict__ out, float* __restrict__ lse) {
+  constexpr int RS = kTileRows;
   const unsigned ctas = unsigned(RS + 3) / 4, task = blockIdx.x / ctas;
   const AttJoin jn = joins[task / unsigned(H)];
   const int h = int(task % unsigned(H)), lane = threadIdx.x & 31;
@@ -532,6 +533,54 @@ __global__ void __launch_bounds__(128) join_forward_kernel(const AttJoin* __rest
     if (d < D) out[at * D + d] = from_float<T>(none ? 0.0f : o[t] * inv);
   }
   if (lane == 0) lse[at] = none ? INFINITY : m + log2f(l);
+}
+
+// The same where one or two rows have many parts: a CTA a (join, head, query), whose warps take every fourth part.
+template <typename T>
+__global__ void __launch_bounds__(128) join_few_kernel(const AttJoin* __restrict__ joins, const float* __restrict__ part,
+                                                       int W, int DP, int D, int H, T* __restrict__ out,
+                                                       float* __restrict__ lse) {
+  __shared__ float s_o[4][kAttMaxWidth];
+  __shared__ float s_m[4], s_l[4];
+  const unsigned task = blockIdx.x / kFewQueries;
+  const AttJoin jn = joins[task / unsigned(H)];
+  const int h = int(task % unsigned(H)), r = int(blockIdx.x % kFewQueries);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (r >= jn.rows) return;
+  const int64_t step = int64_t(H) * kFewQueries * W;
+  const float* p = part + ((int64_t(jn.first) * H + h) * kFewQueries + r) * W;
+  float m = -INFINITY;
+  for (int k = threadIdx.x; k < jn.count; k += 128) m = fmaxf(m, p[k * step + DP]);
+  m = warp_max(m);
+  if (lane == 0) s_m[warp] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float o[kAttMaxWidth / 32] = {}, l = 0.0f;
+#pragma unroll 4
+  for (int k = warp; k < jn.count; k += 4) {
+    // a part without any score above -inf holds no numbers
+    const float mk = p[k * step + DP], lk = p[k * step + DP + 1];
+    const float f = mk == -INFINITY && lk == 0.0f ? 0.0f : exp2f(mk - ref);
+    l += f == 0.0f ? 0.0f : lk * f;
+#pragma unroll
+    for (int t = 0; t < kAttMaxWidth / 32; ++t) {
+      const int d = lane + 32 * t;
+      const float x = d < D ? p[k * step + d] : 0.0f;
+      o[t] = f == 0.0f ? o[t] : fmaf(x, f, o[t]);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < kAttMaxWidth / 32; ++t) s_o[warp][lane + 32 * t] = o[t];
+  if (lane == 0) s_l[warp] = l;
+  __syncthreads();
+  l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+  const bool none = m == -INFINITY && l == 0.0f;
+  const int64_t at = (int64_t(jn.row) + r) * H + h;
+  const int d = threadIdx.x;
+  if (d < D)
+    out[at * D + d] = from_float<T>(none ? 0.0f : ((s_o[0][d] + s_o[1][d]) + (s_o[2][d] + s_o[3][d])) / l);
+  if (d == 0) lse[at] = none ? INFINITY : m + log2f(l);
 }
 
 __device__ __forceinline__ float sum_parts(const float* p, int64_t step, int count) {
@@ -735,9 +784,8 @@ int forward(const y3b_structure_attention_args* p, const AttArgs& a, const AttPl
     const int rc = attention_few_forward<T>(a, reinterpret_cast<const AttItem*>(p->few_items), p->few_item_count, w.DP,
                                             w.DP + 16, part, s);
     if (rc) return rc;
-    join_forward_kernel<T><<<unsigned(p->few_join_count * a.H), 128, 0, s>>>(
-        reinterpret_cast<const AttJoin*>(p->few_joins), part, kFewQueries, w.DP + 16, w.DP, a.D, a.H,
-        static_cast<T*>(out), lse);
+    join_few_kernel<T><<<unsigned(p->few_join_count * a.H * kFewQueries), 128, 0, s>>>(
+        reinterpret_cast<const AttJoin*>(p->few_joins), part, w.DP + 16, w.DP, a.D, a.H, static_cast<T*>(out), lse);
     Y3B_LAUNCH_CHECK();
   }
   if (p->forward_item_count > 0) {
@@ -753,7 +801,7 @@ int forward(const y3b_structure_attention_args* p, const AttArgs& a, const AttPl
     if (rc) return rc;
     if (p->forward_join_count > 0) {
       join_forward_kernel<T><<<unsigned(p->forward_join_count * a.H * kJoinCtas), 128, 0, s>>>(
-          reinterpret_cast<const AttJoin*>(p->forward_joins), t.part, kTileRows, w.Wf, w.DP, a.D, a.H, static_cast<T*>(out), lse);
+          reinterpret_cast<const AttJoin*>(p->forward_joins), t.part, w.Wf, w.DP, a.D, a.H, static_cast<T*>(out), lse);
       Y3B_LAUNCH_CHECK();
     }
   }

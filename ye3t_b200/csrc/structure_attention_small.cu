@@ -79,29 +79,31 @@ __device__ __forceinline__ float quad_max(float v) {
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
 }
 
-// Rows [0, n) of one head into shared memory (ROWS rows of `stride` values), zeros elsewhere.  The copies are
-// asynchronous, so that those of all operands are in flight together: arrived() waits for them.
-template <typename T, int ROWS>
-__device__ __forceinline__ void load_rows(T* dst, int stride, const T* src, int64_t row, int n, int D, bool vec) {
+// Rows [0, n) of one head into shared memory (`rows` rows of `stride` values), zeros elsewhere.  The copies are
+// asynchronous, so that those of all operands are in flight together: arrived() waits for them.  2^shift threads take a
+// row's 16-byte parts.
+template <typename T>
+__device__ __forceinline__ void load_rows(T* dst, int stride, const T* src, int64_t row, int n, int rows, int D, int shift,
+                                          bool vec) {
   constexpr int W = 16 / int(sizeof(T));
   const int width = (D + 7) / 8 * 8;
   if (vec) {
-    const int per = width / W;
-    for (int u = threadIdx.x; u < ROWS * per; u += blockDim.x) {
-      const int r = u / per, d = (u - r * per) * W;
-      tc::cp16(tc::smem_addr(dst + r * stride + d), r < n ? src + r * row + d : src, r < n);
+    const int d = int(threadIdx.x & ((1u << shift) - 1u)) * W;
+    if (d < width) {
+      const uint32_t to = tc::smem_addr(dst) + uint32_t(d) * uint32_t(sizeof(T));
+      for (int r = int(threadIdx.x >> shift); r < rows; r += int(blockDim.x >> shift))
+        tc::cp16(to + uint32_t(r * stride) * uint32_t(sizeof(T)), r < n ? src + r * row + d : src, r < n);
     }
   } else {
-    for (int u = threadIdx.x; u < ROWS * width; u += blockDim.x) {
+    for (int u = threadIdx.x; u < rows * width; u += blockDim.x) {
       const int r = u / width, d = u - r * width;
       dst[r * stride + d] = r < n && d < D ? src[r * row + d] : from_float<T>(0.0f);
     }
   }
 }
 
-template <int ROWS>
-__device__ __forceinline__ void load_places(float* dst, const float* src, int n) {
-  for (int u = threadIdx.x; u < ROWS * 3; u += blockDim.x)
+__device__ __forceinline__ void load_places(float* dst, const float* src, int n, int rows) {
+  for (int u = threadIdx.x; u < rows * 3; u += blockDim.x)
     tc::cp4(tc::smem_addr(dst + u), u < n * 3 ? src + u : src, u < n * 3);
 }
 __device__ __forceinline__ void arrived() {
@@ -231,7 +233,7 @@ __device__ __forceinline__ Softmax softmax(float (&s)[NT][4], int nt, int n, int
 template <typename T, int NT>
 __global__ void __launch_bounds__(16 * NT) small_forward_kernel(const __grid_constant__ AttArgs a,
                                                                 const AttSmall* __restrict__ list, int stride,
-                                                                int vec, T* __restrict__ out) {
+                                                                int shift, int vec, T* __restrict__ out) {
   constexpr int R = 8 * NT, N = Parts<T>::N;
   extern __shared__ __align__(16) unsigned char small_smem[];
   T* s_q = reinterpret_cast<T*>(small_smem);
@@ -243,16 +245,17 @@ __global__ void __launch_bounds__(16 * NT) small_forward_kernel(const __grid_con
   const int h = int(blockIdx.x % unsigned(a.H)), hk = h / a.group;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int width = (a.D + 7) / 8 * 8;
-  load_rows<T, R>(s_q, stride, static_cast<const T*>(a.q) + int64_t(it.q) * a.q_row + h * a.q_head, a.q_row, it.nq, a.D,
-                  vec & 1);
-  load_rows<T, R>(s_k, stride, static_cast<const T*>(a.k) + int64_t(it.k) * a.k_row + hk * a.k_head, a.k_row, it.nk,
-                  a.D, vec & 2);
-  load_rows<T, R>(s_v, stride, static_cast<const T*>(a.v) + int64_t(it.k) * a.v_row + hk * a.v_head, a.v_row, it.nk,
-                  a.D, vec & 4);
+  const int q_rows = (it.nq + 15) / 16 * 16, k_rows = (it.nk + 15) / 16 * 16;  // what the fragments read
+  load_rows<T>(s_q, stride, static_cast<const T*>(a.q) + int64_t(it.q) * a.q_row + h * a.q_head, a.q_row, it.nq, q_rows, a.D,
+               shift, vec & 1);
+  load_rows<T>(s_k, stride, static_cast<const T*>(a.k) + int64_t(it.k) * a.k_row + hk * a.k_head, a.k_row, it.nk, k_rows,
+               a.D, shift, vec & 2);
+  load_rows<T>(s_v, stride, static_cast<const T*>(a.v) + int64_t(it.k) * a.v_row + hk * a.v_head, a.v_row, it.nk, k_rows,
+               a.D, shift, vec & 4);
   const bool bias = a.slopes != nullptr;
   if (bias) {
-    load_places<R>(s_x, a.x + int64_t(it.q) * 3, it.nq);
-    load_places<R>(s_y, a.y + int64_t(it.k) * 3, it.nk);
+    load_places(s_x, a.x + int64_t(it.q) * 3, it.nq, q_rows);
+    load_places(s_y, a.y + int64_t(it.k) * 3, it.nk, k_rows);
   }
   arrived();
   const int r0 = 16 * warp;
@@ -268,6 +271,8 @@ __global__ void __launch_bounds__(16 * NT) small_forward_kernel(const __grid_con
 #pragma unroll
   for (int t = 0; t < NT; ++t)
     if (t < nt) p[t] = frag_a<N, false>(s[t][0], s[t][2], s[t][1], s[t][3]);
+  T* const to = out + ((int64_t(it.q) + r0 + g) * a.H + h) * a.D;
+  const int64_t to8 = int64_t(8) * a.H * a.D;
   for (int d = 0; d < width; d += 8) {
     float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -281,7 +286,7 @@ __global__ void __launch_bounds__(16 * NT) small_forward_kernel(const __grid_con
     for (int u = 0; u < 2; ++u) {
       const int r = r0 + g + 8 * u;
       if (r < it.nq)
-        store_pair(out + ((int64_t(it.q) + r) * a.H + h) * a.D, d + 2 * c, a.D,
+        store_pair(to + u * to8, d + 2 * c, a.D,
                    inv[u] == 0.0f ? 0.0f : o[2 * u] * inv[u], inv[u] == 0.0f ? 0.0f : o[2 * u + 1] * inv[u],
                    (vec & 16) != 0);
     }
@@ -292,7 +297,7 @@ __global__ void __launch_bounds__(16 * NT) small_forward_kernel(const __grid_con
 // that share the key head.
 template <typename T, int NT, int DT>
 __global__ void __launch_bounds__(16 * NT) small_backward_kernel(
-    const __grid_constant__ AttArgs a, const AttSmall* __restrict__ list, int stride, int vec,
+    const __grid_constant__ AttArgs a, const AttSmall* __restrict__ list, int stride, int shift, int vec,
     const T* __restrict__ grad, T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dv,
     float* __restrict__ slope_part, float* __restrict__ dx_part, float* __restrict__ dy_part) {
   constexpr int R = 8 * NT, N = Parts<T>::N, SP = R + 4;
@@ -310,14 +315,15 @@ __global__ void __launch_bounds__(16 * NT) small_backward_kernel(
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int width = (a.D + 7) / 8 * 8, r0 = 16 * warp;
   const int nt = (it.nk + 7) / 8, qt = (it.nq + 7) / 8;
+  const int q_rows = (it.nq + 15) / 16 * 16, k_rows = (it.nk + 15) / 16 * 16;  // what the fragments read
   const bool bias = a.slopes != nullptr, even = (vec & 16) != 0;
-  load_rows<T, R>(s_k, stride, static_cast<const T*>(a.k) + int64_t(it.k) * a.k_row + hk * a.k_head, a.k_row, it.nk,
-                  a.D, vec & 2);
-  load_rows<T, R>(s_v, stride, static_cast<const T*>(a.v) + int64_t(it.k) * a.v_row + hk * a.v_head, a.v_row, it.nk,
-                  a.D, vec & 4);
+  load_rows<T>(s_k, stride, static_cast<const T*>(a.k) + int64_t(it.k) * a.k_row + hk * a.k_head, a.k_row, it.nk, k_rows,
+               a.D, shift, vec & 2);
+  load_rows<T>(s_v, stride, static_cast<const T*>(a.v) + int64_t(it.k) * a.v_row + hk * a.v_head, a.v_row, it.nk, k_rows,
+               a.D, shift, vec & 4);
   if (bias) {
-    load_places<R>(s_x, a.x + int64_t(it.q) * 3, it.nq);
-    load_places<R>(s_y, a.y + int64_t(it.k) * 3, it.nk);
+    load_places(s_x, a.x + int64_t(it.q) * 3, it.nq, q_rows);
+    load_places(s_y, a.y + int64_t(it.k) * 3, it.nk, k_rows);
   }
   float ak[DT][4], av[DT][4], f[2][3];
 #pragma unroll
@@ -328,9 +334,10 @@ __global__ void __launch_bounds__(16 * NT) small_backward_kernel(
   for (int u = 0; u < 2; ++u) f[u][0] = f[u][1] = f[u][2] = 0.0f;
 
   for (int h = hk * a.group; h < (hk + 1) * a.group; ++h) {
-    load_rows<T, R>(s_q, stride, static_cast<const T*>(a.q) + int64_t(it.q) * a.q_row + h * a.q_head, a.q_row, it.nq,
-                    a.D, vec & 1);
-    load_rows<T, R>(s_g, stride, grad + (int64_t(it.q) * a.H + h) * a.D, int64_t(a.H) * a.D, it.nq, a.D, vec & 8);
+    load_rows<T>(s_q, stride, static_cast<const T*>(a.q) + int64_t(it.q) * a.q_row + h * a.q_head, a.q_row, it.nq, q_rows,
+                 a.D, shift, vec & 1);
+    load_rows<T>(s_g, stride, grad + (int64_t(it.q) * a.H + h) * a.D, int64_t(a.H) * a.D, it.nq, q_rows, a.D, shift,
+                 vec & 8);
     arrived();
     const float slope = bias ? a.slopes[h] : 0.0f;
     if (r0 < 8 * qt) {
@@ -389,6 +396,8 @@ __global__ void __launch_bounds__(16 * NT) small_backward_kernel(
 #pragma unroll
       for (int t = 0; t < NT; ++t)
         if (t < nt) ds[t] = frag_a<N, false>(tt[t][0], tt[t][2], tt[t][1], tt[t][3]);
+      T* const to = dq + ((int64_t(it.q) + r0 + g) * a.H + h) * a.D;
+      const int64_t to8 = int64_t(8) * a.H * a.D;
       for (int d = 0; d < width; d += 8) {
         float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -402,7 +411,7 @@ __global__ void __launch_bounds__(16 * NT) small_backward_kernel(
         for (int u = 0; u < 2; ++u) {
           const int r = r0 + g + 8 * u;
           if (r < it.nq)
-            store_pair(dq + ((int64_t(it.q) + r) * a.H + h) * a.D, d + 2 * c, a.D, o[2 * u] * a.scale,
+            store_pair(to + u * to8, d + 2 * c, a.D, o[2 * u] * a.scale,
                        o[2 * u + 1] * a.scale, even);
         }
       }
@@ -410,14 +419,14 @@ __global__ void __launch_bounds__(16 * NT) small_backward_kernel(
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int r = r0 + g + 8 * u;
-          const int64_t to = (int64_t(it.q) + r) * a.H + h;
+          const int64_t at_row = (int64_t(it.q) + r) * a.H + h;
           sd[u] = quad_sum(sd[u]);
 #pragma unroll
           for (int k = 0; k < 3; ++k) fx[u][k] = quad_sum(fx[u][k]);
           if (c == 0 && r < it.nq) {
-            slope_part[to] = -sd[u];
+            slope_part[at_row] = -sd[u];
 #pragma unroll
-            for (int k = 0; k < 3; ++k) dx_part[to * 3 + k] = -slope * fx[u][k];
+            for (int k = 0; k < 3; ++k) dx_part[at_row * 3 + k] = -slope * fx[u][k];
           }
         }
       }
@@ -490,13 +499,22 @@ int row_stride(int D) {
   return width + (width / 8 % 2 == 0 ? 8 : 0);
 }
 
+// log2 of the threads that take a row's 16-byte parts.
+template <typename T>
+int part_shift(int D) {
+  const int parts = (D + 7) / 8 * 8 * int(sizeof(T)) / 16;
+  int shift = 0;
+  while ((1 << shift) < parts) ++shift;
+  return shift;
+}
+
 template <typename T, int NT>
 int forward_class(const AttArgs& a, const AttSmall* list, int64_t n, int vec, T* out, cudaStream_t s) {
   const int stride = row_stride<T>(a.D), R = 8 * NT;
   const int smem = 3 * R * stride * int(sizeof(T)) + 6 * R * 4;
   const auto kernel = small_forward_kernel<T, NT>;
   Y3B_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  kernel<<<unsigned(n * a.H), 16 * NT, smem, s>>>(a, list, stride, vec, out);
+  kernel<<<unsigned(n * a.H), 16 * NT, smem, s>>>(a, list, stride, part_shift<T>(a.D), vec, out);
   Y3B_LAUNCH_CHECK();
   return Y3B_OK;
 }
@@ -508,7 +526,7 @@ int backward_class(const AttArgs& a, const AttSmall* list, int64_t n, int vec, c
   const int smem = 4 * R * stride * int(sizeof(T)) + 2 * R * (R + 4) * 4 + 6 * R * 4;
   const auto kernel = small_backward_kernel<T, NT, DT>;
   Y3B_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  kernel<<<unsigned(n * a.Hk), 16 * NT, smem, s>>>(a, list, stride, vec, grad, dq, dk, dv, slope_part, dx_part, dy_part);
+  kernel<<<unsigned(n * a.Hk), 16 * NT, smem, s>>>(a, list, stride, part_shift<T>(a.D), vec, grad, dq, dk, dv, slope_part, dx_part, dy_part);
   Y3B_LAUNCH_CHECK();
   return Y3B_OK;
 }
