@@ -607,19 +607,19 @@ __global__ void __launch_bounds__(128) join_query_kernel(const AttJoin* __restri
   const int64_t at = (int64_t(jn.row) + r) * H + h;
   const float s = lane < 10 ? sum_parts(p + DP + lane, step, jn.count) : 0.0f;
   const float all = __shfl_sync(0xffffffffu, s, 9), inv = all == 0.0f ? 0.0f : 1.0f / all;
-  const float dl = __shfl_sync(0xffffffffu, s, 0) * inv;
-  const float low = __shfl_sync(0xffffffffu, s, lane < 3 ? 6 + lane : 2);  // what delta multiplies
+  const float off = __shfl_sync(0xffffffffu, s, 0) * inv;  // what delta0 is short of delta
+  const float low = __shfl_sync(0xffffffffu, s, lane < 3 ? 6 + lane : 2);
   const float high = __shfl_sync(0xffffffffu, s, lane < 3 ? 3 + lane : 1);
-  if (lane == 0) delta[at] = dl;
+  if (lane == 0) delta[at] = p[DP + 10] + off;
   for (int d = lane; d < D; d += 32) {
     float x = sum_parts(p + d, step, jn.count);
     // fix: dS was formed with delta from the rounded result, and P K follows the sums
-    if (fix) x = fmaf(p[DP + 10] - dl, sum_parts(p + DP + 16 + d, step, jn.count), x);
+    if (fix) x = fmaf(-off, sum_parts(p + DP + 16 + d, step, jn.count), x);
     dq[at * D + d] = from_float<T>(scale * x);
   }
   if (slopes) {
-    if (lane < 3) place_part[at * 3 + lane] = -slopes[h] * inv * (high - dl * low);
-    if (lane == 3) slope_part[at] = -inv * (high - dl * low);
+    if (lane < 3) place_part[at * 3 + lane] = -slopes[h] * inv * (high - off * low);
+    if (lane == 3) slope_part[at] = -inv * (high - off * low);
   }
 }
 

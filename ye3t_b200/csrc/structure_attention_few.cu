@@ -205,11 +205,11 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_kernel(const __grid_consta
           for (int k = 0; k < W; ++k) x = fmaf(g[r][k], vv[t][k], x);
           x = part_sum<LPK>(x);
           if (there[t]) {
-            const float p = tc::ex2(s[t] - L[r]), pt = p * x, ds = p * (x - delta0[r]);
+            const float p = tc::ex2(s[t] - L[r]), ds = p * (x - delta0[r]);
             const float dx = px[r] - now.x[t], dy = py[r] - now.y[t], dz = pz[r] - now.z[t];
-            const float u = pt * rd[t], w = p * rd[t];
-            sum[r][0] += pt;
-            sum[r][1] = fmaf(d[t], pt, sum[r][1]);
+            const float u = ds * rd[t], w = p * rd[t];
+            sum[r][0] += ds;
+            sum[r][1] = fmaf(d[t], ds, sum[r][1]);
             sum[r][2] = fmaf(d[t], p, sum[r][2]);
             sum[r][3] = fmaf(u, dx, sum[r][3]);
             sum[r][4] = fmaf(u, dy, sum[r][4]);

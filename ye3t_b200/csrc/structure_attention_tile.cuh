@@ -120,7 +120,7 @@ struct AttCfg {
   // to a total in fp32 every FLUSH tiles, and it starts again.  With one piece the
   // query side also accumulates P K, to correct dQ for the rounding of delta.
   static constexpr int OPS = MODE == kKeySide ? 2 : 1;
-  static constexpr int FLUSH = 2;
+  static constexpr int FLUSH = 2;  // 4,096 atoms: errors of 3 to 5e-7 against 64 bits; 8 tiles 9e-7, never 2e-6
   static constexpr int TOTALS = NP == 3 ? OPS : 0;
   static constexpr bool FIX = MODE == kQuerySide && NP == 1;
   static constexpr int HALVES = MODE == kKeySide && NP == 3 && DP == 128 ? 2 : 1;  // CTAs that share a width
@@ -734,14 +734,15 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP, HP>::THREADS, AttCfg<MODE
           const tc::f2 p = tc::pack(p0, p1), tt = tc::pack(tv[cur][c], tv[cur][c + 1]);
           float g0, g1;
           if constexpr (MODE == kQuerySide) {
-            const tc::f2 pt = tc::mul2(p, tt);
-            tc::unpack(tc::mul2(p, tc::sub2(tt, delta02)), g0, g1);
-            acc[0] = tc::add2(acc[0], pt);
+            // with delta from the rounded result; what delta is off by follows from the sums
+            const tc::f2 ds = tc::mul2(p, tc::sub2(tt, delta02));
+            tc::unpack(ds, g0, g1);
+            acc[0] = tc::add2(acc[0], ds);
             acc[9] = tc::add2(acc[9], p);
             if constexpr (BIAS) {
-              acc[1] = tc::fma2(d, pt, acc[1]);
+              acc[1] = tc::fma2(d, ds, acc[1]);
               acc[2] = tc::fma2(d, p, acc[2]);
-              const tc::f2 u = tc::mul2(pt, r), w = tc::mul2(p, r);
+              const tc::f2 u = tc::mul2(ds, r), w = tc::mul2(p, r);
               acc[3] = tc::fma2(u, dx, acc[3]);
               acc[4] = tc::fma2(u, dy, acc[4]);
               acc[5] = tc::fma2(u, dz, acc[5]);
@@ -861,11 +862,11 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP, HP>::THREADS, AttCfg<MODE
         } else if constexpr (MODE == kQuerySide) {
           f0 = split ? 1.0f : a.scale;
         }
-        // query side: the sum of P is 1 up to the rounding of lse; dividing by it takes that out of delta
-        float inv = 0.0f, dl = 0.0f;
+        // query side: delta = delta0 + off; the sum of P is 1 up to the rounding of lse, which dividing by it takes out
+        float inv = 0.0f, off = 0.0f;
         if constexpr (MODE == kQuerySide) {
           inv = none ? 0.0f : 1.0f / sum[9];
-          dl = sum[0] * inv;
+          off = sum[0] * inv;
         }
 #pragma unroll
         for (int op = 0; op < C::OPS; ++op) {
@@ -888,7 +889,7 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP, HP>::THREADS, AttCfg<MODE
 #pragma unroll
                 for (int k = 0; k < 16; ++k) e[k] = 0.0f;
               }
-              const float fe = !C::FIX ? 1.0f : split ? 0.0f : delta0 - dl;
+              const float fe = !C::FIX ? 1.0f : split ? 0.0f : -off;
 #pragma unroll
               for (int k = 0; k < 16; ++k) {
                 if constexpr (C::FIX) {
@@ -927,11 +928,11 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP, HP>::THREADS, AttCfg<MODE
               for (int k = 0; k < 10; ++k) part[DP + k] = sum[k];
               part[DP + 10] = delta0;
             } else {
-              a.delta[at] = dl;
+              a.delta[at] = delta0 + off;
               if constexpr (BIAS) {
-                a.slope_part[at] = -inv * (sum[1] - dl * sum[2]);
+                a.slope_part[at] = -inv * (sum[1] - off * sum[2]);
 #pragma unroll
-                for (int k = 0; k < 3; ++k) a.place_part[at * 3 + k] = -slope[0] * inv * (sum[3 + k] - dl * sum[6 + k]);
+                for (int k = 0; k < 3; ++k) a.place_part[at * 3 + k] = -slope[0] * inv * (sum[3 + k] - off * sum[6 + k]);
               }
             }
           } else if (BIAS && half == 0) {
