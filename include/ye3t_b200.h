@@ -706,8 +706,8 @@ int64_t y3b_structure_layout(const int64_t* query_counts, const int64_t* key_cou
  * arguments.  The tables must be filled in. */
 int64_t y3b_structure_attention_workspace_bytes(const y3b_structure_attention_args* args, int adjoint);
 
-/* out [query_count, heads, width] and lse [query_count, heads] (for the adjoint) are dense.  *status
- * (nullable) takes Y3B_STATUS_TIMEOUT. */
+/* out [query_count, heads, width] and lse [query_count, heads] are dense.  lse, for the adjoint, is the base-2 logarithm
+ * of a row's sum of exponentials, +inf for a row without keys.  *status (nullable) takes Y3B_STATUS_TIMEOUT. */
 int y3b_structure_attention(const y3b_structure_attention_args* args, void* workspace, int64_t workspace_bytes,
                             void* out, float* lse, int32_t* status, void* stream);
 

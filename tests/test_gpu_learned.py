@@ -426,6 +426,39 @@ def test_learned_torch_ops():
         rt.StructureLayout.from_tensors(layout.tables, layout.counts[:-1])
 
 
+# Base-2 log of a row's sum of exponentials.  A score is a sum of D = 48 products of unit normals in fp32: at most
+# 48 * 2^-23 * sum |q k| scale log2(e) = 48 * 1.2e-7 * 31 * 0.3 * 1.44 = 8e-5 off.  With bfloat16 the sum may be that of the
+# rounded probabilities, each within 2^-9: log2(1 + 2^-9) = 2.8e-3 more.
+@pytest.mark.parametrize("dtype,tol", [(torch.float32, 1e-4), (torch.bfloat16, 3e-3)])
+@pytest.mark.parametrize("bias", [True, False])
+@pytest.mark.parametrize("queries,keys", [([70, 1, 0, 30], [70, 1, 0, 30]), ([5, 3, 64, 33], [7, 0, 64, 1]),
+                                          ([1, 2, 1], [5000, 700, 90]), ([3, 90, 20], [200, 0, 40000]),
+                                          ([300, 129], [500, 9000])])
+def test_attention_op_returns_log_sum_exp(queries, keys, bias, dtype, tol):
+    """The registered op's second result is written for every row, whichever kernel takes it; +inf without keys."""
+    import ye3t_b200.torch_ops  # noqa: F401
+    from ye3t_b200 import runtime as rt
+    q, k, v, _, x, y, sl = _inputs(queries, keys, 4, 2, 48, dtype, 11, bias)
+    layout = rt.StructureLayout(queries, keys, heads=4, key_heads=2, device=DEV)
+    want = torch.full((sum(queries), 4), float("inf"), dtype=torch.float64, device=DEV)
+    a = b = 0
+    for nq, nk in zip(queries, keys):
+        if nq and nk:
+            s = 0.3 * torch.einsum("ihd,jhd->hij", q[a:a + nq].double(), k[b:b + nk].double().repeat_interleave(2, 1))
+            if bias:
+                d = (x[a:a + nq, None].double() - y[None, b:b + nk].double()).norm(dim=-1)
+                s = s - sl.double()[:, None, None] * d
+            want[a:a + nq] = torch.logsumexp(s, -1).T / math.log(2.0)
+        a, b = a + nq, b + nk
+    # the allocator hands the results memory that holds NaN
+    for shape, of in (((sum(queries), 4, 48), dtype), ((sum(queries), 4), torch.float32)):
+        torch.full(shape, float("nan"), dtype=of, device=DEV)
+    _, lse = torch.ops.ye3t_b200.structure_attention(q, k, v, layout.tables, layout.counts, x, y, sl, 0.3)
+    assert lse.shape == want.shape and torch.equal(torch.isinf(lse), torch.isinf(want))
+    held = torch.isfinite(want)
+    assert (lse[held].double() - want[held]).abs().max() <= tol and (lse[~held] > 0).all()
+
+
 def test_attention_energies_example():
     import importlib.util
     import os

@@ -771,7 +771,7 @@ int forward(const y3b_structure_attention_args* p, const AttArgs& a, const AttPl
             float* lse, int32_t* status, cudaStream_t s) {
   if (p->small_32_count + p->small_64_count > 0) {
     const int rc = attention_small_forward<T>(a, reinterpret_cast<const AttSmall*>(p->small), p->small_32_count,
-                                              p->small_64_count, static_cast<T*>(out), s);
+                                              p->small_64_count, static_cast<T*>(out), lse, s);
     if (rc) return rc;
   }
   if (p->query_row_count > 0) {

@@ -80,11 +80,11 @@ __device__ __forceinline__ float quad_max(float v) {
 }
 
 // Rows [0, n) of one head into shared memory (`rows` rows of `stride` values), zeros elsewhere.  The copies are
-// asynchronous, so that those of all operands are in flight together: arrived() waits for them.  2^shift threads take a
-// row's 16-byte parts.
+// asynchronous, so that those of all operands are in flight together: arrived() waits for them.  2^shift threads take
+// a row's 16-byte parts.
 template <typename T>
-__device__ __forceinline__ void load_rows(T* dst, int stride, const T* src, int64_t row, int n, int rows, int D, int shift,
-                                          bool vec) {
+__device__ __forceinline__ void load_rows(T* dst, int stride, const T* src, int64_t row, int n, int rows, int D,
+                                          int shift, bool vec) {
   constexpr int W = 16 / int(sizeof(T));
   const int width = (D + 7) / 8 * 8;
   if (vec) {
@@ -233,7 +233,8 @@ __device__ __forceinline__ Softmax softmax(float (&s)[NT][4], int nt, int n, int
 template <typename T, int NT>
 __global__ void __launch_bounds__(16 * NT) small_forward_kernel(const __grid_constant__ AttArgs a,
                                                                 const AttSmall* __restrict__ list, int stride,
-                                                                int shift, int vec, T* __restrict__ out) {
+                                                                int shift, int vec, T* __restrict__ out,
+                                                                float* __restrict__ lse) {
   constexpr int R = 8 * NT, N = Parts<T>::N;
   extern __shared__ __align__(16) unsigned char small_smem[];
   T* s_q = reinterpret_cast<T*>(small_smem);
@@ -271,6 +272,12 @@ __global__ void __launch_bounds__(16 * NT) small_forward_kernel(const __grid_con
 #pragma unroll
   for (int t = 0; t < NT; ++t)
     if (t < nt) p[t] = frag_a<N, false>(s[t][0], s[t][2], s[t][1], s[t][3]);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int r = r0 + g + 8 * u;
+    if (c == u && r < it.nq)
+      lse[(int64_t(it.q) + r) * a.H + h] = inv[u] == 0.0f ? INFINITY : sm.m[u] + log2f(sm.l[u]);
+  }
   T* const to = out + ((int64_t(it.q) + r0 + g) * a.H + h) * a.D;
   const int64_t to8 = int64_t(8) * a.H * a.D;
   for (int d = 0; d < width; d += 8) {
@@ -509,12 +516,12 @@ int part_shift(int D) {
 }
 
 template <typename T, int NT>
-int forward_class(const AttArgs& a, const AttSmall* list, int64_t n, int vec, T* out, cudaStream_t s) {
+int forward_class(const AttArgs& a, const AttSmall* list, int64_t n, int vec, T* out, float* lse, cudaStream_t s) {
   const int stride = row_stride<T>(a.D), R = 8 * NT;
   const int smem = 3 * R * stride * int(sizeof(T)) + 6 * R * 4;
   const auto kernel = small_forward_kernel<T, NT>;
   Y3B_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  kernel<<<unsigned(n * a.H), 16 * NT, smem, s>>>(a, list, stride, part_shift<T>(a.D), vec, out);
+  kernel<<<unsigned(n * a.H), 16 * NT, smem, s>>>(a, list, stride, part_shift<T>(a.D), vec, out, lse);
   Y3B_LAUNCH_CHECK();
   return Y3B_OK;
 }
@@ -550,14 +557,14 @@ int vector_bits(const AttArgs& a, const void* grad, const void* o0, const void* 
 
 template <typename T>
 int attention_small_forward(const AttArgs& a, const AttSmall* list, int64_t up_to_32, int64_t up_to_64, T* out,
-                            cudaStream_t s) {
+                            float* lse, cudaStream_t s) {
   const int vec = vector_bits<T>(a, nullptr, out, nullptr, nullptr);
   if ((up_to_32 + up_to_64) * a.H > INT32_MAX) return fail(Y3B_ERR_UNSUPPORTED, "structure_attention: too many tiles");
   if (up_to_32 > 0) {
-    const int rc = forward_class<T, 4>(a, list, up_to_32, vec, out, s);
+    const int rc = forward_class<T, 4>(a, list, up_to_32, vec, out, lse, s);
     if (rc) return rc;
   }
-  return up_to_64 > 0 ? forward_class<T, 8>(a, list + up_to_32, up_to_64, vec, out, s) : Y3B_OK;
+  return up_to_64 > 0 ? forward_class<T, 8>(a, list + up_to_32, up_to_64, vec, out, lse, s) : Y3B_OK;
 }
 
 template <typename T>
@@ -582,9 +589,10 @@ int attention_small_backward(const AttArgs& a, const AttSmall* list, int64_t up_
   return Y3B_OK;
 }
 
-template int attention_small_forward<float>(const AttArgs&, const AttSmall*, int64_t, int64_t, float*, cudaStream_t);
+template int attention_small_forward<float>(const AttArgs&, const AttSmall*, int64_t, int64_t, float*, float*,
+                                            cudaStream_t);
 template int attention_small_forward<__nv_bfloat16>(const AttArgs&, const AttSmall*, int64_t, int64_t, __nv_bfloat16*,
-                                                    cudaStream_t);
+                                                    float*, cudaStream_t);
 template int attention_small_backward<float>(const AttArgs&, const AttSmall*, int64_t, int64_t, const float*, float*,
                                              float*, float*, float*, float*, float*, cudaStream_t);
 template int attention_small_backward<__nv_bfloat16>(const AttArgs&, const AttSmall*, int64_t, int64_t,

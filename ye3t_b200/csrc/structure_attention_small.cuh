@@ -13,7 +13,7 @@ struct alignas(16) AttSmall {
 // `list` holds the structures of up to 32 queries and keys, then those of up to 64.
 template <typename T>
 int attention_small_forward(const AttArgs& a, const AttSmall* list, int64_t up_to_32, int64_t up_to_64, T* out,
-                            cudaStream_t s);
+                            float* lse, cudaStream_t s);
 
 template <typename T>
 int attention_small_backward(const AttArgs& a, const AttSmall* list, int64_t up_to_32, int64_t up_to_64, const T* grad,

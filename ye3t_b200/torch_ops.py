@@ -254,7 +254,8 @@ def _embedding_backward(ctx, grad):
 species_embedding.register_autograd(_embedding_backward, setup_context=_embedding_setup)
 
 
-# ``tables`` and ``counts`` are a runtime.StructureLayout's; the second result (log-sum-exp) serves the adjoint
+# ``tables`` and ``counts`` are a runtime.StructureLayout's; the second result (base-2 log-sum-exp,
+# +inf for a query without keys) serves the adjoint
 @custom_op("ye3t_b200::structure_attention", mutates_args=())
 def structure_attention(query: Tensor, key: Tensor, value: Tensor, tables: Tensor, counts: List[int],
                         positions: Optional[Tensor], key_positions: Optional[Tensor], slopes: Optional[Tensor],
