@@ -665,10 +665,10 @@ typedef struct {
   const float* slopes;
   const int32_t* query_offsets; /* [structure_count + 1] */
   const int32_t* key_offsets;   /* [structure_count + 1] */
-  /* Work tables.  A structure of up to 64 queries and 64 keys is in small (those of up to 32 of each first).
-   * One or two queries of a larger structure are the rows of an item in few_items, its keys split over items that one
-   * few_joins entry joins.  Every other query is in query_rows (one warp computes it) or in exactly one tile of up to 128 queries
-   * of one structure; a tile is one item, or several items with consecutive slots that split its keys and
+  /* Work tables.  A structure of up to 64 queries and 64 keys may be in small (those of up to 32 of each first).
+   * One or two queries of another structure may be the rows of items in few_items, which split its keys and which one
+   * few_joins entry joins.  Every other query is in query_rows (one warp computes it) or in exactly one tile of up to
+   * 128 queries of one structure; a tile is one item, or several items with consecutive slots that split its keys and
    * one join: in forward_items and forward_joins for the call, in query_items and query_joins for its
    * adjoint.  Keys likewise, with queries as the columns.
    *   row   (query or key, its structure)
@@ -696,9 +696,9 @@ typedef struct {
 
 /* Work tables of a batch (host arrays): query_counts[s] queries and key_counts[s] keys of structure s, one after the
  * other.  counts takes the sixteen table sizes from small_32_count to key_row_count in the order of the struct;
- * tables takes forward_items, query_items, key_items, few_items, forward_joins, query_joins, key_joins, few_joins, small, query_rows, key_rows,
- * query_offsets and key_offsets one after the other, if capacity holds them.  Returns their number of int32 values, or
- * a negative error code. */
+ * tables takes forward_items, query_items, key_items, few_items, forward_joins, query_joins, key_joins, few_joins,
+ * small, query_rows, key_rows, query_offsets and key_offsets one after the other, if capacity holds them.
+ * Returns their number of int32 values, or a negative error code. */
 int64_t y3b_structure_layout(const int64_t* query_counts, const int64_t* key_counts, int64_t structure_count,
                              int64_t heads, int64_t key_heads, int64_t* counts, int32_t* tables, int64_t capacity);
 

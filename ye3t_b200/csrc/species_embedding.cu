@@ -654,7 +654,8 @@ template <typename T, typename I>
 int lookup(const T* table, int64_t V, int C, const I* z, int64_t N, double scale, T* out, int32_t* status,
            cudaStream_t s) {
   constexpr int W = 16 / int(sizeof(T));
-  if (C % W == 0 && aligned(table, 16) && aligned(out, 16)) return lookup<T, I, W>(table, V, C, z, N, scale, out, status, s);
+  if (C % W == 0 && aligned(table, 16) && aligned(out, 16))
+    return lookup<T, I, W>(table, V, C, z, N, scale, out, status, s);
   return lookup<T, I, 1>(table, V, C, z, N, scale, out, status, s);
 }
 

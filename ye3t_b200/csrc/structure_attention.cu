@@ -128,7 +128,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) row_forward_kernel(AttArgs a, 
 template <typename T>
 __global__ void __launch_bounds__(32 * kRowWarps) row_backward_query_kernel(
     AttArgs a, const int2* __restrict__ rows, int64_t row_count, const T* __restrict__ grad,
-    const float* __restrict__ lse, float* __restrict__ delta, T* __restrict__ dq, float* __restrict__ dslope_part, float* __restrict__ dx_part) {
+    const float* __restrict__ lse, float* __restrict__ delta, T* __restrict__ dq, float* __restrict__ dslope_part,
+    float* __restrict__ dx_part) {
   __shared__ float s_q[kRowWarps][kAttMaxWidth];
   __shared__ float s_g[kRowWarps][kAttMaxWidth];
   __shared__ float s_p[kRowWarps][32];
@@ -223,7 +224,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) row_backward_query_kernel(
 template <typename T>
 __global__ void __launch_bounds__(32 * kRowWarps) row_backward_key_kernel(
     AttArgs a, const int2* __restrict__ rows, int64_t row_count, const T* __restrict__ grad,
-    const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ dy_part) {
+    const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv,
+    float* __restrict__ dy_part) {
   __shared__ float s_k[kRowWarps][kAttMaxWidth];
   __shared__ float s_v[kRowWarps][kAttMaxWidth];
   __shared__ float s_p[kRowWarps][32];
@@ -592,8 +594,8 @@ __device__ __forceinline__ float sum_parts(const float* p, int64_t step, int cou
 
 template <typename T>
 __global__ void __launch_bounds__(128) join_query_kernel(const AttJoin* __restrict__ joins,
-                                                         const float* __restrict__ part, int RS, int W, int DP, int D, int H,
-                                                         float scale, bool fix, const float* __restrict__ slopes,
+                                                         const float* __restrict__ part, int RS, int W, int DP, int D,
+                                                         int H, float scale, bool fix, const float* __restrict__ slopes,
                                                          T* __restrict__ dq, float* __restrict__ delta,
                                                          float* __restrict__ slope_part,
                                                          float* __restrict__ place_part) {
@@ -625,8 +627,8 @@ __global__ void __launch_bounds__(128) join_query_kernel(const AttJoin* __restri
 
 template <typename T>
 __global__ void __launch_bounds__(128) join_key_kernel(const AttJoin* __restrict__ joins,
-                                                       const float* __restrict__ part, int RS, int W, int DP, int D, int Hk,
-                                                       float scale, T* __restrict__ dk, T* __restrict__ dv,
+                                                       const float* __restrict__ part, int RS, int W, int DP, int D,
+                                                       int Hk, float scale, T* __restrict__ dk, T* __restrict__ dv,
                                                        float* __restrict__ place_part) {
   const unsigned ctas = unsigned(RS + 3) / 4, task = blockIdx.x / ctas;
   const AttJoin jn = joins[task / unsigned(Hk)];
@@ -652,8 +654,8 @@ unsigned row_grid(int64_t tasks) { return unsigned((tasks + kRowWarps - 1) / kRo
 int check_grids(const y3b_structure_attention_args* p, const char* what) {
   const int64_t most = int64_t(INT32_MAX) / kJoinCtas;
   if (p->query_row_count * p->heads > INT32_MAX || p->key_row_count * p->key_heads > INT32_MAX ||
-      p->query_join_count * p->heads > most || p->forward_join_count * p->heads > most || p->few_join_count * p->heads > most ||
-      p->key_join_count * p->key_heads > most)
+      p->query_join_count * p->heads > most || p->forward_join_count * p->heads > most ||
+      p->few_join_count * p->heads > most || p->key_join_count * p->key_heads > most)
     return fail(Y3B_ERR_UNSUPPORTED, "%s: the batch's tables ask for more than 2^31 - 1 CTAs", what);
   return Y3B_OK;
 }
@@ -834,7 +836,8 @@ int backward(const y3b_structure_attention_args* p, const AttArgs& a, const AttP
   // query side: it also gives delta, which the key side reads
   if (p->query_row_count > 0) {
     row_backward_query_kernel<T><<<row_grid(p->query_row_count * a.H), 32 * kRowWarps, 0, s>>>(
-        a, reinterpret_cast<const int2*>(p->query_rows), p->query_row_count, g, lse, delta, static_cast<T*>(dq), slope_part, dx_part);
+        a, reinterpret_cast<const int2*>(p->query_rows), p->query_row_count, g, lse, delta, static_cast<T*>(dq),
+        slope_part, dx_part);
     Y3B_LAUNCH_CHECK();
   }
   if (p->few_item_count > 0) {
@@ -867,7 +870,8 @@ int backward(const y3b_structure_attention_args* p, const AttArgs& a, const AttP
   }
   if (p->key_row_count > 0) {
     row_backward_key_kernel<T><<<row_grid(p->key_row_count * a.Hk), 32 * kRowWarps, 0, s>>>(
-        a, reinterpret_cast<const int2*>(p->key_rows), p->key_row_count, g, lse, delta, static_cast<T*>(dk), static_cast<T*>(dv), dy_part);
+        a, reinterpret_cast<const int2*>(p->key_rows), p->key_row_count, g, lse, delta, static_cast<T*>(dk),
+        static_cast<T*>(dv), dy_part);
     Y3B_LAUNCH_CHECK();
   }
   if (p->key_item_count > 0) {

@@ -247,8 +247,8 @@ __global__ void __launch_bounds__(16 * NT) small_forward_kernel(const __grid_con
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int width = (a.D + 7) / 8 * 8;
   const int q_rows = (it.nq + 15) / 16 * 16, k_rows = (it.nk + 15) / 16 * 16;  // what the fragments read
-  load_rows<T>(s_q, stride, static_cast<const T*>(a.q) + int64_t(it.q) * a.q_row + h * a.q_head, a.q_row, it.nq, q_rows, a.D,
-               shift, vec & 1);
+  load_rows<T>(s_q, stride, static_cast<const T*>(a.q) + int64_t(it.q) * a.q_row + h * a.q_head, a.q_row, it.nq, q_rows,
+               a.D, shift, vec & 1);
   load_rows<T>(s_k, stride, static_cast<const T*>(a.k) + int64_t(it.k) * a.k_row + hk * a.k_head, a.k_row, it.nk, k_rows,
                a.D, shift, vec & 2);
   load_rows<T>(s_v, stride, static_cast<const T*>(a.v) + int64_t(it.k) * a.v_row + hk * a.v_head, a.v_row, it.nk, k_rows,
@@ -533,7 +533,8 @@ int backward_class(const AttArgs& a, const AttSmall* list, int64_t n, int vec, c
   const int smem = 4 * R * stride * int(sizeof(T)) + 2 * R * (R + 4) * 4 + 6 * R * 4;
   const auto kernel = small_backward_kernel<T, NT, DT>;
   Y3B_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  kernel<<<unsigned(n * a.Hk), 16 * NT, smem, s>>>(a, list, stride, part_shift<T>(a.D), vec, grad, dq, dk, dv, slope_part, dx_part, dy_part);
+  kernel<<<unsigned(n * a.Hk), 16 * NT, smem, s>>>(a, list, stride, part_shift<T>(a.D), vec, grad, dq, dk, dv, slope_part,
+                                               dx_part, dy_part);
   Y3B_LAUNCH_CHECK();
   return Y3B_OK;
 }

@@ -14,10 +14,10 @@
 //
 // What bounds it: the score warps.  A score takes one exp2 and one reciprocal square root on the special-function unit
 // (16 lanes a cycle and SM, so 8 scores a cycle and SM) and 9 to 25 fp32 operations (forward with shared distances, key
-// side 16, query side 25), a packed pair of which takes two issue cycles; the products of a score at D = 64 take 1/32 of a
-// cycle (forward).  The warps issue at about 75 % of what that mix allows.  Two CTAs share an SM, or two score groups, so
-// that one's MMAs and waits lie under another's arithmetic; more warps an SM gained nothing.  16,384 atoms, 8 heads of 64,
-// bf16: forward 1.27 ms (433 TFLOP/s); 8,192 atoms: forward 370, query side 678, key side 564 us.
+// side 16, query side 25), a packed pair of which takes two issue cycles; the products of a score at D = 64 take 1/32
+// of a cycle (forward).  The warps issue at about 75 % of what that mix allows.  Two CTAs share an SM, or two score
+// groups, so that one's MMAs and waits lie under another's arithmetic; more warps an SM gained nothing.  16,384 atoms,
+// 8 heads of 64, bf16: forward 1.27 ms (433 TFLOP/s); 8,192 atoms: forward 370, query side 678, key side 564 us.
 //
 // fp32 data is carried as three bf16 pieces (8 + 8 + 8 bits): six products of pieces give each
 // product to about 2^-24, and P and dS are split likewise.
@@ -344,7 +344,8 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP, HP>::THREADS, AttCfg<MODE
             const int h = u / (2 * NP), op = u / NP % 2, p = u % NP;
 #pragma unroll
             for (int q = 0; q < C::PANELS; ++q)
-              tc::tma_load4(dst + u * C::COL_PIECE + q * (BN * 128), &a.cols[op], full(s), q * 64, head_of(h), int(col), p);
+              tc::tma_load4(dst + u * C::COL_PIECE + q * (BN * 128), &a.cols[op], full(s), q * 64, head_of(h), int(col),
+                            p);
           }
         }
       } else {
@@ -854,7 +855,8 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP, HP>::THREADS, AttCfg<MODE
 #pragma unroll
       for (int h = 0; h < HP; ++h) {
         const int64_t at = row * heads + head0 + h;
-        float* part = split ? a.part + ((int64_t(item.slot) * heads + head0 + h) * kTileRows + r_tile) * C::PART : nullptr;
+        float* part =
+            split ? a.part + ((int64_t(item.slot) * heads + head0 + h) * kTileRows + r_tile) * C::PART : nullptr;
           float f0 = 1.0f;
         bool none = total == 0;
         if constexpr (MODE == kForward) {

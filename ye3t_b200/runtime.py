@@ -630,9 +630,9 @@ _LAYOUT_COUNTS = ("heads", "key_heads", "query_count", "key_count", "structure_c
                   "key_slot_count", "key_row_count")
 # its tables in their order, with the integers of an entry and the count they go by: 32-byte records first, then
 # 16-byte ones
-_LAYOUT_TABLES = (("forward_items", 8, "forward_item_count"), ("query_items", 8, "query_item_count"), ("key_items", 8, "key_item_count"),
-                  ("few_items", 8, "few_item_count"), ("forward_joins", 4, "forward_join_count"),
-                  ("query_joins", 4, "query_join_count"),
+_LAYOUT_TABLES = (("forward_items", 8, "forward_item_count"), ("query_items", 8, "query_item_count"),
+                  ("key_items", 8, "key_item_count"), ("few_items", 8, "few_item_count"),
+                  ("forward_joins", 4, "forward_join_count"), ("query_joins", 4, "query_join_count"),
                   ("key_joins", 4, "key_join_count"), ("few_joins", 4, "few_join_count"),
                   ("small", 4, None), ("query_rows", 2, "query_row_count"), ("key_rows", 2, "key_row_count"),
                   ("query_offsets", 1, "structure_count"), ("key_offsets", 1, "structure_count"))
