@@ -459,6 +459,22 @@ def test_attention_op_returns_log_sum_exp(queries, keys, bias, dtype, tol):
     assert (lse[held].double() - want[held]).abs().max() <= tol and (lse[~held] > 0).all()
 
 
+def test_attention_op_log_sum_exp_takes_no_gradient():
+    """A loss on the registered op's log-sum-exp is refused: it is not silently without a gradient."""
+    import ye3t_b200.torch_ops  # noqa: F401
+    from ye3t_b200 import runtime as rt
+    n = [70, 30]
+    q, k, v, grad, _, _, _ = _inputs(n, n, 2, 2, 16, torch.float32, 3, False)
+    layout = rt.StructureLayout(n, heads=2, device=DEV)
+    q.requires_grad_(True)
+    out, lse = torch.ops.ye3t_b200.structure_attention(q, k, v, layout.tables, layout.counts, None, None, None, 0.25)
+    assert out.requires_grad and not lse.requires_grad
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(lse.sum(), q)
+    (dq,) = torch.autograd.grad((out * lse[..., None]).sum(), q, retain_graph=True)
+    assert torch.equal(dq, torch.autograd.grad(out, q, lse[..., None].expand_as(out))[0])
+
+
 def test_attention_energies_example():
     import importlib.util
     import os

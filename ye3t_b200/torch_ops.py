@@ -301,6 +301,7 @@ def _(grad, query, key, value, tables, counts, positions, key_positions, slopes,
 def _attention_setup(ctx, inputs, output):
     query, key, value, tables, ctx.counts, positions, key_positions, slopes, ctx.scale = inputs
     ctx.save_for_backward(query, key, value, tables, positions, key_positions, slopes, *output)
+    ctx.mark_non_differentiable(output[1])  # no gradient flows through the log-sum-exp
 
 
 def _attention_backward(ctx, grad, _):
