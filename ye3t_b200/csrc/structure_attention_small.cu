@@ -135,7 +135,10 @@ __device__ __forceinline__ float2 pair_at(const __nv_bfloat16* p) {
 }
 
 // Products of 16 rows of X with the rows of Y: out[t] (rows g, g + 8; columns 8 t + 2 c, + 1) = X Y^T.  Both
-// operands take the components of a step in the order 2 c, 2 c + 1, which are read as a pair.
+// operands take the components of a step in the order 2 c, 2 c + 1, which are read as a pair.  fp32: the tensor cores
+// cut a sum towards zero each time that they add to it, which is the same way for every score; each step's products
+// are therefore added to the score outside (a readout's slope gradient 3.4e-6 -> 2.0e-6 off, for 4 % of the backward's
+// time: 512 molecules of 0-63 atoms, 4 heads of 32, 91 -> 95 us).
 template <typename T, int NT>
 __device__ __forceinline__ void scores(float (&out)[NT][4], const T* x, const T* y, int stride, int nt, int width, int g,
                                        int c) {
@@ -151,7 +154,14 @@ __device__ __forceinline__ void scores(float (&out)[NT][4], const T* x, const T*
     for (int t = 0; t < NT; ++t) {
       if (t < nt) {
         const float2 b = pair_at(y + (8 * t + g) * stride + k + 2 * c);
-        product<N>(out[t], a, b.x, b.y);
+        if constexpr (N == 1) {
+          product<N>(out[t], a, b.x, b.y);
+        } else {
+          float step[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          product<N>(step, a, b.x, b.y);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) out[t][u] += step[u];
+        }
       }
     }
   }
