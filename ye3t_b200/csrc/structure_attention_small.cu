@@ -3,13 +3,16 @@
 //
 // Molecules of some ten atoms would fill a sixth of a 128-row tile and take one tile's latency each.  Here a
 // structure's operands sit in shared memory, a warp takes 16 rows, and the products run on
-// mma.sync m16n8k8 with tf32 operands: bf16 data is exact in tf32, fp32 data is split in two tf32 parts with
-// three products (hi hi + hi lo + lo hi, to about 2^-22).  The backward forms P once more from the scores (so it needs
+// mma.sync.  fp32 data is split in two tf32 parts with three products (hi hi + hi lo + lo hi, to about 2^-22).  bf16
+// scores and results use bf16 operands straight from shared memory (ldmatrix): with the conversions to tf32 2,048
+// molecules of 0-39 atoms, 8 heads of 32, took 75 us, now 63.  The backward's other products take bf16 data as tf32,
+// in which it is exact, since P and dS are kept in fp32.  Two heads a CTA, which share their distances, took twice the
+// registers and 88 us.  The backward forms P once more from the scores (so it needs
 // nothing of the forward), keeps P and dS in shared memory and gives every gradient in one launch.
 // Rows and columns past the structure's end are zeros in shared memory.  Bound by the latency of
 // a CTA's few steps (load, scores, softmax, products, store) and by the CTAs an SM holds.
 //
-// Fragments: lane = 4 g + c.  A (16 x 8): rows g, g + 8, columns c, c + 4; B (8 x 8): rows c, c + 4, column g;
+// Fragments of the tf32 products: lane = 4 g + c.  A (16 x 8): rows g, g + 8, columns c, c + 4; B (8 x 8): rows c, c + 4, column g;
 // accumulator: rows g, g + 8, columns 2 c, 2 c + 1.  An accumulator serves as A of the next product
 // with the columns taken in the order 2 c, 2 c + 1, and the rows of B in the same order.
 #include "structure_attention_small.cuh"
@@ -68,6 +71,44 @@ __device__ __forceinline__ void product(float (&d)[4], const FragA<N>& a, float 
     mma8(d, a.v[0], s0.v[1], s1.v[1]);
   }
   mma8(d, a.v[0], s0.v[0], s1.v[0]);
+}
+
+// bf16 operands straight from shared memory: four (two) blocks of 8 x 8 values, one address a row.
+__device__ __forceinline__ void blocks4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void blocks2(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];\n"
+               : "=r"(r[0]), "=r"(r[1]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void blocks4_turned(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void blocks2_turned(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];\n"
+               : "=r"(r[0]), "=r"(r[1]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
+      "%2, %3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%0, %1, %2, %3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(b));
+}
+
+// Two neighbouring values as bf16 and what the rounding left of them, also as bf16: 16 bits of each.
+__device__ __forceinline__ void halves(float x, float y, uint32_t& high, uint32_t& low) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  const float2 f = __bfloat1622float2(h);
+  const __nv_bfloat162 l = __floats2bfloat162_rn(x - f.x, y - f.y);
+  high = *reinterpret_cast<const uint32_t*>(&h);
+  low = *reinterpret_cast<const uint32_t*>(&l);
 }
 
 __device__ __forceinline__ float quad_sum(float v) {
@@ -134,6 +175,42 @@ __device__ __forceinline__ float2 pair_at(const __nv_bfloat16* p) {
   return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p));
 }
 
+// The same for bf16 data, in steps of 16 components (the last one may have 8).  Rows up to the next multiple of 16 are read.
+template <int NT>
+__device__ __forceinline__ void scores_bf16(float (&out)[NT][4], const __nv_bfloat16* x, const __nv_bfloat16* y,
+                                            int stride, int nt, int width, int lane) {
+#pragma unroll
+  for (int t = 0; t < NT; ++t) out[t][0] = out[t][1] = out[t][2] = out[t][3] = 0.0f;
+  const uint32_t xa = tc::smem_addr(x) + 2 * ((lane & 15) * stride + (lane >> 4) * 8);
+  const uint32_t ya = tc::smem_addr(y) + 2 * (((lane & 7) + (lane >> 4) * 8) * stride + (lane >> 3 & 1) * 8);
+  uint32_t a[4], b[4];
+  int k = 0;
+#pragma unroll 2
+  for (; k + 16 <= width; k += 16) {
+    blocks4(a, xa + 2 * k);
+#pragma unroll
+    for (int t = 0; t < NT; t += 2) {
+      if (t < nt) {
+        blocks4(b, ya + 2 * (8 * t * stride + k));
+        mma16(out[t], a, b[0], b[1]);
+        if (t + 1 < nt) mma16(out[t + 1], a, b[2], b[3]);
+      }
+    }
+  }
+  if (k < width) {
+    blocks2(a, xa + 2 * k);
+    const uint32_t y8 = tc::smem_addr(y) + 2 * ((lane & 15) * stride + k);
+#pragma unroll
+    for (int t = 0; t < NT; t += 2) {
+      if (t < nt) {
+        blocks2(b, y8 + 2 * (8 * t * stride));
+        mma8_bf16(out[t], a, b[0]);
+        if (t + 1 < nt) mma8_bf16(out[t + 1], a, b[1]);
+      }
+    }
+  }
+}
+
 // Products of 16 rows of X with the rows of Y: out[t] (rows g, g + 8; columns 8 t + 2 c, + 1) = X Y^T.  Both
 // operands take the components of a step in the order 2 c, 2 c + 1, which are read as a pair.  fp32: the tensor cores
 // cut a sum towards zero each time that they add to it, which is the same way for every score; each step's products
@@ -142,6 +219,10 @@ __device__ __forceinline__ float2 pair_at(const __nv_bfloat16* p) {
 template <typename T, int NT>
 __device__ __forceinline__ void scores(float (&out)[NT][4], const T* x, const T* y, int stride, int nt, int width, int g,
                                        int c) {
+  if constexpr (sizeof(T) == 2) {
+    scores_bf16<NT>(out, x, y, stride, nt, width, 4 * g + c);
+    return;
+  }
   constexpr int N = Parts<T>::N;
 #pragma unroll
   for (int t = 0; t < NT; ++t) out[t][0] = out[t][1] = out[t][2] = out[t][3] = 0.0f;
@@ -240,12 +321,73 @@ __device__ __forceinline__ Softmax softmax(float (&s)[NT][4], int nt, int n, int
   return r;
 }
 
+// out (16 rows x the width, not yet divided by the sums) = P V, row by row into `store`: P as tf32 parts.
+template <typename T, int NT, typename Store>
+__device__ __forceinline__ void weighted(const float (&s)[NT][4], const T* v, int stride, int nt, int width, int g,
+                                         int c, Store store) {
+  constexpr int N = Parts<T>::N;
+  FragA<N> p[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+    if (t < nt) p[t] = frag_a<N, false>(s[t][0], s[t][2], s[t][1], s[t][3]);
+  for (int d = 0; d < width; d += 8) {
+    float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      if (t < nt) {
+        const T* v0 = v + (8 * t + 2 * c) * stride + d + g;
+        product<N>(o, p[t], to_float(v0[0]), to_float(v0[stride]));
+      }
+    }
+    store(d, o);
+  }
+}
+// bf16: P as two bf16 parts (16 bits, so that the result keeps the precision of its own rounding), V as it is.
+template <int NT, typename Store>
+__device__ __forceinline__ void weighted_bf16(const float (&s)[NT][4], const __nv_bfloat16* v, int stride, int nt,
+                                              int width, int lane, Store store) {
+  uint32_t high[NT / 2][4], low[NT / 2][4];
+#pragma unroll
+  for (int t = 0; t < NT; t += 2) {
+    if (t < nt) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        halves(s[t][2 * u], s[t][2 * u + 1], high[t / 2][u], low[t / 2][u]);
+        high[t / 2][2 + u] = low[t / 2][2 + u] = 0u;
+        if (t + 1 < nt) halves(s[t + 1][2 * u], s[t + 1][2 * u + 1], high[t / 2][2 + u], low[t / 2][2 + u]);
+      }
+    }
+  }
+  const uint32_t va = tc::smem_addr(v) + 2 * ((lane & 15) * stride + (lane >> 4) * 8);
+  for (int d = 0; d < width; d += 16) {
+    float o[2][4] = {};
+    const bool two = d + 8 < width;
+#pragma unroll
+    for (int t = 0; t < NT; t += 2) {
+      if (t < nt) {
+        uint32_t b[4];
+        const uint32_t at = va + 2 * (8 * t * stride + d);
+        if (two) blocks4_turned(b, at);
+        else blocks2_turned(b, at);
+        mma16(o[0], low[t / 2], b[0], b[1]);
+        mma16(o[0], high[t / 2], b[0], b[1]);
+        if (two) {
+          mma16(o[1], low[t / 2], b[2], b[3]);
+          mma16(o[1], high[t / 2], b[2], b[3]);
+        }
+      }
+    }
+    store(d, o[0]);
+    if (two) store(d + 8, o[1]);
+  }
+}
+
 template <typename T, int NT>
 __global__ void __launch_bounds__(16 * NT) small_forward_kernel(const __grid_constant__ AttArgs a,
                                                                 const AttSmall* __restrict__ list, int stride,
                                                                 int shift, int vec, T* __restrict__ out,
                                                                 float* __restrict__ lse) {
-  constexpr int R = 8 * NT, N = Parts<T>::N;
+  constexpr int R = 8 * NT;
   extern __shared__ __align__(16) unsigned char small_smem[];
   T* s_q = reinterpret_cast<T*>(small_smem);
   T* s_k = s_q + R * stride;
@@ -257,12 +399,12 @@ __global__ void __launch_bounds__(16 * NT) small_forward_kernel(const __grid_con
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int width = (a.D + 7) / 8 * 8;
   const int q_rows = (it.nq + 15) / 16 * 16, k_rows = (it.nk + 15) / 16 * 16;  // what the fragments read
-  load_rows<T>(s_q, stride, static_cast<const T*>(a.q) + int64_t(it.q) * a.q_row + h * a.q_head, a.q_row, it.nq, q_rows,
-               a.D, shift, vec & 1);
-  load_rows<T>(s_k, stride, static_cast<const T*>(a.k) + int64_t(it.k) * a.k_row + hk * a.k_head, a.k_row, it.nk, k_rows,
-               a.D, shift, vec & 2);
-  load_rows<T>(s_v, stride, static_cast<const T*>(a.v) + int64_t(it.k) * a.v_row + hk * a.v_head, a.v_row, it.nk, k_rows,
-               a.D, shift, vec & 4);
+  load_rows<T>(s_q, stride, static_cast<const T*>(a.q) + int64_t(it.q) * a.q_row + h * a.q_head, a.q_row, it.nq,
+               q_rows, a.D, shift, vec & 1);
+  load_rows<T>(s_k, stride, static_cast<const T*>(a.k) + int64_t(it.k) * a.k_row + hk * a.k_head, a.k_row, it.nk,
+               k_rows, a.D, shift, vec & 2);
+  load_rows<T>(s_v, stride, static_cast<const T*>(a.v) + int64_t(it.k) * a.v_row + hk * a.v_head, a.v_row, it.nk,
+               k_rows, a.D, shift, vec & 4);
   const bool bias = a.slopes != nullptr;
   if (bias) {
     load_places(s_x, a.x + int64_t(it.q) * 3, it.nq, q_rows);
@@ -278,10 +420,6 @@ __global__ void __launch_bounds__(16 * NT) small_forward_kernel(const __grid_con
   if (bias) distances<NT>(at, s_x + 3 * (r0 + g), s_x + 3 * (r0 + g + 8), s_y, nt, c);
   const Softmax sm = softmax<NT>(s, nt, it.nk, c, a.scale2, bias ? a.slopes[h] * kLog2e : 0.0f, bias, at);
   const float inv[2] = {sm.l[0] == 0.0f ? 0.0f : 1.0f / sm.l[0], sm.l[1] == 0.0f ? 0.0f : 1.0f / sm.l[1]};
-  FragA<N> p[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-    if (t < nt) p[t] = frag_a<N, false>(s[t][0], s[t][2], s[t][1], s[t][3]);
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int r = r0 + g + 8 * u;
@@ -290,24 +428,16 @@ __global__ void __launch_bounds__(16 * NT) small_forward_kernel(const __grid_con
   }
   T* const to = out + ((int64_t(it.q) + r0 + g) * a.H + h) * a.D;
   const int64_t to8 = int64_t(8) * a.H * a.D;
-  for (int d = 0; d < width; d += 8) {
-    float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      if (t < nt) {
-        const T* v0 = s_v + (8 * t + 2 * c) * stride + d + g;
-        product<N>(o, p[t], to_float(v0[0]), to_float(v0[stride]));
-      }
-    }
+  const auto store = [&](int d, const float(&o)[4]) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int r = r0 + g + 8 * u;
-      if (r < it.nq)
-        store_pair(to + u * to8, d + 2 * c, a.D,
-                   inv[u] == 0.0f ? 0.0f : o[2 * u] * inv[u], inv[u] == 0.0f ? 0.0f : o[2 * u + 1] * inv[u],
-                   (vec & 16) != 0);
+      if (r0 + g + 8 * u < it.nq)
+        store_pair(to + u * to8, d + 2 * c, a.D, inv[u] == 0.0f ? 0.0f : o[2 * u] * inv[u],
+                   inv[u] == 0.0f ? 0.0f : o[2 * u + 1] * inv[u], (vec & 16) != 0);
     }
-  }
+  };
+  if constexpr (sizeof(T) == 2) weighted_bf16<NT>(s, s_v, stride, nt, width, lane, store);
+  else weighted<T, NT>(s, s_v, stride, nt, width, g, c, store);
 }
 
 // MODE of the accumulators: dk and dv of 16 keys x up to 8 * DT components stay in registers over the query heads
