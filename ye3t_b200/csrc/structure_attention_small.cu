@@ -2,20 +2,26 @@
 // forward and a (structure, key head) on the backward.
 //
 // Molecules of some ten atoms would fill a sixth of a 128-row tile and take one tile's latency each.  Here a
-// structure's operands sit in shared memory, a warp takes 16 rows, and the products run on
-// mma.sync.  fp32 data is split in two tf32 parts with three products (hi hi + hi lo + lo hi, to about 2^-22).  bf16
-// scores and results use bf16 operands straight from shared memory (ldmatrix): with the conversions to tf32 2,048
-// molecules of 0-39 atoms, 8 heads of 32, took 75 us, now 63.  The backward's other products take bf16 data as tf32,
-// in which it is exact, since P and dS are kept in fp32.  Two heads a CTA, which share their distances, took twice the
-// registers and 88 us.  The backward forms P once more from the scores (so it needs
-// nothing of the forward), keeps P and dS in shared memory and gives every gradient in one launch.
-// Rows and columns past the structure's end are zeros in shared memory.  Bound by the latency of
-// a CTA's few steps (load, scores, softmax, products, store) and by the CTAs an SM holds.
+// structure's operands sit in shared memory, a warp takes 16 rows, and the products run on mma.sync.  fp32 data is
+// split in two tf32 parts with three products (hi hi + hi lo + lo hi, to about 2^-22).  bf16 scores and results use
+// bf16 operands straight from shared memory (ldmatrix): with the conversions to tf32 2,048 molecules of 0-39 atoms, 8
+// heads of 32, took 75 us, without them 63.  The backward's other products take bf16 data as tf32, in which it is
+// exact, since P and dS are kept in fp32.  The backward forms P once more from the scores (so it needs nothing of the
+// forward), keeps P and dS in shared memory and gives every gradient in one launch.  Rows and columns past the
+// structure's end are zeros in shared memory.
 //
-// Fragments of the tf32 products: lane = 4 g + c.  A (16 x 8): rows g, g + 8, columns c, c + 4; B (8 x 8): rows c, c + 4, column g;
-// accumulator: rows g, g + 8, columns 2 c, 2 c + 1.  An accumulator serves as A of the next product
+// The forward is bound by instruction issue (70 % of the cycles): of some 1,200 instructions that a warp of 16 rows
+// executes, the 11 scores a lane take about 300, the rest goes into the addresses, loads, masks and stores of rows
+// that hold 20 atoms on average.  Without integer divisions, exact reciprocals and masks of full blocks: 63 -> 57 us.
+// Two heads a CTA, which share their distances, took twice the registers and 88 us.  The backward is bound by latency:
+// 255 registers a thread leave two CTAs an SM.
+//
+// Fragments of the tf32 products: lane = 4 g + c.  A (16 x 8): rows g, g + 8, columns c, c + 4; B (8 x 8): rows c,
+// c + 4, column g; accumulator: rows g, g + 8, columns 2 c, 2 c + 1.  An accumulator serves as A of the next product
 // with the columns taken in the order 2 c, 2 c + 1, and the rows of B in the same order.
 #include "structure_attention_small.cuh"
+
+#include <algorithm>
 
 #include "tcgen05.cuh"
 
@@ -131,9 +137,14 @@ __device__ __forceinline__ void load_rows(T* dst, int stride, const T* src, int6
   if (vec) {
     const int d = int(threadIdx.x & ((1u << shift) - 1u)) * W;
     if (d < width) {
-      const uint32_t to = tc::smem_addr(dst) + uint32_t(d) * uint32_t(sizeof(T));
-      for (int r = int(threadIdx.x >> shift); r < rows; r += int(blockDim.x >> shift))
-        tc::cp16(to + uint32_t(r * stride) * uint32_t(sizeof(T)), r < n ? src + r * row + d : src, r < n);
+      const int r0 = int(threadIdx.x >> shift), step = int(blockDim.x >> shift);
+      uint32_t to = tc::smem_addr(dst) + uint32_t(r0 * stride + d) * uint32_t(sizeof(T));
+      const T* from = src + r0 * row + d;
+      for (int r = r0; r < rows; r += step) {
+        tc::cp16(to, r < n ? from : src, r < n);
+        to += uint32_t(step * stride) * uint32_t(sizeof(T));
+        from += step * row;
+      }
     }
   } else {
     for (int u = threadIdx.x; u < rows * width; u += blockDim.x) {
@@ -294,7 +305,7 @@ __device__ __forceinline__ Softmax softmax(float (&s)[NT][4], int nt, int n, int
       for (int k = 0; k < 4; ++k) {
         float v = s[t][k] * scale2;
         if (bias) v = fmaf(-slope2, at.d[t][k], v);
-        v = 8 * t + 2 * c + (k & 1) < n ? v : -INFINITY;
+        if (8 * t + 8 > n) v = 8 * t + 2 * c + (k & 1) < n ? v : -INFINITY;
         s[t][k] = v;
         r.m[k >> 1] = fmaxf(r.m[k >> 1], v);
       }
@@ -384,8 +395,8 @@ __device__ __forceinline__ void weighted_bf16(const float (&s)[NT][4], const __n
 
 template <typename T, int NT>
 __global__ void __launch_bounds__(16 * NT) small_forward_kernel(const __grid_constant__ AttArgs a,
-                                                                const AttSmall* __restrict__ list, int stride,
-                                                                int shift, int vec, T* __restrict__ out,
+                                                                const AttSmall* __restrict__ list, int64_t n,
+                                                                int stride, int shift, int vec, T* __restrict__ out,
                                                                 float* __restrict__ lse) {
   constexpr int R = 8 * NT;
   extern __shared__ __align__(16) unsigned char small_smem[];
@@ -394,8 +405,10 @@ __global__ void __launch_bounds__(16 * NT) small_forward_kernel(const __grid_con
   T* s_v = s_k + R * stride;
   float* s_x = reinterpret_cast<float*>(s_v + R * stride);
   float* s_y = s_x + R * 3;
-  const AttSmall it = list[blockIdx.x / unsigned(a.H)];
-  const int h = int(blockIdx.x % unsigned(a.H)), hk = h / a.group;
+  const int64_t task = blockIdx.y + int64_t(gridDim.y) * blockIdx.z;
+  if (task >= n) return;
+  const AttSmall it = list[task];
+  const int h = int(blockIdx.x), hk = a.group == 1 ? h : h / a.group;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int width = (a.D + 7) / 8 * 8;
   const int q_rows = (it.nq + 15) / 16 * 16, k_rows = (it.nk + 15) / 16 * 16;  // what the fragments read
@@ -419,12 +432,13 @@ __global__ void __launch_bounds__(16 * NT) small_forward_kernel(const __grid_con
   Places<NT> at;
   if (bias) distances<NT>(at, s_x + 3 * (r0 + g), s_x + 3 * (r0 + g + 8), s_y, nt, c);
   const Softmax sm = softmax<NT>(s, nt, it.nk, c, a.scale2, bias ? a.slopes[h] * kLog2e : 0.0f, bias, at);
-  const float inv[2] = {sm.l[0] == 0.0f ? 0.0f : 1.0f / sm.l[0], sm.l[1] == 0.0f ? 0.0f : 1.0f / sm.l[1]};
+  const float inv[2] = {sm.l[0] == 0.0f ? 0.0f : tc::rcp_approx(sm.l[0]),
+                        sm.l[1] == 0.0f ? 0.0f : tc::rcp_approx(sm.l[1])};
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int r = r0 + g + 8 * u;
     if (c == u && r < it.nq)
-      lse[(int64_t(it.q) + r) * a.H + h] = inv[u] == 0.0f ? INFINITY : sm.m[u] + log2f(sm.l[u]);
+      lse[(int64_t(it.q) + r) * a.H + h] = inv[u] == 0.0f ? INFINITY : sm.m[u] + tc::lg2_approx(sm.l[u]);
   }
   T* const to = out + ((int64_t(it.q) + r0 + g) * a.H + h) * a.D;
   const int64_t to8 = int64_t(8) * a.H * a.D;
@@ -444,7 +458,7 @@ __global__ void __launch_bounds__(16 * NT) small_forward_kernel(const __grid_con
 // that share the key head.
 template <typename T, int NT, int DT>
 __global__ void __launch_bounds__(16 * NT) small_backward_kernel(
-    const __grid_constant__ AttArgs a, const AttSmall* __restrict__ list, int stride, int shift, int vec,
+    const __grid_constant__ AttArgs a, const AttSmall* __restrict__ list, int64_t n, int stride, int shift, int vec,
     const T* __restrict__ grad, T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dv,
     float* __restrict__ slope_part, float* __restrict__ dx_part, float* __restrict__ dy_part) {
   constexpr int R = 8 * NT, N = Parts<T>::N, SP = R + 4;
@@ -457,8 +471,10 @@ __global__ void __launch_bounds__(16 * NT) small_backward_kernel(
   float* s_d = s_p + R * SP;
   float* s_x = s_d + R * SP;
   float* s_y = s_x + R * 3;
-  const AttSmall it = list[blockIdx.x / unsigned(a.Hk)];
-  const int hk = int(blockIdx.x % unsigned(a.Hk));
+  const int64_t task = blockIdx.y + int64_t(gridDim.y) * blockIdx.z;
+  if (task >= n) return;
+  const AttSmall it = list[task];
+  const int hk = int(blockIdx.x);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int width = (a.D + 7) / 8 * 8, r0 = 16 * warp;
   const int nt = (it.nk + 7) / 8, qt = (it.nq + 7) / 8;
@@ -655,13 +671,19 @@ int part_shift(int D) {
   return shift;
 }
 
+// A CTA a head (x) and structure (y and z): no division in the kernel.
+dim3 by_structure(int heads, int64_t n) {
+  const int64_t y = std::min<int64_t>(n, 65535);
+  return dim3(unsigned(heads), unsigned(y), unsigned((n + y - 1) / y));
+}
+
 template <typename T, int NT>
 int forward_class(const AttArgs& a, const AttSmall* list, int64_t n, int vec, T* out, float* lse, cudaStream_t s) {
   const int stride = row_stride<T>(a.D), R = 8 * NT;
   const int smem = 3 * R * stride * int(sizeof(T)) + 6 * R * 4;
   const auto kernel = small_forward_kernel<T, NT>;
   Y3B_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  kernel<<<unsigned(n * a.H), 16 * NT, smem, s>>>(a, list, stride, part_shift<T>(a.D), vec, out, lse);
+  kernel<<<by_structure(a.H, n), 16 * NT, smem, s>>>(a, list, n, stride, part_shift<T>(a.D), vec, out, lse);
   Y3B_LAUNCH_CHECK();
   return Y3B_OK;
 }
@@ -673,8 +695,8 @@ int backward_class(const AttArgs& a, const AttSmall* list, int64_t n, int vec, c
   const int smem = 4 * R * stride * int(sizeof(T)) + 2 * R * (R + 4) * 4 + 6 * R * 4;
   const auto kernel = small_backward_kernel<T, NT, DT>;
   Y3B_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  kernel<<<unsigned(n * a.Hk), 16 * NT, smem, s>>>(a, list, stride, part_shift<T>(a.D), vec, grad, dq, dk, dv, slope_part,
-                                               dx_part, dy_part);
+  kernel<<<by_structure(a.Hk, n), 16 * NT, smem, s>>>(a, list, n, stride, part_shift<T>(a.D), vec, grad, dq, dk, dv,
+                                                      slope_part, dx_part, dy_part);
   Y3B_LAUNCH_CHECK();
   return Y3B_OK;
 }
