@@ -555,29 +555,17 @@ __global__ void __launch_bounds__(16 * NT) small_backward_kernel(
           }
         }
       }
-      FragA<N> ds[NT];
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-        if (t < nt) ds[t] = frag_a<N, false>(tt[t][0], tt[t][2], tt[t][1], tt[t][3]);
       T* const to = dq + ((int64_t(it.q) + r0 + g) * a.H + h) * a.D;
       const int64_t to8 = int64_t(8) * a.H * a.D;
-      for (int d = 0; d < width; d += 8) {
-        float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          if (t < nt) {
-            const T* k0 = s_k + (8 * t + 2 * c) * stride + d + g;
-            product<N>(o, ds[t], to_float(k0[0]), to_float(k0[stride]));
-          }
-        }
+      const auto store = [&](int d, const float(&o)[4]) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const int r = r0 + g + 8 * u;
-          if (r < it.nq)
-            store_pair(to + u * to8, d + 2 * c, a.D, o[2 * u] * a.scale,
-                       o[2 * u + 1] * a.scale, even);
+          if (r0 + g + 8 * u < it.nq)
+            store_pair(to + u * to8, d + 2 * c, a.D, o[2 * u] * a.scale, o[2 * u + 1] * a.scale, even);
         }
-      }
+      };
+      if constexpr (sizeof(T) == 2) weighted_bf16<NT>(tt, s_k, stride, nt, width, lane, store);
+      else weighted<T, NT>(tt, s_k, stride, nt, width, g, c, store);
       if (bias) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
