@@ -14,7 +14,7 @@
 // executes, the 11 scores a lane take about 300, the rest goes into the addresses, loads, masks and stores of rows
 // that hold 20 atoms on average.  Without integer divisions, exact reciprocals and masks of full blocks: 63 -> 57 us.
 // Two heads a CTA, which share their distances, took twice the registers and 88 us.  The backward is bound by latency:
-// 255 registers a thread leave two CTAs an SM.
+// its registers leave two or three CTAs an SM.
 //
 // Fragments of the tf32 products: lane = 4 g + c.  A (16 x 8): rows g, g + 8, columns c, c + 4; B (8 x 8): rows c,
 // c + 4, column g; accumulator: rows g, g + 8, columns 2 c, 2 c + 1.  An accumulator serves as A of the next product
@@ -186,7 +186,8 @@ __device__ __forceinline__ float2 pair_at(const __nv_bfloat16* p) {
   return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p));
 }
 
-// The same for bf16 data, in steps of 16 components (the last one may have 8).  Rows up to the next multiple of 16 are read.
+// The same for bf16 data, in steps of 16 components (the last one may have 8).  Rows up to the next multiple of 16 are
+// read.
 template <int NT>
 __device__ __forceinline__ void scores_bf16(float (&out)[NT][4], const __nv_bfloat16* x, const __nv_bfloat16* y,
                                             int stride, int nt, int width, int lane) {
@@ -226,10 +227,10 @@ __device__ __forceinline__ void scores_bf16(float (&out)[NT][4], const __nv_bflo
 // operands take the components of a step in the order 2 c, 2 c + 1, which are read as a pair.  fp32: the tensor cores
 // cut a sum towards zero each time that they add to it, which is the same way for every score; each step's products
 // are therefore added to the score outside (a readout's slope gradient 3.4e-6 -> 2.0e-6 off, for 4 % of the backward's
-// time: 512 molecules of 0-63 atoms, 4 heads of 32, 91 -> 95 us).
+// time).
 template <typename T, int NT>
-__device__ __forceinline__ void scores(float (&out)[NT][4], const T* x, const T* y, int stride, int nt, int width, int g,
-                                       int c) {
+__device__ __forceinline__ void scores(float (&out)[NT][4], const T* x, const T* y, int stride, int nt, int width,
+                                       int g, int c) {
   if constexpr (sizeof(T) == 2) {
     scores_bf16<NT>(out, x, y, stride, nt, width, 4 * g + c);
     return;
@@ -274,7 +275,8 @@ __device__ __forceinline__ float square(const Apart3& a) {
   return fmaf(a.z, a.z, fmaf(a.y, a.y, fmaf(a.x, a.x, 1e-30f)));
 }
 template <int NT>
-__device__ __forceinline__ void distances(Places<NT>& p, const float* x0, const float* x8, const float* y, int nt, int c) {
+__device__ __forceinline__ void distances(Places<NT>& p, const float* x0, const float* x8, const float* y, int nt,
+                                          int c) {
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     if (t < nt) {
@@ -454,10 +456,16 @@ __global__ void __launch_bounds__(16 * NT) small_forward_kernel(const __grid_con
   else weighted<T, NT>(s, s_v, stride, nt, width, g, c, store);
 }
 
+// CTAs an SM that the registers are held to: 168 a thread where that spills little (512 molecules, 4 heads of 32, up to
+// 32 atoms in fp32: 28.4 -> 27.2 us; bf16, 8 heads, up to 64 atoms: 101 -> 91 us), else as many as it takes (bf16 of up
+// to 32 atoms takes 168 by itself: 115 us, held to them 122; width 64, up to 64 atoms: 105 us against 133).
+template <typename T, int NT, int DT>
+constexpr int backward_ctas = DT == 4 && (sizeof(T) == 4) == (NT == 4) ? 24 / NT : 1;
+
 // MODE of the accumulators: dk and dv of 16 keys x up to 8 * DT components stay in registers over the query heads
 // that share the key head.
 template <typename T, int NT, int DT>
-__global__ void __launch_bounds__(16 * NT) small_backward_kernel(
+__global__ void __launch_bounds__(16 * NT, backward_ctas<T, NT, DT>) small_backward_kernel(
     const __grid_constant__ AttArgs a, const AttSmall* __restrict__ list, int64_t n, int stride, int shift, int vec,
     const T* __restrict__ grad, T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dv,
     float* __restrict__ slope_part, float* __restrict__ dx_part, float* __restrict__ dy_part) {
@@ -480,10 +488,10 @@ __global__ void __launch_bounds__(16 * NT) small_backward_kernel(
   const int nt = (it.nk + 7) / 8, qt = (it.nq + 7) / 8;
   const int q_rows = (it.nq + 15) / 16 * 16, k_rows = (it.nk + 15) / 16 * 16;  // what the fragments read
   const bool bias = a.slopes != nullptr, even = (vec & 16) != 0;
-  load_rows<T>(s_k, stride, static_cast<const T*>(a.k) + int64_t(it.k) * a.k_row + hk * a.k_head, a.k_row, it.nk, k_rows,
-               a.D, shift, vec & 2);
-  load_rows<T>(s_v, stride, static_cast<const T*>(a.v) + int64_t(it.k) * a.v_row + hk * a.v_head, a.v_row, it.nk, k_rows,
-               a.D, shift, vec & 4);
+  load_rows<T>(s_k, stride, static_cast<const T*>(a.k) + int64_t(it.k) * a.k_row + hk * a.k_head, a.k_row, it.nk,
+               k_rows, a.D, shift, vec & 2);
+  load_rows<T>(s_v, stride, static_cast<const T*>(a.v) + int64_t(it.k) * a.v_row + hk * a.v_head, a.v_row, it.nk,
+               k_rows, a.D, shift, vec & 4);
   if (bias) {
     load_places(s_x, a.x + int64_t(it.q) * 3, it.nq, q_rows);
     load_places(s_y, a.y + int64_t(it.k) * 3, it.nk, k_rows);
@@ -497,8 +505,8 @@ __global__ void __launch_bounds__(16 * NT) small_backward_kernel(
   for (int u = 0; u < 2; ++u) f[u][0] = f[u][1] = f[u][2] = 0.0f;
 
   for (int h = hk * a.group; h < (hk + 1) * a.group; ++h) {
-    load_rows<T>(s_q, stride, static_cast<const T*>(a.q) + int64_t(it.q) * a.q_row + h * a.q_head, a.q_row, it.nq, q_rows,
-                 a.D, shift, vec & 1);
+    load_rows<T>(s_q, stride, static_cast<const T*>(a.q) + int64_t(it.q) * a.q_row + h * a.q_head, a.q_row, it.nq,
+                 q_rows, a.D, shift, vec & 1);
     load_rows<T>(s_g, stride, grad + (int64_t(it.q) * a.H + h) * a.D, int64_t(a.H) * a.D, it.nq, q_rows, a.D, shift,
                  vec & 8);
     arrived();
@@ -537,8 +545,10 @@ __global__ void __launch_bounds__(16 * NT) small_backward_kernel(
             tt[t][k] = ds;
             if (bias) {
               const Apart3 v = apart3(x_of[u], s_y + 3 * col);
-              const float w = ds * at.r[t][k];
-              sd[u] = fmaf(ds, at.d[t][k], sd[u]);
+              // 64 columns: distances formed again are cheaper than 64 registers over the softmax (95 -> 87 us)
+              const float q = NT == 4 ? 0.0f : square(v), r = NT == 4 ? at.r[t][k] : tc::rsqrt_approx(q);
+              const float w = ds * r;
+              sd[u] = fmaf(ds, NT == 4 ? at.d[t][k] : q * r, sd[u]);
               fx[u][0] = fmaf(w, v.x, fx[u][0]);
               fx[u][1] = fmaf(w, v.y, fx[u][1]);
               fx[u][2] = fmaf(w, v.z, fx[u][2]);
