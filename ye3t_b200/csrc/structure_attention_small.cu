@@ -13,7 +13,7 @@
 // The forward is bound by instruction issue (70 % of the cycles): of some 1,200 instructions that a warp of 16 rows
 // executes, the 11 scores a lane take about 300, the rest goes into the addresses, loads, masks and stores of rows
 // that hold 20 atoms on average.  Without integer divisions, exact reciprocals and masks of full blocks: 63 -> 57 us.
-// Two heads a CTA, which share their distances, took twice the registers and 88 us.  The backward is bound by latency:
+// Two heads a CTA, which share their distances, took twice the registers and 87 us.  The backward is bound by latency:
 // its registers leave two or three CTAs an SM.
 //
 // Fragments of the tf32 products: lane = 4 g + c.  A (16 x 8): rows g, g + 8, columns c, c + 4; B (8 x 8): rows c,

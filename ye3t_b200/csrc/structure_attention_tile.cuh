@@ -102,7 +102,8 @@ struct AttCfg {
   static constexpr int EXTRA = 5 * BN;  // floats a stage: x, y, z, lse, delta of the columns
   // Three pieces: the row operands lie in tensor memory where they fit.  A product of 128 rows and 32 columns reads
   // 4 KB of rows from shared memory for 1 KB of columns, and six products of pieces make that the bound
-  // (4,096 atoms, 4 heads of 64: query side 578 us, key side 650, without the products 189 and 207).
+  // (4,096 atoms, 4 heads of 64, rows in shared memory: query side 578 us, key side 650, without the products 189 and
+  // 207; rows in tensor memory and the MMA loop entered by the whole warp: 263 and 350).
   static constexpr bool ROWS_TMEM = NP == 3 && (DP == 64 || MODE == kForward);
   static constexpr int ROW_BYTES = ROWS_TMEM ? 0 : HP * ROWOPS * NP * ROW_PIECE;
   // Tensor memory columns.  P and dS (NP * BN / 2 columns each) take the place of the scores they come from.
