@@ -404,7 +404,8 @@ int unpack(const y3b_structure_attention_args* p, const char* what, AttArgs* a) 
                 "%s: bad table of the forward", what);
   Y3B_CHECK_ARG(p->query_item_count >= 0 && p->query_join_count >= 0 && p->query_slot_count >= 0 &&
                     p->query_row_count >= 0 && p->key_item_count >= 0 && p->key_join_count >= 0 &&
-                    p->key_slot_count >= 0 && p->key_row_count >= 0,
+                    p->key_slot_count >= 0 && p->key_row_count >= 0 && p->few_key_count >= 0 &&
+                    p->few_key_count <= p->key_row_count && (p->few_key_count == 0 || p->query_count > 0),
                 "%s: negative table size", what);
   Y3B_CHECK_ARG((p->query_item_count == 0 || p->query_items) && (p->query_join_count == 0 || p->query_joins) &&
                     (p->query_row_count == 0 || p->query_rows) && (p->key_item_count == 0 || p->key_items) &&
@@ -868,9 +869,16 @@ int backward(const y3b_structure_attention_args* p, const AttArgs& a, const AttP
       Y3B_LAUNCH_CHECK();
     }
   }
-  if (p->key_row_count > 0) {
-    row_backward_key_kernel<T><<<row_grid(p->key_row_count * a.Hk), 32 * kRowWarps, 0, s>>>(
-        a, reinterpret_cast<const int2*>(p->key_rows), p->key_row_count, g, lse, delta, static_cast<T*>(dk),
+  const int2* key_rows = reinterpret_cast<const int2*>(p->key_rows);
+  const int64_t other_rows = p->key_row_count - p->few_key_count;
+  if (p->few_key_count > 0) {
+    const int rc = attention_few_key<T>(a, key_rows + other_rows, p->few_key_count, g, lse, delta, static_cast<T*>(dk),
+                                        static_cast<T*>(dv), dy_part, s);
+    if (rc) return rc;
+  }
+  if (other_rows > 0) {
+    row_backward_key_kernel<T><<<row_grid(other_rows * a.Hk), 32 * kRowWarps, 0, s>>>(
+        a, key_rows, other_rows, g, lse, delta, static_cast<T*>(dk),
         static_cast<T*>(dv), dy_part);
     Y3B_LAUNCH_CHECK();
   }

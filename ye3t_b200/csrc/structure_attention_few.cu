@@ -307,6 +307,109 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_kernel(const __grid_consta
   }
 }
 
+// Gradients of keys that one or two queries see: LPK lanes hold a key's components of K and V and those of its gradients,
+// in fp32, and go over the query heads that share the key head.  The loads of kFewSteps keys are in flight together.
+// Bound by reading K and V and writing their gradients once.
+template <typename T, int LPK, bool VEC>
+__global__ void __launch_bounds__(32 * kFewWarps) few_key_kernel(const __grid_constant__ AttArgs a,
+                                                                const int2* __restrict__ rows, int64_t count, int vec,
+                                                                const T* __restrict__ grad,
+                                                                const float* __restrict__ lse,
+                                                                const float* __restrict__ delta, T* __restrict__ dk,
+                                                                T* __restrict__ dv, float* __restrict__ dy_part) {
+  constexpr int W = 16 / int(sizeof(T)), KPW = 32 / LPK;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, slot = lane / LPK, d0 = (lane % LPK) * W;
+  const int hk = int(blockIdx.y);
+  const int64_t e0 = (blockIdx.x * int64_t(kFewWarps) + warp) * (KPW * kFewSteps) + slot;
+  const bool bias = a.slopes != nullptr;
+  int2 of[kFewSteps];  // (key, structure); past the end the last one, which is not stored again
+#pragma unroll
+  for (int t = 0; t < kFewSteps; ++t) of[t] = rows[e0 + t * KPW < count ? e0 + t * KPW : count - 1];
+  const T* kp = static_cast<const T*>(a.k) + hk * a.k_head + d0;
+  const T* vp = static_cast<const T*>(a.v) + hk * a.v_head + d0;
+  uint4 kr[kFewSteps], vr[kFewSteps];
+  float y[kFewSteps][3];
+  int first[kFewSteps], queries[kFewSteps];
+#pragma unroll
+  for (int t = 0; t < kFewSteps; ++t) {
+    kr[t] = raw_part<T, W, VEC>(kp + int64_t(of[t].x) * a.k_row, a.D - d0);
+    vr[t] = raw_part<T, W, VEC>(vp + int64_t(of[t].x) * a.v_row, a.D - d0);
+#pragma unroll
+    for (int c = 0; c < 3; ++c) y[t][c] = bias ? a.y[3 * int64_t(of[t].x) + c] : 0.0f;
+    first[t] = a.q_off[of[t].y];
+    queries[t] = a.q_off[of[t].y + 1] - first[t];
+  }
+#pragma unroll
+  for (int t = 0; t < kFewSteps; ++t) {
+    float kv[W], vv[W], gk[W], gv[W], f[3] = {0.0f, 0.0f, 0.0f};
+    widen_part<T, W>(kv, kr[t]);
+    widen_part<T, W>(vv, vr[t]);
+#pragma unroll
+    for (int k = 0; k < W; ++k) gk[k] = gv[k] = 0.0f;
+    for (int n = 0; n < kFewQueries; ++n) {
+      const bool seen = n < queries[t];
+      if (!__any_sync(0xffffffffu, seen)) break;
+      const int64_t i = seen ? first[t] + n : 0;
+      for (int h = hk * a.group; h < (hk + 1) * a.group; ++h) {
+        float q[W], g[W], s = 0.0f, x = 0.0f;
+        load_part<T, W>(q, static_cast<const T*>(a.q) + i * a.q_row + h * a.q_head + d0, a.D - d0, vec & 1);
+        load_part<T, W>(g, grad + (i * a.H + h) * a.D + d0, a.D - d0, vec & 8);
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+          s = fmaf(q[k] * a.scale2, kv[k], s);
+          x = fmaf(g[k], vv[k], x);
+        }
+        s = part_sum<LPK>(s);
+        x = part_sum<LPK>(x);
+        if (!seen) continue;
+        float away[3] = {0.0f, 0.0f, 0.0f}, rd = 0.0f, slope = 0.0f;
+        if (bias) {
+          slope = a.slopes[h];
+#pragma unroll
+          for (int c = 0; c < 3; ++c) away[c] = a.x[3 * i + c] - y[t][c];
+          const float sq = fmaf(away[2], away[2], fmaf(away[1], away[1], fmaf(away[0], away[0], 1e-30f)));
+          rd = tc::rsqrt_approx(sq);
+          s = fmaf(sq * rd, -slope * kLog2e, s);
+        }
+        const float p = tc::ex2(s - lse[i * a.H + h]), ds = p * (x - delta[i * a.H + h]), e = slope * ds * rd;
+#pragma unroll
+        for (int c = 0; c < 3; ++c) f[c] = fmaf(e, away[c], f[c]);
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+          gk[k] = fmaf(ds, q[k], gk[k]);
+          gv[k] = fmaf(p, g[k], gv[k]);
+        }
+      }
+    }
+    if (e0 + t * KPW >= count) continue;
+    const int64_t at = int64_t(of[t].x) * a.Hk + hk;
+    alignas(16) T ok[W], ov[W];
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      ok[k] = from_float<T>(gk[k] * a.scale);
+      ov[k] = from_float<T>(gv[k]);
+    }
+    if (vec & 16) {
+      if (d0 < a.D) {
+        *reinterpret_cast<uint4*>(dk + at * a.D + d0) = *reinterpret_cast<const uint4*>(ok);
+        *reinterpret_cast<uint4*>(dv + at * a.D + d0) = *reinterpret_cast<const uint4*>(ov);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        if (d0 + k < a.D) {
+          dk[at * a.D + d0 + k] = ok[k];
+          dv[at * a.D + d0 + k] = ov[k];
+        }
+      }
+    }
+    if (bias && lane % LPK == 0) {
+#pragma unroll
+      for (int c = 0; c < 3; ++c) dy_part[at * 3 + c] = f[c];
+    }
+  }
+}
+
 template <typename T, bool BACKWARD>
 int few(const AttArgs& a, const AttItem* items, int64_t count, int DP, int width, const T* out, const T* grad,
         const float* lse, float* part, cudaStream_t s) {
@@ -343,6 +446,38 @@ int few(const AttArgs& a, const AttItem* items, int64_t count, int DP, int width
 }  // namespace
 
 template <typename T>
+int attention_few_key(const AttArgs& a, const int2* rows, int64_t count, const T* grad, const float* lse,
+                      const float* delta, T* dk, T* dv, float* dy_part, cudaStream_t s) {
+  constexpr int W = 16 / int(sizeof(T));
+  const auto fits = [&](const void* p, int64_t row, int64_t head) {
+    return a.D % W == 0 && row % W == 0 && head % W == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+  };
+  const int vec = (fits(a.q, a.q_row, a.q_head) ? 1 : 0) | (fits(grad, int64_t(a.H) * a.D, a.D) ? 8 : 0) |
+                  (fits(dk, a.D, a.D) && fits(dv, a.D, a.D) ? 16 : 0);
+  const bool loads = fits(a.k, a.k_row, a.k_head) && fits(a.v, a.v_row, a.v_head);
+#define Y3B_FEW_KEY(LPK)                                                                                       \
+  do {                                                                                                         \
+    const int64_t keys = kFewWarps * (32 / LPK) * kFewSteps, grid = (count + keys - 1) / keys;                 \
+    if (grid > INT32_MAX) return fail(Y3B_ERR_UNSUPPORTED, "structure_attention: too many keys");              \
+    const dim3 ctas(unsigned(grid), unsigned(a.Hk));                                                           \
+    if (loads)                                                                                                 \
+      few_key_kernel<T, LPK, true><<<ctas, 32 * kFewWarps, 0, s>>>(a, rows, count, vec, grad, lse, delta, dk,  \
+                                                                   dv, dy_part);                               \
+    else                                                                                                       \
+      few_key_kernel<T, LPK, false><<<ctas, 32 * kFewWarps, 0, s>>>(a, rows, count, vec, grad, lse, delta, dk, \
+                                                                    dv, dy_part);                              \
+  } while (0)
+  const int lanes = (a.D + W - 1) / W;
+  if (lanes <= 4) Y3B_FEW_KEY(4);
+  else if (lanes <= 8) Y3B_FEW_KEY(8);
+  else if (lanes <= 16) Y3B_FEW_KEY(16);
+  else if constexpr (sizeof(T) == 4) Y3B_FEW_KEY(32);
+#undef Y3B_FEW_KEY
+  Y3B_LAUNCH_CHECK();
+  return Y3B_OK;
+}
+
+template <typename T>
 int attention_few_forward(const AttArgs& a, const AttItem* items, int64_t count, int DP, int width, float* part,
                           cudaStream_t s) {
   return few<T, false>(a, items, count, DP, width, nullptr, nullptr, nullptr, part, s);
@@ -354,6 +489,10 @@ int attention_few_query(const AttArgs& a, const AttItem* items, int64_t count, i
   return few<T, true>(a, items, count, DP, width, out, grad, lse, part, s);
 }
 
+template int attention_few_key<float>(const AttArgs&, const int2*, int64_t, const float*, const float*, const float*,
+                                      float*, float*, float*, cudaStream_t);
+template int attention_few_key<__nv_bfloat16>(const AttArgs&, const int2*, int64_t, const __nv_bfloat16*, const float*,
+                                              const float*, __nv_bfloat16*, __nv_bfloat16*, float*, cudaStream_t);
 template int attention_few_forward<float>(const AttArgs&, const AttItem*, int64_t, int, int, float*, cudaStream_t);
 template int attention_few_forward<__nv_bfloat16>(const AttArgs&, const AttItem*, int64_t, int, int, float*,
                                                   cudaStream_t);

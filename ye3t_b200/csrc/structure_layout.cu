@@ -7,7 +7,7 @@
 //   row     no or a single key: its weight is exactly 1 and its gradients through the softmax exactly 0, which the
 //           row kernels keep;
 //   few     up to two queries: a tile would hold 2 rows of 128 (8 structures of 16,384 keys, 8 heads: 111 us on tiles,
-//           64 on the few-query kernels); their keys keep to the tile kernels;
+//           64 on the few-query kernels; their keys' gradients 209 us on tiles, 122 by a few lanes a key);
 //   tile    the rest.
 // A tile's columns are cut into parts, which are joined, where that makes the last wave of CTAs shorter (16,384 atoms, 8
 // heads: forward 1,273 us and 39 to join against 1,431 uncut).
@@ -144,9 +144,9 @@ int64_t build(const int64_t* queries, const int64_t* keys, int64_t n, int64_t he
     } else if (keys[s] <= 1) {
       by_row.push_back(s);
     } else {
-      key_tiled.push_back(s);
       if (queries[s] > kFew) tiled.push_back(s);
       else if (queries[s] > 0) few.push_back(s);
+      if (queries[s] > kFew || queries[s] == 0) key_tiled.push_back(s);
     }
   }
   // Places: two CTAs an SM of the tile kernels, and the forward's take two heads where their number is even; four of
@@ -158,13 +158,15 @@ int64_t build(const int64_t* queries, const int64_t* keys, int64_t n, int64_t he
   add_tiles(&one, q, k, few, key_heads, kSMs * 4, true);
   add_rows(&query, q, by_row);
   add_rows(&key, k, by_row);
+  const int64_t other_rows = int64_t(key.rows.size()) / 2;
+  add_rows(&key, k, few);
   const auto entries = [](const std::vector<int32_t>& v, int width) { return int64_t(v.size()) / width; };
   const int64_t all[] = {int64_t(low.size()),      int64_t(high.size()),     entries(one.items, 8),
                          entries(one.joins, 4),    one.slots,                entries(forward.items, 8),
                          entries(forward.joins, 4), forward.slots,           entries(query.items, 8),
                          entries(query.joins, 4),  query.slots,              entries(query.rows, 2),
                          entries(key.items, 8),    entries(key.joins, 4),    key.slots,
-                         entries(key.rows, 2)};
+                         entries(key.rows, 2),     entries(key.rows, 2) - other_rows};
   std::copy(std::begin(all), std::end(all), counts);
   const std::vector<int32_t>* const tables[] = {&forward.items, &query.items, &key.items, &one.items,
                                                 &forward.joins, &query.joins, &key.joins, &one.joins};
