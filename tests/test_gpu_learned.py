@@ -459,6 +459,20 @@ def test_attention_op_returns_log_sum_exp(queries, keys, bias, dtype, tol):
     assert (lse[held].double() - want[held]).abs().max() <= tol and (lse[~held] > 0).all()
 
 
+@pytest.mark.parametrize("keys", [[65, 700, 3000], [2, 90, 131]])
+@pytest.mark.parametrize("D", [7, 20, 64, 128])
+def test_attention_key_gradients_of_one_query_are_rounded_once(keys, D):
+    """With one query and one head a key, dk = scale dS q and dv = P g are single products in fp32: what bfloat16 adds is
+    the rounding of the result, at most 2^-9 of each value."""
+    from ye3t_b200 import runtime as rt
+    queries = [1] * len(keys)
+    q, k, v, grad, x, y, sl = _inputs(queries, keys, 2, 2, D, torch.bfloat16, D)
+    _, grads, _ = _run(rt, q, k, v, grad, x, y, sl, queries, keys, 0.2, False)
+    ref = _plain(q, k, v, x, y, sl, 0.2, queries, keys, grad)
+    for got, want in zip(grads[1:3], ref[2:4]):
+        _close(got, want, 2.0 ** -9 + TOL[torch.float32])
+
+
 def test_attention_op_log_sum_exp_takes_no_gradient():
     """A loss on the registered op's log-sum-exp is refused: it is not silently without a gradient."""
     import ye3t_b200.torch_ops  # noqa: F401

@@ -5,7 +5,8 @@
 // 32 / LPK keys at a time, four steps in flight.  Each group of lanes keeps its own running maximum, sum and
 // accumulator in fp32; they are joined at the end of the chunk, and the chunks by the join kernels.  Bound by
 // reading K and V once (two rows of arithmetic a key take about half of that time); a tile of the tensor cores would
-// hold two rows of 128.  Readout of 8 structures of 16,384 keys on average, 8 heads of 64 on 4 key heads: 50 us, 3.0 TB/s.
+// hold two rows of 128.  Readout of 8 structures of 16,384 keys on average, 8 heads of 64 on 4 key heads: 50 us,
+// 3.0 TB/s.
 #include "structure_attention_few.cuh"
 #include "structure_attention_tile.cuh"
 
@@ -15,6 +16,9 @@ namespace {
 constexpr int kFewWarps = 4;
 constexpr int kFewSteps = 4;  // two steps and more CTAs an SM take 64 us where four take 50 (the readout below)
 constexpr int kFewRows = 2;
+// Keys in flight on the key side and CTAs an SM that the registers are held to: 20 structures of 5,000 keys, 3 heads of
+// 128, fp32, 139 us; four keys and 120 registers 167, one key 180.
+constexpr int kFewKeySteps = 2, kFewKeyCtas = 8;
 
 // W components of a row from `p`, as fp32, zeros from `left` on.
 template <typename T, int W>
@@ -307,11 +311,13 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_kernel(const __grid_consta
   }
 }
 
-// Gradients of keys that one or two queries see: LPK lanes hold a key's components of K and V and those of its gradients,
-// in fp32, and go over the query heads that share the key head.  The loads of kFewSteps keys are in flight together.
-// Bound by reading K and V and writing their gradients once.
+// Gradients of keys that one or two queries see: LPK lanes hold a key's components of K and V and those of its
+// gradients, in fp32, and go over the query heads that share the key head.  The loads of two keys are in flight
+// together.  fp32 is bound by reading K and V and writing their gradients once (705 MB of the case above: 5.1 TB/s),
+// bf16 by the arithmetic of its eight components a lane (8 structures of 16,384 keys, 8 heads of 64 on 4: 297 MB, 121
+// us, 2.5 TB/s; on tiles 209).
 template <typename T, int LPK, bool VEC>
-__global__ void __launch_bounds__(32 * kFewWarps) few_key_kernel(const __grid_constant__ AttArgs a,
+__global__ void __launch_bounds__(32 * kFewWarps, kFewKeyCtas) few_key_kernel(const __grid_constant__ AttArgs a,
                                                                 const int2* __restrict__ rows, int64_t count, int vec,
                                                                 const T* __restrict__ grad,
                                                                 const float* __restrict__ lse,
@@ -320,18 +326,18 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_key_kernel(const __grid_co
   constexpr int W = 16 / int(sizeof(T)), KPW = 32 / LPK;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, slot = lane / LPK, d0 = (lane % LPK) * W;
   const int hk = int(blockIdx.y);
-  const int64_t e0 = (blockIdx.x * int64_t(kFewWarps) + warp) * (KPW * kFewSteps) + slot;
+  const int64_t e0 = (blockIdx.x * int64_t(kFewWarps) + warp) * (KPW * kFewKeySteps) + slot;
   const bool bias = a.slopes != nullptr;
-  int2 of[kFewSteps];  // (key, structure); past the end the last one, which is not stored again
+  int2 of[kFewKeySteps];  // (key, structure); past the end the last one, which is not stored again
 #pragma unroll
-  for (int t = 0; t < kFewSteps; ++t) of[t] = rows[e0 + t * KPW < count ? e0 + t * KPW : count - 1];
+  for (int t = 0; t < kFewKeySteps; ++t) of[t] = rows[e0 + t * KPW < count ? e0 + t * KPW : count - 1];
   const T* kp = static_cast<const T*>(a.k) + hk * a.k_head + d0;
   const T* vp = static_cast<const T*>(a.v) + hk * a.v_head + d0;
-  uint4 kr[kFewSteps], vr[kFewSteps];
-  float y[kFewSteps][3];
-  int first[kFewSteps], queries[kFewSteps];
+  uint4 kr[kFewKeySteps], vr[kFewKeySteps];
+  float y[kFewKeySteps][3];
+  int first[kFewKeySteps], queries[kFewKeySteps];
 #pragma unroll
-  for (int t = 0; t < kFewSteps; ++t) {
+  for (int t = 0; t < kFewKeySteps; ++t) {
     kr[t] = raw_part<T, W, VEC>(kp + int64_t(of[t].x) * a.k_row, a.D - d0);
     vr[t] = raw_part<T, W, VEC>(vp + int64_t(of[t].x) * a.v_row, a.D - d0);
 #pragma unroll
@@ -340,7 +346,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_key_kernel(const __grid_co
     queries[t] = a.q_off[of[t].y + 1] - first[t];
   }
 #pragma unroll
-  for (int t = 0; t < kFewSteps; ++t) {
+  for (int t = 0; t < kFewKeySteps; ++t) {
     float kv[W], vv[W], gk[W], gv[W], f[3] = {0.0f, 0.0f, 0.0f};
     widen_part<T, W>(kv, kr[t]);
     widen_part<T, W>(vv, vr[t]);
@@ -354,6 +360,13 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_key_kernel(const __grid_co
         float q[W], g[W], s = 0.0f, x = 0.0f;
         load_part<T, W>(q, static_cast<const T*>(a.q) + i * a.q_row + h * a.q_head + d0, a.D - d0, vec & 1);
         load_part<T, W>(g, grad + (i * a.H + h) * a.D + d0, a.D - d0, vec & 8);
+        const float L = lse[i * a.H + h], about = delta[i * a.H + h];
+        float away[3] = {0.0f, 0.0f, 0.0f}, slope = 0.0f;
+        if (bias) {
+          slope = a.slopes[h];
+#pragma unroll
+          for (int c = 0; c < 3; ++c) away[c] = a.x[3 * i + c] - y[t][c];
+        }
 #pragma unroll
         for (int k = 0; k < W; ++k) {
           s = fmaf(q[k] * a.scale2, kv[k], s);
@@ -362,16 +375,13 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_key_kernel(const __grid_co
         s = part_sum<LPK>(s);
         x = part_sum<LPK>(x);
         if (!seen) continue;
-        float away[3] = {0.0f, 0.0f, 0.0f}, rd = 0.0f, slope = 0.0f;
+        float rd = 0.0f;
         if (bias) {
-          slope = a.slopes[h];
-#pragma unroll
-          for (int c = 0; c < 3; ++c) away[c] = a.x[3 * i + c] - y[t][c];
           const float sq = fmaf(away[2], away[2], fmaf(away[1], away[1], fmaf(away[0], away[0], 1e-30f)));
           rd = tc::rsqrt_approx(sq);
           s = fmaf(sq * rd, -slope * kLog2e, s);
         }
-        const float p = tc::ex2(s - lse[i * a.H + h]), ds = p * (x - delta[i * a.H + h]), e = slope * ds * rd;
+        const float p = tc::ex2(s - L), ds = p * (x - about), e = slope * ds * rd;
 #pragma unroll
         for (int c = 0; c < 3; ++c) f[c] = fmaf(e, away[c], f[c]);
 #pragma unroll
@@ -457,7 +467,7 @@ int attention_few_key(const AttArgs& a, const int2* rows, int64_t count, const T
   const bool loads = fits(a.k, a.k_row, a.k_head) && fits(a.v, a.v_row, a.v_head);
 #define Y3B_FEW_KEY(LPK)                                                                                       \
   do {                                                                                                         \
-    const int64_t keys = kFewWarps * (32 / LPK) * kFewSteps, grid = (count + keys - 1) / keys;                 \
+    const int64_t keys = kFewWarps * (32 / LPK) * kFewKeySteps, grid = (count + keys - 1) / keys;              \
     if (grid > INT32_MAX) return fail(Y3B_ERR_UNSUPPORTED, "structure_attention: too many keys");              \
     const dim3 ctas(unsigned(grid), unsigned(a.Hk));                                                           \
     if (loads)                                                                                                 \
