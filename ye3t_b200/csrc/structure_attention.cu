@@ -593,17 +593,20 @@ __device__ __forceinline__ float sum_parts(const float* p, int64_t step, int cou
   return s;
 }
 
-template <typename T>
+// FEW: one row a CTA, its components over all threads (few rows of many parts: 8 structures of 16,384 keys, 8 heads,
+// 14 us, by a warp a row 36); else four rows.
+template <typename T, bool FEW>
 __global__ void __launch_bounds__(128) join_query_kernel(const AttJoin* __restrict__ joins,
                                                          const float* __restrict__ part, int RS, int W, int DP, int D,
                                                          int H, float scale, bool fix, const float* __restrict__ slopes,
                                                          T* __restrict__ dq, float* __restrict__ delta,
                                                          float* __restrict__ slope_part,
                                                          float* __restrict__ place_part) {
-  const unsigned ctas = unsigned(RS + 3) / 4, task = blockIdx.x / ctas;
+  constexpr int ROWS = FEW ? 1 : 4;
+  const unsigned ctas = unsigned(RS + ROWS - 1) / ROWS, task = blockIdx.x / ctas;
   const AttJoin jn = joins[task / unsigned(H)];
   const int h = int(task % unsigned(H)), lane = threadIdx.x & 31;
-  const int r = int(blockIdx.x % ctas) * 4 + (threadIdx.x >> 5);
+  const int r = int(blockIdx.x % ctas) * ROWS + (FEW ? 0 : threadIdx.x >> 5), mine = FEW ? int(threadIdx.x) : lane;
   if (r >= jn.rows) return;
   const int64_t step = int64_t(H) * RS * W;
   const float* p = part + ((int64_t(jn.first) * H + h) * RS + r) * W;
@@ -613,16 +616,16 @@ __global__ void __launch_bounds__(128) join_query_kernel(const AttJoin* __restri
   const float off = __shfl_sync(0xffffffffu, s, 0) * inv;  // what delta0 is short of delta
   const float low = __shfl_sync(0xffffffffu, s, lane < 3 ? 6 + lane : 2);
   const float high = __shfl_sync(0xffffffffu, s, lane < 3 ? 3 + lane : 1);
-  if (lane == 0) delta[at] = p[DP + 10] + off;
-  for (int d = lane; d < D; d += 32) {
+  if (mine == 0) delta[at] = p[DP + 10] + off;
+  for (int d = mine; d < D; d += 128 / ROWS) {
     float x = sum_parts(p + d, step, jn.count);
     // fix: dS was formed with delta from the rounded result, and P K follows the sums
     if (fix) x = fmaf(-off, sum_parts(p + DP + 16 + d, step, jn.count), x);
     dq[at * D + d] = from_float<T>(scale * x);
   }
   if (slopes) {
-    if (lane < 3) place_part[at * 3 + lane] = -slopes[h] * inv * (high - off * low);
-    if (lane == 3) slope_part[at] = -inv * (high - off * low);
+    if (mine < 3) place_part[at * 3 + mine] = -slopes[h] * inv * (high - off * low);
+    if (mine == 3) slope_part[at] = -inv * (high - off * low);
   }
 }
 
@@ -846,7 +849,7 @@ int backward(const y3b_structure_attention_args* p, const AttArgs& a, const AttP
     const int rc = attention_few_query<T>(a, reinterpret_cast<const AttItem*>(p->few_items), p->few_item_count, w.DP,
                                           2 * w.DP + 16, static_cast<const T*>(out), g, lse, part, s);
     if (rc) return rc;
-    join_query_kernel<T><<<unsigned(p->few_join_count * a.H), 128, 0, s>>>(
+    join_query_kernel<T, true><<<unsigned(p->few_join_count * a.H * kFewQueries), 128, 0, s>>>(
         reinterpret_cast<const AttJoin*>(p->few_joins), part, kFewQueries, 2 * w.DP + 16, w.DP, a.D, a.H, a.scale, true,
         a.slopes, static_cast<T*>(dq), delta, slope_part, dx_part);
     Y3B_LAUNCH_CHECK();
@@ -862,7 +865,7 @@ int backward(const y3b_structure_attention_args* p, const AttArgs& a, const AttP
     const int rc = attention_query_tiles(w.pieces, t, p->query_item_count, s);
     if (rc) return rc;
     if (p->query_join_count > 0) {
-      join_query_kernel<T><<<unsigned(p->query_join_count * a.H * kJoinCtas), 128, 0, s>>>(
+      join_query_kernel<T, false><<<unsigned(p->query_join_count * a.H * kJoinCtas), 128, 0, s>>>(
           reinterpret_cast<const AttJoin*>(p->query_joins), t.part, kTileRows, w.Wq, w.DP, a.D, a.H, a.scale,
           w.pieces == 1, a.slopes,
           static_cast<T*>(dq), delta, slope_part, dx_part);
