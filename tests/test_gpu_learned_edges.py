@@ -1,0 +1,89 @@
+"""Structure attention on rows and values that are not finite, against its definition in float64.
+
+A score that is not a number makes its row one, as does a value that is not a number, however small its weight: the
+definition multiplies it all the same.  Tolerances are those of the finite cases: float32 2e-5 of the result's norm
+(some thousand products rounded to 2^-24 and exp2 to 2^-22), bfloat16 6e-3 (the result's own rounding, 1.7e-3 rms, and
+that of the probabilities before their product).
+"""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+TOL = {torch.float32: 2e-5, torch.bfloat16: 6e-3}
+
+
+def _inputs(queries, keys, H, Hk, D, dtype, seed):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    nq, nk = sum(queries), sum(keys)
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=g, device=DEV).to(dtype)
+
+    x, y = (torch.rand(n, 3, generator=g, device=DEV) * 6.0 for n in (nq, nk))
+    return (normal(nq, H, D), normal(nk, Hk, D), normal(nk, Hk, D), normal(nq, H, D), x, y,
+            torch.rand(H, generator=g, device=DEV) - 0.2)
+
+
+def _definition(q, k, v, x, y, slopes, scale, queries, keys):
+    """Output and base-2 log-sum-exp in float64, structure by structure."""
+    q, k, v, x, y, slopes = (t.double() for t in (q, k, v, x, y, slopes))
+    m = q.shape[1] // k.shape[1]
+    out, lse = torch.zeros_like(q), torch.full(q.shape[:2], math.inf, dtype=torch.float64, device=DEV)
+    a = b = 0
+    for nq, nk in zip(queries, keys):
+        i, j = slice(a, a + nq), slice(b, b + nk)
+        a, b = a + nq, b + nk
+        d = (x[i, None] - y[None, j]).norm(dim=-1)
+        s = scale * torch.einsum("ihd,jhd->hij", q[i], k[j].repeat_interleave(m, 1)) - slopes[:, None, None] * d
+        out[i] = torch.einsum("hij,jhd->ihd", torch.softmax(s, -1), v[j].repeat_interleave(m, 1))
+        lse[i] = torch.logsumexp(s, -1).T / math.log(2.0)
+    return out, lse
+
+
+def _same_numbers(got, want, tol, what):
+    got, want = got.detach().double(), want.double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), what
+    held = torch.isfinite(want)
+    assert torch.isfinite(got[held]).all(), what
+    assert float((got[held] - want[held]).norm()) <= tol * max(float(want[held].norm()), 1e-30), what
+
+
+# 385 keys: three parts, the last of which holds one key; 700 several; 70 a single part
+FEW = ([1, 2, 1], [385, 700, 70])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("where", ["query", "infinite query", "positions", "slopes", "keys", "last key", "all but one key"])
+def test_few_queries_keep_what_is_not_a_number(where, dtype):
+    import ye3t_b200.torch_ops  # noqa: F401
+    from ye3t_b200 import runtime as rt
+    queries, keys = FEW
+    q, k, v, _, x, y, sl = _inputs(queries, keys, 4, 2, 48, dtype, 3)
+    nan = float("nan")
+    if where == "query":
+        q[0, 1, 5] = q[2, 0, 0] = nan
+    elif where == "infinite query":
+        q[0, 1, 5] = float("inf")
+    elif where == "positions":
+        x[1, 2] = nan
+    elif where == "slopes":
+        sl[3] = nan
+    elif where == "keys":
+        k[:385, 1, 7] = nan
+    elif where == "last key":
+        k[384, 0, 7] = nan
+    else:
+        k[385 + 1:385 + 700, 0, 7] = k[1085 + 1:, 1, 0] = nan
+    layout = rt.StructureLayout(queries, keys, heads=4, key_heads=2, device=DEV)
+    assert dict(zip(rt._LAYOUT_COUNTS, layout.counts))["few_item_count"] > 3
+    out, lse = torch.ops.ye3t_b200.structure_attention(q, k, v, layout.tables, layout.counts, x, y, sl, 0.15)
+    want, want_lse = _definition(q, k, v, x, y, sl, 0.15, queries, keys)
+    assert torch.isnan(want).any() and not torch.isnan(want).all()
+    _same_numbers(out, want, TOL[dtype], "out")
+    if where != "infinite query":  # of which the definition in torch is infinite, and not a number here
+        _same_numbers(lse, want_lse, 1e-4, "log-sum-exp")

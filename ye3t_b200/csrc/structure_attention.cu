@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(128) join_few_kernel(const AttJoin* __restrict
     // a part without any score above -inf holds no numbers
     const float mk = p[k * step + DP], lk = p[k * step + DP + 1];
     const float f = mk == -INFINITY && lk == 0.0f ? 0.0f : exp2f(mk - ref);
-    l += f == 0.0f ? 0.0f : lk * f;
+    l += lk * f;  // NaN where the part's scores held one, whatever its maximum
 #pragma unroll
     for (int t = 0; t < kAttMaxWidth / 32; ++t) {
       const int d = lane + 32 * t;

@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_kernel(const __grid_consta
     for (int w = 0; w < kFewWarps; ++w) {
       const float mw = s_sum[w][r][0], lw = s_sum[w][r][1];
       f[w] = mw == -INFINITY && lw == 0.0f ? 0.0f : tc::ex2(mw - (top == -INFINITY ? 0.0f : top));
-      l += f[w] == 0.0f ? 0.0f : lw * f[w];
+      l += lw * f[w];  // the maxima pass over NaN, so that only the sums carry it
     }
     if (lane == 0) {
       p[DP] = top;
