@@ -87,3 +87,32 @@ def test_few_queries_keep_what_is_not_a_number(where, dtype):
     _same_numbers(out, want, TOL[dtype], "out")
     if where != "infinite query":  # of which the definition in torch is infinite, and not a number here
         _same_numbers(lse, want_lse, 1e-4, "log-sum-exp")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [48, 100])
+@pytest.mark.parametrize("queries,keys", [([150], [200]), ([150], [9000]), ([40], [50]), ([2], [700])])
+def test_a_row_without_finite_scores_gives_zeros(queries, keys, D, dtype):
+    """A row whose scores are all -inf gives zeros and takes part in no gradient, whichever kernel has it."""
+    from ye3t_b200 import runtime as rt
+    q, k, v, grad, x, y, sl = _inputs(queries, keys, 2, 1, D, dtype, D)
+    dead = queries[0] // 2
+    # powers of two, so that the products of the pieces of a value stay exact: -2^200 is past fp32
+    k[:, :, 0], q[:, :, 0], q[dead, :, 0] = 2.0 ** 100, 0.0, -(2.0 ** 100)
+    leaves = [t.requires_grad_(True) for t in (q, k, v, x, y, sl)]
+    layout = rt.StructureLayout(queries, keys, heads=2, key_heads=1, device=DEV)
+    out = rt.structure_attention(q, k, v, layout, positions=x, key_positions=y, slopes=sl, scale=0.25)
+    dq, dk, dv, dx, dy, dsl = torch.autograd.grad(out, leaves, grad)
+    for got in (out, dq, dx):
+        assert not got[dead].any()
+    # the other rows, by themselves
+    keep = torch.arange(queries[0], device=DEV) != dead
+    wide = [t.detach().double().requires_grad_(True) for t in (q[keep], k, v, x[keep], y, sl)]
+    want = _definition(*wide, 0.25, [queries[0] - 1], keys)[0]
+    ref = torch.autograd.grad(want, wide, grad[keep].double())
+    tol, fine = TOL[dtype], TOL[torch.float32]
+    _same_numbers(out[keep], want, tol, "out")
+    _same_numbers(dq[keep][:, :, 1:], ref[0][:, :, 1:], tol, "dq")  # component 0 is a difference of 2^100s
+    for got, expect, t, what in ((dk, ref[1], tol, "dk"), (dv, ref[2], tol, "dv"), (dx[keep], ref[3], fine, "dx"),
+                                 (dy, ref[4], fine, "dy"), (dsl, ref[5], fine, "dslopes")):
+        _same_numbers(got, expect, t, what)

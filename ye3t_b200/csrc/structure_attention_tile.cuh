@@ -866,10 +866,11 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP, HP>::THREADS, AttCfg<MODE
         } else if constexpr (MODE == kQuerySide) {
           f0 = split ? 1.0f : a.scale;
         }
-        // query side: delta = delta0 + off; the sum of P is 1 up to the rounding of lse, which dividing by it takes out
+        // query side: delta = delta0 + off; the sum of P is 1 up to the rounding of lse, which dividing by it takes out.
+        // It is 0 for a row without a score above -inf, whose lse is +inf.
         float inv = 0.0f, off = 0.0f;
         if constexpr (MODE == kQuerySide) {
-          inv = none ? 0.0f : 1.0f / sum[9];
+          inv = none || sum[9] == 0.0f ? 0.0f : 1.0f / sum[9];
           off = sum[0] * inv;
         }
 #pragma unroll
