@@ -46,7 +46,7 @@ def _definition(q, k, v, x, y, slopes, scale, queries, keys):
 
 
 def _same_numbers(got, want, tol, what):
-    got, want = got.detach().double(), want.double()
+    got, want = got.detach().double(), want.detach().double()
     assert torch.equal(torch.isnan(got), torch.isnan(want)), what
     held = torch.isfinite(want)
     assert torch.isfinite(got[held]).all(), what
@@ -116,3 +116,19 @@ def test_a_row_without_finite_scores_gives_zeros(queries, keys, D, dtype):
     for got, expect, t, what in ((dk, ref[1], tol, "dk"), (dv, ref[2], tol, "dv"), (dx[keep], ref[3], fine, "dx"),
                                  (dy, ref[4], fine, "dy"), (dsl, ref[5], fine, "dslopes")):
         _same_numbers(got, expect, t, what)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("queries,keys", [(40, 60), (150, 200), (150, 9000), (1, 9000), (2, 300)])
+def test_a_value_that_is_not_a_number_is_not_lost_to_a_small_weight(queries, keys, dtype):
+    """The weight of a far key underflows; its value still counts, whether or not the keys are split over CTAs."""
+    from ye3t_b200 import runtime as rt
+    q, k, v, _, x, y, sl = _inputs([queries], [keys], 2, 2, 48, dtype, 5)
+    y[keys // 2:] += 1000.0
+    sl.fill_(1.0)
+    v[keys - 3, 0, 11] = float("nan")
+    layout = rt.StructureLayout([queries], [keys], heads=2, device=DEV)
+    out = rt.structure_attention(q, k, v, layout, positions=x, key_positions=y, slopes=sl, scale=0.15)
+    want, _ = _definition(q, k, v, x, y, sl, 0.15, [queries], [keys])
+    assert torch.isnan(want[:, 0, 11]).all() and torch.isfinite(want[:, 1]).all()
+    _same_numbers(out, want, TOL[dtype], "out")

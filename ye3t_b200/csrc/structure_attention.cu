@@ -510,7 +510,8 @@ __global__ void __launch_bounds__(128) join_forward_kernel(const AttJoin* __rest
   const float inv = none ? 0.0f : 1.0f / l;
   float o[kAttMaxWidth / 32] = {};
   for (int k0 = 0; k0 < jn.count; k0 += 32) {
-    // lane k weighs part k0 + k; a part without any score above -inf holds no numbers
+    // lane k weighs part k0 + k; a part without any score above -inf holds zeros, one whose weight underflows may
+    // hold NaN
     float weight = 0.0f;
     if (k0 + lane < jn.count) {
       const float mk = p[(k0 + lane) * step + DP];
@@ -524,8 +525,7 @@ __global__ void __launch_bounds__(128) join_forward_kernel(const AttJoin* __rest
       for (int t = 0; t < kAttMaxWidth / 32; ++t) {
         const int d = lane + 32 * t;
         if (d < D) {
-          const float x = p[(k0 + k) * step + d];
-          o[t] = f == 0.0f ? o[t] : fmaf(x, f, o[t]);
+          o[t] = fmaf(p[(k0 + k) * step + d], f, o[t]);
         }
       }
     }
@@ -562,7 +562,7 @@ __global__ void __launch_bounds__(128) join_few_kernel(const AttJoin* __restrict
   float o[kAttMaxWidth / 32] = {}, l = 0.0f;
 #pragma unroll 4
   for (int k = warp; k < jn.count; k += 4) {
-    // a part without any score above -inf holds no numbers
+    // a part without any score above -inf holds zeros, one whose weight underflows may hold NaN
     const float mk = p[k * step + DP], lk = p[k * step + DP + 1];
     const float f = mk == -INFINITY && lk == 0.0f ? 0.0f : exp2f(mk - ref);
     l += lk * f;  // NaN where the part's scores held one, whatever its maximum
@@ -570,7 +570,7 @@ __global__ void __launch_bounds__(128) join_few_kernel(const AttJoin* __restrict
     for (int t = 0; t < kAttMaxWidth / 32; ++t) {
       const int d = lane + 32 * t;
       const float x = d < D ? p[k * step + d] : 0.0f;
-      o[t] = f == 0.0f ? o[t] : fmaf(x, f, o[t]);
+      o[t] = fmaf(x, f, o[t]);
     }
   }
 #pragma unroll

@@ -237,12 +237,14 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_kernel(const __grid_consta
 #pragma unroll
   for (int r = 0; r < kFewRows; ++r) {
     float f = 1.0f;
+    bool none = false;
     if constexpr (!BACKWARD) {
       float top = m[r];
 #pragma unroll
       for (int o = LPK; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      // a group that saw no key above -inf has nothing to add
-      f = m[r] == -INFINITY && sum[r][1] == 0.0f ? 0.0f : tc::ex2(m[r] - (top == -INFINITY ? 0.0f : top));
+      // a group that saw no key above -inf has nothing to add; one whose weight underflows may hold NaN
+      none = m[r] == -INFINITY && sum[r][1] == 0.0f;
+      f = none ? 0.0f : tc::ex2(m[r] - (top == -INFINITY ? 0.0f : top));
       sum[r][0] = top;
       sum[r][1] *= f;
     }
@@ -250,7 +252,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_kernel(const __grid_consta
     for (int u = 0; u < ACC; ++u) {
 #pragma unroll
       for (int k = 0; k < W; ++k) {
-        float x = f == 0.0f ? 0.0f : acc[r][u][k] * f;
+        float x = none ? 0.0f : acc[r][u][k] * f;
 #pragma unroll
         for (int o = LPK; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
         if (slot == 0) s_acc[warp][r][u][d0 + k] = x;
@@ -305,7 +307,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_kernel(const __grid_consta
     for (int c = 0; c < ACC; ++c) {
       float x = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kFewWarps; ++w) x += f[w] == 0.0f ? 0.0f : s_acc[w][r][c][d] * f[w];
+      for (int w = 0; w < kFewWarps; ++w) x += s_acc[w][r][c][d] * f[w];
       p[c * (DP + 16) + d] = x;
     }
   }
