@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define Y3B_ABI_VERSION 10
+#define Y3B_ABI_VERSION 11
 
 /* dtype codes */
 #define Y3B_F32 0
@@ -674,10 +674,10 @@ typedef struct {
    * those of one or two queries may be the last of key_rows.
    *   row   (query or key, its structure)
    *   small (first query, queries, first key, keys)
-   *   item  (first row, rows, first column, columns, slot or -1, 0, 0, 0)
+   *   item  (first row, rows, first column, columns, slot or -1, 0, 0, 0); every few item has a slot
    *   join  (first row, rows, first slot, slots) */
   int64_t small_32_count, small_64_count;
-  int64_t few_item_count, few_join_count, few_slot_count;
+  int64_t few_item_count, few_join_count; /* a slot an item */
   int64_t forward_item_count, forward_join_count, forward_slot_count;
   int64_t query_item_count, query_join_count, query_slot_count, query_row_count;
   int64_t key_item_count, key_join_count, key_slot_count, key_row_count;
@@ -697,7 +697,7 @@ typedef struct {
 } y3b_structure_attention_args;
 
 /* Work tables of a batch (host arrays): query_counts[s] queries and key_counts[s] keys of structure s, one after the
- * other.  counts takes the seventeen table sizes from small_32_count to few_key_count in the order of the struct;
+ * other.  counts takes the sixteen table sizes from small_32_count to few_key_count in the order of the struct;
  * tables takes forward_items, query_items, key_items, few_items, forward_joins, query_joins, key_joins, few_joins,
  * small, query_rows, key_rows, query_offsets and key_offsets one after the other, if capacity holds them.
  * Returns their number of int32 values, or a negative error code. */

@@ -16,7 +16,7 @@ import torch
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libye3t_b200.so")
 
-ABI_VERSION = 10
+ABI_VERSION = 11
 F32, F64, C64, C128, BF16 = 0, 1, 2, 3, 4
 STATUS_INDEX_RANGE = 1
 STATUS_CAPACITY = 2
@@ -104,7 +104,7 @@ class StructureAttentionArgs(ctypes.Structure):
         ("positions", VP), ("key_positions", VP), ("slopes", VP),
         ("query_offsets", VP), ("key_offsets", VP),
         ("small_32_count", I64), ("small_64_count", I64),
-        ("few_item_count", I64), ("few_join_count", I64), ("few_slot_count", I64),
+        ("few_item_count", I64), ("few_join_count", I64),
         ("forward_item_count", I64), ("forward_join_count", I64), ("forward_slot_count", I64),
         ("query_item_count", I64), ("query_join_count", I64), ("query_slot_count", I64), ("query_row_count", I64),
         ("key_item_count", I64), ("key_join_count", I64), ("key_slot_count", I64), ("key_row_count", I64),

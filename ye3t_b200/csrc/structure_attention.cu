@@ -396,7 +396,7 @@ int unpack(const y3b_structure_attention_args* p, const char* what, AttArgs* a) 
   Y3B_CHECK_ARG(p->small_32_count >= 0 && p->small_64_count >= 0 &&
                     (p->small_32_count + p->small_64_count == 0 || p->small),
                 "%s: bad table of small structures", what);
-  Y3B_CHECK_ARG(p->few_item_count >= 0 && p->few_join_count >= 0 && p->few_slot_count >= 0 &&
+  Y3B_CHECK_ARG(p->few_item_count >= 0 && p->few_join_count >= 0 &&
                     (p->few_item_count == 0 || (p->few_items && p->few_joins && p->few_join_count > 0)),
                 "%s: bad table of few-query structures", what);
   Y3B_CHECK_ARG(p->forward_item_count >= 0 && p->forward_join_count >= 0 && p->forward_slot_count >= 0 &&
@@ -711,7 +711,7 @@ AttPlan make_plan(const y3b_structure_attention_args* p, bool adjoint) {
   w.part_q = take(adjoint ? p->query_slot_count * H * kTileRows * w.Wq * 4
                           : p->forward_slot_count * H * kTileRows * w.Wf * 4);
   w.part_k = take(adjoint ? p->key_slot_count * Hk * kTileRows * w.Wk * 4 : 0);
-  w.part_few = take(p->few_slot_count * H * kFewQueries * ((adjoint ? 2 : 1) * w.DP + 16) * 4);
+  w.part_few = take(p->few_item_count * H * kFewQueries * ((adjoint ? 2 : 1) * w.DP + 16) * 4);
   w.bytes = at;
   return w;
 }

@@ -162,11 +162,12 @@ int64_t build(const int64_t* queries, const int64_t* keys, int64_t n, int64_t he
   add_rows(&key, k, few);
   const auto entries = [](const std::vector<int32_t>& v, int width) { return int64_t(v.size()) / width; };
   const int64_t all[] = {int64_t(low.size()),      int64_t(high.size()),     entries(one.items, 8),
-                         entries(one.joins, 4),    one.slots,                entries(forward.items, 8),
-                         entries(forward.joins, 4), forward.slots,           entries(query.items, 8),
-                         entries(query.joins, 4),  query.slots,              entries(query.rows, 2),
-                         entries(key.items, 8),    entries(key.joins, 4),    key.slots,
-                         entries(key.rows, 2),     entries(key.rows, 2) - other_rows};
+                         entries(one.joins, 4),    entries(forward.items, 8), entries(forward.joins, 4),
+                         forward.slots,            entries(query.items, 8),  entries(query.joins, 4),
+                         query.slots,              entries(query.rows, 2),   entries(key.items, 8),
+                         entries(key.joins, 4),    key.slots,                entries(key.rows, 2),
+                         entries(key.rows, 2) - other_rows};
+  static_assert(sizeof(all) == 16 * sizeof(int64_t), "what callers reserve for counts");
   std::copy(std::begin(all), std::end(all), counts);
   const std::vector<int32_t>* const tables[] = {&forward.items, &query.items, &key.items, &one.items,
                                                 &forward.joins, &query.joins, &key.joins, &one.joins};

@@ -640,7 +640,7 @@ _LAYOUT_TABLES = (("forward_items", 8, "forward_item_count"), ("query_items", 8,
 
 def _layout_tables(queries, keys, heads, key_heads):
     """A layout's tables, one after the other, and the counts of their entries (``small_32_count`` on)."""
-    lib, counts = nat.lib(), np.empty(17, np.int64)
+    lib, counts = nat.lib(), np.empty(16, np.int64)
     # room for a few entries a structure; a batch that needs more says how much
     tables = np.empty(16 * queries.size + 256, np.int32)
     for _ in range(2):
@@ -651,7 +651,8 @@ def _layout_tables(queries, keys, heads, key_heads):
         if n <= tables.size:
             break
         tables = np.empty(n, np.int32)
-    return tables[:n], counts.tolist()
+    counts = counts.tolist()
+    return tables[:n], counts[:4] + [counts[2]] + counts[4:]  # every few-query item has a slot
 
 
 class StructureLayout:
@@ -692,7 +693,7 @@ class StructureLayout:
         self._stream = _raw_stream(self.device)
         a = self._args = nat.StructureAttentionArgs()
         for name in _LAYOUT_COUNTS:
-            if name != "shared":
+            if name not in ("shared", "few_slot_count"):
                 setattr(a, name, c[name])
         at = 0
         for name, width, count in _LAYOUT_TABLES:
