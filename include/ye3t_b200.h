@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define Y3B_ABI_VERSION 11
+#define Y3B_ABI_VERSION 12
 
 /* dtype codes */
 #define Y3B_F32 0
@@ -671,7 +671,7 @@ typedef struct {
    * 128 queries of one structure; a tile is one item, or several items with consecutive slots that split its keys and
    * one join: in forward_items and forward_joins for the call, in query_items and query_joins for its
    * adjoint.  Keys likewise, with queries as the columns;
-   * those of one or two queries may be the last of key_rows.
+   * up to 128 keys of one or two queries may be one of the last key_items, without a slot.
    *   row   (query or key, its structure)
    *   small (first query, queries, first key, keys)
    *   item  (first row, rows, first column, columns, slot or -1, 0, 0, 0); every few item has a slot
@@ -681,7 +681,7 @@ typedef struct {
   int64_t forward_item_count, forward_join_count, forward_slot_count;
   int64_t query_item_count, query_join_count, query_slot_count, query_row_count;
   int64_t key_item_count, key_join_count, key_slot_count, key_row_count;
-  int64_t few_key_count; /* the last key_rows, whose structures have one or two queries */
+  int64_t few_key_item_count; /* the last key_items, whose structures have one or two queries */
   const int32_t* small;       /* 16-byte aligned */
   const int32_t* few_items;   /* 32-byte aligned */
   const int32_t* few_joins;   /* 16-byte aligned */
@@ -697,7 +697,7 @@ typedef struct {
 } y3b_structure_attention_args;
 
 /* Work tables of a batch (host arrays): query_counts[s] queries and key_counts[s] keys of structure s, one after the
- * other.  counts takes the sixteen table sizes from small_32_count to few_key_count in the order of the struct;
+ * other.  counts takes the sixteen table sizes from small_32_count to few_key_item_count in the order of the struct;
  * tables takes forward_items, query_items, key_items, few_items, forward_joins, query_joins, key_joins, few_joins,
  * small, query_rows, key_rows, query_offsets and key_offsets one after the other, if capacity holds them.
  * Returns their number of int32 values, or a negative error code. */

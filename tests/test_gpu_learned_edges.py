@@ -132,3 +132,21 @@ def test_a_value_that_is_not_a_number_is_not_lost_to_a_small_weight(queries, key
     want, _ = _definition(q, k, v, x, y, sl, 0.15, [queries], [keys])
     assert torch.isnan(want[:, 0, 11]).all() and torch.isfinite(want[:, 1]).all()
     _same_numbers(out, want, TOL[dtype], "out")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [5, 24, 64, 128])
+def test_gradients_of_keys_in_items_of_128(D, dtype):
+    """One and two queries over numbers of keys about the length of an item, heads that share keys."""
+    from ye3t_b200 import runtime as rt
+    queries, keys = [1, 2, 0, 1, 2, 1, 2], [127, 128, 140, 129, 256, 257, 65]
+    q, k, v, grad, x, y, sl = _inputs(queries, keys, 4, 2, D, dtype, D)
+    leaves = [t.requires_grad_(True) for t in (q, k, v, x, y, sl)]
+    layout = rt.StructureLayout(queries, keys, heads=4, key_heads=2, device=DEV)
+    assert dict(zip(rt._LAYOUT_COUNTS, layout.counts))["few_item_count"] >= 6
+    out = rt.structure_attention(q, k, v, layout, positions=x, key_positions=y, slopes=sl, scale=0.2)
+    got = torch.autograd.grad(out, leaves, grad)
+    wide = [t.detach().double().requires_grad_(True) for t in (q, k, v, x, y, sl)]
+    ref = torch.autograd.grad(_definition(*wide, 0.2, queries, keys)[0], wide, grad.double())
+    for n, (a, b) in enumerate(zip(got, ref)):
+        _same_numbers(a, b, TOL[dtype if n < 3 else torch.float32], n)

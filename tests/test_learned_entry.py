@@ -19,3 +19,13 @@ def test_layout_writes_sixteen_counts(queries, keys):
     assert len(sizes) == len(named) == len(rt._LAYOUT_COUNTS) - 6
     assert named["few_slot_count"] == named["few_item_count"]
     assert sizes[:4] + sizes[5:] == counts[:16].tolist()
+
+
+@pytest.mark.parametrize("queries,keys", [([1] * 8, [5000, 32000, 16384, 9000, 20011, 12000, 30001, 6000]),
+                                          ([2] * 200, [5000] * 200)])
+def test_layout_of_few_queries_has_no_entry_a_key(queries, keys):
+    """A readout's tables go by chunks of its keys: the host work of a batch is not that of its keys."""
+    from ye3t_b200 import runtime as rt
+    packed, _ = rt._layout_tables(np.array(queries), np.array(keys), 8, 4)
+    # an item of eight values a hundred keys in two tables, and some for each structure
+    assert packed.size <= 16 * (sum(keys) // 100) + 64 * len(keys)

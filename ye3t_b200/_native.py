@@ -16,7 +16,7 @@ import torch
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libye3t_b200.so")
 
-ABI_VERSION = 11
+ABI_VERSION = 12
 F32, F64, C64, C128, BF16 = 0, 1, 2, 3, 4
 STATUS_INDEX_RANGE = 1
 STATUS_CAPACITY = 2
@@ -108,7 +108,7 @@ class StructureAttentionArgs(ctypes.Structure):
         ("forward_item_count", I64), ("forward_join_count", I64), ("forward_slot_count", I64),
         ("query_item_count", I64), ("query_join_count", I64), ("query_slot_count", I64), ("query_row_count", I64),
         ("key_item_count", I64), ("key_join_count", I64), ("key_slot_count", I64), ("key_row_count", I64),
-        ("few_key_count", I64),
+        ("few_key_item_count", I64),
         ("small", VP), ("few_items", VP), ("few_joins", VP), ("forward_items", VP),
         ("forward_joins", VP), ("query_items", VP), ("query_joins", VP), ("query_rows", VP), ("key_items", VP), ("key_joins", VP),
         ("key_rows", VP), ("scale", ctypes.c_float),

@@ -404,8 +404,8 @@ int unpack(const y3b_structure_attention_args* p, const char* what, AttArgs* a) 
                 "%s: bad table of the forward", what);
   Y3B_CHECK_ARG(p->query_item_count >= 0 && p->query_join_count >= 0 && p->query_slot_count >= 0 &&
                     p->query_row_count >= 0 && p->key_item_count >= 0 && p->key_join_count >= 0 &&
-                    p->key_slot_count >= 0 && p->key_row_count >= 0 && p->few_key_count >= 0 &&
-                    p->few_key_count <= p->key_row_count && (p->few_key_count == 0 || p->query_count > 0),
+                    p->key_slot_count >= 0 && p->key_row_count >= 0 && p->few_key_item_count >= 0 &&
+                    p->few_key_item_count <= p->key_item_count && (p->few_key_item_count == 0 || p->query_count > 0),
                 "%s: negative table size", what);
   Y3B_CHECK_ARG((p->query_item_count == 0 || p->query_items) && (p->query_join_count == 0 || p->query_joins) &&
                     (p->query_row_count == 0 || p->query_rows) && (p->key_item_count == 0 || p->key_items) &&
@@ -689,7 +689,7 @@ AttPlan make_plan(const y3b_structure_attention_args* p, bool adjoint) {
   w.Wf = w.DP + 16;
   w.Wq = (w.pieces == 1 ? 2 : 1) * w.DP + 16;
   w.Wk = 2 * w.DP + 16;
-  w.tiles = adjoint ? p->query_item_count > 0 || p->key_item_count > 0 : p->forward_item_count > 0;
+  w.tiles = adjoint ? p->query_item_count > 0 || p->key_item_count > p->few_key_item_count : p->forward_item_count > 0;
   w.direct[0] = in_place(p, p->query, p->query_row_stride, p->query_head_stride);
   w.direct[1] = in_place(p, p->key, p->key_row_stride, p->key_head_stride);
   w.direct[2] = in_place(p, p->value, p->value_row_stride, p->value_head_stride);
@@ -872,27 +872,27 @@ int backward(const y3b_structure_attention_args* p, const AttArgs& a, const AttP
       Y3B_LAUNCH_CHECK();
     }
   }
-  const int2* key_rows = reinterpret_cast<const int2*>(p->key_rows);
-  const int64_t other_rows = p->key_row_count - p->few_key_count;
-  if (p->few_key_count > 0) {
-    const int rc = attention_few_key<T>(a, key_rows + other_rows, p->few_key_count, g, lse, delta, static_cast<T*>(dk),
-                                        static_cast<T*>(dv), dy_part, s);
+  const AttItem* key_items = reinterpret_cast<const AttItem*>(p->key_items);
+  const int64_t key_tiles = p->key_item_count - p->few_key_item_count;
+  if (p->few_key_item_count > 0) {
+    const int rc = attention_few_key<T>(a, key_items + key_tiles, p->few_key_item_count, g, lse, delta,
+                                        static_cast<T*>(dk), static_cast<T*>(dv), dy_part, s);
     if (rc) return rc;
   }
-  if (other_rows > 0) {
-    row_backward_key_kernel<T><<<row_grid(other_rows * a.Hk), 32 * kRowWarps, 0, s>>>(
-        a, key_rows, other_rows, g, lse, delta, static_cast<T*>(dk),
+  if (p->key_row_count > 0) {
+    row_backward_key_kernel<T><<<row_grid(p->key_row_count * a.Hk), 32 * kRowWarps, 0, s>>>(
+        a, reinterpret_cast<const int2*>(p->key_rows), p->key_row_count, g, lse, delta, static_cast<T*>(dk),
         static_cast<T*>(dv), dy_part);
     Y3B_LAUNCH_CHECK();
   }
-  if (p->key_item_count > 0) {
-    t.items = reinterpret_cast<const AttItem*>(p->key_items);
+  if (key_tiles > 0) {
+    t.items = key_items;
     t.place_part = dy_part;
     t.out0 = dv;
     t.out1 = dk;
     t.part = reinterpret_cast<float*>(ws + w.part_k);
     t.vec = a.D * sizeof(T) % 16 == 0 && on16(dk) && on16(dv);
-    const int rc = attention_key_tiles(w.pieces, t, p->key_item_count, s);
+    const int rc = attention_key_tiles(w.pieces, t, key_tiles, s);
     if (rc) return rc;
     if (p->key_join_count > 0) {
       join_key_kernel<T><<<unsigned(p->key_join_count * a.Hk * kJoinCtas), 128, 0, s>>>(

@@ -315,37 +315,39 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_kernel(const __grid_consta
 
 // Gradients of keys that one or two queries see: LPK lanes hold a key's components of K and V and those of its
 // gradients, in fp32, and go over the query heads that share the key head.  The loads of two keys are in flight
-// together.  fp32 is bound by reading K and V and writing their gradients once (705 MB of the case above: 5.1 TB/s),
-// bf16 by the arithmetic of its eight components a lane (8 structures of 16,384 keys, 8 heads of 64 on 4: 297 MB, 121
-// us, 2.5 TB/s; on tiles 209).
+// together.  A CTA takes part of an item of up to kTileRows keys that the same queries see.  fp32 is bound by reading K
+// and V and writing their gradients once (705 MB of the case above: 143 us, 4.9 TB/s; by an entry a key 139), bf16 by the
+// arithmetic of its eight components a lane (8 structures of 16,384 keys, 8 heads of 64 on 4: 297 MB, 111 us, 2.7
+// TB/s; by an entry a key 124, on tiles 209).
 template <typename T, int LPK, bool VEC>
 __global__ void __launch_bounds__(32 * kFewWarps, kFewKeyCtas) few_key_kernel(const __grid_constant__ AttArgs a,
-                                                                const int2* __restrict__ rows, int64_t count, int vec,
+                                                                const AttItem* __restrict__ items, int vec,
                                                                 const T* __restrict__ grad,
                                                                 const float* __restrict__ lse,
                                                                 const float* __restrict__ delta, T* __restrict__ dk,
                                                                 T* __restrict__ dv, float* __restrict__ dy_part) {
   constexpr int W = 16 / int(sizeof(T)), KPW = 32 / LPK;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, slot = lane / LPK, d0 = (lane % LPK) * W;
-  const int hk = int(blockIdx.y);
-  const int64_t e0 = (blockIdx.x * int64_t(kFewWarps) + warp) * (KPW * kFewKeySteps) + slot;
+  constexpr int KEYS = kFewWarps * KPW * kFewKeySteps;  // of a CTA
+  constexpr unsigned CTAS = kTileRows / KEYS;           // of an item
+  const int hk = int(blockIdx.y), cta0 = int(blockIdx.x % CTAS) * KEYS;
+  const AttItem it = items[blockIdx.x / CTAS];
+  if (cta0 >= it.rows) return;
+  const int e0 = cta0 + warp * (KPW * kFewKeySteps) + slot;
   const bool bias = a.slopes != nullptr;
-  int2 of[kFewKeySteps];  // (key, structure); past the end the last one, which is not stored again
+  int key[kFewKeySteps];  // past the end the last one, which is not stored again
 #pragma unroll
-  for (int t = 0; t < kFewKeySteps; ++t) of[t] = rows[e0 + t * KPW < count ? e0 + t * KPW : count - 1];
+  for (int t = 0; t < kFewKeySteps; ++t) key[t] = it.row + min(e0 + t * KPW, it.rows - 1);
   const T* kp = static_cast<const T*>(a.k) + hk * a.k_head + d0;
   const T* vp = static_cast<const T*>(a.v) + hk * a.v_head + d0;
   uint4 kr[kFewKeySteps], vr[kFewKeySteps];
   float y[kFewKeySteps][3];
-  int first[kFewKeySteps], queries[kFewKeySteps];
 #pragma unroll
   for (int t = 0; t < kFewKeySteps; ++t) {
-    kr[t] = raw_part<T, W, VEC>(kp + int64_t(of[t].x) * a.k_row, a.D - d0);
-    vr[t] = raw_part<T, W, VEC>(vp + int64_t(of[t].x) * a.v_row, a.D - d0);
+    kr[t] = raw_part<T, W, VEC>(kp + int64_t(key[t]) * a.k_row, a.D - d0);
+    vr[t] = raw_part<T, W, VEC>(vp + int64_t(key[t]) * a.v_row, a.D - d0);
 #pragma unroll
-    for (int c = 0; c < 3; ++c) y[t][c] = bias ? a.y[3 * int64_t(of[t].x) + c] : 0.0f;
-    first[t] = a.q_off[of[t].y];
-    queries[t] = a.q_off[of[t].y + 1] - first[t];
+    for (int c = 0; c < 3; ++c) y[t][c] = bias ? a.y[3 * int64_t(key[t]) + c] : 0.0f;
   }
 #pragma unroll
   for (int t = 0; t < kFewKeySteps; ++t) {
@@ -354,10 +356,8 @@ __global__ void __launch_bounds__(32 * kFewWarps, kFewKeyCtas) few_key_kernel(co
     widen_part<T, W>(vv, vr[t]);
 #pragma unroll
     for (int k = 0; k < W; ++k) gk[k] = gv[k] = 0.0f;
-    for (int n = 0; n < kFewQueries; ++n) {
-      const bool seen = n < queries[t];
-      if (!__any_sync(0xffffffffu, seen)) break;
-      const int64_t i = seen ? first[t] + n : 0;
+    for (int n = 0; n < it.cols; ++n) {
+      const int64_t i = int64_t(it.col) + n;
       for (int h = hk * a.group; h < (hk + 1) * a.group; ++h) {
         float q[W], g[W], s = 0.0f, x = 0.0f;
         load_part<T, W>(q, static_cast<const T*>(a.q) + i * a.q_row + h * a.q_head + d0, a.D - d0, vec & 1);
@@ -376,7 +376,6 @@ __global__ void __launch_bounds__(32 * kFewWarps, kFewKeyCtas) few_key_kernel(co
         }
         s = part_sum<LPK>(s);
         x = part_sum<LPK>(x);
-        if (!seen) continue;
         float rd = 0.0f;
         if (bias) {
           const float sq = fmaf(away[2], away[2], fmaf(away[1], away[1], fmaf(away[0], away[0], 1e-30f)));
@@ -393,8 +392,8 @@ __global__ void __launch_bounds__(32 * kFewWarps, kFewKeyCtas) few_key_kernel(co
         }
       }
     }
-    if (e0 + t * KPW >= count) continue;
-    const int64_t at = int64_t(of[t].x) * a.Hk + hk;
+    if (e0 + t * KPW >= it.rows) continue;
+    const int64_t at = int64_t(key[t]) * a.Hk + hk;
     alignas(16) T ok[W], ov[W];
 #pragma unroll
     for (int k = 0; k < W; ++k) {
@@ -458,7 +457,7 @@ int few(const AttArgs& a, const AttItem* items, int64_t count, int DP, int width
 }  // namespace
 
 template <typename T>
-int attention_few_key(const AttArgs& a, const int2* rows, int64_t count, const T* grad, const float* lse,
+int attention_few_key(const AttArgs& a, const AttItem* items, int64_t count, const T* grad, const float* lse,
                       const float* delta, T* dk, T* dv, float* dy_part, cudaStream_t s) {
   constexpr int W = 16 / int(sizeof(T));
   const auto fits = [&](const void* p, int64_t row, int64_t head) {
@@ -469,15 +468,15 @@ int attention_few_key(const AttArgs& a, const int2* rows, int64_t count, const T
   const bool loads = fits(a.k, a.k_row, a.k_head) && fits(a.v, a.v_row, a.v_head);
 #define Y3B_FEW_KEY(LPK)                                                                                       \
   do {                                                                                                         \
-    const int64_t keys = kFewWarps * (32 / LPK) * kFewKeySteps, grid = (count + keys - 1) / keys;              \
+    const int64_t grid = count * (kTileRows / (kFewWarps * (32 / LPK) * kFewKeySteps));                        \
     if (grid > INT32_MAX) return fail(Y3B_ERR_UNSUPPORTED, "structure_attention: too many keys");              \
     const dim3 ctas(unsigned(grid), unsigned(a.Hk));                                                           \
     if (loads)                                                                                                 \
-      few_key_kernel<T, LPK, true><<<ctas, 32 * kFewWarps, 0, s>>>(a, rows, count, vec, grad, lse, delta, dk,  \
-                                                                   dv, dy_part);                               \
+      few_key_kernel<T, LPK, true><<<ctas, 32 * kFewWarps, 0, s>>>(a, items, vec, grad, lse, delta, dk, dv,    \
+                                                                   dy_part);                                   \
     else                                                                                                       \
-      few_key_kernel<T, LPK, false><<<ctas, 32 * kFewWarps, 0, s>>>(a, rows, count, vec, grad, lse, delta, dk, \
-                                                                    dv, dy_part);                              \
+      few_key_kernel<T, LPK, false><<<ctas, 32 * kFewWarps, 0, s>>>(a, items, vec, grad, lse, delta, dk, dv,   \
+                                                                    dy_part);                                  \
   } while (0)
   const int lanes = (a.D + W - 1) / W;
   if (lanes <= 4) Y3B_FEW_KEY(4);
@@ -501,9 +500,9 @@ int attention_few_query(const AttArgs& a, const AttItem* items, int64_t count, i
   return few<T, true>(a, items, count, DP, width, out, grad, lse, part, s);
 }
 
-template int attention_few_key<float>(const AttArgs&, const int2*, int64_t, const float*, const float*, const float*,
+template int attention_few_key<float>(const AttArgs&, const AttItem*, int64_t, const float*, const float*, const float*,
                                       float*, float*, float*, cudaStream_t);
-template int attention_few_key<__nv_bfloat16>(const AttArgs&, const int2*, int64_t, const __nv_bfloat16*, const float*,
+template int attention_few_key<__nv_bfloat16>(const AttArgs&, const AttItem*, int64_t, const __nv_bfloat16*, const float*,
                                               const float*, __nv_bfloat16*, __nv_bfloat16*, float*, cudaStream_t);
 template int attention_few_forward<float>(const AttArgs&, const AttItem*, int64_t, int, int, float*, cudaStream_t);
 template int attention_few_forward<__nv_bfloat16>(const AttArgs&, const AttItem*, int64_t, int, int, float*,

@@ -20,10 +20,10 @@ template <typename T>
 int attention_few_query(const AttArgs& a, const AttItem* items, int64_t count, int DP, int width, const T* out,
                         const T* grad, const float* lse, float* part, cudaStream_t s);
 
-// dk, dv and the position parts of the keys in `rows` (key, structure), whose structures have at most kFewQueries
-// queries.
+// dk, dv and the position parts of the keys of `items` (rows: up to kTileRows keys of one structure, columns: its one to
+// kFewQueries queries).
 template <typename T>
-int attention_few_key(const AttArgs& a, const int2* rows, int64_t count, const T* grad, const float* lse,
+int attention_few_key(const AttArgs& a, const AttItem* items, int64_t count, const T* grad, const float* lse,
                       const float* delta, T* dk, T* dv, float* dy_part, cudaStream_t s);
 
 }  // namespace y3b

@@ -7,7 +7,8 @@
 //   row     no or a single key: its weight is exactly 1 and its gradients through the softmax exactly 0, which the
 //           row kernels keep;
 //   few     up to two queries: a tile would hold 2 rows of 128 (8 structures of 16,384 keys, 8 heads: 111 us on tiles,
-//           64 on the few-query kernels; their keys' gradients 209 us on tiles, 121 by a few lanes a key);
+//           64 on the few-query kernels; their keys' gradients 209 us on tiles, 121 by a few lanes a key, in items of 128
+//           keys: with an entry a key this table took 1.1 ms and 1.2 MB, in items 0.05 ms and 41 KB);
 //   tile    the rest.
 // A tile's columns are cut into parts, which are joined, where that makes the last wave of CTAs shorter (16,384 atoms, 8
 // heads: forward 1,273 us and 39 to join against 1,431 uncut).
@@ -123,6 +124,18 @@ void add_rows(Side* side, const std::vector<Range>& row, const std::vector<int64
   }
 }
 
+// Keys whose structure has one or two queries, in items of up to kTile of one structure.
+void add_few_keys(Side* side, const std::vector<Range>& key, const std::vector<Range>& query,
+                  const std::vector<int64_t>& which) {
+  for (const int64_t s : which) {
+    for (int64_t r = 0; r < key[s].count; r += kTile) {
+      const int32_t item[8] = {int32_t(key[s].first + r), int32_t(std::min(kTile, key[s].count - r)),
+                               int32_t(query[s].first), int32_t(query[s].count), -1, 0, 0, 0};
+      side->items.insert(side->items.end(), item, item + 8);
+    }
+  }
+}
+
 int64_t build(const int64_t* queries, const int64_t* keys, int64_t n, int64_t heads, int64_t key_heads,
               int64_t* counts, int32_t* out, int64_t capacity) {
   std::vector<Range> q(n), k(n);
@@ -158,15 +171,15 @@ int64_t build(const int64_t* queries, const int64_t* keys, int64_t n, int64_t he
   add_tiles(&one, q, k, few, key_heads, kSMs * 4, true);
   add_rows(&query, q, by_row);
   add_rows(&key, k, by_row);
-  const int64_t other_rows = int64_t(key.rows.size()) / 2;
-  add_rows(&key, k, few);
+  const int64_t key_tiles = int64_t(key.items.size()) / 8;
+  add_few_keys(&key, k, q, few);
   const auto entries = [](const std::vector<int32_t>& v, int width) { return int64_t(v.size()) / width; };
   const int64_t all[] = {int64_t(low.size()),      int64_t(high.size()),     entries(one.items, 8),
                          entries(one.joins, 4),    entries(forward.items, 8), entries(forward.joins, 4),
                          forward.slots,            entries(query.items, 8),  entries(query.joins, 4),
                          query.slots,              entries(query.rows, 2),   entries(key.items, 8),
                          entries(key.joins, 4),    key.slots,                entries(key.rows, 2),
-                         entries(key.rows, 2) - other_rows};
+                         entries(key.items, 8) - key_tiles};
   static_assert(sizeof(all) == 16 * sizeof(int64_t), "what callers reserve for counts");
   std::copy(std::begin(all), std::end(all), counts);
   const std::vector<int32_t>* const tables[] = {&forward.items, &query.items, &key.items, &one.items,

@@ -627,7 +627,7 @@ _LAYOUT_COUNTS = ("heads", "key_heads", "query_count", "key_count", "structure_c
                   "small_64_count", "few_item_count", "few_join_count", "few_slot_count", "forward_item_count",
                   "forward_join_count", "forward_slot_count", "query_item_count",
                   "query_join_count", "query_slot_count", "query_row_count", "key_item_count", "key_join_count",
-                  "key_slot_count", "key_row_count", "few_key_count")
+                  "key_slot_count", "key_row_count", "few_key_item_count")
 # its tables in their order, with the integers of an entry and the count they go by: 32-byte records first, then
 # 16-byte ones
 _LAYOUT_TABLES = (("forward_items", 8, "forward_item_count"), ("query_items", 8, "query_item_count"),
@@ -641,8 +641,8 @@ _LAYOUT_TABLES = (("forward_items", 8, "forward_item_count"), ("query_items", 8,
 def _layout_tables(queries, keys, heads, key_heads):
     """A layout's tables, one after the other, and the counts of their entries (``small_32_count`` on)."""
     lib, counts = nat.lib(), np.empty(16, np.int64)
-    # room for a few entries a structure; a batch that needs more says how much
-    tables = np.empty(16 * queries.size + 256, np.int32)
+    # room for a few entries a structure and for every 128 of its rows; a batch that needs more says how much
+    tables = np.empty(24 * queries.size + int(queries.sum() + keys.sum()) // 4 + 256, np.int32)
     for _ in range(2):
         n = int(lib.y3b_structure_layout(queries.ctypes.data, keys.ctypes.data, queries.size, heads, key_heads,
                                          counts.ctypes.data, tables.ctypes.data, tables.size))
