@@ -150,3 +150,62 @@ def test_gradients_of_keys_in_items_of_128(D, dtype):
     ref = torch.autograd.grad(_definition(*wide, 0.2, queries, keys)[0], wide, grad.double())
     for n, (a, b) in enumerate(zip(got, ref)):
         _same_numbers(a, b, TOL[dtype if n < 3 else torch.float32], n)
+
+
+def _in_two_threads(calls, times):
+    """Each call, many times over, in a thread and on a stream of its own; the return codes that are not zero."""
+    import threading
+    streams = [torch.cuda.Stream(DEV) for _ in calls]
+    failed = []
+
+    def work(call, stream):
+        torch.cuda.set_device(DEV)
+        for _ in range(times):
+            rc = call(stream)
+            if rc:
+                failed.append(rc)
+                return
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(call, s.cuda_stream)) for call, s in zip(calls, streams)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    return failed
+
+
+def test_calls_of_two_threads_do_not_limit_each_other():
+    """Two widths of small structures, and two small tables, on the same kernels: what shared memory a launch may have is
+    not what another thread's call needs."""
+    import ctypes
+
+    from ye3t_b200 import _native as nat
+    from ye3t_b200 import runtime as rt
+    lib, layout = nat.lib(), rt.StructureLayout([64, 50], heads=2, device=DEV)
+    hold, attention, adjoint, tables = [], [], [], []
+    for D in (8, 128):
+        q, k, v, g, x, _, sl = _inputs([64, 50], [64, 50], 2, 2, D, torch.float32, D)
+        args = rt._attention_args(q, k, v, x, x, sl, layout, 0.2)
+        out, lse = rt._attention_forward(q, k, v, x, x, sl, layout, 0.2, False)
+        ws, size = rt._attention_workspace(args, 1, q.device)
+        grads = [torch.empty_like(t) for t in (q, k, v, x, sl)]
+        hold += [q, k, v, g, x, sl, out, lse, ws, args] + grads
+        at = [t.data_ptr() for t in (out, g, lse, ws)]
+        to = [t.data_ptr() for t in grads]
+        attention.append(lambda s, a=args, at=at: lib.y3b_structure_attention(ctypes.byref(a), at[3], 0, at[0], at[2], 0, s))
+        adjoint.append(lambda s, a=args, at=at, to=to, size=size: lib.y3b_structure_attention_adjoint(
+            ctypes.byref(a), at[0], at[1], at[2], at[3], size, to[0], to[1], to[2], to[3], 0, to[4], 0, s))
+    for species in (2, 24):
+        grad, z = torch.ones(500, 128, device=DEV), torch.arange(500, device=DEV) % species
+        size = int(lib.y3b_species_embedding_adjoint_workspace_bytes(nat.F32, 500, species, 128))
+        ws, out = torch.empty(max(size, 1), dtype=torch.uint8, device=DEV), torch.empty(species, 128, device=DEV)
+        hold += [grad, z, ws, out]
+        p = [t.data_ptr() for t in (grad, z, ws, out)]
+        tables.append(lambda s, p=p, n=species, size=size: lib.y3b_species_embedding_adjoint(
+            nat.F32, p[0], p[1], 8, 500, n, 128, 1.0, p[2], size, p[3], 0, s))
+    for calls in (attention, adjoint, tables):
+        assert all(call(0) == 0 for call in calls)
+        assert not _in_two_threads(calls, 20000)
+    del hold

@@ -75,6 +75,7 @@ __global__ void __launch_bounds__(256) embedding_kernel(const T* __restrict__ ta
 // them taken from registers).
 constexpr int kTableRows = 8;
 constexpr int kTableThreads = 256;
+constexpr int kTableSmem = 109 * 1024;  // of the copies: two CTAs an SM
 
 template <typename T, typename I, int VEC, int L>
 __global__ void __launch_bounds__(kTableThreads) table_sum_kernel(
@@ -600,7 +601,7 @@ AdjointPlan adjoint_plan(int dtype, int64_t N, int64_t V, int64_t C) {
   p.vec = C % wide == 0 ? wide : 1;
   p.lanes = unit_lanes(C, p.vec);
   const int64_t units = kTableThreads / p.lanes, copies = units * (V + 1) * p.lanes * p.vec * real;
-  p.small = 2 * (copies + 1024) <= 220 * 1024;
+  p.small = copies <= kTableSmem;
   if (p.small) {
     const int64_t slabs = (C + p.lanes * p.vec - 1) / (p.lanes * p.vec);
     const int64_t per_sm = std::min<int64_t>(2048 / kTableThreads, 220 * 1024 / (copies + 1024));
@@ -685,7 +686,8 @@ int table_sums(const AdjointPlan& p, const T* grad, const I* z, int64_t N, int64
   using A = typename Acc<T>::type;
   const auto kernel = table_sum_kernel<T, I, VEC, L>;
   const int smem = int(kTableThreads * (V + 1) * VEC * int64_t(sizeof(A))), slabs = (C + L * VEC - 1) / (L * VEC);
-  Y3B_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  // the kernel's limit is that of every table, so that calls of several threads only ever set the same value
+  Y3B_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTableSmem));
   A* part = p.parts > 1 ? reinterpret_cast<A*>(ws + p.head) : nullptr;
   kernel<<<dim3(unsigned(p.parts), unsigned(slabs)), kTableThreads, smem, s>>>(grad, z, N, int(V), C, p.rows_per_unit,
                                                                               A(scale), dtable, part, status);

@@ -676,12 +676,24 @@ dim3 by_structure(int heads, int64_t n) {
 }
 
 template <typename T, int NT>
+int forward_smem(int D) {
+  return 3 * 8 * NT * row_stride<T>(D) * int(sizeof(T)) + 6 * 8 * NT * 4;
+}
+template <typename T, int NT>
+int backward_smem(int D) {
+  constexpr int R = 8 * NT;
+  return 4 * R * row_stride<T>(D) * int(sizeof(T)) + 2 * R * (R + 4) * 4 + 6 * R * 4;
+}
+
+// A kernel may have what its widest head needs, whatever this call does: the limit is the kernel's, and another thread's
+// call of fewer components must not lower it between the setting and the launch.
+template <typename T, int NT>
 int forward_class(const AttArgs& a, const AttSmall* list, int64_t n, int vec, T* out, float* lse, cudaStream_t s) {
-  const int stride = row_stride<T>(a.D), R = 8 * NT;
-  const int smem = 3 * R * stride * int(sizeof(T)) + 6 * R * 4;
   const auto kernel = small_forward_kernel<T, NT>;
-  Y3B_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  kernel<<<by_structure(a.H, n), 16 * NT, smem, s>>>(a, list, n, stride, part_shift<T>(a.D), vec, out, lse);
+  Y3B_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    forward_smem<T, NT>(kAttMaxWidth)));
+  kernel<<<by_structure(a.H, n), 16 * NT, forward_smem<T, NT>(a.D), s>>>(a, list, n, row_stride<T>(a.D),
+                                                                         part_shift<T>(a.D), vec, out, lse);
   Y3B_LAUNCH_CHECK();
   return Y3B_OK;
 }
@@ -689,12 +701,11 @@ int forward_class(const AttArgs& a, const AttSmall* list, int64_t n, int vec, T*
 template <typename T, int NT, int DT>
 int backward_class(const AttArgs& a, const AttSmall* list, int64_t n, int vec, const T* grad, T* dq, T* dk, T* dv,
                    float* slope_part, float* dx_part, float* dy_part, cudaStream_t s) {
-  const int stride = row_stride<T>(a.D), R = 8 * NT;
-  const int smem = 4 * R * stride * int(sizeof(T)) + 2 * R * (R + 4) * 4 + 6 * R * 4;
   const auto kernel = small_backward_kernel<T, NT, DT>;
-  Y3B_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  kernel<<<by_structure(a.Hk, n), 16 * NT, smem, s>>>(a, list, n, stride, part_shift<T>(a.D), vec, grad, dq, dk, dv,
-                                                      slope_part, dx_part, dy_part);
+  Y3B_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    backward_smem<T, NT>(8 * DT)));
+  kernel<<<by_structure(a.Hk, n), 16 * NT, backward_smem<T, NT>(a.D), s>>>(
+      a, list, n, row_stride<T>(a.D), part_shift<T>(a.D), vec, grad, dq, dk, dv, slope_part, dx_part, dy_part);
   Y3B_LAUNCH_CHECK();
   return Y3B_OK;
 }
