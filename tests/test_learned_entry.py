@@ -29,3 +29,73 @@ def test_layout_of_few_queries_has_no_entry_a_key(queries, keys):
     packed, _ = rt._layout_tables(np.array(queries), np.array(keys), 8, 4)
     # an item of eight values a hundred keys in two tables, and some for each structure
     assert packed.size <= 16 * (sum(keys) // 100) + 64 * len(keys)
+
+
+class _Library:
+    """Stands in for the native library: notes which calls are made, and whether the device was current then."""
+
+    def __init__(self):
+        self.current, self.calls = 0, {}
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls[name] = self.current
+            return 64 if name.endswith("_bytes") else 0
+        return call
+
+
+@pytest.mark.parametrize("current", [0, 1])
+def test_native_calls_run_with_the_tensors_device_current(monkeypatch, current):
+    """The kernels launch on the current device, which need not be that of the tensors."""
+    import contextlib
+    from types import SimpleNamespace
+
+    import torch
+    from ye3t_b200 import _native as nat
+    from ye3t_b200 import runtime as rt
+    lib = _Library()
+    lib.current = current
+
+    @contextlib.contextmanager
+    def device(wanted):
+        before, lib.current = lib.current, wanted.index
+        yield
+        lib.current = before
+
+    class Device(SimpleNamespace):
+        type, index = "cuda", 1
+
+    class Tensor(SimpleNamespace):
+        """A tensor of the second device, of which only the shape matters."""
+
+        def __init__(self, *shape, dtype=torch.float32):
+            super().__init__(shape=torch.Size(shape), dtype=dtype, device=Device())
+
+        def contiguous(self):
+            return self
+
+        def new_empty(self, shape, dtype=None):
+            return Tensor(*shape, dtype=dtype or self.dtype)
+
+        def stride(self, dim=None):
+            return (1, 1, 1) if dim is None else 1
+
+        data_ptr = element_size = numel = lambda self: 4
+
+    monkeypatch.setattr(nat, "lib", lambda: lib)
+    monkeypatch.setattr(rt, "_raw_stream", lambda dev: 0)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: lib.current)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch, "empty", lambda shape, dtype=None, device=None: Tensor(*np.atleast_1d(shape), dtype=dtype))
+    monkeypatch.setattr(torch, "empty_like", lambda t: t)
+    z = Tensor(5, dtype=torch.int64)
+    rt._embedding_forward(Tensor(3, 4), z, 1.0, False)
+    rt._embedding_adjoint(Tensor(5, 4), z, 3, 1.0)
+    layout = SimpleNamespace(_args=nat.StructureAttentionArgs(), device=Device(), _stream=0)
+    q, x, slopes = Tensor(5, 2, 8), Tensor(5, 3), Tensor(2)
+    out, lse = rt._attention_forward(q, q, q, x, x, slopes, layout, 1.0, False)
+    rt._attention_adjoint(out, q, q, q, x, x, slopes, out, lse, layout, 1.0, True, False)
+    launches = {name: dev for name, dev in lib.calls.items() if not name.endswith("_bytes")}
+    assert launches == {"y3b_species_embedding": 1, "y3b_species_embedding_adjoint": 1, "y3b_structure_attention": 1,
+                        "y3b_structure_attention_adjoint": 1}
+    assert lib.current == current

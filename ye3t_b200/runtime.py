@@ -15,6 +15,7 @@ status word is set, matching the reference CPU path's eager checks
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -536,14 +537,23 @@ def _raw_stream(device):
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def _on_device(device):
+    """Makes the tensors' device the current one, where it is not: the native calls launch on the current device."""
+    if torch.cuda.current_device() == device.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
 def _embedding_forward(table, species, scale, validate):
     dev = table.device
     t, z = table.contiguous(), species.contiguous()
     out = torch.empty(z.shape + (t.shape[1],), dtype=t.dtype, device=dev)
     status = _status(dev) if validate else None
-    nat.check(nat.lib().y3b_species_embedding(nat.learned_dtype_code(t.dtype), t.data_ptr(), t.shape[0], t.shape[1],
-                                              z.data_ptr(), z.element_size(), z.numel(), scale, out.data_ptr(),
-                                              nat.ptr(status), _raw_stream(dev)), "species_embedding")
+    with _on_device(dev):
+        nat.check(nat.lib().y3b_species_embedding(nat.learned_dtype_code(t.dtype), t.data_ptr(), t.shape[0],
+                                                  t.shape[1], z.data_ptr(), z.element_size(), z.numel(), scale,
+                                                  out.data_ptr(), nat.ptr(status), _raw_stream(dev)),
+                  "species_embedding")
     if validate:
         _raise_on_status(status, "species_embedding")
     return out
@@ -560,9 +570,10 @@ def _embedding_adjoint(grad, species, species_count, scale):
     if ws_bytes < 0:
         raise ValueError("species_embedding: the gradient takes up to 2^31 - 1 atoms and species")
     ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=dev)
-    nat.check(lib.y3b_species_embedding_adjoint(code, g.data_ptr(), z.data_ptr(), z.element_size(), z.numel(),
-                                                species_count, C, scale, ws.data_ptr(), ws_bytes, out.data_ptr(), 0,
-                                                _raw_stream(dev)), "species_embedding adjoint")
+    with _on_device(dev):
+        nat.check(lib.y3b_species_embedding_adjoint(code, g.data_ptr(), z.data_ptr(), z.element_size(), z.numel(),
+                                                    species_count, C, scale, ws.data_ptr(), ws_bytes, out.data_ptr(),
+                                                    0, _raw_stream(dev)), "species_embedding adjoint")
     return out
 
 
@@ -750,9 +761,10 @@ def _attention_forward(query, key, value, x, y, slopes, layout, scale, validate)
     args = _attention_args(q, k, v, x, y, slopes, layout, scale)
     ws, ws_bytes = _attention_workspace(args, 0, q.device)
     status = _status(q.device) if validate else None
-    nat.check(nat.lib().y3b_structure_attention(ctypes.byref(args), ws.data_ptr(), ws_bytes, out.data_ptr(),
-                                                lse.data_ptr(), nat.ptr(status), _raw_stream(q.device)),
-              "structure_attention")
+    with _on_device(q.device):
+        nat.check(nat.lib().y3b_structure_attention(ctypes.byref(args), ws.data_ptr(), ws_bytes, out.data_ptr(),
+                                                    lse.data_ptr(), nat.ptr(status), _raw_stream(q.device)),
+                  "structure_attention")
     if validate:
         _raise_on_status(status, "structure_attention")
     return out, lse
@@ -769,10 +781,11 @@ def _attention_adjoint(grad, query, key, value, x, y, slopes, out, lse, layout, 
     args = _attention_args(q, k, v, x, y, slopes, layout, scale)
     ws, ws_bytes = _attention_workspace(args, 1, dev)
     status = _status(dev) if validate else None
-    nat.check(nat.lib().y3b_structure_attention_adjoint(
-        ctypes.byref(args), out.data_ptr(), g.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws_bytes, dq.data_ptr(),
-        dk.data_ptr(), dv.data_ptr(), nat.ptr(dx), nat.ptr(dy), nat.ptr(dslopes), nat.ptr(status), _raw_stream(dev)),
-        "structure_attention adjoint")
+    with _on_device(dev):
+        nat.check(nat.lib().y3b_structure_attention_adjoint(
+            ctypes.byref(args), out.data_ptr(), g.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws_bytes, dq.data_ptr(),
+            dk.data_ptr(), dv.data_ptr(), nat.ptr(dx), nat.ptr(dy), nat.ptr(dslopes), nat.ptr(status),
+            _raw_stream(dev)), "structure_attention adjoint")
     if validate:
         _raise_on_status(status, "structure_attention adjoint")
     return dq, dk, dv, dx, dy, dslopes
