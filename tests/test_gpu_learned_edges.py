@@ -209,3 +209,20 @@ def test_calls_of_two_threads_do_not_limit_each_other():
         assert all(call(0) == 0 for call in calls)
         assert not _in_two_threads(calls, 20000)
     del hold
+
+
+@pytest.mark.parametrize("on", [False, True])
+def test_registered_operators_read_the_status_where_validation_is_on(monkeypatch, on):
+    """YE3T_B200_VALIDATE holds for torch.ops as for the runtime's functions."""
+    import ye3t_b200.torch_ops  # noqa: F401
+    from ye3t_b200 import runtime as rt
+    monkeypatch.setenv("YE3T_B200_VALIDATE", "1" if on else "0")
+    read = []
+    monkeypatch.setattr(rt, "_raise_on_status", lambda status, what: read.append((what, int(status))))
+    n = [100, 7]
+    q, k, v, grad, x, _, sl = _inputs(n, n, 2, 2, 16, torch.float32, 1)
+    layout = rt.StructureLayout(n, heads=2, device=DEV)
+    q.requires_grad_(True)
+    out, _ = torch.ops.ye3t_b200.structure_attention(q, k, v, layout.tables, layout.counts, x, None, sl, 0.3)
+    torch.autograd.grad(out, q, grad)
+    assert read == ([("structure_attention", 0), ("structure_attention adjoint", 0)] if on else [])

@@ -263,7 +263,7 @@ def structure_attention(query: Tensor, key: Tensor, value: Tensor, tables: Tenso
     layout = rt.StructureLayout.from_tensors(tables, counts)
     rt._check_attention(query, key, value, layout, positions, key_positions, slopes)
     x, y, slopes = _places(positions, key_positions, slopes)
-    return rt._attention_forward(query, key, value, x, y, slopes, layout, scale, False)
+    return rt._attention_forward(query, key, value, x, y, slopes, layout, scale, rt._validate_default(None))
 
 
 def _places(positions, key_positions, slopes):
@@ -287,7 +287,7 @@ def structure_attention_adjoint(grad: Tensor, query: Tensor, key: Tensor, value:
     rt._check_attention(query, key, value, layout, positions, key_positions, slopes)
     x, y, slopes = _places(positions, key_positions, slopes)
     grads = rt._attention_adjoint(grad, query, key, value, x, y, slopes, out, lse, layout, scale,
-                                  key_positions is None, False)
+                                  key_positions is None, rt._validate_default(None))
     # an absent argument's gradient is an empty tensor
     return tuple(lse.new_empty(0) if g is None else g for g in grads)
 
