@@ -328,7 +328,8 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP, HP>::THREADS, AttCfg<MODE
     // cp.async, with zeros past it: rows of the next structure, whatever they hold, stay out.
     const int t = lane;
     bool ok = true;
-    for (int j = 0; j < total; ++j) {
+    int j = 0;
+    for (; j < total; ++j) {
       const int s = j % C::STAGES;
       if (j >= C::STAGES) ok = tc::mbar_wait(empty(s), ((j / C::STAGES) - 1) & 1);
       if (!ok) break;
@@ -377,6 +378,8 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP, HP>::THREADS, AttCfg<MODE
       tc::mbar_arrive(full(s));
     }
     if (!ok) s_abort = 1;
+    // no copy is in flight when the CTA ends, also where a warp gave up before it came
+    for (int k = j > C::STAGES ? j - C::STAGES : 0; k < j; ++k) tc::mbar_wait(full(k % C::STAGES), (k / C::STAGES) & 1);
   } else if (warp == C::MMA_WARP) {
     // ---- MMA issue: scores of tile j, then (when P is back) its accumulating product
     {
@@ -459,11 +462,10 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP, HP>::THREADS, AttCfg<MODE
         __syncwarp();
         if (C::BUFS == 1 && j + 1 < total) ok = issue_scores(j + 1);
       }
-      if (!ok) {
-        s_abort = 1;
-        if (lead) tc::commit(drain);
-        tc::mbar_wait(drain, 0);
-      }
+      if (!ok) s_abort = 1;
+      if (lead) tc::commit(drain);
+      __syncwarp();
+      tc::mbar_wait(drain, 0);  // no product either
     }
     __syncwarp();
   } else {
@@ -838,12 +840,14 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP, HP>::THREADS, AttCfg<MODE
     // the groups' sums: every thread gets the other group's of its row, through the stages' memory
     if constexpr (C::GROUPS == 2) {
       float* shared = reinterpret_cast<float*>(tile_smem + (cols - tc::smem_addr(tile_smem)));
+      if (!ok) s_abort = 1;
       asm volatile("bar.sync 1, 256;\n" ::: "memory");
       if (ok) {
 #pragma unroll
         for (int k = 0; k < SUMS; ++k) shared[(group * SUMS + k) * kTileRows + r_tile] = sum[k];
       }
       asm volatile("bar.sync 1, 256;\n" ::: "memory");
+      ok = ok && *static_cast<volatile int*>(&s_abort) == 0;  // a row needs both groups
       if (ok) {
         const float* other = shared + (1 - group) * SUMS * kTileRows + r_tile;
 #pragma unroll
@@ -951,6 +955,30 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP, HP>::THREADS, AttCfg<MODE
       }
     } else {
       s_abort = 1;
+      // a wait ran out: NaN, so that what is missing cannot pass as a result where no status is read
+      if (valid) {
+        const float nan = __int_as_float(0x7fffffff);
+#pragma unroll 1
+        for (int h = 0; h < HP; ++h) {
+          const int64_t at = row * heads + head0 + h;
+          if (item.slot >= 0) {
+            float* part = a.part + ((int64_t(item.slot) * heads + head0 + h) * kTileRows + r_tile) * C::PART;
+#pragma unroll 1
+            for (int k = group; k < C::PART; k += C::GROUPS) part[k] = nan;
+            continue;
+          }
+#pragma unroll 1
+          for (int d = d_first + group; d < d_first + d_count; d += C::GROUPS) {
+            static_cast<T*>(a.out0)[at * a.D + d] = from_float<T>(nan);
+            if constexpr (C::OPS == 2) static_cast<T*>(a.out1)[at * a.D + d] = from_float<T>(nan);
+          }
+          if constexpr (MODE == kForward) a.lse[at] = nan;
+          if constexpr (MODE == kQuerySide) a.delta[at] = nan;
+          if constexpr (MODE == kQuerySide && BIAS) a.slope_part[at] = nan;
+          if constexpr (MODE != kForward && BIAS)
+            for (int k = 0; k < 3; ++k) a.place_part[at * 3 + k] = nan;
+        }
+      }
     }
   }
   tc::fence_before();
