@@ -226,3 +226,33 @@ def test_registered_operators_read_the_status_where_validation_is_on(monkeypatch
     out, _ = torch.ops.ye3t_b200.structure_attention(q, k, v, layout.tables, layout.counts, x, None, sl, 0.3)
     torch.autograd.grad(out, q, grad)
     assert read == ([("structure_attention", 0), ("structure_attention adjoint", 0)] if on else [])
+
+
+def test_registered_adjoints_refuse_what_does_not_fit():
+    """The adjoints are operators of their own: a gradient of another size or type is refused, not read past its end."""
+    import ye3t_b200.torch_ops  # noqa: F401
+    from ye3t_b200 import runtime as rt
+    ops = torch.ops.ye3t_b200
+    grad, z = torch.ones(5, 8, device=DEV), torch.tensor([0, 1, 2, 1, 0], device=DEV)
+    assert ops.species_embedding_adjoint(grad, z, 3, 1.0).shape == (3, 8)
+    for g, s, n in ((grad[:3], z, 3), (grad[None], z, 3), (grad, z.reshape(1, 5), 3), (grad[:, :0], z, 3), (grad, z, -1)):
+        with pytest.raises(ValueError):
+            ops.species_embedding_adjoint(g, s, n, 1.0)
+    for g, s in ((grad.half(), z), (grad, z.float())):
+        with pytest.raises(TypeError):
+            ops.species_embedding_adjoint(g, s, 3, 1.0)
+    n = [4, 6]
+    q, k, v, grad, x, _, sl = _inputs(n, n, 4, 2, 16, torch.float32, 0)
+    layout = rt.StructureLayout(n, heads=4, key_heads=2, device=DEV)
+    out, lse = ops.structure_attention(q, k, v, layout.tables, layout.counts, x, None, sl, 0.25)
+
+    def adjoint(grad=grad, out=out, lse=lse):
+        return ops.structure_attention_adjoint(grad, q, k, v, layout.tables, layout.counts, x, None, sl, out, lse, 0.25)
+
+    assert adjoint()[0].shape == q.shape
+    assert torch.equal(adjoint()[0], adjoint(out=out.transpose(0, 1).contiguous().transpose(0, 1),
+                                             lse=lse.t().contiguous().t())[0])
+    for wrong in ({"grad": grad[:9]}, {"grad": grad.bfloat16()}, {"out": out[:, :2]}, {"out": out.double()},
+                  {"lse": lse[:4]}, {"lse": lse.double()}, {"lse": lse.cpu()}):
+        with pytest.raises(ValueError):
+            adjoint(**wrong)

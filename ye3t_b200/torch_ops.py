@@ -232,6 +232,11 @@ def _(table, species, scale):
 @custom_op("ye3t_b200::species_embedding_adjoint", mutates_args=())
 def species_embedding_adjoint(grad: Tensor, species: Tensor, species_count: int, scale: float) -> Tensor:
     nat.require_cuda(grad, species, what="species_embedding_adjoint")
+    if species.dtype not in (torch.int32, torch.int64):
+        raise TypeError("species must be int32 or int64")
+    if grad.ndim < 1 or grad.shape[:-1] != species.shape or grad.shape[-1] < 1 or species_count < 0:
+        raise ValueError(f"species_embedding_adjoint: grad {tuple(grad.shape)} of species {tuple(species.shape)} and a "
+                         f"table of {species_count} rows")
     return rt._embedding_adjoint(grad, species, species_count, scale)
 
 
@@ -285,8 +290,14 @@ def structure_attention_adjoint(grad: Tensor, query: Tensor, key: Tensor, value:
                                 scale: float) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
     layout = rt.StructureLayout.from_tensors(tables, counts)
     rt._check_attention(query, key, value, layout, positions, key_positions, slopes)
+    nat.require_cuda(query, grad, out, lse, what="structure_attention_adjoint")
+    for t, what, dtype, shape in ((grad, "grad", query.dtype, query.shape), (out, "out", query.dtype, query.shape),
+                                  (lse, "lse", torch.float32, query.shape[:2])):
+        if t.dtype != dtype or t.shape != shape:
+            raise ValueError(f"structure_attention_adjoint: {what} must be {dtype} {tuple(shape)}, got {t.dtype} "
+                             f"{tuple(t.shape)}")
     x, y, slopes = _places(positions, key_positions, slopes)
-    grads = rt._attention_adjoint(grad, query, key, value, x, y, slopes, out, lse, layout, scale,
+    grads = rt._attention_adjoint(grad, query, key, value, x, y, slopes, out.contiguous(), lse.contiguous(), layout, scale,
                                   key_positions is None, rt._validate_default(None))
     # an absent argument's gradient is an empty tensor
     return tuple(lse.new_empty(0) if g is None else g for g in grads)
