@@ -256,3 +256,31 @@ def test_registered_adjoints_refuse_what_does_not_fit():
                   {"lse": lse[:4]}, {"lse": lse.double()}, {"lse": lse.cpu()}):
         with pytest.raises(ValueError):
             adjoint(**wrong)
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent is not dropped without a word, with or without gradients recorded."""
+    import torch.autograd.forward_ad as forward_ad
+    import ye3t_b200.torch_ops  # noqa: F401
+    from ye3t_b200 import runtime as rt
+    n = [4, 6]
+    q, k, v, _, x, _, sl = _inputs(n, n, 2, 2, 16, torch.float32, 0)
+    layout = rt.StructureLayout(n, heads=2, device=DEV)
+    table, z = torch.ones(3, 4, device=DEV), torch.tensor([0, 2], device=DEV)
+    given = [q, k, v, x, sl]
+    with forward_ad.dual_level():
+        dual = [forward_ad.make_dual(t.clone(), torch.ones_like(t)) for t in given + [table]]
+        for recorded in (True, False):
+            with torch.set_grad_enabled(recorded):
+                for call in (lambda t: rt.species_embedding(t, z),
+                             lambda t: torch.ops.ye3t_b200.species_embedding(t, z, 1.0)):
+                    with pytest.raises(NotImplementedError):
+                        call(dual[5])
+                    assert call(table).shape == (2, 4)
+                for number in range(5):
+                    q1, k1, v1, x1, s1 = (dual[m] if m == number else t for m, t in enumerate(given))
+                    with pytest.raises(NotImplementedError):
+                        rt.structure_attention(q1, k1, v1, layout, positions=x1, slopes=s1)
+                    with pytest.raises(NotImplementedError):
+                        torch.ops.ye3t_b200.structure_attention(q1, k1, v1, layout.tables, layout.counts, x1, None, s1, 0.25)
+                assert rt.structure_attention(q, k, v, layout, positions=x, slopes=sl).shape == q.shape

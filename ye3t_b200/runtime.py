@@ -21,6 +21,7 @@ import os
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native as nat
@@ -544,6 +545,14 @@ def _on_device(device):
     return torch.cuda.device(device)
 
 
+def _refuse_tangents(what, *tensors):
+    """The learned operators have no forward-mode derivatives; a dual tensor would come out without its tangent."""
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivatives")
+
+
 def _embedding_forward(table, species, scale, validate):
     dev = table.device
     t, z = table.contiguous(), species.contiguous()
@@ -613,6 +622,7 @@ def species_embedding(table, species, *, scale=1.0, backend="auto", validate=Non
         raise ValueError("table must be [species_count, channels] with at least one channel")
     if species.dtype not in (torch.int32, torch.int64):
         raise TypeError("species must be int32 or int64")
+    _refuse_tangents("species_embedding", table)
     scale, validate = float(scale), _validate_default(validate)
     if table.requires_grad and torch.is_grad_enabled():
         return _SpeciesEmbedding.apply(table, species, scale, validate)
@@ -848,6 +858,7 @@ def _check_attention(query, key, value, layout, positions, key_positions, slopes
             raise ValueError("the layout has keys of its own: give key_positions")
         if slopes.dtype != torch.float32 or tuple(slopes.shape) != (layout.heads,):
             raise ValueError(f"slopes must be float32 [{layout.heads}], got {slopes.dtype} {tuple(slopes.shape)}")
+    _refuse_tangents("structure_attention", *given)
 
 
 def structure_attention(query, key, value, layout, *, positions=None, key_positions=None, slopes=None, scale=None,
