@@ -284,3 +284,20 @@ def test_forward_mode_derivatives_are_refused():
                     with pytest.raises(NotImplementedError):
                         torch.ops.ye3t_b200.structure_attention(q1, k1, v1, layout.tables, layout.counts, x1, None, s1, 0.25)
                 assert rt.structure_attention(q, k, v, layout, positions=x, slopes=sl).shape == q.shape
+
+
+@pytest.mark.parametrize("queries,keys", [([70, 1, 0, 30], [70, 1, 0, 30]), ([5, 3, 64, 33], [7, 2, 64, 1]),
+                                          ([1, 2, 1], [5000, 700, 90]), ([300, 129], [500, 9000])])
+def test_log_sum_exp_of_bfloat16_is_that_of_float32(queries, keys):
+    """Every kernel sums the probabilities as they are, before any is rounded to bfloat16: products of bfloat16 values are
+    exact in float32, so that the bound is that of float32 data.  Widths of 48 products of unit normals: 48 * 2^-23 * 31 *
+    0.3 * 1.44 = 8e-5."""
+    import ye3t_b200.torch_ops  # noqa: F401
+    from ye3t_b200 import runtime as rt
+    q, k, v, _, x, y, sl = _inputs(queries, keys, 4, 2, 48, torch.bfloat16, 12)
+    layout = rt.StructureLayout(queries, keys, heads=4, key_heads=2, device=DEV)
+    _, lse = torch.ops.ye3t_b200.structure_attention(q, k, v, layout.tables, layout.counts, x, y, sl, 0.3)
+    want = _definition(q, k, v, x, y, sl, 0.3, queries, keys)[1]
+    held = torch.isfinite(want)
+    assert torch.equal(held, torch.isfinite(lse))
+    assert float((lse[held].double() - want[held]).abs().max()) <= 1e-4
