@@ -301,3 +301,25 @@ def test_log_sum_exp_of_bfloat16_is_that_of_float32(queries, keys):
     held = torch.isfinite(want)
     assert torch.equal(held, torch.isfinite(lse))
     assert float((lse[held].double() - want[held]).abs().max()) <= 1e-4
+
+
+@pytest.mark.parametrize("queries,keys,H,Hk,D", [([300, 129], [300, 129], 4, 2, 64), ([200], [4000], 2, 2, 48),
+                                                 ([700], [700], 3, 3, 32), ([260], [400], 2, 1, 128), ([1, 2], [900, 300], 4, 2, 64)])
+@pytest.mark.parametrize("bias", [True, False])
+def test_bfloat16_results_are_rounded_once(queries, keys, H, Hk, D, bias):
+    """What bfloat16 results are off by is their own rounding: they are the rounded float64 results but for values beside
+    a rounding's edge.  Before it they are within d = 2^-16 of the norm (probabilities in two pieces of 8 bits, sums of
+    float32); a value within d of an edge goes to the other side, a step of r = 2^-7 at most, in a share d / r of all:
+    sqrt(d r) = 3.5e-4 of the norm, and twice that is allowed."""
+    from ye3t_b200 import runtime as rt
+    q, k, v, grad, x, y, sl = _inputs(queries, keys, H, Hk, D, torch.bfloat16, D)
+    layout = rt.StructureLayout(queries, keys, heads=H, key_heads=Hk, device=DEV)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    places = dict(positions=x, key_positions=y, slopes=sl) if bias else {}
+    out = rt.structure_attention(q, k, v, layout, **places)
+    got = (out,) + torch.autograd.grad(out, leaves, grad)
+    wide = [t.detach().double().requires_grad_(True) for t in leaves]
+    want = _definition(*wide, x, y, sl if bias else 0.0 * sl, D ** -0.5, queries, keys)[0]
+    for a, b, what in zip(got, (want,) + torch.autograd.grad(want, wide, grad.double()), ("out", "dq", "dk", "dv")):
+        off = (a.detach().double() - b.detach().bfloat16().double()).norm() / b.detach().norm()
+        assert float(off) <= 2.0 * 2.0 ** -11.5, (what, float(off))

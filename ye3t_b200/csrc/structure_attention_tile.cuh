@@ -7,7 +7,7 @@
 //   key side   rows = keys,    columns = queries  S = K Q^T, T = V G^T dV += P G, dK += dS Q
 // (G = gradient of the output.)  Per tile of BN columns: tcgen05.mma forms the score products in
 // tensor memory; thread r of the four score warps reads row r, does the softmax arithmetic in fp32 and
-// writes P or dS back to tensor memory as bf16, where it is the A operand of the accumulating product
+// writes P or dS back to tensor memory in bf16 pieces, where it is the A operand of the accumulating product
 // (B: the same shared-memory column tile, read MN-major).  One warp issues the MMAs, one
 // warp brings the column tiles (TMA; a tile cut by the structure's end with cp.async and zeros), so that
 // nothing of another structure enters a product.
@@ -20,7 +20,10 @@
 // 8 heads of 64, bf16: forward 1.27 ms (433 TFLOP/s); 8,192 atoms: forward 370, query side 678, key side 564 us.
 //
 // fp32 data is carried as three bf16 pieces (8 + 8 + 8 bits): six products of pieces give each
-// product to about 2^-24, and P and dS are split likewise.
+// product to about 2^-24, and P and dS are split likewise.  With bf16 data P and dS are two pieces, 2^-17: results are then
+// as far from 64 bits as their own rounding (8,192 atoms, 8 heads of 64: 1.66e-3 of the norm, the result and all
+// gradients; with one piece 2.16e-3 and 2.35e-3).  The second piece costs the forward 382 -> 411 us, the query side 697 ->
+// 730, the key side 571 -> 687.
 #pragma once
 
 #include <cuda.h>
@@ -106,7 +109,12 @@ struct AttCfg {
   // 207; rows in tensor memory and the MMA loop entered by the whole warp: 263 and 350).
   static constexpr bool ROWS_TMEM = NP == 3 && (DP == 64 || MODE == kForward);
   static constexpr int ROW_BYTES = ROWS_TMEM ? 0 : HP * ROWOPS * NP * ROW_PIECE;
-  // Tensor memory columns.  P and dS (NP * BN / 2 columns each) take the place of the scores they come from.
+  // Tensor memory columns.  P and dS, in AP pieces of BN / 2 columns each, take the place of the scores they come from.
+  // Two pieces lie by turns, so that those of 16 columns fill these columns and no others.
+  static constexpr int AP = NP == 1 ? 2 : 3;
+  __device__ static constexpr int piece_at(int piece, int step) {
+    return AP == 2 ? step * 16 + piece * 8 : piece * (BN / 2) + step * 8;
+  }
   // Score buffers: with two, the products of tile j + 1 run under the arithmetic of tile j (a single
   // stage of columns allows one).
   static constexpr int BUFS = STAGES > 1 && !KEY_BF16 ? 2 : 1;
@@ -156,6 +164,13 @@ template <> struct Pieces<3> {
   __device__ static constexpr int a(int n) { return n == 0 ? 2 : n == 2 ? 1 : n == 3 ? 1 : 0; }
   __device__ static constexpr int b(int n) { return n == 1 ? 2 : n == 2 ? 1 : n == 4 ? 1 : 0; }
 };
+// The same of the accumulating products, whose A operand has two pieces where the data has one.
+template <int NP> struct AccPieces : Pieces<NP> {};
+template <> struct AccPieces<1> {
+  static constexpr int N = 2;
+  __device__ static constexpr int a(int n) { return 1 - n; }
+  __device__ static constexpr int b(int) { return 0; }
+};
 
 // Rows [0, valid) of an operand into a tile of ROWS x DP in the 128-byte swizzle, zeros elsewhere.
 template <int ROWS, int DP, int NP>
@@ -180,12 +195,11 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const AttOperand& o, int
 template <int NP>
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&r)[NP]) {
   r[0] = tc::bf16x2(a, b);
-  if constexpr (NP == 3) {
-    float ra = a - __uint_as_float(r[0] << 16), rb = b - __uint_as_float(r[0] & 0xffff0000u);
-    r[1] = tc::bf16x2(ra, rb);
-    ra -= __uint_as_float(r[1] << 16);
-    rb -= __uint_as_float(r[1] & 0xffff0000u);
-    r[2] = tc::bf16x2(ra, rb);
+#pragma unroll
+  for (int p = 1; p < NP; ++p) {
+    a -= __uint_as_float(r[p - 1] << 16);
+    b -= __uint_as_float(r[p - 1] & 0xffff0000u);
+    r[p] = tc::bf16x2(a, b);
   }
 }
 
@@ -442,18 +456,20 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP, HP>::THREADS, AttCfg<MODE
         if (lead) {
           constexpr int kOps = C::OPS + (C::FIX ? 1 : 0);
 #pragma unroll
-          for (int n = 0; n < Pieces<NP>::N; ++n) {
+          for (int n = 0; n < AccPieces<NP>::N; ++n) {
 #pragma unroll
             for (int ks = 0; ks < BN / 16; ++ks) {
 #pragma unroll
               for (int u = 0; u < HP * kOps; ++u) {
                 const int h = u / kOps, op = u % kOps;
+                const bool one = C::FIX && op == 1;  // P K, the small correction's factor, has one piece
+                if (one && AccPieces<NP>::a(n) > 0) continue;
                 const int second = MODE == kForward || (MODE == kKeySide && op == 0) ? 1 : 0;  // V or G
                 tc::mma_ts(tmem + C::ACC + (h * C::NACC + op) * C::W,
-                           buf + h * C::BUF + (op == 0 ? C::A0 : C::A1) + Pieces<NP>::a(n) * (BN / 2) + ks * 8,
-                           b0 + uint64_t((h * C::COL_HEAD + (second * NP + Pieces<NP>::b(n)) * C::COL_PIECE + ks * 2048) /
-                                         16),
-                           id_a, n > 0 || ks > 0 ? 1u : go_on);
+                           buf + h * C::BUF + (op == 0 ? C::A0 : C::A1) + C::piece_at(AccPieces<NP>::a(n), ks),
+                           b0 + uint64_t((h * C::COL_HEAD + (second * NP + AccPieces<NP>::b(n)) * C::COL_PIECE +
+                                          ks * 2048) / 16),
+                           id_a, ks > 0 || (n > 0 && !one) ? 1u : go_on);
               }
             }
           }
@@ -666,7 +682,7 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP, HP>::THREADS, AttCfg<MODE
         const uint32_t dst = lane_base + C::A0 + ((j % C::BUFS) * HP + h) * C::BUF;
 #pragma unroll
         for (int c0 = 0; c0 < BN; c0 += 16) {
-          uint32_t pr[NP][8];
+          uint32_t pr[C::AP][8];
 #pragma unroll
           for (int c = 0; c < 16; c += 2) {
             float e0, e1;
@@ -675,13 +691,13 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP, HP>::THREADS, AttCfg<MODE
             e1 = tc::ex2(e1);
             if (c & 2) l1 = tc::add2(l1, tc::pack(e0, e1));
             else l0 = tc::add2(l0, tc::pack(e0, e1));
-            uint32_t r[NP];
-            split_pair<NP>(e0, e1, r);
+            uint32_t r[C::AP];
+            split_pair<C::AP>(e0, e1, r);
 #pragma unroll
-            for (int p = 0; p < NP; ++p) pr[p][c / 2] = r[p];
+            for (int p = 0; p < C::AP; ++p) pr[p][c / 2] = r[p];
           }
 #pragma unroll
-          for (int p = 0; p < NP; ++p) tc::st8(dst + p * (BN / 2) + c0 / 2, pr[p]);
+          for (int p = 0; p < C::AP; ++p) tc::st8(dst + C::piece_at(p, c0 / 16), pr[p]);
         }
         float s0, s1;
         tc::unpack(tc::add2(l0, l1), s0, s1);
@@ -693,8 +709,8 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP, HP>::THREADS, AttCfg<MODE
     const auto backward_tile = [&](auto cut, int j, int n, const float* ex, uint32_t buf) {
       constexpr bool CUT = decltype(cut)::value;
       const uint32_t dst = lane_base + (j % C::BUFS) * C::BUF;
-      // One piece: the next 16 columns load under these; P and dS of columns c0 .. take half of the columns that were
-      // read.  Several pieces take more than that: all scores come to registers first.
+      // bf16 data: the next 16 columns load under these; P and dS of columns c0 .. take the columns that were read.  Three
+      // pieces take more than that: all scores come to registers first.
       constexpr int HOLD = NP == 1 ? 2 : BN / 16;
       float sv[HOLD][16], tv[HOLD][16];
 #pragma unroll
@@ -711,8 +727,9 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP, HP>::THREADS, AttCfg<MODE
           tc::ld16(buf + c0 + 16, sv[cur ^ 1]);
           tc::ld16(buf + C::T + c0 + 16, tv[cur ^ 1]);
         }
-        [[maybe_unused]] uint32_t pr[NP][8];
-        uint32_t dr[NP][8];
+        constexpr int PP = MODE == kKeySide ? C::AP : 1;  // pieces of P
+        [[maybe_unused]] uint32_t pr[PP][8];
+        uint32_t dr[C::AP][8];
 #pragma unroll
         for (int c = 0; c < 16; c += 2) {
           const int cc = c0 + c;
@@ -766,23 +783,24 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP, HP>::THREADS, AttCfg<MODE
             }
           }
           if constexpr (MODE == kKeySide || C::FIX) {
-            uint32_t q[NP];
-            split_pair<NP>(p0, p1, q);
+            uint32_t q[PP];
+            split_pair<PP>(p0, p1, q);
 #pragma unroll
-            for (int k = 0; k < NP; ++k) pr[k][c / 2] = q[k];
+            for (int k = 0; k < PP; ++k) pr[k][c / 2] = q[k];
           }
-          uint32_t q[NP];
-          split_pair<NP>(g0, g1, q);
+          uint32_t q[C::AP];
+          split_pair<C::AP>(g0, g1, q);
 #pragma unroll
-          for (int k = 0; k < NP; ++k) dr[k][c / 2] = q[k];
+          for (int k = 0; k < C::AP; ++k) dr[k][c / 2] = q[k];
         }
+        // key side: P first, then dS, stored by turns (8,192 atoms, 8 heads: 687 us, one after the other 723); query side: dS
+        // first
 #pragma unroll
-        for (int k = 0; k < NP; ++k) {
-          // key side: P first, then dS; query side: dS first
-          tc::st8(dst + (MODE == kKeySide ? C::A1 : C::A0) + k * (BN / 2) + c0 / 2, dr[k]);
-          if constexpr (MODE == kKeySide || C::FIX)
-            tc::st8(dst + (MODE == kKeySide ? C::A0 : C::A1) + k * (BN / 2) + c0 / 2, pr[k]);
+        for (int k = 0; k < C::AP; ++k) {
+          tc::st8(dst + (MODE == kKeySide ? C::A1 : C::A0) + C::piece_at(k, c0 / 16), dr[k]);
+          if constexpr (MODE == kKeySide) tc::st8(dst + C::A0 + C::piece_at(k, c0 / 16), pr[k]);
         }
+        if constexpr (C::FIX) tc::st8(dst + C::A1 + C::piece_at(0, c0 / 16), pr[0]);
       }
       return true;
     };
