@@ -430,14 +430,14 @@ int few(const AttArgs& a, const AttItem* items, int64_t count, int DP, int width
     return a.D % W == 0 && row % W == 0 && head % W == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0;
   };
   const int64_t dense = int64_t(a.H) * a.D;
-  const int vec = (fits(a.q, a.q_row, a.q_head) ? 1 : 0) | (fits(a.k, a.k_row, a.k_head) ? 2 : 0) |
-                  (fits(a.v, a.v_row, a.v_head) ? 4 : 0) |
+  const int vec = (fits(a.q, a.q_row, a.q_head) ? 1 : 0) |
                   (BACKWARD && fits(out, dense, a.D) && fits(grad, dense, a.D) ? 8 : 0);
+  const bool loads = fits(a.k, a.k_row, a.k_head) && fits(a.v, a.v_row, a.v_head);
   const int64_t blocks = (kFewQueries * a.group + kFewRows - 1) / kFewRows, grid = count * a.Hk * blocks;
   if (grid > INT32_MAX) return fail(Y3B_ERR_UNSUPPORTED, "structure_attention: too many chunks");
 #define Y3B_FEW(LPK)                                                                                           \
   do {                                                                                                         \
-    if ((vec & 6) == 6)                                                                                        \
+    if (loads)                                                                                                 \
       few_kernel<T, LPK, BACKWARD, true>                                                                       \
           <<<unsigned(grid), 32 * kFewWarps, 0, s>>>(a, items, DP, width, vec, out, grad, lse, part);          \
     else                                                                                                       \

@@ -5,10 +5,12 @@
 // structure's operands sit in shared memory, a warp takes 16 rows, and the products run on mma.sync.  fp32 data is
 // split in two tf32 parts with three products (hi hi + hi lo + lo hi, to about 2^-22).  bf16 scores and results use
 // bf16 operands straight from shared memory (ldmatrix): with the conversions to tf32 2,048 molecules of 0-39 atoms, 8
-// heads of 32, took 75 us, without them 63.  The backward's other products take bf16 data as tf32, in which it is
-// exact, since P and dS are kept in fp32.  The backward forms P once more from the scores (so it needs nothing of the
-// forward), keeps P and dS in shared memory and gives every gradient in one launch.  Rows and columns past the
-// structure's end are zeros in shared memory.
+// heads of 32, took 75 us, without them 63.  dK and dV of bf16 data take P and dS, which are kept in fp32, as one tf32
+// part (11 bits: 2^-12 of a probability beside the result's rounding of 2^-8; 512 molecules of 32 atoms 1.67e-3 of the
+// norm off 64 bits, the rounding alone 1.66e-3) and the data itself, which tf32 holds exactly.  fp32 leaves out the
+// product of both low parts: results are 3 to 4e-7 of the norm off, those of fp32 arithmetic 2e-7.  The backward forms P
+// once more from the scores (so it needs nothing of the forward), keeps P and dS in shared memory and gives every
+// gradient in one launch.  Rows and columns past the structure's end are zeros in shared memory.
 //
 // The forward is bound by instruction issue (70 % of the cycles): of some 1,200 instructions that a warp of 16 rows
 // executes, the 11 scores a lane take about 300, the rest goes into the addresses, loads, masks and stores of rows
@@ -182,12 +184,9 @@ __device__ __forceinline__ void store_pair(T* dst, int d, int D, float a, float 
 
 // Two neighbouring values of a row.
 __device__ __forceinline__ float2 pair_at(const float* p) { return *reinterpret_cast<const float2*>(p); }
-__device__ __forceinline__ float2 pair_at(const __nv_bfloat16* p) {
-  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p));
-}
 
-// The same for bf16 data, in steps of 16 components (the last one may have 8).  Rows up to the next multiple of 16 are
-// read.
+// Products of 16 rows of X with the rows of Y in bf16, in steps of 16 components (the last one may have 8): out[t] (rows
+// g, g + 8; columns 8 t + 2 c, + 1) = X Y^T.  Rows up to the next multiple of 16 are read.
 template <int NT>
 __device__ __forceinline__ void scores_bf16(float (&out)[NT][4], const __nv_bfloat16* x, const __nv_bfloat16* y,
                                             int stride, int nt, int width, int lane) {
@@ -223,33 +222,28 @@ __device__ __forceinline__ void scores_bf16(float (&out)[NT][4], const __nv_bflo
   }
 }
 
-// Products of 16 rows of X with the rows of Y: out[t] (rows g, g + 8; columns 8 t + 2 c, + 1) = X Y^T.  Both
-// operands take the components of a step in the order 2 c, 2 c + 1, which are read as a pair.  fp32: the tensor cores
-// cut a sum towards zero each time that they add to it, which is the same way for every score; each step's products
-// are therefore added to the score outside (a readout's slope gradient 3.4e-6 -> 2.0e-6 off, for 4 % of the backward's
-// time).
+// The same for either type.  fp32: both operands take the components of a step in the order 2 c, 2 c + 1, which are read
+// as a pair.  The tensor cores cut a sum towards zero each time that they add to it, which is the same way for every
+// score; each step's products are therefore added to the score outside (a readout's slope gradient 3.4e-6 -> 2.0e-6 off,
+// for 4 % of the backward's time).
 template <typename T, int NT>
 __device__ __forceinline__ void scores(float (&out)[NT][4], const T* x, const T* y, int stride, int nt, int width,
                                        int g, int c) {
   if constexpr (sizeof(T) == 2) {
     scores_bf16<NT>(out, x, y, stride, nt, width, 4 * g + c);
-    return;
-  }
-  constexpr int N = Parts<T>::N;
+  } else {
+    constexpr int N = Parts<T>::N;
 #pragma unroll
-  for (int t = 0; t < NT; ++t) out[t][0] = out[t][1] = out[t][2] = out[t][3] = 0.0f;
+    for (int t = 0; t < NT; ++t) out[t][0] = out[t][1] = out[t][2] = out[t][3] = 0.0f;
 #pragma unroll 2
-  for (int k = 0; k < width; k += 8) {
-    const T* x0 = x + g * stride + k + 2 * c;
-    const float2 a0 = pair_at(x0), a1 = pair_at(x0 + 8 * stride);
-    const FragA<N> a = frag_a<N, true>(a0.x, a1.x, a0.y, a1.y);
+    for (int k = 0; k < width; k += 8) {
+      const T* x0 = x + g * stride + k + 2 * c;
+      const float2 a0 = pair_at(x0), a1 = pair_at(x0 + 8 * stride);
+      const FragA<N> a = frag_a<N, true>(a0.x, a1.x, a0.y, a1.y);
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      if (t < nt) {
-        const float2 b = pair_at(y + (8 * t + g) * stride + k + 2 * c);
-        if constexpr (N == 1) {
-          product<N>(out[t], a, b.x, b.y);
-        } else {
+      for (int t = 0; t < NT; ++t) {
+        if (t < nt) {
+          const float2 b = pair_at(y + (8 * t + g) * stride + k + 2 * c);
           float step[4] = {0.0f, 0.0f, 0.0f, 0.0f};
           product<N>(step, a, b.x, b.y);
 #pragma unroll
@@ -462,8 +456,8 @@ __global__ void __launch_bounds__(16 * NT) small_forward_kernel(const __grid_con
 template <typename T, int NT, int DT>
 constexpr int backward_ctas = DT == 4 && (sizeof(T) == 4) == (NT == 4) ? 24 / NT : 1;
 
-// MODE of the accumulators: dk and dv of 16 keys x up to 8 * DT components stay in registers over the query heads
-// that share the key head.
+// The accumulators of dk and dv of 16 keys x up to 8 * DT components stay in registers over the query heads that share
+// the key head.
 template <typename T, int NT, int DT>
 __global__ void __launch_bounds__(16 * NT, backward_ctas<T, NT, DT>) small_backward_kernel(
     const __grid_constant__ AttArgs a, const AttSmall* __restrict__ list, int64_t n, int stride, int shift, int vec,
