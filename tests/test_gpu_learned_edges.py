@@ -304,7 +304,8 @@ def test_log_sum_exp_of_bfloat16_is_that_of_float32(queries, keys):
 
 
 @pytest.mark.parametrize("queries,keys,H,Hk,D", [([300, 129], [300, 129], 4, 2, 64), ([200], [4000], 2, 2, 48),
-                                                 ([700], [700], 3, 3, 32), ([260], [400], 2, 1, 128), ([1, 2], [900, 300], 4, 2, 64)])
+                                                 ([700], [700], 3, 3, 32), ([260], [400], 2, 1, 128),
+                                                 ([1, 2], [900, 300], 4, 2, 64)])
 @pytest.mark.parametrize("bias", [True, False])
 def test_bfloat16_results_are_rounded_once(queries, keys, H, Hk, D, bias):
     """What bfloat16 results are off by is their own rounding: they are the rounded float64 results but for values beside

@@ -3,10 +3,10 @@
 //   out[i, c]   = scale * table[z_i, c]
 //   dtable[v, c] = scale * sum_{i : z_i = v} grad[i, c]
 //
-// The lookup is one pass over the output.  The gradient of a small table (a few hundred species) is summed
-// in copies of the table in shared memory; that of a larger one orders the atoms by species (stable
-// radix sort of the indices) and sums runs of equal species.  Neither needs floating-point atomics, and
-// results are bitwise repeatable.
+// The lookup is one pass over the output.  The gradient of a small table (up to 26 species; 108, in fp64 53, where the
+// channels are no multiple of the vectors' width) is summed in copies of the table in shared memory; that of a larger one
+// orders the atoms by species (stable radix sort of the indices) and sums runs of equal species.  Neither needs
+// floating-point atomics, and results are bitwise repeatable.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -34,7 +34,8 @@ __device__ __forceinline__ int64_t species_at(const I* z, int64_t i, int64_t V) 
 }
 
 // A CTA is X threads along the channels by 256 / X along the atoms; a thread writes VEC channels of kLookups atoms.
-// Bound by the output's store: the table stays in L2.
+// The table stays in L2.  2^20 atoms x 32 in fp32: 37 us, 3.6 TB/s of output; issue is 63 % active and DRAM writes 2 TB/s
+// (the rest of the output is still in L2), so that neither is the bound by itself.
 constexpr int kLookups = 4;
 
 template <typename T, typename I, int VEC>

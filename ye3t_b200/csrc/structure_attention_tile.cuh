@@ -13,11 +13,11 @@
 // nothing of another structure enters a product.
 //
 // What bounds it: the score warps.  A score takes one exp2 and one reciprocal square root on the special-function unit
-// (16 lanes a cycle and SM, so 8 scores a cycle and SM) and 9 to 25 fp32 operations (forward with shared distances, key
-// side 16, query side 25), a packed pair of which takes two issue cycles; the products of a score at D = 64 take 1/32
-// of a cycle (forward).  The warps issue at about 75 % of what that mix allows.  Two CTAs share an SM, or two score
-// groups, so that one's MMAs and waits lie under another's arithmetic; more warps an SM gained nothing.  16,384 atoms,
-// 8 heads of 64, bf16: forward 1.27 ms (433 TFLOP/s); 8,192 atoms: forward 370, query side 678, key side 564 us.
+// (16 lanes a cycle and SM, so 8 scores a cycle and SM) and 12 to 28 operations (forward with shared distances, key
+// side 22, query side 28), a packed fp32 pair of which takes two issue cycles; the products of a score at D = 64 take 3/64
+// of a cycle (forward).  The warps issue in 52 to 60 % of the cycles, packed pairs counted once.  Two CTAs share an SM, or
+// two score groups, so that one's MMAs and waits lie under another's arithmetic; more warps an SM gained nothing.  16,384
+// atoms, 8 heads of 64, bf16: forward 1.40 ms (393 TFLOP/s); 8,192 atoms: forward 406, query side 721, key side 684 us.
 //
 // fp32 data is carried as three bf16 pieces (8 + 8 + 8 bits): six products of pieces give each
 // product to about 2^-24, and P and dS are split likewise.  With bf16 data P and dS are two pieces, 2^-17: results are then
@@ -92,7 +92,7 @@ struct AttCfg {
   static constexpr int STAGES = NP == 3 ? (DP == 128 && MODE != kForward ? 1 : 2) : DP == 128 ? 2 : 4;
   // Score groups of four warps; with two, each takes every other column tile: for what leaves an SM a single CTA.
   // Two CTAs of one group with 64 columns a tile and one buffer (key side), or 32 and two (query side), are 6 and 7 %
-  // faster than two of two groups (8,192 atoms, 8 heads of 64: 636 against 677 us, 777 against 837).
+  // faster than two of two groups (8,192 atoms, 8 heads of 64, one piece of P and dS: 636 against 677 us, 777 against 837).
   static constexpr int GROUPS = MODE != kForward && STAGES > 1 && (NP == 3 || DP == 128) ? 2 : 1;
   static constexpr int MMA_WARP = 4 * GROUPS, LOAD_WARP = MMA_WARP + 1;
   static constexpr int THREADS = 32 * (LOAD_WARP + 1);
@@ -793,8 +793,8 @@ __global__ void __launch_bounds__(AttCfg<MODE, DP, NP, HP>::THREADS, AttCfg<MODE
 #pragma unroll
           for (int k = 0; k < C::AP; ++k) dr[k][c / 2] = q[k];
         }
-        // key side: P first, then dS, stored by turns (8,192 atoms, 8 heads: 687 us, one after the other 723); query side: dS
-        // first
+        // key side: P first, then dS, stored by turns (8,192 atoms, 8 heads: 687 us, one after the other 723); query side:
+        // dS first
 #pragma unroll
         for (int k = 0; k < C::AP; ++k) {
           tc::st8(dst + (MODE == kKeySide ? C::A1 : C::A0) + C::piece_at(k, c0 / 16), dr[k]);

@@ -11,7 +11,7 @@
 //           keys: with an entry a key this table took 1.1 ms and 1.2 MB, in items 0.05 ms and 41 KB);
 //   tile    the rest.
 // A tile's columns are cut into parts, which are joined, where that makes the last wave of CTAs shorter (16,384 atoms, 8
-// heads: forward 1,273 us and 39 to join against 1,431 uncut).
+// heads: forward 1,273 us and 39 to join against 1,431 uncut, when P had one piece).
 #include <algorithm>
 #include <iterator>
 #include <new>
@@ -162,8 +162,12 @@ int64_t build(const int64_t* queries, const int64_t* keys, int64_t n, int64_t he
       if (queries[s] > kFew || queries[s] == 0) key_tiled.push_back(s);
     }
   }
-  // Places: two CTAs an SM of the tile kernels, and the forward's take two heads where their number is even; four of
-  // the few-query kernels.
+  // Places: two CTAs an SM of the tile kernels; four of the few-query kernels.  The forward's are counted as those of the
+  // kernel that takes two heads a CTA, where their number is even: a layout knows neither the type nor the width, and
+  // that kernel (bf16 with distances, widths up to 64) gains more by it (8,192 atoms, 8 heads of 64: 410 us against 454 cut
+  // for half the places; 16,384 atoms 1,423 and 1,414) than the others mostly lose (fp32, 4,096 atoms, 4 heads of 64: 164 us
+  // against 158; 8,192 atoms 535 and 534; 16 clusters of 300, 8 heads on 2, fp32: 70 and 58; bf16, 8,192 atoms, 8 heads of
+  // 128: 565 and 538).
   Side forward, query, key, one;
   add_tiles(&forward, q, k, tiled, heads, kSMs * (heads % 2 == 0 ? 4 : 2), false);
   add_tiles(&query, q, k, tiled, heads, kSMs * 2, false);
