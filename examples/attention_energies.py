@@ -6,7 +6,8 @@ The ACE features of every atom (fixed, from ``ACEEvaluator``) and a learned vect
 (``runtime.species_embedding``) make its state; one attention layer exchanges states among the atoms of each
 structure, weaker with distance (``runtime.structure_attention``); a second one, with a single query per structure,
 pools them into an energy.  The model is fitted to energies of a pair potential, which the features alone, with
-their cutoff, describe in part.
+their cutoff, describe in part.  The features' neighbours are those of a periodic box; the attention and the energies
+know the atoms in it and none of their images.
 """
 
 import argparse
