@@ -7,8 +7,9 @@
 //   row     no or a single key: its weight is exactly 1 and its gradients through the softmax exactly 0, which the
 //           row kernels keep;
 //   few     up to two queries: a tile would hold 2 rows of 128 (8 structures of 16,384 keys, 8 heads: 111 us on tiles,
-//           64 on the few-query kernels; their keys' gradients 209 us on tiles, 121 by a few lanes a key, in items of 128
-//           keys: with an entry a key this table took 1.1 ms and 1.2 MB, in items 0.05 ms and 41 KB);
+//           64 on the few-query kernels; their keys' gradients 209 us on tiles, 111 by a few lanes a key, in items of 128
+//           keys: with an entry a key the tables of 8 structures of 14,000 keys took 701 us and 889 KB on the host, in
+//           items 22 us and 33 KB);
 //   tile    the rest.
 // A tile's columns are cut into parts, which are joined, where that makes the last wave of CTAs shorter (16,384 atoms, 8
 // heads: forward 1,273 us and 39 to join against 1,431 uncut, when P had one piece).
